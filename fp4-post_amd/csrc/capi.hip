@@ -627,4 +627,34 @@ int metis_linear_wgrad_ws(const void* dyt_codes, const void* dyt_scales, const f
                       nullptr, grad_weight, out_dtype, (hipStream_t)stream, workspace, workspace_bytes);
 }
 
+int metis_residual_norm(const void* x, int x_dtype, const void* y, int y_dtype, const void* weight, const void* post_weight, const void* gate,
+                        int64_t gate_rows, float scale, float eps, int64_t rows, int64_t cols, void* h, void* n, void* stream)
+{
+    return residual_norm(x, x_dtype, y, y_dtype, weight, post_weight, gate, gate_rows, scale, eps, rows, cols, h, n, (hipStream_t)stream);
+}
+
+size_t metis_residual_norm_backward_workspace_bytes(int64_t rows, int64_t cols, int64_t gate_rows)
+{
+    return residual_norm_backward_workspace_bytes(rows, cols, gate_rows);
+}
+
+int metis_residual_norm_backward(const void* h, int x_dtype, const void* y, int y_dtype, const void* weight, const void* post_weight, const void* gate,
+                                 int64_t gate_rows, float scale, float eps, int64_t rows, int64_t cols, const void* grad_h, const void* grad_n, void* grad_x,
+                                 void* grad_y, void* grad_weight, void* grad_post_weight, void* grad_gate, void* workspace, size_t workspace_bytes, void* stream)
+{
+    return residual_norm_backward(h, x_dtype, y, y_dtype, weight, post_weight, gate, gate_rows, scale, eps, rows, cols, grad_h, grad_n, grad_x, grad_y, grad_weight,
+                                  grad_post_weight, grad_gate, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int metis_swiglu(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int64_t rows, int64_t cols, int dtype, void* out, void* stream)
+{
+    return swiglu(gate, ld_gate, up, ld_up, nullptr, rows, cols, dtype, false, out, nullptr, (hipStream_t)stream);
+}
+
+int metis_swiglu_backward(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, const void* grad, int64_t rows, int64_t cols, int dtype,
+                          void* grad_gate, void* grad_up, void* stream)
+{
+    return swiglu(gate, ld_gate, up, ld_up, grad, rows, cols, dtype, true, grad_gate, grad_up, (hipStream_t)stream);
+}
+
 }  // extern "C"

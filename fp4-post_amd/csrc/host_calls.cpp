@@ -129,6 +129,10 @@ constexpr Entry kEntries[] = {
     METIS_ENTRY(metis_lowrank_project_rows_ws),
     METIS_ENTRY(metis_lowrank_project_rows_grouped),
     METIS_ENTRY(metis_lowrank_backward),
+    METIS_ENTRY(metis_residual_norm),
+    METIS_ENTRY(metis_residual_norm_backward),
+    METIS_ENTRY(metis_swiglu),
+    METIS_ENTRY(metis_swiglu_backward),
 };
 constexpr size_t kMaxArgs = 32, kMaxOuts = 32;
 constexpr bool all_counted()

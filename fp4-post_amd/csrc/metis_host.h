@@ -114,6 +114,16 @@ int token_mean_quant(const void* x, int64_t rows, int64_t cols, int after_norm, 
 size_t rmsnorm_backward_workspace_bytes(int64_t rows, int64_t cols);
 int rmsnorm_backward(const void* x, const void* g, const void* gamma, float eps, int64_t rows, int64_t cols, void* gx, void* ggamma,
                      int ggamma_bf16, void* workspace, size_t workspace_bytes, hipStream_t st);
+// residual sum with the norms before and after a block, and its gradients; residual_norm.hip
+int residual_norm(const void* x, int x_dtype, const void* y, int y_dtype, const void* weight, const void* post, const void* gate, int64_t gate_rows, float scale,
+                  float eps, int64_t rows, int64_t cols, void* h, void* n, hipStream_t st);
+size_t residual_norm_backward_workspace_bytes(int64_t rows, int64_t cols, int64_t gate_rows);
+int residual_norm_backward(const void* h, int x_dtype, const void* y, int y_dtype, const void* weight, const void* post, const void* gate, int64_t gate_rows,
+                           float scale, float eps, int64_t rows, int64_t cols, const void* gh, const void* gn, void* gx, void* gy, void* gweight, void* gpost,
+                           void* ggate, void* workspace, size_t workspace_bytes, hipStream_t st);
+// silu(gate) * up (back: its gradients into out and gup); swiglu.hip
+int swiglu(const void* gate, int64_t ldg, const void* up, int64_t ldu, const void* grad, int64_t rows, int64_t cols, int dtype, bool back, void* out, void* gup,
+           hipStream_t st);
 int gemm_nvfp4(const void* a_codes, const void* a_scales, const float* a_unit, const void* b_codes, const void* b_scales,
                const float* b_unit, int64_t M, int64_t N, int64_t K, const void* t, const void* u, int64_t r,
                const void* bias, void* out, int out_dtype, hipStream_t st, void* workspace = nullptr,

@@ -126,6 +126,11 @@ SIGNATURES = {
     "metis_linear_fwd_ws": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _sz, _vp]),
     "metis_linear_dgrad_ws": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _vp, _sz, _vp]),
     "metis_linear_wgrad_ws": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _vp, _sz, _vp]),
+    "metis_residual_norm": (_i32, [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _i64, _f32, _f32, _i64, _i64, _vp, _vp, _vp]),
+    "metis_residual_norm_backward_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "metis_residual_norm_backward": (_i32, [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _i64, _f32, _f32, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "metis_swiglu": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _vp]),
+    "metis_swiglu_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
 }
 
 _lib = None

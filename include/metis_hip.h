@@ -938,6 +938,46 @@ int metis_linear_fwd_f32bias(const void *a_codes, const void *a_scales, const fl
                              int64_t r, const float *bias, void *out, int out_dtype,
                              void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * The residual sum behind a block with the norms before and after it, in binary32 with each result rounded once:
+ *   z = y, or with post_weight  y * rstd(y) * post_weight           rstd(t) = 1 / sqrt(mean(t^2) + eps)
+ *   h = x + scale * gate * z                                        stored in x's type
+ *   n = h * rstd(h) * weight                                        of h as it is stored, in y's type
+ * (The reference's decoder layers do this in separate operations, src/Metis/models/llama.py:23-31 being the norm; unlike
+ * metis_rmsnorm, which follows that module, n is not rounded between the two products.)
+ *   x, h     [rows, cols] bf16 or float (x_dtype); y, n and all vectors bf16 or float (y_dtype), float only where x is float
+ *   gate     [gate_rows, cols], row g for rows g * rows / gate_rows ..; or NULL with gate_rows = 0
+ *   cols     a multiple of 8, at most 8192; every pointer 16-byte aligned; post_weight may be NULL
+ * Gradients, with grad_h and grad_n those of h and n (NULL: zero) and h the forward's result; d, dz as written:
+ *   grad_x = d = grad_h + rstd(h) (grad_n weight - hh mean(grad_n weight hh)),  hh = h rstd(h)
+ *   grad_y = dz = scale gate d, or through the norm of y;  grad_weight, grad_post_weight, grad_gate: binary32 sums in a
+ *   fixed order, rounded once.  Outputs may be NULL when they are not wanted (grad_y then also where it equals grad_x).
+ *   y        needed with post_weight or for grad_gate, else NULL
+ *   workspace metis_residual_norm_backward_workspace_bytes(rows, cols, gate_rows) bytes, no initialisation needed
+ */
+int metis_residual_norm(const void *x, int x_dtype, const void *y, int y_dtype, const void *weight,
+                        const void *post_weight, const void *gate, int64_t gate_rows, float scale,
+                        float eps, int64_t rows, int64_t cols, void *h, void *n, void *stream);
+size_t metis_residual_norm_backward_workspace_bytes(int64_t rows, int64_t cols, int64_t gate_rows);
+int metis_residual_norm_backward(const void *h, int x_dtype, const void *y, int y_dtype,
+                                 const void *weight, const void *post_weight, const void *gate,
+                                 int64_t gate_rows, float scale, float eps, int64_t rows, int64_t cols,
+                                 const void *grad_h, const void *grad_n, void *grad_x, void *grad_y,
+                                 void *grad_weight, void *grad_post_weight, void *grad_gate,
+                                 void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * out = silu(gate) * up between two projections of an MLP, and its gradients, in binary32 with each result rounded once.
+ *   gate, up  [rows, cols] bf16 or float (dtype), row strides ld_gate, ld_up (the halves of one product's rows as they
+ *             are); out, grad, grad_gate, grad_up dense.  Any sizes and alignment of whole elements; 16-byte aligned rows
+ *             of a multiple of 8 columns are read in whole pieces.
+ */
+int metis_swiglu(const void *gate, int64_t ld_gate, const void *up, int64_t ld_up, int64_t rows,
+                 int64_t cols, int dtype, void *out, void *stream);
+int metis_swiglu_backward(const void *gate, int64_t ld_gate, const void *up, int64_t ld_up,
+                          const void *grad, int64_t rows, int64_t cols, int dtype, void *grad_gate,
+                          void *grad_up, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

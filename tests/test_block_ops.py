@@ -1,0 +1,84 @@
+"""residual_norm and swiglu: what is refused, without a device."""
+import ctypes
+
+import pytest
+import torch
+
+from metis_hip import MetisHipError, _lib, ops, residual_norm, swiglu
+
+
+def test_host_tensors_are_refused():
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    w = torch.ones(64, dtype=torch.bfloat16)
+    with pytest.raises(MetisHipError, match="no CPU path"):
+        residual_norm(x, x, w)
+    with pytest.raises(MetisHipError, match="no CPU path"):
+        swiglu(x, x)
+
+
+@pytest.mark.parametrize("shape,gate,rows", [((2, 3, 8), (8,), 1), ((2, 3, 8), (2, 1, 8), 2), ((2, 3, 8), (1, 1, 8), 1), ((2, 3, 8), (2, 3, 8), 6),
+                                             ((5, 8), (5, 8), 5), ((5, 8), (1, 8), 1), ((8,), (8,), 1), ((1, 3, 8), (1, 3, 8), 3)])
+def test_gate_rows(shape, gate, rows):
+    assert ops.residual_norm_gate_rows(torch.empty(shape), torch.empty(gate)) == rows
+
+
+@pytest.mark.parametrize("shape,gate", [((2, 3, 8), (2, 8)), ((2, 3, 8), (3, 1, 8)), ((2, 3, 8), (1, 3, 8)), ((5, 8), (1, 5, 8)), ((5, 8), (4, 8))])
+def test_gates_of_other_shapes_are_refused(shape, gate):
+    with pytest.raises(ValueError, match="leading sizes"):
+        ops.residual_norm_gate_rows(torch.empty(shape), torch.empty(gate))
+
+
+def _norm_args(**changes):
+    """metis_residual_norm's arguments for 4 x 64 in bf16 with addresses that are never read."""
+    args = dict(x=4096, x_dtype=0, y=4096, y_dtype=0, weight=4096, post=None, gate=None, gate_rows=0, scale=1.0, eps=1e-6, rows=4, cols=64, h=4096, n=4096, stream=None)
+    args.update(changes)
+    return tuple(args.values())
+
+
+@pytest.mark.parametrize("changes", [dict(cols=60), dict(cols=0), dict(cols=8200), dict(rows=-1), dict(rows=1 << 31), dict(x_dtype=2), dict(y_dtype=1), dict(x=None), dict(y=None),
+                                     dict(weight=None), dict(h=None), dict(n=None), dict(x=4098), dict(weight=4104), dict(gate=4096), dict(gate_rows=2),
+                                     dict(gate=4096, gate_rows=3), dict(gate=4096, gate_rows=-1), dict(post=4100)])
+def test_the_abi_refuses_before_a_launch(changes):
+    assert _lib.load().metis_residual_norm(*_norm_args(**changes)) == _lib.E_ARG
+
+
+def test_no_rows_are_no_work():
+    assert _lib.load().metis_residual_norm(*_norm_args(rows=0, x=None, y=None)) == _lib.OK
+
+
+def _backward_args(**changes):
+    args = dict(h=4096, x_dtype=0, y=None, y_dtype=0, weight=4096, post=None, gate=None, gate_rows=0, scale=1.0, eps=1e-6, rows=4, cols=64, gh=4096, gn=4096, gx=4096, gy=4096,
+                gw=4096, gp=None, gg=None, workspace=4096, bytes=1 << 30, stream=None)
+    args.update(changes)
+    return tuple(args.values())
+
+
+@pytest.mark.parametrize("changes", [dict(rows=0), dict(cols=12), dict(h=None), dict(post=4096), dict(gp=4096), dict(gg=4096), dict(gate=4096, gate_rows=2, gg=4096),
+                                     dict(gh=4097), dict(gx=4100), dict(gw=4104)])
+def test_the_backward_refuses_before_a_launch(changes):
+    assert _lib.load().metis_residual_norm_backward(*_backward_args(**changes)) == _lib.E_ARG
+
+
+def test_the_backward_wants_its_workspace():
+    L = _lib.load()
+    need = L.metis_residual_norm_backward_workspace_bytes(4, 64, 0)
+    assert need > 0 and L.metis_residual_norm_backward_workspace_bytes(0, 64, 0) == 0 and L.metis_residual_norm_backward_workspace_bytes(4, 60, 0) == 0
+    assert L.metis_residual_norm_backward_workspace_bytes(4, 64, 3) == 0                        # 3 does not divide 4
+    for changes in (dict(workspace=None), dict(bytes=need - 1), dict(workspace=4100)):
+        assert L.metis_residual_norm_backward(*_backward_args(**changes)) == _lib.E_WORKSPACE
+
+
+@pytest.mark.parametrize("changes", [dict(rows=-1), dict(cols=-1), dict(dtype=2), dict(gate=None), dict(up=None), dict(out=None), dict(gate=4097), dict(ldg=63), dict(ldu=63),
+                                     dict(cols=1 << 31), dict(rows=1 << 40, cols=1 << 20, ldg=1 << 20, ldu=1 << 20)])
+def test_swiglu_refuses_before_a_launch(changes):
+    args = dict(gate=4096, ldg=64, up=4096, ldu=64, rows=4, cols=64, dtype=0, out=4096, stream=None)
+    args.update(changes)
+    L = _lib.load()
+    assert L.metis_swiglu(*args.values()) == _lib.E_ARG
+    back = (args["gate"], args["ldg"], args["up"], args["ldu"], ctypes.c_void_p(4096), args["rows"], args["cols"], args["dtype"], args["out"], 4096, None)
+    assert L.metis_swiglu_backward(*back) == _lib.E_ARG
+
+
+def test_swiglu_refuses_more_pieces_than_it_counts():
+    rows = (1 << 31) // 8
+    assert _lib.load().metis_swiglu(4096, 64, 4096, 64, rows, 64, 0, 4096, None) == _lib.E_TOO_LARGE
