@@ -657,4 +657,29 @@ int metis_swiglu_backward(const void* gate, int64_t ld_gate, const void* up, int
     return swiglu(gate, ld_gate, up, ld_up, grad, rows, cols, dtype, true, grad_gate, grad_up, (hipStream_t)stream);
 }
 
+size_t metis_head_index_bytes(int64_t tokens) { return head_index_bytes(tokens); }
+
+size_t metis_head_logprobs_workspace_bytes(int64_t tokens, int64_t H, int64_t V, int entropy) { return head_logprobs_workspace_bytes(tokens, H, V, entropy); }
+
+int metis_head_logprobs(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const void* targets, int64_t ignore_index, int64_t tokens,
+                        int64_t H, int64_t V, float temperature, float* logp, float* lse, float* entropy, void* index, void* workspace, size_t workspace_bytes,
+                        void* stream)
+{
+    return head_logprobs(hidden, ld_hidden, weight, ld_weight, targets, ignore_index, tokens, H, V, temperature, logp, lse, entropy, index, workspace, workspace_bytes,
+                         (hipStream_t)stream);
+}
+
+size_t metis_head_logprobs_backward_workspace_bytes(int64_t tokens, int64_t H, int64_t V, int want_hidden, int want_weight)
+{
+    return head_logprobs_backward_workspace_bytes(tokens, H, V, want_hidden, want_weight);
+}
+
+int metis_head_logprobs_backward(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const void* targets, int64_t tokens, int64_t H,
+                                 int64_t V, float temperature, const float* lse, const float* entropy, const float* grad_logp, const float* grad_entropy,
+                                 const void* index, void* grad_hidden, void* grad_weight, void* workspace, size_t workspace_bytes, void* stream)
+{
+    return head_logprobs_backward(hidden, ld_hidden, weight, ld_weight, targets, tokens, H, V, temperature, lse, entropy, grad_logp, grad_entropy, index, grad_hidden,
+                                  grad_weight, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
 }  // extern "C"

@@ -133,6 +133,8 @@ constexpr Entry kEntries[] = {
     METIS_ENTRY(metis_residual_norm_backward),
     METIS_ENTRY(metis_swiglu),
     METIS_ENTRY(metis_swiglu_backward),
+    METIS_ENTRY(metis_head_logprobs),
+    METIS_ENTRY(metis_head_logprobs_backward),
 };
 constexpr size_t kMaxArgs = 32, kMaxOuts = 32;
 constexpr bool all_counted()

@@ -124,6 +124,15 @@ int residual_norm_backward(const void* h, int x_dtype, const void* y, int y_dtyp
 // silu(gate) * up (back: its gradients into out and gup); swiglu.hip
 int swiglu(const void* gate, int64_t ldg, const void* up, int64_t ldu, const void* grad, int64_t rows, int64_t cols, int dtype, bool back, void* out, void* gup,
            hipStream_t st);
+// log-probabilities of given tokens under a large head, and their gradients; head_loss.hip
+size_t head_index_bytes(int64_t tokens);
+size_t head_logprobs_workspace_bytes(int64_t tokens, int64_t H, int64_t V, int entropy);
+int head_logprobs(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, const void* targets, int64_t ignore, int64_t tokens, int64_t H, int64_t V, float temperature,
+                  float* logp, float* lse, float* entropy, void* index, void* workspace, size_t workspace_bytes, hipStream_t st);
+size_t head_logprobs_backward_workspace_bytes(int64_t tokens, int64_t H, int64_t V, int want_hidden, int want_weight);
+int head_logprobs_backward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, const void* targets, int64_t tokens, int64_t H, int64_t V, float temperature,
+                           const float* lse, const float* entropy, const float* g_logp, const float* g_entropy, const void* index, void* grad_hidden, void* grad_weight,
+                           void* workspace, size_t workspace_bytes, hipStream_t st);
 int gemm_nvfp4(const void* a_codes, const void* a_scales, const float* a_unit, const void* b_codes, const void* b_scales,
                const float* b_unit, int64_t M, int64_t N, int64_t K, const void* t, const void* u, int64_t r,
                const void* bias, void* out, int out_dtype, hipStream_t st, void* workspace = nullptr,

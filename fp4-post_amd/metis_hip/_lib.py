@@ -131,6 +131,11 @@ SIGNATURES = {
     "metis_residual_norm_backward": (_i32, [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _i64, _f32, _f32, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "metis_swiglu": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _vp]),
     "metis_swiglu_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "metis_head_index_bytes": (_sz, [_i64]),
+    "metis_head_logprobs_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32]),
+    "metis_head_logprobs": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "metis_head_logprobs_backward_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
+    "metis_head_logprobs_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 
 _lib = None

@@ -1,0 +1,61 @@
+"""Log-probabilities of tokens under a model's head, and losses on them, without a tensor of logits.
+
+The reference's trainers take them from the logits that the model returns: log_softmax over [tokens, vocabulary] and a gather of the
+sampled tokens (its GRPO and DPO entries, src/grpo/grpo.py and src/dpo/dpo.py, through TRL), or cross entropy.  A head of 131072 rows makes
+that 2 GB in binary32 for 4096 tokens, several times over with the gradient.  Here the head's product, the softmax and the gather are one
+operator on the last hidden states and the head's weight.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, ignore_index, temperature, entropy):
+        logp, lse, ent, index = ops.head_logprobs(hidden, weight, targets, ignore_index, temperature, entropy)
+        ctx.save_for_backward(hidden, weight, targets, lse, ent, index)
+        ctx.temperature = temperature
+        ctx.set_materialize_grads(False)
+        return (logp, ent) if entropy else logp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_logp, grad_entropy=None):
+        if grad_logp is None and grad_entropy is None:
+            return (None,) * 6
+        hidden, weight, targets, lse, ent, index = ctx.saved_tensors
+        gx, gw = ops.head_logprobs_backward(hidden, weight, targets, ctx.temperature, lse, ent, index, grad_logp, grad_entropy, *ctx.needs_input_grad[:2])
+        return gx, gw, None, None, None, None
+
+
+def token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, temperature: float = 1.0, ignore_index: int = -100,
+                   entropy: bool = False):
+    """log softmax(hidden weight^T / temperature) at each token's target, float32 of targets' shape; with entropy=True also the entropy of each
+    token's distribution.
+
+    hidden    bf16 [..., H], the last hidden states (behind the final norm); H a multiple of 16
+    weight    bf16 [V, H], the head's weight; any V up to 2^22
+    targets   int64 [...]; a token whose target is ignore_index has 0 and no gradient, and its hidden state is not looked at.  Any other
+              target outside the vocabulary makes its results NaN.
+
+    Differentiable (once) in hidden and weight; the logits are formed in pieces, in both directions, and never kept."""
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _TokenLogprobs.apply(hidden, weight, targets, int(ignore_index), float(temperature), bool(entropy))
+    logp, _, ent, _ = ops.head_logprobs(hidden, weight, targets, ignore_index, temperature, entropy)
+    return (logp, ent) if entropy else logp
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, temperature: float = 1.0, ignore_index: int = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """Cross entropy of softmax(hidden weight^T / temperature) with the targets, as torch.nn.functional.cross_entropy on the logits would
+    give it ("mean": over the targets that are not ignored; NaN where all are), float32.  Operands as in token_logprobs."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"linear_cross_entropy: reduction is 'mean', 'sum' or 'none', not {reduction!r}")
+    loss = -token_logprobs(hidden, weight, targets, temperature=temperature, ignore_index=ignore_index)
+    if reduction == "none":
+        return loss
+    return loss.sum() if reduction == "sum" else loss.sum() / (targets != ignore_index).sum()

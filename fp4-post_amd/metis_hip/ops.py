@@ -1441,6 +1441,93 @@ def swiglu_backward(gate: torch.Tensor, up: torch.Tensor, grad: torch.Tensor) ->
     return new[0], new[1]
 
 
+@functools.lru_cache(maxsize=4096)
+def _head_bytes(tokens: int, H: int, V: int, entropy: bool) -> tuple[int, int]:
+    L = load()
+    return int(L.metis_head_index_bytes(tokens)), int(L.metis_head_logprobs_workspace_bytes(tokens, H, V, entropy))
+
+
+@functools.lru_cache(maxsize=4096)
+def _head_backward_bytes(tokens: int, H: int, V: int, want_hidden: bool, want_weight: bool, device_index: int) -> int:
+    return int(load().metis_head_logprobs_backward_workspace_bytes(tokens, H, V, want_hidden, want_weight))      # depends on the device's CU count only
+
+
+def _head_operand(t: torch.Tensor) -> torch.Tensor:
+    """[rows, H] bf16 whose rows are dense and 16-byte aligned, at any stride that keeps them so; a copy only where it has to be one."""
+    t = t.reshape(-1, t.shape[-1])
+    if t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) < t.shape[1] or t.stride(0) % 8)) or t.data_ptr() % 16:
+        t = t.contiguous()
+        t = t if t.data_ptr() % 16 == 0 else t.clone()
+    return t
+
+
+def _check_head(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, temperature: float) -> None:
+    _same_device("token_logprobs", hidden, weight, targets)
+    if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise ValueError(f"token_logprobs: hidden and weight are bf16, not {hidden.dtype} and {weight.dtype}")
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"token_logprobs: hidden [..., H] and weight [V, H], not {tuple(hidden.shape)} and {tuple(weight.shape)}")
+    V, H = weight.shape
+    if H % 16 or not 0 < H <= 65536 or not 0 < V <= 1 << 22:
+        raise ValueError(f"token_logprobs: H a multiple of 16 up to 65536 and 1 to 2^22 rows of weight, not {H} and {V}")
+    if targets.shape != hidden.shape[:-1] or targets.dtype != torch.int64:
+        raise ValueError(f"token_logprobs: targets int64 {tuple(hidden.shape[:-1])}, not {targets.dtype} {tuple(targets.shape)}")
+    if targets.numel() > 1 << 24:
+        raise ValueError(f"token_logprobs: at most 2^24 tokens, not {targets.numel()}")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"token_logprobs: a positive temperature, not {temperature}")
+
+
+@_on_own_device
+def head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100, temperature: float = 1.0, entropy: bool = False):
+    """(logp, lse, entropy or None, index): log-probability of every target under softmax(hidden weight^T / temperature), the logits' log-sum-exp and
+    the entropy, float32 of targets' shape, without the logits; `index` is for head_logprobs_backward.  hidden bf16 [..., H], weight bf16 [V, H]."""
+    _check_head(hidden, weight, targets, temperature)
+    x, w, t = _head_operand(hidden), _head_operand(weight), targets.reshape(-1).contiguous()
+    (V, H), tokens = weight.shape, t.numel()
+    if tokens == 0:
+        zero = torch.zeros(targets.shape, dtype=torch.float32, device=hidden.device)
+        return zero, zero.clone(), zero.clone() if entropy else None, torch.zeros(0, dtype=torch.uint8, device=hidden.device)
+    index, need = _head_bytes(tokens, H, V, entropy)
+    shape = (F32, *targets.shape)
+    new = _lib.call("metis_head_logprobs", hidden.device.index, (shape, shape, (U8, index), (U8, need), shape if entropy else (F32, 0)),
+                    (x, max(x.stride(0), H), w, max(w.stride(0), H), t, int(ignore_index), tokens, H, V, float(temperature), "0", "1", "4" if entropy else None, "2", "3", need, _stream()))
+    if new.__class__ is int:
+        check(new, "metis_head_logprobs", hidden.shape)
+    return new[0], new[1], new[4] if entropy else None, new[2]
+
+
+@_on_own_device
+def head_logprobs_backward(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, temperature: float, lse: torch.Tensor, entropy: torch.Tensor | None,
+                           index: torch.Tensor, grad_logp: torch.Tensor | None, grad_entropy: torch.Tensor | None, want_hidden: bool = True, want_weight: bool = True):
+    """(gradient of hidden, gradient of weight), bf16 or None where not wanted, for those of head_logprobs' logp and entropy (either may be None); lse, entropy
+    and index are its results."""
+    _check_head(hidden, weight, targets, temperature)
+    for name, g in (("lse", lse), ("entropy", entropy), ("grad_logp", grad_logp), ("grad_entropy", grad_entropy)):
+        if g is not None and (g.shape != targets.shape or g.dtype != torch.float32 or g.device != hidden.device):
+            raise ValueError(f"head_logprobs_backward: {name} is float32 {tuple(targets.shape)}, not {g.dtype} {tuple(g.shape)}")
+    if lse is None or (grad_entropy is not None and entropy is None):
+        raise ValueError("head_logprobs_backward: lse, and for grad_entropy also entropy, of the forward call")
+    x, w, t = _head_operand(hidden), _head_operand(weight), targets.reshape(-1).contiguous()
+    (V, H), tokens = weight.shape, t.numel()
+    if tokens == 0 or (grad_logp is None and grad_entropy is None):
+        return torch.zeros(hidden.shape, dtype=hidden.dtype, device=hidden.device) if want_hidden else None, torch.zeros((V, H), dtype=weight.dtype, device=hidden.device) if want_weight else None
+    if index.dtype != torch.uint8 or index.numel() != _head_bytes(tokens, H, V, False)[0] or index.device != hidden.device:
+        raise ValueError("head_logprobs_backward: the index of the forward call on these tokens")
+    lse, entropy, grad_logp, grad_entropy = (None if g is None else g.contiguous() for g in (lse, entropy, grad_logp, grad_entropy))
+    need = _head_backward_bytes(tokens, H, V, want_hidden, want_weight, hidden.device.index)
+    specs, place = [(U8, need)], [None, None]
+    for k, (wanted, shape) in enumerate(((want_hidden, hidden.shape), (want_weight, (V, H)))):
+        if wanted:
+            place[k] = str(len(specs))
+            specs.append((B16, *shape))
+    new = _lib.call("metis_head_logprobs_backward", hidden.device.index, tuple(specs),
+                    (x, max(x.stride(0), H), w, max(w.stride(0), H), t, tokens, H, V, float(temperature), lse, entropy, grad_logp, grad_entropy, index, *place, "0", need, _stream()))
+    if new.__class__ is int:
+        check(new, "metis_head_logprobs_backward", hidden.shape)
+    return tuple(None if k is None else new[int(k)] for k in place)
+
+
 @functools.lru_cache(maxsize=16)
 def _device_cus(device_index: int) -> int:
     return int(torch.cuda.get_device_properties(device_index).multi_processor_count)

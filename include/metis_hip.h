@@ -978,6 +978,40 @@ int metis_swiglu_backward(const void *gate, int64_t ld_gate, const void *up, int
                           const void *grad, int64_t rows, int64_t cols, int dtype, void *grad_gate,
                           void *grad_up, void *stream);
 
+/*
+ * Log-probabilities of given tokens under a large head without its logits, and their gradients: what the reference's
+ * trainers take from a [tokens, V] tensor of logits (log_softmax and a gather behind lm_head).
+ *   l[t, v] = sum_k hidden[t, k] weight[v, k] / temperature,   lse = log sum_v exp l
+ *   logp[t] = l[t, targets[t]] - lse[t],   entropy[t] = lse[t] - sum_v p l,   p = exp(l - lse)
+ *   hidden   bf16 [tokens, H], weight bf16 [V, H], row strides ld_hidden, ld_weight (multiples of 8), 16-byte aligned;
+ *            H a multiple of 16 up to 65536, tokens up to 2^24, V up to 2^22
+ *   targets  int64 [tokens]; tokens whose target is ignore_index take no part: logp, lse and entropy 0, no gradient, their
+ *            rows of hidden are not read into any sum.  Any other target outside [0, V) makes its token's results NaN (and
+ *            the gradients that they enter).
+ *   logp, lse, entropy  float [tokens]; entropy may be NULL
+ *   index    metis_head_index_bytes(tokens) bytes, 256-byte aligned: written by the forward, read by the backward
+ * Backward, for gradients of logp and entropy (float [tokens], NULL: zero; with grad_entropy also entropy):
+ *   dl = (grad_logp (1[v = target] - p) - grad_entropy p (l - lse + entropy)) / temperature, rounded to bf16 once
+ *   grad_hidden = dl weight, grad_weight = dl^T hidden, dense bf16, sums in binary32 in a fixed order; NULL: not wanted
+ * The logits are formed again in pieces of the vocabulary.  Workspaces need no initialisation; the backward's holds one
+ * piece of dl (at most the larger of 256 MiB and twice the binary32 gradient of hidden, at least 256 columns) beside the
+ * binary32 gradient of hidden.
+ */
+size_t metis_head_index_bytes(int64_t tokens);
+size_t metis_head_logprobs_workspace_bytes(int64_t tokens, int64_t H, int64_t V, int entropy);
+int metis_head_logprobs(const void *hidden, int64_t ld_hidden, const void *weight, int64_t ld_weight,
+                        const void *targets, int64_t ignore_index, int64_t tokens, int64_t H, int64_t V,
+                        float temperature, float *logp, float *lse, float *entropy, void *index,
+                        void *workspace, size_t workspace_bytes, void *stream);
+size_t metis_head_logprobs_backward_workspace_bytes(int64_t tokens, int64_t H, int64_t V,
+                                                    int want_hidden, int want_weight);
+int metis_head_logprobs_backward(const void *hidden, int64_t ld_hidden, const void *weight,
+                                 int64_t ld_weight, const void *targets, int64_t tokens, int64_t H,
+                                 int64_t V, float temperature, const float *lse, const float *entropy,
+                                 const float *grad_logp, const float *grad_entropy, const void *index,
+                                 void *grad_hidden, void *grad_weight, void *workspace,
+                                 size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,68 @@
+"""token_logprobs: what is refused, and the sizes a caller asks for, without a device."""
+import pytest
+import torch
+
+from metis_hip import MetisHipError, _lib, linear_cross_entropy, token_logprobs
+
+
+def test_host_tensors_are_refused():
+    x, w, t = torch.zeros(3, 32, dtype=torch.bfloat16), torch.zeros(7, 32, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(MetisHipError, match="no CPU path"):
+        token_logprobs(x, w, t)
+    with pytest.raises(MetisHipError, match="no CPU path"):
+        linear_cross_entropy(x, w, t)
+    with pytest.raises(ValueError, match="reduction"):
+        linear_cross_entropy(x, w, t, reduction="max")
+
+
+def _forward(**changes):
+    a = dict(hidden=4096, ldh=64, weight=4096, ldw=64, targets=4096, ignore=-100, tokens=4, H=64, V=100, temperature=1.0, logp=4096, lse=4096, entropy=None, index=4096,
+             workspace=4096, bytes=1 << 30, stream=None)
+    a.update(changes)
+    return _lib.load().metis_head_logprobs(*a.values())
+
+
+BAD = [dict(H=60), dict(H=0), dict(H=65552, ldh=65552, ldw=65552), dict(V=0), dict(V=(1 << 22) + 1), dict(tokens=-1), dict(tokens=(1 << 24) + 1), dict(hidden=None), dict(weight=None),
+       dict(targets=None), dict(index=None), dict(ldh=56), dict(ldw=56), dict(ldh=68), dict(ldw=68), dict(hidden=4104), dict(weight=4104), dict(targets=4100), dict(index=4112),
+       dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("inf")), dict(temperature=float("nan"))]
+
+
+@pytest.mark.parametrize("changes", BAD + [dict(logp=None), dict(lse=None), dict(lse=4098), dict(entropy=4098)])
+def test_the_forward_refuses_before_a_launch(changes):
+    assert _forward(**changes) == _lib.E_ARG
+
+
+def test_workspaces():
+    L = _lib.load()
+    need = L.metis_head_logprobs_workspace_bytes(4, 64, 100, 0)
+    assert 0 < need < L.metis_head_logprobs_workspace_bytes(4, 64, 100, 1)
+    assert L.metis_head_logprobs_workspace_bytes(0, 64, 100, 0) == 0 and L.metis_head_logprobs_workspace_bytes(4, 60, 100, 0) == 0
+    assert L.metis_head_index_bytes(10) >= (64 + 20) * 4 and L.metis_head_index_bytes(-1) == 0
+    for changes in (dict(workspace=None), dict(bytes=need - 1), dict(workspace=4096 + 16)):
+        assert _forward(**changes) == _lib.E_WORKSPACE
+    assert _forward(tokens=0, hidden=None, workspace=None) == _lib.OK
+    back = L.metis_head_logprobs_backward_workspace_bytes
+    assert back(4, 64, 100, 1, 1) >= back(4, 64, 100, 0, 1) > 0 and back(4, 64, 100, 1, 0) > 0 and back(0, 64, 100, 1, 1) == 0
+    # a piece of the gradient of the logits, not the whole: 4096 x 131072 of it would be 1 GiB
+    assert back(4096, 3584, 131072, 0, 0) <= 256 << 20
+    # and with many tokens at most twice the binary32 gradient of hidden
+    assert back(1 << 20, 4096, 131072, 0, 0) <= 8 * (1 << 20) * 4096
+
+
+def _backward(**changes):
+    a = dict(hidden=4096, ldh=64, weight=4096, ldw=64, targets=4096, tokens=4, H=64, V=100, temperature=1.0, lse=4096, entropy=None, g_logp=4096, g_entropy=None, index=4096,
+             gh=4096, gw=4096, workspace=4096, bytes=1 << 40, stream=None)
+    a.update(changes)
+    return _lib.load().metis_head_logprobs_backward(*a.values())
+
+
+@pytest.mark.parametrize("changes", BAD + [dict(tokens=0), dict(lse=None), dict(g_entropy=4096), dict(gh=4104), dict(gw=4104), dict(g_logp=4098)])
+def test_the_backward_refuses_before_a_launch(changes):
+    assert _backward(**changes) == _lib.E_ARG
+
+
+def test_the_backward_wants_its_workspace():
+    need = _lib.load().metis_head_logprobs_backward_workspace_bytes(4, 64, 100, 1, 1)
+    for changes in (dict(workspace=None), dict(bytes=need - 1), dict(workspace=4096 + 16)):
+        assert _backward(**changes) == _lib.E_WORKSPACE
+    assert _backward(gh=None, gw=None, workspace=None) == _lib.OK
