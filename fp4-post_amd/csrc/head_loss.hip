@@ -15,6 +15,7 @@
 // Tokens whose target is ignored take no part: a first launch lists the others ("live"), the products run over the listed rows, and what an ignored
 // row of hidden holds (padding: anything) is never read into a sum.
 #include "gemm_common.h"
+#include <type_traits>
 
 namespace metis {
 
@@ -23,7 +24,7 @@ namespace {
 constexpr int HL_BN = 256, HL_TN = 2, HL_THREADS = 512;
 
 __host__ __device__ constexpr int hl_stage_bytes(int TM) { return (64 * TM + HL_BN) * 64; }
-__host__ __device__ constexpr int hl_slots(int TM) { return 4; }
+constexpr int HL_NS = 5;
 
 __host__ __device__ constexpr int hl_waitcnt(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | ((lgkm & 15) << 8); }
 #define HL_WAIT(VM, LGKM) __builtin_amdgcn_s_waitcnt(hl_waitcnt(VM, LGKM))
@@ -34,8 +35,9 @@ typedef uint32_t hl_u32x4_t __attribute__((ext_vector_type(4)));
 typedef hl_short4_t __attribute__((address_space(3))) * hl_lds_ptr_t;
 
 // ---------------------------------------------------------------------------------------------
-// The tile engine: 64 TM x 256 of a product per workgroup, eight waves (2 x 4) of 32 TM x 64, stages of 32 along the contraction in a ring of four
-// LDS slots, filled by direct loads three stages ahead; one barrier a stage, waits that never drain the queue.
+// The tile engine: 64 TM x 256 of a product per workgroup, eight waves (2 x 4) of 32 TM x 64, stages of 32 along the contraction in a ring of five
+// LDS slots, filled by direct loads three stages ahead; one barrier a stage, waits that never drain the queue.  Loads go out for two stages at a time (a
+// plain operand's 64 bytes of either are the halves of one 128-byte line) and spread over both iterations between the products.
 //
 // An operand lies in memory either along the contraction ("plain": [row][k]) or across it ("turned": [k][row]); both go to LDS as they are, 1 KiB per load
 // instruction.  Plain: 16 rows of 64 bytes, the four 16-byte pieces of row q in the order c ^ swz(q), read back as ds_read_b128.  Turned: rows of k, whose
@@ -51,21 +53,22 @@ struct Operand {
     int limit;                   // rows from here on are not there: the last one is read in their place
     const int* index;            // plain: the rows' numbers, or nullptr for rows as they come
     int rest;                    // k of the last stage that are there: 16 or 32 (plain), 1 .. 32 (turned); in place of others some that are there are read
+    int64_t panel;               // A in panels: elements between panels of 64 columns of the stored matrix, whose rows are then 64 long (ld 64)
 };
 
 // Stages [0, steps) of 32 along the contraction; half: only the first sixteen k of the last one count.  Where fewer count otherwise, one operand holds zeros
-// beyond them.
-template <int TM, bool AT, bool BT>
+// beyond them.  PANELS: A is stored in panels.
+template <int TM, bool AT, bool BT, bool PANELS>
 __device__ __forceinline__ void hl_main_loop(float16_t (&acc)[TM][HL_TN], uint8_t* lds, const Operand& a, const Operand& b, int steps, bool half)
 {
-    constexpr int BM = 64 * TM, NA = BM / 16, TOTAL = NA + HL_BN / 16, LPW = (TOTAL + 7) / 8, STAGE = hl_stage_bytes(TM), NS = hl_slots(TM), B_AT = NA * 1024;
+    constexpr int BM = 64 * TM, NA = BM / 16, TOTAL = NA + HL_BN / 16, LPW = (TOTAL + 7) / 8, STAGE = hl_stage_bytes(TM), NS = HL_NS, B_AT = NA * 1024;
     constexpr int A_RB = BM * 2, B_RB = HL_BN * 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 2, wn = wave & 3;
 
     // ---- this wave's load instructions of a stage: where its lanes read in the first one, how far they go per stage, and back in the last
     const uint8_t* src[LPW];
-    int64_t inc[LPW];
+    int64_t inc[LPW], inc_odd[LPW];                            // behind even and odd stages (64 where both operands are plain)
     uint32_t back[LPW];
     int place[LPW];
 #pragma unroll
@@ -80,8 +83,8 @@ __device__ __forceinline__ void hl_main_loop(float16_t (&acc)[TM][HL_TN], uint8_
             const int rb = is_a ? A_RB : B_RB, k = q * (1024 / rb) + lane * 16 / rb, at = lane * 16 % rb;
             int col = (at ^ (is_a ? hl_turn<A_RB>(k) : hl_turn<B_RB>(k))) >> 1;
             if (col >= o.limit) col = 0;                       // (columns in eights: all there or none)
-            src[j] = reinterpret_cast<const uint8_t*>(o.base + (int64_t)k * o.ld + col);
-            inc[j] = o.ld * 64;
+            src[j] = reinterpret_cast<const uint8_t*>(o.base + (int64_t)k * o.ld + (PANELS && is_a ? (col >> 6) * o.panel + (col & 63) : col));
+            inc[j] = inc_odd[j] = o.ld * 64;
             back[j] = k >= o.rest ? (uint32_t)((k - (o.rest - 1)) * (o.ld * 2)) : 0u;
         } else {
             const int row = q * 16 + (lane >> 2), chunk = (lane & 3) ^ hl_swz(row & 15);
@@ -89,14 +92,17 @@ __device__ __forceinline__ void hl_main_loop(float16_t (&acc)[TM][HL_TN], uint8_
             const int64_t at = o.index ? o.index[r] : r;
             src[j] = reinterpret_cast<const uint8_t*>(o.base + at * o.ld + chunk * 8);
             inc[j] = 64;
+            inc_odd[j] = PANELS && is_a ? o.panel * 2 - 64 : 64;
             back[j] = chunk * 8 >= o.rest ? 32u : 0u;
         }
     }
-    auto issue_one = [&](int slot, int j, bool last) {
+    auto issue_one = [&](int slot, int j, bool odd, bool last) {
         const uint8_t* g = src[j] - (last ? back[j] : 0u);
         const uint32_t dst = (uint32_t)(slot * STAGE + place[j]);
         asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(g), "s"(dst) : "memory");
-        src[j] += inc[j];
+        if constexpr (!AT && !BT && !PANELS) src[j] += 64;
+        else if constexpr (!AT && PANELS) src[j] += odd ? inc_odd[j] : inc[j];
+        else src[j] += inc[j];
     };
 
     // ---- fragments: lane -> row l % 32 of a 32-row tile, k 8 (l / 32) .. + 7 of a half stage
@@ -150,58 +156,81 @@ __device__ __forceinline__ void hl_main_loop(float16_t (&acc)[TM][HL_TN], uint8_
     constexpr int NM = TM * HL_TN, NF = TM * (AT ? 2 : 1) + HL_TN * (BT ? 2 : 1);
 
     if (steps <= 0) return;
+    // Two stages are requested together, piece by piece: a plain operand's two pieces are the halves of the same 128-byte lines.
+    auto issue_pair = [&](int slot0, int slot1, int j, int stage0) {
+        if (stage0 < steps) issue_one(slot0, j, false, stage0 == steps - 1);
+        if (stage0 + 1 < steps) issue_one(slot1, j, true, stage0 + 1 == steps - 1);
+    };
 #pragma unroll
-    for (int p = 0; p < NS; ++p)
-        if (p < steps) {
+    for (int p = 0; p < 4; p += 2)
 #pragma unroll
-            for (int j = 0; j < LPW; ++j) issue_one(p, j, p == steps - 1);
-        }
-    if (steps >= NS) HL_WAIT((NS - 1) * LPW, 15);
+        for (int j = 0; j < LPW; ++j) issue_pair(p, p + 1, j, p);
+    if (steps >= 4) HL_WAIT(2 * LPW + 1, 15);
     else HL_WAIT(0, 15);
     __syncthreads();
     load_frags(0, 0);
     int s = 0, slot = 0;
-    for (; s + NS < steps; ++s) {
-        const int nslot = slot + 1 == NS ? 0 : slot + 1;
-        const bool last = s + NS == steps - 1;
+    auto next_of = [](int k) { return k + 1 == NS ? 0 : k + 1; };
+    auto before = [](int k) { return k == 0 ? NS - 1 : k - 1; };
+    // Stage s in `slot`.  FIRST (s even): half of the load instructions of stages s + 4 and s + 5, into the slots before `slot` and `slot` itself, whose
+    // stages every wave has in registers behind this barrier; the iteration after it the other half.  Behind a barrier at most MOST loads are outstanding.
+    auto iterate = [&](auto first, auto most) {
+        constexpr bool FIRST = decltype(first)::value;
+        constexpr int H0 = LPW / 2, J0 = FIRST ? 0 : H0, COUNT = FIRST ? H0 : LPW - H0;
         load_frags(slot, 1);
         mfmas(0);
         sched_substep<NM, 0, NF, 0>();
-        HL_WAIT((NS - 2) * LPW, 0);                            // own loads of stage s + 1 are there, own reads of stage s done
+        HL_WAIT(decltype(most)::value, 0);                     // own loads of stage s + 1 are there, own reads of stage s done
         __syncthreads();
-        load_frags(nslot, 0);
+        load_frags(next_of(slot), 0);
+        const int slot1 = FIRST ? slot : before(slot), slot0 = before(slot1);
+        const bool last = (FIRST ? s + 5 : s + 4) == steps - 1;
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
 #pragma unroll
-            for (int j = 0; j < LPW; ++j)
-                if (j * NM / LPW == m) issue_one(slot, j, last);
+            for (int j = J0; j < J0 + COUNT; ++j)
+                if ((j - J0) * NM / COUNT == m) {
+                    issue_one(slot0, j, false, false);
+                    issue_one(slot1, j, true, last);
+                }
             mfma_one(1, m / HL_TN, m % HL_TN);
         }
-        slot = nslot;
+        slot = next_of(slot);
+        ++s;
+    };
+    // when stage s + 1 has to be there: s even, all of its pair (all but the next pair); s odd, the even half of its pair (all but the last load of it
+    // and the first half of the next pair)
+    while (s + 5 < steps) {
+        iterate(std::true_type{}, std::integral_constant<int, 2 * LPW>{});
+        iterate(std::false_type{}, std::integral_constant<int, 2 * (LPW / 2) + 1>{});
     }
     for (; s < steps; ++s) {
-        const int nslot = slot + 1 == NS ? 0 : slot + 1;
         const bool both = s + 1 < steps || !half;
         if (both) load_frags(slot, 1);
         mfmas(0);
         HL_WAIT(0, 0);
         __syncthreads();
-        if (s + 1 < steps) load_frags(nslot, 0);
+        if (s + 1 < steps) load_frags(next_of(slot), 0);
+        if ((s & 1) == 0) {
+#pragma unroll
+            for (int j = 0; j < LPW; ++j) issue_pair(before(slot), slot, j, s + 4);
+        }
         if (both) mfmas(1);
-        slot = nslot;
+        slot = next_of(slot);
     }
     __syncthreads();                                           // the ring is free
 }
 
 // acc[i][j][e] of lane l: row 32 (TM wm + i) + l % 32, column 64 wn + 32 j + 8 (e / 4) + 4 (l / 32) + e % 4 of the tile.
-// The tile as bf16, rows of `ld` elements from `out` on: through the wave's own part of LDS, 32 rows at a time, so that a store writes 8 rows of 128 bytes.
+// The tile as bf16, the wave's 64 columns in rows of `ld` elements from `out` on: through the wave's own part of LDS, 32 rows at a time, so that a store
+// writes 8 rows of 128 bytes.
 template <int TM>
 __device__ __forceinline__ void hl_store_bf16(const float16_t (&acc)[TM][HL_TN], uint8_t* lds, uint16_t* out, int64_t ld, int rows, int cols)
 {
     constexpr int CROW = 72;                                   // 144 bytes
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 2, wn = wave & 3, lr = lane & 31, hi = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 2, lr = lane & 31, hi = lane >> 5;
     uint16_t* cw = reinterpret_cast<uint16_t*>(lds) + wave * (32 * CROW);
-    const int n = wn * 64 + (lane & 7) * 8;
+    const int n = (lane & 7) * 8;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -243,13 +272,38 @@ __device__ __forceinline__ int hl_logical(int total)
     const int per = (total + 7) >> 3, logical = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     return (int)(blockIdx.x >> 3) < per && logical < total ? logical : -1;
 }
-// groups of four tile rows, walked column by column
+// groups of up to five tile rows, as even as they come, walked column by column: 32 compute units of an XCD share the operands of a few rows and columns.
+// (Groups of up to 6, 8, 16 rows: 16 rows of tiles, all three products, 1 to 6 % slower.)
 __device__ __forceinline__ void hl_origin(int logical, int tiles_m, int tiles_n, int& tm, int& tn)
 {
-    constexpr int GM = 4;
-    const int group = logical / (GM * tiles_n), first = group * GM, size = min(tiles_m - first, GM), in = logical - group * GM * tiles_n;
+    constexpr int MOST = 5;
+    const int groups = (tiles_m + MOST - 1) / MOST, gm = (tiles_m + groups - 1) / groups;
+    const int group = logical / (gm * tiles_n), first = group * gm, size = min(tiles_m - first, gm), in = logical - group * gm * tiles_n;
     tm = first + in % size;
     tn = in / size;
+}
+
+// Rows of a tile over tokens, 64 TM, by the live tokens' number.  A tile takes 57, 80, 100 parts of time with TM = 2, 3, 4 (65536 x 2048: 33, 46, 58 us each),
+// so fewer rows pay only where the last tile of more would be mostly empty: 300 tokens 119 -> 101 us, 540 176 -> 147, 100 63 -> 51; but 400 stay (124,
+// 142 with TM = 3).  The number is known on the device alone: the launches for up to kFewTokens tokens hold all three, beyond that it is always 4.
+constexpr int kListTokens = 64, kFewTokens = 2048;
+__host__ __device__ __forceinline__ int hl_row_tiles(int count)
+{
+    if (count <= 128) return 2;
+    return (count + 191) / 192 * 80 < (count + 255) / 256 * 100 ? 3 : 4;
+}
+enum Rows { kList, kFew, kMany };                              // up to kListTokens tokens (TM = 1), up to kFewTokens, more
+// f with the TM that counts
+template <int ROWS, class F> __device__ __forceinline__ void with_row_tiles(int count, F&& f)
+{
+    if constexpr (ROWS == kList) f(std::integral_constant<int, 1>{});
+    else if constexpr (ROWS == kMany) f(std::integral_constant<int, 4>{});
+    else {
+        const int tm = hl_row_tiles(count);
+        if (tm == 2) f(std::integral_constant<int, 2>{});
+        else if (tm == 3) f(std::integral_constant<int, 3>{});
+        else f(std::integral_constant<int, 4>{});
+    }
 }
 
 template <int TM> __device__ __forceinline__ void hl_clear(float16_t (&acc)[TM][HL_TN])
@@ -267,12 +321,11 @@ template <int TM> __device__ __forceinline__ void hl_clear(float16_t (&acc)[TM][
 // 2^(l - maximum) (l - maximum); the target's logit from the tile that has it.
 // ---------------------------------------------------------------------------------------------
 template <int TM, bool ENT>
-__global__ __launch_bounds__(HL_THREADS, TM == 1 ? 4 : 2) void head_stats_kernel(const Tokens tk, const uint16_t* __restrict__ weight, int64_t ldw, int stride,
-                                                                               float2* __restrict__ part, float* __restrict__ part_e, float* __restrict__ hit)
+__device__ __forceinline__ void hl_stats_tile(uint8_t* hl_lds, const Tokens& tk, int count, const int* live, const uint16_t* weight, int64_t ldw, int stride, float2* part, float* part_e,
+                                              float* hit)
 {
-    extern __shared__ __attribute__((aligned(1024))) uint8_t hl_lds[];
     constexpr int BM = 64 * TM;
-    const int count = tk.index[0], tiles_m = (count + BM - 1) / BM, tiles_n = (tk.V + HL_BN - 1) / HL_BN;
+    const int tiles_m = (count + BM - 1) / BM, tiles_n = (tk.V + HL_BN - 1) / HL_BN;
     const int logical = hl_logical(tiles_m * tiles_n);
     if (logical < 0) return;
     int tm, tn;
@@ -281,8 +334,8 @@ __global__ __launch_bounds__(HL_THREADS, TM == 1 ? 4 : 2) void head_stats_kernel
     float16_t acc[TM][HL_TN];
     hl_clear<TM>(acc);
     const int rest = tk.H % 32 ? 16 : 32;
-    const Operand a = {tk.hidden, tk.ld, count - m0, live_rows(tk.index) + m0, rest}, b = {weight + (int64_t)n0 * ldw, ldw, tk.V - n0, nullptr, rest};
-    hl_main_loop<TM, false, false>(acc, hl_lds, a, b, (tk.H + 31) / 32, rest == 16);
+    const Operand a = {tk.hidden, tk.ld, count - m0, live + m0, rest, 0}, b = {weight + (int64_t)n0 * ldw, ldw, tk.V - n0, nullptr, rest, 0};
+    hl_main_loop<TM, false, false, false>(acc, hl_lds, a, b, (tk.H + 31) / 32, rest == 16);
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3, lr = lane & 31, hi = lane >> 5;
     const int there = tk.V - (n0 + wn * 64);                   // columns of this wave that exist
@@ -313,7 +366,7 @@ __global__ __launch_bounds__(HL_THREADS, TM == 1 ? 4 : 2) void head_stats_kernel
             sum += __shfl_xor(sum, 32, 64);
             if constexpr (ENT) ent += __shfl_xor(ent, 32, 64);
             int64_t want = -1;
-            if (m < count) want = tk.targets[live_rows(tk.index)[m]] - (n0 + wn * 64);
+            if (m < count) want = tk.targets[live[m]] - (n0 + wn * 64);
             if (__any(want >= 0 && want < 64)) {
 #pragma unroll
                 for (int j = 0; j < HL_TN; ++j)
@@ -345,32 +398,90 @@ __global__ __launch_bounds__(HL_THREADS, TM == 1 ? 4 : 2) void head_stats_kernel
     if constexpr (ENT) part_e[(size_t)tn * stride + m0 + row] = ent;
 }
 
-// The tiles of a token folded: 64 chains of every 64th tile, then the chains in order; 16 tokens per workgroup.
+// kList: every workgroup lists the live tokens for itself, in LDS behind the ring, and the first writes the list down for the launches to come: a launch less
+// (5 x 1536 against 131072: 91 -> 83 us with the fold of the tiles in fewer steps).
+template <int ROWS, bool ENT>
+__global__ __launch_bounds__(HL_THREADS, 2) void head_stats_kernel(const Tokens tk, const uint16_t* __restrict__ weight, int64_t ldw, int stride,
+                                                                 float2* __restrict__ part, float* __restrict__ part_e, float* __restrict__ hit, int64_t ignore,
+                                                                 int* __restrict__ list)
+{
+    extern __shared__ __attribute__((aligned(1024))) uint8_t hl_lds[];
+    int count;
+    const int* live;
+    if constexpr (ROWS == kList) {
+        int* own = reinterpret_cast<int*>(hl_lds + HL_NS * hl_stage_bytes(1));
+        const int t = threadIdx.x & 63;
+        const bool on = t < tk.tokens && tk.targets[t] != ignore;
+        const uint64_t mask = __ballot(on);
+        const int at = __popcll(mask & ((1ull << t) - 1ull));
+        count = __popcll(mask);
+        if (threadIdx.x < 64) {
+            if (on) own[at] = t;
+            if (blockIdx.x == 0) {
+                if (t == 0) list[0] = count;
+                if (on) list[64 + at] = t;
+                if (t < tk.tokens) list[64 + tk.tokens + t] = on ? at : -1;
+            }
+        }
+        __syncthreads();
+        live = own;
+    } else {
+        count = tk.index[0];
+        live = live_rows(tk.index);
+    }
+    with_row_tiles<ROWS>(count, [&](auto tm) { hl_stats_tile<decltype(tm)::value, ENT>(hl_lds, tk, count, live, weight, ldw, stride, part, part_e, hit); });
+}
+
+// A maximum with its sum of 2^(l - maximum) and, for the entropy, of 2^(l - maximum) (l - maximum); empty: -infinity, 0, 0.
+struct Fold {
+    float top, sum, ent;
+};
+template <bool ENT> __device__ __forceinline__ Fold fold(const Fold& a, const Fold& b)
+{
+    Fold r;
+    r.top = fmaxf(a.top, b.top);
+    const float da = a.sum != 0.0f ? a.top - r.top : 0.0f, db = b.sum != 0.0f ? b.top - r.top : 0.0f;     // (nothing in it: no infinity less infinity)
+    const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
+    r.sum = fa * a.sum + fb * b.sum;
+    r.ent = ENT ? fa * fmaf(da, a.sum, a.ent) + fb * fmaf(db, b.sum, b.ent) : 0.0f;
+    return r;
+}
+
+// The tiles of a token folded, 16 tokens per workgroup: 64 chains of every 64th tile, eight requested together, then the four chains of a wave by lanes and
+// the sixteen waves in order.
 template <bool ENT>
 __global__ __launch_bounds__(1024) void head_finish_kernel(const int64_t* __restrict__ targets, const int* __restrict__ index, int tokens, int V, int tiles_n, int stride,
                                                            const float2* __restrict__ part, const float* __restrict__ part_e, const float* __restrict__ hit,
                                                            float* __restrict__ logp, float* __restrict__ lse, float* __restrict__ entropy)
 {
-    __shared__ float red[64][16][3];
-    const int r = threadIdx.x & 15, chain = threadIdx.x >> 4, t = blockIdx.x * 16 + r;
+    __shared__ float red[16][16][3];
+    const int r = threadIdx.x & 15, chain = threadIdx.x >> 4, wave = threadIdx.x >> 6, t = blockIdx.x * 16 + r;
     const int pos = t < tokens ? live_rows(index)[tokens + t] : -1;
-    float top = -INFINITY, sum = 0.0f, ent = 0.0f;
-    auto fold = [&](float t1, float s1, float e1) {
-        const float up = fmaxf(top, t1);
-        if (up == -INFINITY && s1 == 0.0f) return;             // nothing yet and nothing new
-        const float f0 = __builtin_amdgcn_exp2f(top - up), f1 = __builtin_amdgcn_exp2f(t1 - up);
-        if constexpr (ENT) ent = (sum != 0.0f ? f0 * fmaf(top - up, sum, ent) : 0.0f) + f1 * fmaf(t1 - up, s1, e1);
-        sum = (sum != 0.0f ? f0 * sum : 0.0f) + f1 * s1;
-        top = up;
-    };
-    if (pos >= 0)
-        for (int k = chain; k < tiles_n; k += 64) {
-            const float2 p = part[(size_t)k * stride + pos];
-            fold(p.x, p.y, ENT ? part_e[(size_t)k * stride + pos] : 0.0f);
+    Fold mine = {-INFINITY, 0.0f, 0.0f};
+    for (int k0 = chain; k0 < tiles_n; k0 += 8 * 64) {
+        float2 p[8];
+        float e[8];
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+            p[b] = make_float2(-INFINITY, 0.0f);
+            e[b] = 0.0f;
+            const int k = k0 + b * 64;
+            if (pos >= 0 && k < tiles_n) {
+                p[b] = part[(size_t)k * stride + pos];
+                if constexpr (ENT) e[b] = part_e[(size_t)k * stride + pos];
+            }
         }
-    red[chain][r][0] = top;
-    red[chain][r][1] = sum;
-    red[chain][r][2] = ent;
+#pragma unroll
+        for (int b = 0; b < 8; ++b) mine = fold<ENT>(mine, Fold{p[b].x, p[b].y, e[b]});
+    }
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1)
+        mine = fold<ENT>(mine, Fold{__shfl_xor(mine.top, o, 64), __shfl_xor(mine.sum, o, 64), ENT ? __shfl_xor(mine.ent, o, 64) : 0.0f});
+    if ((threadIdx.x & 63) < 16) {
+        red[wave][r][0] = mine.top;
+        red[wave][r][1] = mine.sum;
+        red[wave][r][2] = mine.ent;
+    }
     __syncthreads();
     if (chain || t >= tokens) return;
     if (pos < 0) {
@@ -378,14 +489,15 @@ __global__ __launch_bounds__(1024) void head_finish_kernel(const int64_t* __rest
         if constexpr (ENT) entropy[t] = 0.0f;
         return;
     }
-    for (int k = 1; k < 64 && k < tiles_n; ++k) fold(red[k][r][0], red[k][r][1], red[k][r][2]);
+#pragma unroll
+    for (int k = 1; k < 16; ++k) mine = fold<ENT>(mine, Fold{red[k][r][0], red[k][r][1], red[k][r][2]});
     constexpr float kLn2 = 0.693147180559945f;
     const int64_t want = targets[t];
     const bool there = want >= 0 && want < V;                  // (a target outside of the vocabulary shows: everything of its row is NaN)
-    const float l2 = __log2f(sum), nan = __uint_as_float(0x7fc00000u);
-    lse[t] = there ? (top + l2) * kLn2 : nan;
-    logp[t] = there ? ((hit[pos] - top) - l2) * kLn2 : nan;
-    if constexpr (ENT) entropy[t] = there ? (l2 - ent / sum) * kLn2 : nan;
+    const float l2 = __log2f(mine.sum), nan = __uint_as_float(0x7fc00000u);
+    lse[t] = there ? (mine.top + l2) * kLn2 : nan;
+    logp[t] = there ? ((hit[pos] - mine.top) - l2) * kLn2 : nan;
+    if constexpr (ENT) entropy[t] = there ? (l2 - mine.ent / mine.sum) * kLn2 : nan;
 }
 
 // The live tokens in order, one workgroup.
@@ -416,20 +528,19 @@ __global__ __launch_bounds__(1024) void head_index_kernel(const int64_t* __restr
 }
 
 // ---------------------------------------------------------------------------------------------
-// Backward, first launch of a piece: dl of the vocabulary's columns v0 .. v0 + width - 1 as bf16 [live tokens, padded to the tile][ld], zero where tokens or
-// columns are not there.
+// Backward, first launch of a piece: dl of the vocabulary's columns v0 .. v0 + width - 1 as bf16, in panels of 64 columns, [panel][live tokens, padded][64]
+// (whole lines that lie side by side for both products; rows of a whole piece would be a power of two apart), zero where tokens of a tile or columns are not there.
 // ---------------------------------------------------------------------------------------------
 struct RowGrads {
     const float *lse, *entropy, *g_logp, *g_entropy;           // by token; entropy and g_entropy may be nullptr
 };
 template <int TM>
-__global__ __launch_bounds__(HL_THREADS, 2) void head_dlogits_kernel(const Tokens tk, const uint16_t* __restrict__ weight, int64_t ldw, int v0, int width, const RowGrads rg,
-                                                                     uint16_t* __restrict__ dl, int64_t ld)
+__device__ __forceinline__ void hl_dlogits_tile(uint8_t* hl_lds, const Tokens& tk, int count, const uint16_t* weight, int64_t ldw, int v0, int width, const RowGrads& rg, uint16_t* dl,
+                                                int64_t panel)
 {
-    extern __shared__ __attribute__((aligned(1024))) uint8_t hl_lds[];
     constexpr int BM = 64 * TM;
     constexpr float kLn2 = 0.693147180559945f, kLog2e = 1.44269504088896f;
-    const int count = tk.index[0], tiles_m = (count + BM - 1) / BM, tiles_n = (width + HL_BN - 1) / HL_BN;
+    const int tiles_m = (count + BM - 1) / BM, tiles_n = (width + HL_BN - 1) / HL_BN;
     const int logical = hl_logical(tiles_m * tiles_n);
     if (logical < 0) return;
     int tm, tn;
@@ -439,8 +550,8 @@ __global__ __launch_bounds__(HL_THREADS, 2) void head_dlogits_kernel(const Token
     hl_clear<TM>(acc);
     const int* live = live_rows(tk.index);
     const int rest = tk.H % 32 ? 16 : 32;
-    const Operand a = {tk.hidden, tk.ld, count - m0, live + m0, rest}, b = {weight + (int64_t)(v0 + n0) * ldw, ldw, width - n0, nullptr, rest};
-    hl_main_loop<TM, false, false>(acc, hl_lds, a, b, (tk.H + 31) / 32, rest == 16);
+    const Operand a = {tk.hidden, tk.ld, count - m0, live + m0, rest, 0}, b = {weight + (int64_t)(v0 + n0) * ldw, ldw, width - n0, nullptr, rest, 0};
+    hl_main_loop<TM, false, false, false>(acc, hl_lds, a, b, (tk.H + 31) / 32, rest == 16);
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3, lr = lane & 31, hi = lane >> 5;
     const int there = width - (n0 + wn * 64);
@@ -473,7 +584,16 @@ __global__ __launch_bounds__(HL_THREADS, 2) void head_dlogits_kernel(const Token
                 acc[i][j][e] = on && n < there ? v : 0.0f;
             }
     }
-    hl_store_bf16<TM>(acc, hl_lds, dl + (int64_t)m0 * ld + n0, ld, BM, HL_BN);
+    hl_store_bf16<TM>(acc, hl_lds, dl + (int64_t)(n0 / 64 + wn) * panel + m0 * 64, 64, BM, 64);
+}
+
+template <int ROWS>
+__global__ __launch_bounds__(HL_THREADS, 2) void head_dlogits_kernel(const Tokens tk, const uint16_t* __restrict__ weight, int64_t ldw, int v0, int width, const RowGrads rg,
+                                                                     uint16_t* __restrict__ dl, int64_t panel)
+{
+    extern __shared__ __attribute__((aligned(1024))) uint8_t hl_lds[];
+    const int count = tk.index[0];
+    with_row_tiles<ROWS>(count, [&](auto tm) { hl_dlogits_tile<decltype(tm)::value>(hl_lds, tk, count, weight, ldw, v0, width, rg, dl, panel); });
 }
 
 // The live rows of hidden side by side, then zero rows up to a multiple of 32.
@@ -493,8 +613,8 @@ __global__ __launch_bounds__(256) void head_gather_kernel(const Tokens tk, uint4
 //   grad_weight: rows v0 .. of the gradient, complete
 // ---------------------------------------------------------------------------------------------
 struct Products {
-    const uint16_t* dl;          // [padded tokens][ld]
-    int64_t ld;
+    const uint16_t* dl;
+    int64_t rows;                // of its panels, and of a slab: the tokens, padded to grad_hidden's tiles
     const uint16_t* weight;      // the piece's first row
     int64_t ldw;
     const uint16_t* gathered;    // live rows of hidden
@@ -502,56 +622,59 @@ struct Products {
     uint16_t* grad_weight;       // nullptr: grad_weight is not wanted
     const int* index;
     int width, H, splits, first; // first: the slabs hold nothing yet
-    int64_t slab_rows;
 };
-__global__ __launch_bounds__(HL_THREADS, 2) void head_products_kernel(const Products p)
+// Tile `job` of grad_hidden.
+template <int TMX>
+__device__ __forceinline__ void hl_hidden_tile(uint8_t* hl_lds, const Products& p, int count, int job, int tiles_t, int tiles_h)
 {
-    extern __shared__ __attribute__((aligned(1024))) uint8_t hl_lds[];
-    constexpr int TM = 4, BM = 256;
-    const int count = p.index[0], tiles_t = (count + BM - 1) / BM, tiles_h = (p.H + HL_BN - 1) / HL_BN, tiles_v = (p.width + BM - 1) / BM;
-    const int xcd = blockIdx.x & 7;
-    int li = blockIdx.x >> 3;
-    const int hidden_jobs = p.slabs ? tiles_t * tiles_h * p.splits : 0, hidden_x = (hidden_jobs + 7) >> 3;
-    float16_t acc[TM][HL_TN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3, lr = lane & 31, hi = lane >> 5;
-    if (li < hidden_x) {
-        const int job = xcd * hidden_x + li;
-        if (job >= hidden_jobs) return;
-        const int split = job / (tiles_t * tiles_h);
-        int tm, tn;
-        hl_origin(job - split * tiles_t * tiles_h, tiles_t, tiles_h, tm, tn);
-        const int m0 = tm * BM, n0 = tn * HL_BN, kt = (p.width + 31) / 32;
-        const int begin = (int)((int64_t)split * kt / p.splits), end = (int)((int64_t)(split + 1) * kt / p.splits);
-        float* slab = p.slabs + ((int64_t)split * p.slab_rows + m0) * p.H + n0;
-        if (p.first) {
-            hl_clear<TM>(acc);
-        } else {
+    const int split = job / (tiles_t * tiles_h);
+    int tm, tn;
+    hl_origin(job - split * tiles_t * tiles_h, tiles_t, tiles_h, tm, tn);
+    const int m0 = tm * 64 * TMX, n0 = tn * HL_BN, kt = (p.width + 31) / 32, pairs = (kt + 1) / 2;
+    const int begin = 2 * (int)((int64_t)split * pairs / p.splits), end = min(kt, 2 * (int)((int64_t)(split + 1) * pairs / p.splits));
+    float* slab = p.slabs + ((int64_t)split * p.rows + m0) * p.H + n0;
+    float16_t acc[TMX][HL_TN];
+    hl_clear<TMX>(acc);
+    // the lane's places in the slab, four columns at a time
+    auto each = [&](auto&& f) {
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < HL_TN; ++j)
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int n = wn * 64 + j * 32 + 8 * g + 4 * hi;
-                        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (n0 + n < p.H) v = *reinterpret_cast<const float4*>(slab + (int64_t)((wm * TM + i) * 32 + lr) * p.H + n);
-                        acc[i][j][4 * g] = v.x; acc[i][j][4 * g + 1] = v.y; acc[i][j][4 * g + 2] = v.z; acc[i][j][4 * g + 3] = v.w;
-                    }
-        }
-        const Operand a = {p.dl + (int64_t)m0 * p.ld + begin * 32, p.ld, BM, nullptr, 32};
-        const Operand b = {p.weight + (int64_t)begin * 32 * p.ldw + n0, p.ldw, p.H - n0, nullptr, end == kt && p.width % 32 ? p.width % 32 : 32};
-        hl_main_loop<TM, false, true>(acc, hl_lds, a, b, end - begin, false);
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TMX; ++i) {
+            const int row = (wm * TMX + i) * 32 + lr;
+            if (m0 + row >= count) continue;
 #pragma unroll
             for (int j = 0; j < HL_TN; ++j)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const int n = wn * 64 + j * 32 + 8 * g + 4 * hi;
-                    if (n0 + n < p.H)
-                        *reinterpret_cast<float4*>(slab + (int64_t)((wm * TM + i) * 32 + lr) * p.H + n) =
-                            make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+                    if (n0 + n < p.H) f(acc[i][j], 4 * g, reinterpret_cast<float4*>(slab + (int64_t)row * p.H + n));
                 }
+        }
+    };
+    if (!p.first)
+        each([](float16_t& v, int e, const float4* q) {
+            const float4 x = *q;
+            v[e] = x.x; v[e + 1] = x.y; v[e + 2] = x.z; v[e + 3] = x.w;
+        });
+    const Operand a = {p.dl + (int64_t)(begin / 2) * p.rows * 64 + m0 * 64, 64, 64 * TMX, nullptr, 32, p.rows * 64};
+    const Operand b = {p.weight + (int64_t)begin * 32 * p.ldw + n0, p.ldw, p.H - n0, nullptr, end == kt && p.width % 32 ? p.width % 32 : 32, 0};
+    hl_main_loop<TMX, false, true, true>(acc, hl_lds, a, b, end - begin, false);
+    each([](const float16_t& v, int e, float4* q) { *q = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]); });
+}
+
+template <int ROWS>
+__global__ __launch_bounds__(HL_THREADS, 2) void head_products_kernel(const Products p)
+{
+    extern __shared__ __attribute__((aligned(1024))) uint8_t hl_lds[];
+    const int count = p.index[0], tmx = ROWS == kList ? 1 : ROWS == kMany ? 4 : hl_row_tiles(count);
+    const int tiles_t = (count + 64 * tmx - 1) / (64 * tmx), tiles_h = (p.H + HL_BN - 1) / HL_BN, tiles_v = (p.width + 255) / 256;
+    const int xcd = blockIdx.x & 7;
+    int li = blockIdx.x >> 3;
+    const int hidden_jobs = p.slabs ? tiles_t * tiles_h * p.splits : 0, hidden_x = (hidden_jobs + 7) >> 3;
+    if (li < hidden_x) {
+        const int job = xcd * hidden_x + li;
+        if (job < hidden_jobs)
+            with_row_tiles<ROWS>(count, [&](auto tm) { hl_hidden_tile<decltype(tm)::value>(hl_lds, p, count, job, tiles_t, tiles_h); });
         return;
     }
     if (!p.grad_weight) return;
@@ -560,11 +683,13 @@ __global__ __launch_bounds__(HL_THREADS, 2) void head_products_kernel(const Prod
     if (li >= per || job >= jobs) return;
     int tm, tn;
     hl_origin(job, tiles_v, tiles_h, tm, tn);
-    const int m0 = tm * BM, n0 = tn * HL_BN;
-    hl_clear<TM>(acc);
-    const Operand a = {p.dl + m0, p.ld, BM, nullptr, 32}, b = {p.gathered + n0, p.H, p.H - n0, nullptr, 32};
-    hl_main_loop<TM, true, true>(acc, hl_lds, a, b, (count + 31) / 32, false);
-    hl_store_bf16<TM>(acc, hl_lds, p.grad_weight + (int64_t)m0 * p.H + n0, p.H, p.width - m0, p.H - n0);
+    const int m0 = tm * 256, n0 = tn * HL_BN;
+    float16_t acc[4][HL_TN];
+    hl_clear<4>(acc);
+    const Operand a = {p.dl + (int64_t)(m0 / 64) * p.rows * 64, 64, 256, nullptr, 32, p.rows * 64}, b = {p.gathered + n0, p.H, p.H - n0, nullptr, 32, 0};
+    hl_main_loop<4, true, true, true>(acc, hl_lds, a, b, (count + 31) / 32, false);
+    const int wn = (threadIdx.x >> 6) & 3;
+    hl_store_bf16<4>(acc, hl_lds, p.grad_weight + (int64_t)m0 * p.H + n0 + wn * 64, p.H, p.width - m0, p.H - (n0 + wn * 64));
 }
 
 // grad_hidden of every token: the slabs of a live one added in order, zero for the others.
@@ -587,7 +712,9 @@ __global__ __launch_bounds__(256) void head_hidden_kernel(const float* __restric
 // ---------------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------------
-int row_tiles(int64_t tokens) { return tokens <= 64 ? 1 : tokens <= 128 ? 2 : 4; }    // TM of the products over hidden
+int rows_kind(int64_t tokens) { return tokens <= kListTokens ? kList : tokens <= kFewTokens ? kFew : kMany; }
+// the most tiles over tokens that a launch may have
+int64_t most_row_tiles(int64_t tokens) { return tokens <= kListTokens ? 1 : tokens <= kFewTokens ? (tokens + 191) / 192 : (tokens + 255) / 256; }
 int64_t padded(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 bool sizes_ok(int64_t tokens, int64_t H, int64_t V)
@@ -605,15 +732,15 @@ struct BackwardPlan {
 BackwardPlan backward_plan(int64_t tokens, int64_t H, int64_t V, bool want_weight)
 {
     BackwardPlan p;
-    p.rows = padded(tokens, 256);
+    p.rows = tokens <= kListTokens ? 64 : tokens <= kFewTokens ? padded(tokens, 64) + 192 : padded(tokens, 256);      // (a tile begins with a token)
     int64_t bytes = 8 * p.rows * H;
     if (bytes < ((int64_t)256 << 20)) bytes = (int64_t)256 << 20;
     int64_t most = bytes / (2 * p.rows) / 256 * 256;
     if (most < 256) most = 256;
     const int64_t pieces = (V + most - 1) / most;
     p.width = padded((V + pieces - 1) / pieces, 256);
-    const int64_t tiles_h = (H + 255) / 256, tiles = p.rows / 256 * tiles_h, stages = p.width / 32;
-    const int64_t all = tiles * stages + (want_weight ? p.width / 256 * tiles_h * (p.rows / 32) : 0), cus = device_cus();
+    const int64_t tiles_h = (H + 255) / 256, tiles = most_row_tiles(tokens) * tiles_h, stages = p.width / 32;
+    const int64_t all = tiles * stages + (want_weight ? p.width / 256 * tiles_h * ((tokens + 31) / 32) : 0), cus = device_cus();
     int64_t share = (all + cus - 1) / cus;
     if (share < 16) share = 16;
     int64_t s = (stages + share - 1) / share;
@@ -623,25 +750,48 @@ BackwardPlan backward_plan(int64_t tokens, int64_t H, int64_t V, bool want_weigh
 }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
-template <int TM, bool ENT>
-int launch_stats(const Tokens& tk, const void* weight, int64_t ldw, int stride, float2* part, float* part_e, float* hit, hipStream_t st)
+// f with the kind of launch
+template <class F> int with_rows(int64_t tokens, F&& f)
+{
+    switch (rows_kind(tokens)) {
+        case kList: return f(std::integral_constant<int, kList>{});
+        case kFew: return f(std::integral_constant<int, kFew>{});
+        default: return f(std::integral_constant<int, kMany>{});
+    }
+}
+// LDS of a kernel whose tiles have at most 64 TM rows
+constexpr size_t ring_bytes(int TM) { return (size_t)HL_NS * hl_stage_bytes(TM); }
+
+template <int ROWS, bool ENT>
+int launch_stats(const Tokens& tk, const void* weight, int64_t ldw, int stride, float2* part, float* part_e, float* hit, int64_t ignore, int* list, hipStream_t st)
 {
     static bool done[64] = {};
-    const size_t lds = (size_t)hl_slots(TM) * hl_stage_bytes(TM);
-    if (const int rc = allow_dynamic_lds((const void*)head_stats_kernel<TM, ENT>, lds, done)) return rc;
-    const int64_t tiles = ((tk.tokens + 64 * TM - 1) / (64 * TM)) * (int64_t)((tk.V + HL_BN - 1) / HL_BN);
-    hipLaunchKernelGGL((head_stats_kernel<TM, ENT>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(HL_THREADS), lds, st, tk, (const uint16_t*)weight, ldw, stride, part, part_e, hit);
+    const size_t lds = ROWS == kList ? ring_bytes(1) + kListTokens * sizeof(int) : ring_bytes(4);
+    if (const int rc = allow_dynamic_lds((const void*)head_stats_kernel<ROWS, ENT>, lds, done)) return rc;
+    const int64_t tiles = most_row_tiles(tk.tokens) * ((tk.V + HL_BN - 1) / HL_BN);
+    hipLaunchKernelGGL((head_stats_kernel<ROWS, ENT>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(HL_THREADS), lds, st, tk, (const uint16_t*)weight, ldw, stride, part, part_e, hit,
+                       ignore, list);
     return hipGetLastError() == hipSuccess ? METIS_OK : METIS_E_LAUNCH;
 }
 
-template <int TM>
-int launch_dlogits(const Tokens& tk, const void* weight, int64_t ldw, int v0, int width, const RowGrads& rg, uint16_t* dl, int64_t ld, hipStream_t st)
+template <int ROWS>
+int launch_dlogits(const Tokens& tk, const void* weight, int64_t ldw, int v0, int width, const RowGrads& rg, uint16_t* dl, int64_t panel, hipStream_t st)
 {
     static bool done[64] = {};
-    const size_t lds = (size_t)hl_slots(TM) * hl_stage_bytes(TM);
-    if (const int rc = allow_dynamic_lds((const void*)head_dlogits_kernel<TM>, lds, done)) return rc;
-    const int64_t tiles = ((tk.tokens + 64 * TM - 1) / (64 * TM)) * (int64_t)((width + HL_BN - 1) / HL_BN);
-    hipLaunchKernelGGL((head_dlogits_kernel<TM>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(HL_THREADS), lds, st, tk, (const uint16_t*)weight, ldw, v0, width, rg, dl, ld);
+    const size_t lds = ring_bytes(ROWS == kList ? 1 : 4);
+    if (const int rc = allow_dynamic_lds((const void*)head_dlogits_kernel<ROWS>, lds, done)) return rc;
+    const int64_t tiles = most_row_tiles(tk.tokens) * ((width + HL_BN - 1) / HL_BN);
+    hipLaunchKernelGGL((head_dlogits_kernel<ROWS>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(HL_THREADS), lds, st, tk, (const uint16_t*)weight, ldw, v0, width, rg, dl, panel);
+    return hipGetLastError() == hipSuccess ? METIS_OK : METIS_E_LAUNCH;
+}
+
+template <int ROWS>
+int launch_products(const Products& p, unsigned grid, hipStream_t st)
+{
+    static bool done[64] = {};
+    const size_t lds = ring_bytes(4);
+    if (const int rc = allow_dynamic_lds((const void*)head_products_kernel<ROWS>, lds, done)) return rc;
+    hipLaunchKernelGGL((head_products_kernel<ROWS>), dim3(grid), dim3(HL_THREADS), lds, st, p);
     return hipGetLastError() == hipSuccess ? METIS_OK : METIS_E_LAUNCH;
 }
 
@@ -679,15 +829,15 @@ int head_logprobs(const void* hidden, int64_t ldh, const void* weight, int64_t l
     float2* part = static_cast<float2*>(workspace);
     float* hit = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256((size_t)stride * tiles_n * 8));
     float* part_e = entropy ? reinterpret_cast<float*>(reinterpret_cast<char*>(hit) + align256((size_t)stride * 4)) : nullptr;
-    hipLaunchKernelGGL(head_index_kernel, dim3(1), dim3(1024), 0, st, (const int64_t*)targets, ignore, (int)tokens, (int*)index);
-    if (hipGetLastError() != hipSuccess) return METIS_E_LAUNCH;
+    if (tokens > kListTokens) {
+        hipLaunchKernelGGL(head_index_kernel, dim3(1), dim3(1024), 0, st, (const int64_t*)targets, ignore, (int)tokens, (int*)index);
+        if (hipGetLastError() != hipSuccess) return METIS_E_LAUNCH;
+    }
     const Tokens tk = tokens_of(hidden, ldh, targets, index, tokens, H, V, temperature);
-    const int tm = row_tiles(tokens);
-    int rc;
-    if (entropy) rc = tm == 1 ? launch_stats<1, true>(tk, weight, ldw, stride, part, part_e, hit, st) : tm == 2 ? launch_stats<2, true>(tk, weight, ldw, stride, part, part_e, hit, st)
-                                                                                                       : launch_stats<4, true>(tk, weight, ldw, stride, part, part_e, hit, st);
-    else rc = tm == 1 ? launch_stats<1, false>(tk, weight, ldw, stride, part, part_e, hit, st) : tm == 2 ? launch_stats<2, false>(tk, weight, ldw, stride, part, part_e, hit, st)
-                                                                                                 : launch_stats<4, false>(tk, weight, ldw, stride, part, part_e, hit, st);
+    const int rc = with_rows(tokens, [&](auto rows) {
+        return entropy ? launch_stats<decltype(rows)::value, true>(tk, weight, ldw, stride, part, part_e, hit, ignore, (int*)index, st)
+                       : launch_stats<decltype(rows)::value, false>(tk, weight, ldw, stride, part, part_e, hit, ignore, (int*)index, st);
+    });
     if (rc != METIS_OK) return rc;
     const dim3 grid((unsigned)((tokens + 15) / 16));
     if (entropy)
@@ -731,22 +881,17 @@ int head_logprobs_backward(const void* hidden, int64_t ldh, const void* weight, 
         hipLaunchKernelGGL(head_gather_kernel, dim3((unsigned)(tokens + 31 < 8 * (int64_t)cus ? tokens + 31 : 8 * (int64_t)cus)), dim3(256), 0, st, tk, (uint4*)gathered);
         if (hipGetLastError() != hipSuccess) return METIS_E_LAUNCH;
     }
-    static bool done[64] = {};
-    const size_t lds = (size_t)hl_slots(4) * hl_stage_bytes(4);
-    if (const int rc = allow_dynamic_lds((const void*)head_products_kernel, lds, done)) return rc;
-    const int tm = row_tiles(tokens);
     const int64_t tiles_h = (H + 255) / 256;
     for (int64_t v0 = 0; v0 < V; v0 += p.width) {
         const int width = (int)(V - v0 < p.width ? V - v0 : p.width);
-        const int rc = tm == 1 ? launch_dlogits<1>(tk, weight, ldw, (int)v0, width, rg, dl, p.width, st)
-                     : tm == 2 ? launch_dlogits<2>(tk, weight, ldw, (int)v0, width, rg, dl, p.width, st) : launch_dlogits<4>(tk, weight, ldw, (int)v0, width, rg, dl, p.width, st);
+        int rc = with_rows(tokens, [&](auto rows) { return launch_dlogits<decltype(rows)::value>(tk, weight, ldw, (int)v0, width, rg, dl, p.rows * 64, st); });
         if (rc != METIS_OK) return rc;
-        const Products pr = {dl, p.width, (const uint16_t*)weight + v0 * ldw, ldw, gathered, slabs, grad_weight ? (uint16_t*)grad_weight + v0 * H : nullptr, (const int*)index, width, (int)H,
-                             p.splits, v0 == 0, p.rows};
-        const int64_t hidden_jobs = slabs ? p.rows / 256 * tiles_h * p.splits : 0, weight_jobs = grad_weight ? (width + 255) / 256 * tiles_h : 0;
+        const Products pr = {dl, p.rows, (const uint16_t*)weight + v0 * ldw, ldw, gathered, slabs, grad_weight ? (uint16_t*)grad_weight + v0 * H : nullptr, (const int*)index, width,
+                             (int)H, p.splits, v0 == 0};
+        const int64_t hidden_jobs = slabs ? most_row_tiles(tokens) * tiles_h * p.splits : 0, weight_jobs = grad_weight ? (width + 255) / 256 * tiles_h : 0;
         const unsigned grid = 8u * (unsigned)((hidden_jobs + 7) / 8 + (weight_jobs + 7) / 8);
-        hipLaunchKernelGGL(head_products_kernel, dim3(grid), dim3(HL_THREADS), lds, st, pr);
-        if (hipGetLastError() != hipSuccess) return METIS_E_LAUNCH;
+        rc = with_rows(tokens, [&](auto rows) { return launch_products<decltype(rows)::value>(pr, grid, st); });
+        if (rc != METIS_OK) return rc;
     }
     if (grad_hidden) {
         const int64_t need = (tokens * (H / 4) + 255) / 256, cap = (int64_t)cus * 16;
