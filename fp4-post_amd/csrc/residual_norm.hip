@@ -11,7 +11,7 @@
 //   gy    = rstd(y) (dz post_weight - yh mean(dz post_weight yh))
 //   gweight = sum gn hh,   gpost = sum dz yh,   ggate = sum over the rows of a gate's row of scale d z
 //
-// A row belongs to W waves (one up to 1024 columns, then four or eight), lane l of wave w holding the chunks of eight elements
+// A row belongs to W waves (one per 512 columns up to 2048, then four or eight), lane l of wave w holding the chunks of eight elements
 // (i W + w) 64 + l: every access instruction of a wave covers consecutive bytes, the row is read once, its sums are folded across the lanes with
 // DPP moves and across the waves through LDS.  Bound by memory.
 #include "chunk8.h"
@@ -39,7 +39,7 @@ __device__ __forceinline__ float rn_wave_sum(float v)
 // Sums of up to three numbers over the waves of a row.  Two areas in turn: a wave writes an area again only behind the barrier of the
 // other one, which every wave passes after it has read the first.
 template <int W> struct RowSums {
-    static constexpr int kWords = W > 1 ? 2 * 3 * W : 1;
+    static constexpr int kWords = W > 1 ? 2 * 3 * W : 1;       // for the waves of one row
     float* area;
     int turn = 0;
     template <int N> __device__ __forceinline__ void operator()(float (&v)[N], int wave)
@@ -72,9 +72,9 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void residual_norm_kernel(con
                                                                              void* __restrict__ n)
 {
     constexpr int WAVES = W > 4 ? W : 4, ROWS = WAVES / W;
-    __shared__ float area[RowSums<W>::kWords];
-    RowSums<W> fold{area};
-    const uint32_t cpr = cols / 8u, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, part = wave % W;
+    __shared__ float area[ROWS][RowSums<W>::kWords];
+    const uint32_t cpr = cols / 8u, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, part = wave % W, team = wave / W;
+    RowSums<W> fold{area[team]};
     const float fcols = (float)cols;
     B wt[NL], pw[POST ? NL : 1];
 #pragma unroll
@@ -87,18 +87,20 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void residual_norm_kernel(con
             if (c < cpr) pw[i].load(post, c);
         }
     }
-    // (with several waves to a row all of a workgroup's waves are on the same one: the barriers inside are met by all)
-    for (uint32_t row = blockIdx.x * ROWS + wave / W; row < rows; row += gridDim.x * ROWS) {
+    // (all teams go round as often as the first: the folds hold barriers for all of them)
+    for (uint32_t row0 = blockIdx.x * ROWS; row0 < rows; row0 += gridDim.x * ROWS) {
+        const uint32_t row = row0 + team;
+        const bool live = row < rows;
         R xr[NL];
         B yr[NL], gr[NL];
-        const size_t at = (size_t)row * cpr, gate_at = gate ? (size_t)(row / gate_every) * cpr : 0;
+        const size_t at = (size_t)row * cpr, gate_at = gate && live ? (size_t)(row / gate_every) * cpr : 0;
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const uint32_t c = (i * W + part) * 64u + lane;
             xr[i].zero();
             yr[i].zero();
             gr[i].zero();
-            if (c < cpr) {
+            if (live && c < cpr) {
                 yr[i].load(y, at + c);
                 xr[i].load(x, at + c);
                 if (gate) gr[i].load(gate, gate_at + c);
@@ -133,7 +135,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void residual_norm_kernel(con
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const uint32_t c = (i * W + part) * 64u + lane;
-            if (c >= cpr) continue;
+            if (!live || c >= cpr) continue;
             float f[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] = xr[i].get(j) * rh * wt[i].get(j);
@@ -148,17 +150,27 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void residual_norm_kernel(con
 // Gradients.  A workgroup owns every slabs-th row (set of ROWS) of one gate row's rows and keeps the column sums of its rows in registers; they go to
 // partial rows of the workspace, [sum][gate row][slab][column], which residual_norm_sums_kernel adds in order.  No gate: one gate row for all rows.
 // Where there are more gate rows than workgroups a workgroup takes several, one after the other, and writes the gate's gradient itself.
+//
+// The sums' registers leave room for two waves per SIMD, one workgroup of eight per compute unit (two of four would leave twice the partial rows: 2103 x 4096
+// with a norm behind the block and gates, binary32 stream, 42 us, now 37), so a row's reads have to be under way while the one before is
+// worked on: the next row is requested before the folds (AHEAD; where the registers hold it).  weight, post_weight and the gate stay in LDS, every lane reading what it put there itself.
+template <class R, class B> struct RowIn {                    // one chunk of the lane's share of a row
+    R h, gh;
+    B gn, y;
+};
 template <class R, class B, int NL, int W, bool POST>
-__global__ __launch_bounds__(W > 4 ? 64 * W : 256) void residual_norm_backward_kernel(
+__global__ __launch_bounds__(512, 2) void residual_norm_backward_kernel(
     const void* __restrict__ h, const void* __restrict__ y, const void* __restrict__ weight, const void* __restrict__ post, const void* __restrict__ gate,
     uint32_t groups, uint32_t group_rows, uint32_t slabs, float scale, float eps, uint32_t cols, const void* __restrict__ gh, const void* __restrict__ gn,
     void* __restrict__ gx, void* __restrict__ gy, float* __restrict__ sum_w, float* __restrict__ sum_p, float* __restrict__ sum_g, void* __restrict__ ggate)
 {
-    constexpr int WAVES = W > 4 ? W : 4, ROWS = WAVES / W;
-    __shared__ float area[RowSums<W>::kWords];
-    __shared__ float turn[ROWS > 1 ? NL * 64 * 8 : 1];
-    RowSums<W> fold{area};
-    const uint32_t cpr = cols / 8u, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, part = wave % W;
+    constexpr int ROWS = 8 / W, THREADS = 512;                 // rows at once
+    constexpr bool AHEAD = !(POST && NL == 2 && R::bytes == 32 && (W != 4 || B::bytes == 32));
+    __shared__ float area[ROWS][RowSums<W>::kWords];
+    __shared__ float turn[ROWS > 1 ? W * NL * 64 * 8 : 1];
+    __shared__ B vec_w[NL][THREADS], vec_p[POST ? NL : 1][POST ? THREADS : 1], vec_g[NL][THREADS];
+    const uint32_t cpr = cols / 8u, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, part = wave % W, team = wave / W;
+    RowSums<W> fold{area[team]};
     const float inv_cols = 1.0f / (float)cols, fcols = (float)cols;
     float acc_w[NL][8], acc_p[POST ? NL : 1][8], acc_g[NL][8];
     auto clear = [](float(&a)[8]) {
@@ -167,33 +179,44 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void residual_norm_backward_k
     };
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
+        const uint32_t c = (i * W + part) * 64u + lane;
         clear(acc_w[i]);
         clear(acc_g[i]);
         if constexpr (POST) clear(acc_p[i]);
+        B v;
+        v.zero();
+        if (c < cpr) v.load(weight, c);
+        vec_w[i][threadIdx.x] = v;
+        if constexpr (POST) {
+            v.zero();
+            if (c < cpr) v.load(post, c);
+            vec_p[i][threadIdx.x] = v;
+        }
     }
-    // the sums of a workgroup: its waves' in wave order where they hold different rows of the same columns
+    // the sums of a workgroup: those of its teams in order
     auto write_sums = [&](float(&a)[NL][8], float* out, void* rounded) {
         if constexpr (ROWS > 1) {
-            for (int v = 0; v < ROWS; ++v) {
-                if ((int)wave == v) {
+            float* mine = turn + part * (NL * 64 * 8) + lane;
+            for (uint32_t v = 0; v < (uint32_t)ROWS; ++v) {
+                if (team == v) {
 #pragma unroll
                     for (int i = 0; i < NL; ++i)
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            float* t = turn + (i * 8 + j) * 64 + lane;
+                            float* t = mine + (i * 8 + j) * 64;
                             *t = v ? *t + a[i][j] : a[i][j];
                         }
                 }
                 __syncthreads();
             }
-            if (wave == 0) {
+            if (team == 0) {
 #pragma unroll
                 for (int i = 0; i < NL; ++i)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) a[i][j] = turn[(i * 8 + j) * 64 + lane];
+                    for (int j = 0; j < 8; ++j) a[i][j] = mine[(i * 8 + j) * 64];
             }
             __syncthreads();
-            if (wave != 0) return;
+            if (team) return;
         }
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
@@ -212,66 +235,90 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void residual_norm_backward_k
     };
     const uint32_t slab = blockIdx.x % slabs;
     for (uint32_t group = blockIdx.x / slabs; group < groups; group += gridDim.x / slabs) {
-        B gt[NL];
+        RowIn<R, B> in[NL];
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const uint32_t c = (i * W + part) * 64u + lane;
-            gt[i].zero();
-            if (gate && c < cpr) gt[i].load(gate, (size_t)group * cpr + c);
+            B v;
+            v.zero();
+            if (gate && c < cpr) v.load(gate, (size_t)group * cpr + c);
+            vec_g[i][threadIdx.x] = v;
+            in[i].h.zero();
+            in[i].gh.zero();
+            in[i].gn.zero();
+            in[i].y.zero();
         }
-        for (uint32_t r = slab * ROWS + wave / W; r < group_rows; r += slabs * ROWS) {
+        auto request = [&](uint32_t r) {
             const size_t at = ((size_t)group * group_rows + r) * cpr;
-            R hr[NL], dr[NL];
-            B nr[NL], yr[NL], wt[NL], pw[NL];
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
                 const uint32_t c = (i * W + part) * 64u + lane;
-                hr[i].zero(); dr[i].zero(); nr[i].zero(); yr[i].zero(); wt[i].zero(); pw[i].zero();
                 if (c < cpr) {
-                    hr[i].load(h, at + c);
-                    if (gn) nr[i].load(gn, at + c);
-                    if (gh) dr[i].load(gh, at + c);
-                    if (y) yr[i].load(y, at + c);
-                    wt[i].load(weight, c);
-                    if constexpr (POST) pw[i].load(post, c);
+                    in[i].h.load(h, at + c);
+                    if (gn) in[i].gn.load(gn, at + c);
+                    if (gh) in[i].gh.load(gh, at + c);
+                    if (y) in[i].y.load(y, at + c);
+                }
+            }
+        };
+        // (all teams go round as often as the first: the folds hold barriers for all; one without a row adds nothing)
+        const uint32_t step = slabs * ROWS;
+        if (AHEAD && slab * ROWS + team < group_rows) request(slab * ROWS + team);
+        for (uint32_t r0 = slab * ROWS; r0 < group_rows; r0 += step) {
+            const uint32_t r = r0 + team;
+            const bool live = r < group_rows;
+            const size_t at = ((size_t)group * group_rows + r) * cpr;
+            if (!AHEAD && live) request(r);
+            RowIn<R, B> cur[NL];
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                cur[i] = in[i];
+                if (ROWS > 1 && !live) {
+                    cur[i].h.zero();
+                    cur[i].gh.zero();
+                    cur[i].gn.zero();
+                    cur[i].y.zero();
                 }
             }
             float s[POST ? 3 : 2] = {};                        // sum h^2, sum (gn weight) h, sum y^2
 #pragma unroll
-            for (int i = 0; i < NL; ++i)
+            for (int i = 0; i < NL; ++i) {
+                const B wt = vec_w[i][threadIdx.x];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float hv = hr[i].get(j);
+                    const float hv = cur[i].h.get(j);
                     s[0] = fmaf(hv, hv, s[0]);
-                    s[1] = fmaf(nr[i].get(j) * wt[i].get(j), hv, s[1]);
-                    if constexpr (POST) s[2] = fmaf(yr[i].get(j), yr[i].get(j), s[2]);
+                    s[1] = fmaf(cur[i].gn.get(j) * wt.get(j), hv, s[1]);
+                    if constexpr (POST) s[2] = fmaf(cur[i].y.get(j), cur[i].y.get(j), s[2]);
                 }
+            }
+            if (AHEAD && r + step < group_rows) request(r + step);
             fold(s, part);
-            const float rh = 1.0f / sqrtf(s[0] / fcols + eps), mean = s[1] * rh * inv_cols;
-            float ry = 1.0f;
-            if constexpr (POST) ry = 1.0f / sqrtf(s[2] / fcols + eps);
+            const float rh = live ? 1.0f / sqrtf(s[0] / fcols + eps) : 0.0f, mean = s[1] * rh * inv_cols;
+            float ry = live ? 1.0f : 0.0f;
+            if constexpr (POST) ry = live ? 1.0f / sqrtf(s[2] / fcols + eps) : 0.0f;
             float dz[NL][8], dot[1] = {0.0f};
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
                 const uint32_t c = (i * W + part) * 64u + lane;
+                const B wt = vec_w[i][threadIdx.x], gt = vec_g[i][threadIdx.x], pw = vec_p[POST ? i : 0][POST ? threadIdx.x : 0];
                 float d[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float hh = hr[i].get(j) * rh, gv = nr[i].get(j);
+                    const float hh = cur[i].h.get(j) * rh, gv = cur[i].gn.get(j);
                     acc_w[i][j] = fmaf(gv, hh, acc_w[i][j]);
-                    d[j] = fmaf(rh, fmaf(gv, wt[i].get(j), -hh * mean), dr[i].get(j));
-                    const float sd = scale * d[j], yh = yr[i].get(j) * ry;
+                    d[j] = fmaf(rh, fmaf(gv, wt.get(j), -hh * mean), cur[i].gh.get(j));
+                    const float sd = scale * d[j], yh = cur[i].y.get(j) * ry;
+                    dz[i][j] = gate ? sd * gt.get(j) : sd;
                     if constexpr (POST) {
-                        acc_g[i][j] = fmaf(sd, yh * pw[i].get(j), acc_g[i][j]);
-                        dz[i][j] = gate ? sd * gt[i].get(j) : sd;
+                        acc_g[i][j] = fmaf(sd, yh * pw.get(j), acc_g[i][j]);
                         acc_p[i][j] = fmaf(dz[i][j], yh, acc_p[i][j]);
-                        dot[0] = fmaf(dz[i][j] * pw[i].get(j), yh, dot[0]);
+                        dot[0] = fmaf(dz[i][j] * pw.get(j), yh, dot[0]);
                     } else {
                         acc_g[i][j] = fmaf(sd, yh, acc_g[i][j]);
-                        dz[i][j] = gate ? sd * gt[i].get(j) : sd;
                     }
                 }
-                if (gx && c < cpr) {
+                if (gx && live && c < cpr) {
                     R o;
                     o.set(d);
                     o.store(gx, at + c);
@@ -282,12 +329,13 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void residual_norm_backward_k
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
                 const uint32_t c = (i * W + part) * 64u + lane;
-                if (c >= cpr) continue;
+                if (!live || c >= cpr) continue;
+                const B pw = vec_p[POST ? i : 0][POST ? threadIdx.x : 0];
                 float f[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     f[j] = dz[i][j];
-                    if constexpr (POST) f[j] = ry * fmaf(dz[i][j], pw[i].get(j), -(yr[i].get(j) * ry) * (dot[0] * inv_cols));
+                    if constexpr (POST) f[j] = ry * fmaf(dz[i][j], pw.get(j), -(cur[i].y.get(j) * ry) * (dot[0] * inv_cols));
                 }
                 B o;
                 o.set(f);
@@ -340,20 +388,19 @@ __global__ __launch_bounds__(1024) void residual_norm_sums_kernel(const float* _
 
 namespace {
 
-// waves of a row, and the rows that a workgroup takes at once
-int row_waves(int64_t cols) { return cols <= 1024 ? 1 : cols <= 4096 ? 4 : 8; }
-int rows_at_once(int64_t cols) { return cols <= 1024 ? 4 : 1; }
+// waves of a row; a workgroup has eight, forward four where these are enough
+int row_waves(int64_t cols, int y_dtype) { return cols <= 512 ? 1 : cols <= 1024 ? 2 : cols <= 2048 || (cols <= 4096 && y_dtype == METIS_DTYPE_BF16) ? 4 : 8; }
 
 struct BackwardPlan {
     uint32_t groups, group_rows, slabs, grid;
     bool direct;                                               // more gate rows than workgroups: each writes its gate's gradient itself
 };
-BackwardPlan backward_plan(int64_t rows, int64_t cols, int64_t gate_rows)
+BackwardPlan backward_plan(int64_t rows, int64_t cols, int y_dtype, int64_t gate_rows)
 {
     BackwardPlan p;
     p.groups = gate_rows > 0 ? (uint32_t)gate_rows : 1u;
     p.group_rows = (uint32_t)(rows / p.groups);
-    const uint32_t cap = (uint32_t)device_cus() * 2u, at_once = (uint32_t)rows_at_once(cols), need = (p.group_rows + at_once - 1) / at_once;
+    const uint32_t cap = (uint32_t)device_cus(), at_once = 8u / (uint32_t)row_waves(cols, y_dtype), need = (p.group_rows + at_once - 1) / at_once;
     p.slabs = p.groups >= cap ? 1u : cap / p.groups;
     if (p.slabs > need) p.slabs = need;
     p.grid = p.slabs * (p.groups < cap ? p.groups : cap);
@@ -373,13 +420,13 @@ bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
 }  // namespace
 
 // calls F with the kernel's types and widths
-#define METIS_RN_WIDTH(F, R, B, P)                                  \
-    do {                                                            \
-        if (cols <= 512) F(R, B, 1, 1, P);                          \
-        else if (cols <= 1024) F(R, B, 2, 1, P);                    \
-        else if (cols <= 2048) F(R, B, 1, 4, P);                    \
-        else if (cols <= 4096) F(R, B, 2, 4, P);                    \
-        else F(R, B, 2, 8, P);                                      \
+#define METIS_RN_WIDTH(F, R, B, P)                                                                                              \
+    do {                                                                                                                        \
+        if (cols <= 512) F(R, B, 1, 1, P);                                                                                      \
+        else if (cols <= 1024) F(R, B, 1, 2, P);                                                                                \
+        else if (cols <= 2048) F(R, B, 1, 4, P);                                                                                \
+        else if (cols <= 4096) F(R, B, (B::bytes == 16 ? 2 : 1), (B::bytes == 16 ? 4 : 8), P);                                  \
+        else F(R, B, 2, 8, P);                                                                                                  \
     } while (0)
 #define METIS_RN_TYPES(F, P)                                                                    \
     do {                                                                                        \
@@ -395,8 +442,9 @@ int residual_norm(const void* x, int x_dtype, const void* y, int y_dtype, const 
     if (rows == 0) return METIS_OK;
     if (!x || !y || !weight || !h || !n || (gate_rows > 0) != (gate != nullptr)) return METIS_E_ARG;
     if (!aligned(x) || !aligned(y) || !aligned(weight) || !aligned(post) || !aligned(gate) || !aligned(h) || !aligned(n)) return METIS_E_ARG;
-    const int64_t at_once = rows_at_once(cols), need = (rows + at_once - 1) / at_once, cap = (int64_t)device_cus() * (row_waves(cols) == 8 ? 4 : 8);
-    const unsigned grid = (unsigned)(need < cap ? need : cap), threads = row_waves(cols) == 8 ? 512 : 256;
+    const int waves = row_waves(cols, y_dtype);
+    const int64_t at_once = waves == 8 ? 1 : 4 / waves, need = (rows + at_once - 1) / at_once, cap = (int64_t)device_cus() * (waves == 8 ? 4 : 8);
+    const unsigned grid = (unsigned)(need < cap ? need : cap), threads = waves == 8 ? 512 : 256;
     const uint32_t every = gate ? (uint32_t)(rows / gate_rows) : 1u;
 #define METIS_RN_FWD(R, B, NL, W, P) hipLaunchKernelGGL((residual_norm_kernel<R, B, NL, W, P>), dim3(grid), dim3(threads), 0, st, x, y, weight, post, gate, every, \
                                                         scale, eps, (uint32_t)rows, (uint32_t)cols, h, n)
@@ -409,7 +457,7 @@ int residual_norm(const void* x, int x_dtype, const void* y, int y_dtype, const 
 size_t residual_norm_backward_workspace_bytes(int64_t rows, int64_t cols, int64_t gate_rows)
 {
     if (rows <= 0 || !sizes_ok(rows, cols, METIS_DTYPE_F32, METIS_DTYPE_F32, gate_rows)) return 0;
-    const BackwardPlan p = backward_plan(rows, cols, gate_rows);
+    const BackwardPlan p = backward_plan(rows, cols, METIS_DTYPE_F32, gate_rows);       // (its rows take the most waves: the most workgroups of the two types)
     return (size_t)p.grid * (size_t)cols * sizeof(float) * (gate_rows > 0 && !p.direct ? 3 : 2);
 }
 
@@ -423,8 +471,7 @@ int residual_norm_backward(const void* h, int x_dtype, const void* y, int y_dtyp
         !aligned(gweight) || !aligned(gpost) || !aligned(ggate))
         return METIS_E_ARG;
     if (!workspace || !aligned(workspace) || workspace_bytes < residual_norm_backward_workspace_bytes(rows, cols, gate_rows)) return METIS_E_WORKSPACE;
-    const BackwardPlan p = backward_plan(rows, cols, gate_rows);
-    const unsigned threads = row_waves(cols) == 8 ? 512 : 256;
+    const BackwardPlan p = backward_plan(rows, cols, y_dtype, gate_rows);
     float* sum_w = static_cast<float*>(workspace);
     float* sum_p = sum_w + (size_t)p.grid * cols;
     float* sum_g = ggate && !p.direct ? sum_p + (size_t)p.grid * cols : nullptr;
@@ -432,7 +479,7 @@ int residual_norm_backward(const void* h, int x_dtype, const void* y, int y_dtyp
     if (!gpost) sum_p = nullptr;
     const void* yy = (post || ggate) ? y : nullptr;
     void* direct = p.direct ? ggate : nullptr;
-#define METIS_RN_BWD(R, B, NL, W, P) hipLaunchKernelGGL((residual_norm_backward_kernel<R, B, NL, W, P>), dim3(p.grid), dim3(threads), 0, st, h, yy, weight, post, gate, \
+#define METIS_RN_BWD(R, B, NL, W, P) hipLaunchKernelGGL((residual_norm_backward_kernel<R, B, NL, W, P>), dim3(p.grid), dim3(512), 0, st, h, yy, weight, post, gate, \
                                                         p.groups, p.group_rows, p.slabs, scale, eps, (uint32_t)cols, gh, gn, gx, gy, sum_w, sum_p, sum_g, direct)
     if (post) METIS_RN_TYPES(METIS_RN_BWD, true);
     else METIS_RN_TYPES(METIS_RN_BWD, false);

@@ -7,6 +7,8 @@
 
 namespace metis {
 
+constexpr uint64_t kStreamBytes = (uint64_t)256 << 20;         // the memory-side cache
+
 // The sigmoid of a bf16 value needs no more than the hardware's exponential and reciprocal; a binary32 one takes the library's and a true division.
 template <bool F32> __device__ __forceinline__ float sigmoid(float g)
 {
@@ -24,41 +26,54 @@ template <bool F32> __device__ __forceinline__ void gated_back(float g, float u,
 // position of unit `at` (eight elements or one) in rows of `per` units and `ld` units' stride
 template <class I> __device__ __forceinline__ size_t strided(I at, uint32_t per, uint64_t ld) { return ld == per ? at : at / per * ld + at % per; }
 
-template <class C>
+// STREAM: more bytes than the memory-side cache holds (kStreamBytes) go by it with the non-temporal hint, and the backward takes two chunks a lane at once.
+// 4096 x 18944 bf16, halves of one product: 87 -> 69 us and 148 -> 122 (6.8 and 6.3 TB/s); of 1024 rows, which stay in the cache, 19 and 31 us with or without
+// the hint, 512 x 8960 8.4 us without and 9.4 with it.
+template <class C, bool STREAM>
 __global__ __launch_bounds__(256) void swiglu_kernel(const void* __restrict__ gate, uint64_t ldg, const void* __restrict__ up, uint64_t ldu, uint32_t total,
                                                      uint32_t per, void* __restrict__ out)
 {
     constexpr bool F32 = C::bytes == 32;
-    for (uint32_t at = blockIdx.x * 256u + threadIdx.x; at < total; at += gridDim.x * 256u) {
-        C g, u, o;
-        g.load(gate, strided(at, per, ldg));
-        u.load(up, strided(at, per, ldu));
-        float f[8];
+    const uint32_t at = blockIdx.x * 256u + threadIdx.x;
+    if (at >= total) return;
+    C g, u, o;
+    g.template load<STREAM>(gate, strided(at, per, ldg));
+    u.template load<STREAM>(up, strided(at, per, ldu));
+    float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = gated<F32>(g.get(j), u.get(j));
-        o.set(f);
-        o.store(out, at);
-    }
+    for (int j = 0; j < 8; ++j) f[j] = gated<F32>(g.get(j), u.get(j));
+    o.set(f);
+    o.template store<STREAM>(out, at);
 }
 
-template <class C>
+template <class C, bool STREAM>
 __global__ __launch_bounds__(256) void swiglu_backward_kernel(const void* __restrict__ gate, uint64_t ldg, const void* __restrict__ up, uint64_t ldu,
                                                               const void* __restrict__ grad, uint32_t total, uint32_t per, void* __restrict__ ggate,
                                                               void* __restrict__ gup)
 {
     constexpr bool F32 = C::bytes == 32;
-    for (uint32_t at = blockIdx.x * 256u + threadIdx.x; at < total; at += gridDim.x * 256u) {
-        C g, u, a;
-        g.load(gate, strided(at, per, ldg));
-        u.load(up, strided(at, per, ldu));
-        a.load(grad, at);
+    constexpr int N = STREAM ? 2 : 1;                          // chunks of a lane, a workgroup's width apart
+    const uint32_t first = blockIdx.x * 256u * N + threadIdx.x;
+    C g[N], u[N], a[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const uint32_t at = first + 256u * k;
+        if (at >= total) break;
+        g[k].template load<STREAM>(gate, strided(at, per, ldg));
+        u[k].template load<STREAM>(up, strided(at, per, ldu));
+        a[k].template load<STREAM>(grad, at);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const uint32_t at = first + 256u * k;
+        if (at >= total) break;
         float dg[8], du[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) gated_back<F32>(g.get(j), u.get(j), a.get(j), dg[j], du[j]);
-        g.set(dg);
-        u.set(du);
-        g.store(ggate, at);
-        u.store(gup, at);
+        for (int j = 0; j < 8; ++j) gated_back<F32>(g[k].get(j), u[k].get(j), a[k].get(j), dg[j], du[j]);
+        g[k].set(dg);
+        u[k].set(du);
+        g[k].template store<STREAM>(ggate, at);
+        u[k].template store<STREAM>(gup, at);
     }
 }
 
@@ -102,17 +117,23 @@ int swiglu(const void* gate, int64_t ldg, const void* up, int64_t ldu, const voi
     if (any % size) return METIS_E_ARG;
     if (rows == 1) ldg = ldu = cols;
     const bool whole = cols % 8 == 0 && ldg % 8 == 0 && ldu % 8 == 0 && any % 16 == 0;
-    const uint64_t unit = whole ? 8 : 1, total = (uint64_t)rows * (uint64_t)cols / unit, need = (total + 255) / 256, cap = (uint64_t)device_cus() * 16;
-    const dim3 grid((unsigned)(need < cap ? need : cap)), block(256);
-    if (whole && total > (uint64_t)INT32_MAX) return METIS_E_TOO_LARGE;   // (units are counted in 32 bits, a stride beyond the last one included)
+    const uint64_t unit = whole ? 8 : 1, total = (uint64_t)rows * (uint64_t)cols / unit;
+    if (whole && total > (uint64_t)INT32_MAX) return METIS_E_TOO_LARGE;         // (units are counted in 32 bits)
+    const bool stream = whole && total * 8 * size * (back ? 5 : 3) > kStreamBytes;
+    const uint64_t lane = back && stream ? 2 : 1, need = (total + 256 * lane - 1) / (256 * lane), cap = (uint64_t)device_cus() * 16;
+    const dim3 grid((unsigned)(whole || need < cap ? need : cap)), block(256);
     const uint32_t per = (uint32_t)(cols / unit);
     const uint64_t lg = (uint64_t)ldg / unit, lu = (uint64_t)ldu / unit;
+#define METIS_SGF(C, S) hipLaunchKernelGGL((swiglu_kernel<C, S>), grid, block, 0, st, gate, lg, up, lu, (uint32_t)total, per, out)
+#define METIS_SGB(C, S) hipLaunchKernelGGL((swiglu_backward_kernel<C, S>), grid, block, 0, st, gate, lg, up, lu, grad, (uint32_t)total, per, out, gup)
     if (whole && !back) {
-        if (f32) hipLaunchKernelGGL((swiglu_kernel<F32x8>), grid, block, 0, st, gate, lg, up, lu, (uint32_t)total, per, out);
-        else hipLaunchKernelGGL((swiglu_kernel<Bf16x8>), grid, block, 0, st, gate, lg, up, lu, (uint32_t)total, per, out);
+        if (f32) { if (stream) METIS_SGF(F32x8, true); else METIS_SGF(F32x8, false); }
+        else { if (stream) METIS_SGF(Bf16x8, true); else METIS_SGF(Bf16x8, false); }
     } else if (whole) {
-        if (f32) hipLaunchKernelGGL((swiglu_backward_kernel<F32x8>), grid, block, 0, st, gate, lg, up, lu, grad, (uint32_t)total, per, out, gup);
-        else hipLaunchKernelGGL((swiglu_backward_kernel<Bf16x8>), grid, block, 0, st, gate, lg, up, lu, grad, (uint32_t)total, per, out, gup);
+        if (f32) { if (stream) METIS_SGB(F32x8, true); else METIS_SGB(F32x8, false); }
+        else { if (stream) METIS_SGB(Bf16x8, true); else METIS_SGB(Bf16x8, false); }
+#undef METIS_SGF
+#undef METIS_SGB
     } else {
 #define METIS_SG(F, K) hipLaunchKernelGGL((swiglu_single_kernel<F, K>), grid, block, 0, st, gate, lg, up, lu, grad, total, per, out, gup)
         if (f32) { if (back) METIS_SG(true, true); else METIS_SG(true, false); }

@@ -44,9 +44,10 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, *, pos
     gate      in y's type: [C], or x's leading sizes followed by ones ([B, 1, C]: one for each sequence of [B, S, C])
 
     Returns (h in x's type, n in y's type); n is the norm of h as it is stored.  Differentiable (once) in all tensors."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, weight, post_weight, gate)):
+    if torch.is_grad_enabled() and (x.requires_grad or y.requires_grad or weight.requires_grad or (post_weight is not None and post_weight.requires_grad)
+                                    or (gate is not None and gate.requires_grad)):
         return _ResidualNorm.apply(x, y, weight, post_weight, gate, float(residual_scale), float(eps))
-    return ops.residual_norm(x, y, weight, post_weight, gate, residual_scale, eps)
+    return ops.residual_norm(x, y, weight, post_weight, gate, float(residual_scale), float(eps))
 
 
 class _SwiGLU(torch.autograd.Function):

@@ -1271,7 +1271,7 @@ def _on_own_device(fn):
     """The call runs on the current stream of its first tensor's device, whichever device is current."""
     @functools.wraps(fn)
     def run(first: torch.Tensor, *args, **kwargs):
-        if first.is_cuda and first.device.index != torch.cuda.current_device():
+        if first.is_cuda and first.get_device() != (_raw_device or torch.cuda.current_device)():
             with torch.cuda.device(first.device):
                 return fn(first, *args, **kwargs)
         return fn(first, *args, **kwargs)
@@ -1281,20 +1281,21 @@ def _on_own_device(fn):
 _FLOATS = {torch.bfloat16: (DTYPE_BF16, B16), torch.float32: (DTYPE_F32, F32)}      # the ABI's type, call()'s
 
 
-def _dense_rows(t: torch.Tensor | None, cols: int) -> torch.Tensor | None:
-    """[-1, cols], contiguous and 16-byte aligned; a copy only where it has to be one."""
-    if t is None:
-        return None
-    t = t.reshape(-1, cols)
-    t = t if t.is_contiguous() else t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+def _flat(t: torch.Tensor | None) -> torch.Tensor | None:
+    """Contiguous and 16-byte aligned; a copy only where it has to be one."""
+    if t is None or (t.is_contiguous() and not t.data_ptr() & 15):
+        return t
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
 
 
 def _same_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
     if not first.is_cuda:
         raise _lib.MetisHipError("metis_hip ops need a ROCm device tensor; there is no CPU path")
-    if any(t is not None and t.device != first.device for t in others):
-        raise ValueError(f"{what}: all tensors on one device")
+    device = first.device
+    for t in others:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: all tensors on one device")
 
 
 RESIDUAL_NORM_MAX_COLS = 8192
@@ -1320,11 +1321,12 @@ def residual_norm_gate_rows(x: torch.Tensor, gate: torch.Tensor | None) -> int:
 
 def _check_residual_norm(x, y, weight, post_weight, gate, y_dtype: torch.dtype) -> None:
     _same_device("residual_norm", x, y, weight, post_weight, gate)
-    if x.dim() == 0 or (y is not None and y.shape != x.shape):
-        raise ValueError(f"residual_norm: x and y have the same shape: {tuple(x.shape)} and {tuple(y.shape) if y is not None else None}")
-    if x.dtype not in _FLOATS or y_dtype not in _FLOATS or (y is not None and y.dtype != y_dtype) or (y_dtype == torch.float32 and x.dtype != torch.float32):
-        raise ValueError(f"residual_norm: bf16 or float32, x no narrower than y: {x.dtype} and {y_dtype if y is None else y.dtype}")
-    cols = x.shape[-1]
+    shape, x_dtype = x.shape, x.dtype
+    if len(shape) == 0 or (y is not None and y.shape != shape):
+        raise ValueError(f"residual_norm: x and y have the same shape: {tuple(shape)} and {tuple(y.shape) if y is not None else None}")
+    if x_dtype not in _FLOATS or y_dtype not in _FLOATS or (y is not None and y.dtype != y_dtype) or (x_dtype != y_dtype and x_dtype != torch.float32):
+        raise ValueError(f"residual_norm: bf16 or float32, x no narrower than y: {x_dtype} and {y_dtype if y is None else y.dtype}")
+    cols = shape[-1]
     if cols % 8 or not 0 < cols <= RESIDUAL_NORM_MAX_COLS:
         raise ValueError(f"residual_norm: a multiple of 8 columns up to {RESIDUAL_NORM_MAX_COLS}, not {cols}")
     for name, t in (("weight", weight), ("post_weight", post_weight)):
@@ -1341,18 +1343,17 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, post_w
     over x and y; binary32 arithmetic, each result rounded once.  x and y bf16 or float32 (x no narrower than y), up to 8192 columns; gate as in
     residual_norm_gate_rows."""
     _check_residual_norm(x, y, weight, post_weight, gate, y.dtype)
+    shape = x.shape
+    cols, rows = shape[-1], x.numel() // shape[-1]
+    (xt, xs), (yt, ys) = _FLOATS[x.dtype], _FLOATS[y.dtype]
     gate_rows = residual_norm_gate_rows(x, gate)
-    cols = x.shape[-1]
-    x2, y2, w, p, g = (_dense_rows(t, cols) for t in (x, y, weight, post_weight, gate))
-    rows = x2.shape[0]
     if rows == 0:
         return torch.empty_like(x), torch.empty_like(y)
-    (xt, xs), (yt, ys) = _FLOATS[x.dtype], _FLOATS[y.dtype]
-    new = _lib.call("metis_residual_norm", x.device.index, ((xs, *x.shape), (ys, *x.shape)),
-                    (x2, xt, y2, yt, w, p, g, gate_rows, float(scale), float(eps), rows, cols, "0", "1", _stream()))
+    new = _lib.call("metis_residual_norm", x.get_device(), ((xs, *shape), (ys, *shape)),
+                    (_flat(x), xt, _flat(y), yt, _flat(weight), _flat(post_weight), _flat(gate), gate_rows, scale, eps, rows, cols, "0", "1", _stream()))
     if new.__class__ is int:
-        check(new, "metis_residual_norm", x.shape)
-    return new[0], new[1]
+        check(new, "metis_residual_norm", shape)
+    return new
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1366,42 +1367,59 @@ def residual_norm_backward(h: torch.Tensor, y: torch.Tensor | None, weight: torc
                            want: tuple[bool, bool, bool, bool, bool] = (True,) * 5):
     """Gradients of residual_norm's x, y, weight, post_weight and gate (None for those that `want` leaves out or that are not there) for those of h and
     n, either of which may be None.  h is the forward's result; y may be None where neither a post_weight nor the gate's gradient asks for it."""
-    cols = h.shape[-1]
     _check_residual_norm(h, y, weight, post_weight, gate, y_dtype)
+    shape = h.shape
     for name, t, dtype in (("grad_h", grad_h, h.dtype), ("grad_n", grad_n, y_dtype)):
-        if t is not None and (t.shape != h.shape or t.dtype != dtype or t.device != h.device):
-            raise ValueError(f"residual_norm_backward: {name} is {tuple(h.shape)} of {dtype}, not {tuple(t.shape)} of {t.dtype}")
-    if y is None and (post_weight is not None or (gate is not None and want[4])):
+        if t is not None and (t.shape != shape or t.dtype != dtype or t.device != h.device):
+            raise ValueError(f"residual_norm_backward: {name} is {tuple(shape)} of {dtype}, not {tuple(t.shape)} of {t.dtype}")
+    want_x, want_y, want_w, want_p, want_g = want
+    want_p, want_g = want_p and post_weight is not None, want_g and gate is not None
+    if post_weight is None and not want_g:
+        y = None
+    elif y is None:
         raise ValueError("residual_norm_backward: a post_weight and the gate's gradient need y")
-    gate_rows = residual_norm_gate_rows(h, gate)
-    want_x, want_y, want_w = want[:3]
-    want_p, want_g = want[3] and post_weight is not None, want[4] and gate is not None
+    cols, gate_rows = shape[-1], residual_norm_gate_rows(h, gate)
+    rows = h.numel() // cols
     same = post_weight is None and gate is None and scale == 1.0 and h.dtype == y_dtype          # the gradient of y is that of x
-    if h.numel() == 0:
+    if rows == 0:
         zero = [None if not w or t is None else torch.zeros_like(t) for w, t in ((want_w, weight), (want_p, post_weight), (want_g, gate))]
-        return (torch.zeros_like(h) if want_x else None, torch.zeros(h.shape, dtype=y_dtype, device=h.device) if want_y else None, *zero)
-    h2, y2, w, p, g, gh, gn = (_dense_rows(t, cols) for t in (h, y if post_weight is not None or want_g else None, weight, post_weight, gate, grad_h, grad_n))
-    rows = h2.shape[0]
+        return (torch.zeros_like(h) if want_x else None, torch.zeros(shape, dtype=y_dtype, device=h.device) if want_y else None, *zero)
     (xt, xs), (yt, ys) = _FLOATS[h.dtype], _FLOATS[y_dtype]
-    need = _residual_norm_backward_bytes(rows, cols, gate_rows, h.device.index)
-    specs, place = [(U8, need)], {}
-    for key, wanted, spec in (("x", want_x or (same and want_y), (xs, *h.shape)), ("y", want_y and not same, (ys, *h.shape)), ("w", want_w, (ys, cols)),
-                              ("p", want_p, (ys, cols)), ("g", want_g, (ys, *(gate.shape if gate is not None else ())))):
-        if wanted:
-            place[key] = str(len(specs))
-            specs.append(spec)
-    new = _lib.call("metis_residual_norm_backward", h.device.index, tuple(specs),
-                    (h2, xt, y2, yt, w, p, g, gate_rows, float(scale), float(eps), rows, cols, gh, gn, *(place.get(k) for k in "xywpg"), "0", need, _stream()))
+    need = _residual_norm_backward_bytes(rows, cols, gate_rows, h.get_device())
+    # the workspace, then whatever is wanted: each one's place among the new tensors as the call names it
+    specs, gx, gy, gw, gp, gg = [(U8, need)], None, None, None, None, None
+    if want_x or (same and want_y):
+        gx = "1"
+        specs.append((xs, *shape))
+    if want_y and not same:
+        gy = str(len(specs))
+        specs.append((ys, *shape))
+    if want_w:
+        gw = str(len(specs))
+        specs.append((ys, cols))
+    if want_p:
+        gp = str(len(specs))
+        specs.append((ys, cols))
+    if want_g:
+        gg = str(len(specs))
+        specs.append((ys, *gate.shape))
+    new = _lib.call("metis_residual_norm_backward", h.get_device(), tuple(specs),
+                    (_flat(h), xt, _flat(y), yt, _flat(weight), _flat(post_weight), _flat(gate), gate_rows, scale, eps, rows, cols, _flat(grad_h), _flat(grad_n),
+                     gx, gy, gw, gp, gg, "0", need, _stream()))
     if new.__class__ is int:
-        check(new, "metis_residual_norm_backward", h.shape)
-    got = {k: new[int(v)] for k, v in place.items()}
-    return (got.get("x") if want_x else None, (got["x"] if same else got["y"]) if want_y else None, got.get("w"), got.get("p"), got.get("g"))
+        check(new, "metis_residual_norm_backward", shape)
+    return (new[1] if want_x else None, (new[1] if same else new[int(gy)]) if want_y else None, None if gw is None else new[int(gw)],
+            None if gp is None else new[int(gp)], None if gg is None else new[int(gg)])
 
 
-def _swiglu_rows(t: torch.Tensor) -> torch.Tensor:
-    """[-1, cols] with dense rows of any stride (halves of one product's rows are taken as they are)."""
-    t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 and (t.shape[0] < 2 or t.stride(0) >= t.shape[1]) else t.contiguous()
+def _swiglu_rows(t: torch.Tensor, rows: int, cols: int) -> tuple[torch.Tensor, int]:
+    """The tensor with dense rows of any stride, and that stride (halves of one product's rows are taken as they are)."""
+    if t.is_contiguous():
+        return t, cols
+    t = t.reshape(rows, cols)
+    if t.stride(1) != 1 or (rows > 1 and t.stride(0) < cols):
+        t = t.contiguous()
+    return t, max(t.stride(0), cols)
 
 
 def _check_swiglu(gate: torch.Tensor, up: torch.Tensor) -> None:
@@ -1414,13 +1432,15 @@ def _check_swiglu(gate: torch.Tensor, up: torch.Tensor) -> None:
 def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     """silu(gate) * up in binary32, rounded once; bf16 or float32, rows of any stride."""
     _check_swiglu(gate, up)
-    if gate.numel() == 0:
+    shape, total = gate.shape, gate.numel()
+    if total == 0:
         return torch.empty_like(gate, memory_format=torch.contiguous_format)
-    g, u = _swiglu_rows(gate), _swiglu_rows(up)
-    dt, spec = _FLOATS[gate.dtype]
-    new = _lib.call("metis_swiglu", gate.device.index, ((spec, *gate.shape),), (g, g.stride(0), u, u.stride(0), g.shape[0], g.shape[1], dt, "0", _stream()))
+    cols, (dt, spec) = shape[-1], _FLOATS[gate.dtype]
+    rows = total // cols
+    (g, ldg), (u, ldu) = _swiglu_rows(gate, rows, cols), _swiglu_rows(up, rows, cols)
+    new = _lib.call("metis_swiglu", gate.get_device(), ((spec, *shape),), (g, ldg, u, ldu, rows, cols, dt, "0", _stream()))
     if new.__class__ is int:
-        check(new, "metis_swiglu", gate.shape)
+        check(new, "metis_swiglu", shape)
     return new[0]
 
 
@@ -1428,17 +1448,19 @@ def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 def swiglu_backward(gate: torch.Tensor, up: torch.Tensor, grad: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Gradients of gate and up for the gradient of swiglu(gate, up): one pass."""
     _check_swiglu(gate, up)
-    if grad.shape != gate.shape or grad.dtype != gate.dtype or grad.device != gate.device:
-        raise ValueError(f"swiglu_backward: the gradient is {tuple(gate.shape)} of {gate.dtype}, not {tuple(grad.shape)} of {grad.dtype}")
-    if gate.numel() == 0:
+    shape, total = gate.shape, gate.numel()
+    if grad.shape != shape or grad.dtype != gate.dtype or grad.device != gate.device:
+        raise ValueError(f"swiglu_backward: the gradient is {tuple(shape)} of {gate.dtype}, not {tuple(grad.shape)} of {grad.dtype}")
+    if total == 0:
         return torch.zeros_like(gate), torch.zeros_like(up)
-    g, u, a = _swiglu_rows(gate), _swiglu_rows(up), grad.reshape(-1, gate.shape[-1]).contiguous()
-    dt, spec = _FLOATS[gate.dtype]
-    new = _lib.call("metis_swiglu_backward", gate.device.index, ((spec, *gate.shape), (spec, *gate.shape)),
-                    (g, g.stride(0), u, u.stride(0), a, g.shape[0], g.shape[1], dt, "0", "1", _stream()))
+    cols, (dt, spec) = shape[-1], _FLOATS[gate.dtype]
+    rows = total // cols
+    (g, ldg), (u, ldu) = _swiglu_rows(gate, rows, cols), _swiglu_rows(up, rows, cols)
+    new = _lib.call("metis_swiglu_backward", gate.get_device(), ((spec, *shape), (spec, *shape)),
+                    (g, ldg, u, ldu, grad.contiguous(), rows, cols, dt, "0", "1", _stream()))
     if new.__class__ is int:
-        check(new, "metis_swiglu_backward", gate.shape)
-    return new[0], new[1]
+        check(new, "metis_swiglu_backward", shape)
+    return new
 
 
 @functools.lru_cache(maxsize=4096)
