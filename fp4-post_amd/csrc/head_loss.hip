@@ -345,23 +345,25 @@ __device__ __forceinline__ void hl_stats_tile(uint8_t* hl_lds, const Tokens& tk,
         const int row = (wm * TM + i) * 32 + lr, m = m0 + row;
         float top = -INFINITY, sum = 0.0f, ent = 0.0f;
         if (there > 0) {
+            if (there < 64) {                                  // columns that do not exist
+#pragma unroll
+                for (int j = 0; j < HL_TN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (j * 32 + 8 * (e >> 2) + 4 * hi + (e & 3) >= there) acc[i][j][e] = -INFINITY;
+            }
+#pragma unroll
+            for (int j = 0; j < HL_TN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, acc[i][j][e]);
+            top = fmaxf(top, __shfl_xor(top, 32, 64)) * tk.scale2;
 #pragma unroll
             for (int j = 0; j < HL_TN; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    float v = acc[i][j][e] * tk.scale2;
-                    if (there < 64 && j * 32 + 8 * (e >> 2) + 4 * hi + (e & 3) >= there) v = -INFINITY;
-                    acc[i][j][e] = v;
-                    top = fmaxf(top, v);
-                }
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-#pragma unroll
-            for (int j = 0; j < HL_TN; ++j)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float d = acc[i][j][e] - top, p = __builtin_amdgcn_exp2f(d);
+                    const float d = fmaf(acc[i][j][e], tk.scale2, -top), p = __builtin_amdgcn_exp2f(d);
                     sum += p;
-                    if constexpr (ENT) ent = there < 64 && j * 32 + 8 * (e >> 2) + 4 * hi + (e & 3) >= there ? ent : fmaf(p, d, ent);
+                    if constexpr (ENT) ent = fmaf(p, there < 64 ? fmaxf(d, -1e30f) : d, ent);      // (0 * -infinity of a column that does not exist)
                 }
             sum += __shfl_xor(sum, 32, 64);
             if constexpr (ENT) ent += __shfl_xor(ent, 32, 64);
@@ -372,7 +374,7 @@ __device__ __forceinline__ void hl_stats_tile(uint8_t* hl_lds, const Tokens& tk,
                 for (int j = 0; j < HL_TN; ++j)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (want == j * 32 + 8 * (e >> 2) + 4 * hi + (e & 3)) hit[m] = acc[i][j][e];
+                        if (want == j * 32 + 8 * (e >> 2) + 4 * hi + (e & 3)) hit[m] = acc[i][j][e] * tk.scale2;
             }
         }
         if (hi == 0) {
@@ -573,16 +575,37 @@ __device__ __forceinline__ void hl_dlogits_tile(uint8_t* hl_lds, const Tokens& t
             const int64_t w = tk.targets[t] - (v0 + n0 + wn * 64);
             want = w >= 0 && w < 64 ? (int)w : -1;
         }
+        // -p f everywhere, then g more at the target, then zero where nothing is: the last two in few tiles
+        const float ge2 = ge * kLn2;
+        if (rg.g_entropy) {
+            g = fmaf(ge, h, g);                                // f = g + ge (d ln 2 + h)
 #pragma unroll
-        for (int j = 0; j < HL_TN; ++j)
+            for (int j = 0; j < HL_TN; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int n = j * 32 + 8 * (e >> 2) + 4 * hi + (e & 3);
-                const float d = acc[i][j][e] * tk.scale2 - lse2, p = __builtin_amdgcn_exp2f(d);
-                const float f = rg.g_entropy ? fmaf(ge, fmaf(d, kLn2, h), g) : g;
-                const float v = n == want ? fmaf(-p, f, g) : -p * f;
-                acc[i][j][e] = on && n < there ? v : 0.0f;
-            }
+                for (int e = 0; e < 16; ++e) {
+                    const float d = fmaf(acc[i][j][e], tk.scale2, -lse2);
+                    acc[i][j][e] = -__builtin_amdgcn_exp2f(d) * fmaf(ge2, d, g);
+                }
+            g = on && rg.g_logp ? rg.g_logp[live[m]] * inv_t : 0.0f;
+        } else {
+#pragma unroll
+            for (int j = 0; j < HL_TN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = -__builtin_amdgcn_exp2f(fmaf(acc[i][j][e], tk.scale2, -lse2)) * g;
+        }
+        if (__any(want >= 0)) {
+#pragma unroll
+            for (int j = 0; j < HL_TN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] += j * 32 + 8 * (e >> 2) + 4 * hi + (e & 3) == want ? g : 0.0f;
+        }
+        if (__any(!on) || there < 64) {
+#pragma unroll
+            for (int j = 0; j < HL_TN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!on || j * 32 + 8 * (e >> 2) + 4 * hi + (e & 3) >= there) acc[i][j][e] = 0.0f;
+        }
     }
     hl_store_bf16<TM>(acc, hl_lds, dl + (int64_t)(n0 / 64 + wn) * panel + m0 * 64, 64, BM, 64);
 }
