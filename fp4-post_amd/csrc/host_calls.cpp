@@ -26,6 +26,7 @@
 #include <vector>
 
 #include "../../include/metis_hip.h"
+#include "host_autograd.h"
 
 namespace {
 
@@ -290,6 +291,10 @@ PyObject* call(PyObject*, PyObject* const* a, Py_ssize_t n)
 
 PyMethodDef methods[] = {{"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&call)), METH_FASTCALL,
                           "call(name, device_index, specs, args): allocate, call an entry point, return the new tensors or its return code"},
+                         {"recorded_residual_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&metis_recorded_residual_norm)), METH_FASTCALL,
+                          "recorded_residual_norm(x, y, weight, post_weight, gate, gate_rows, scale, eps): residual_norm of checked arguments as a node of autograd"},
+                         {"recorded_swiglu", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&metis_recorded_swiglu)), METH_FASTCALL,
+                          "recorded_swiglu(gate, up): swiglu of checked arguments as a node of autograd"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_metis_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

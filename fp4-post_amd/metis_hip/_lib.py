@@ -173,12 +173,23 @@ def call(name: str, device_index: int, specs: tuple, args: tuple):
     """One entry point of the library with new tensors as outputs and scratch (csrc/host_calls.cpp): the tensors, or the return code if it
     is not OK.  Replaced by the compiled function on first use; raises MetisHipError if it has not been built."""
     global call
-    load()
-    if not os.path.exists(HOST_PATH):
-        raise MetisHipError(f"{HOST_PATH} not found: build it with `make -C fp4-post_amd/csrc` (or __graft_entry__.build()); there is no fallback path")
-    from . import _metis_host
-    call = _metis_host.call
+    call = host().call
     return call(name, device_index, specs, args)
+
+
+_host = None
+
+
+def host():
+    """Python's compiled way into the library (csrc/host_calls.cpp, csrc/host_autograd.cpp); raises MetisHipError if it has not been built."""
+    global _host
+    if _host is None:
+        load()
+        if not os.path.exists(HOST_PATH):
+            raise MetisHipError(f"{HOST_PATH} not found: build it with `make -C fp4-post_amd/csrc` (or __graft_entry__.build()); there is no fallback path")
+        from . import _metis_host
+        _host = _metis_host
+    return _host
 
 
 def check(rc: int, what: str, shape=None):

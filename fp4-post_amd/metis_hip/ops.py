@@ -1448,9 +1448,10 @@ def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 def swiglu_backward(gate: torch.Tensor, up: torch.Tensor, grad: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Gradients of gate and up for the gradient of swiglu(gate, up): one pass."""
     _check_swiglu(gate, up)
-    shape, total = gate.shape, gate.numel()
+    shape = gate.shape
     if grad.shape != shape or grad.dtype != gate.dtype or grad.device != gate.device:
         raise ValueError(f"swiglu_backward: the gradient is {tuple(shape)} of {gate.dtype}, not {tuple(grad.shape)} of {grad.dtype}")
+    total = gate.numel()
     if total == 0:
         return torch.zeros_like(gate), torch.zeros_like(up)
     cols, (dt, spec) = shape[-1], _FLOATS[gate.dtype]

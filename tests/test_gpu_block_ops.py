@@ -283,8 +283,10 @@ def test_swiglu_far_values_and_shapes():
         near(a[live], want[live], dtype, want[live].abs() * (1 + g[live].double().abs()))
         dg, du = __import__("metis_hip").ops.swiglu_backward(g.to(dtype), u, torch.ones_like(u))
         assert bool(dg[live].isfinite().all()) and bool(du[live].isfinite().all())
-    e = torch.zeros(0, 5, dtype=BF, device="cuda")
-    assert swiglu(e, e).shape == (0, 5)
+    for shape in ((0, 5), (3, 0)):
+        e = torch.zeros(shape, dtype=BF, device="cuda", requires_grad=True)
+        a = swiglu(e, e)
+        assert a.shape == shape and torch.autograd.grad(a.sum(), e)[0].shape == shape
 
 
 def _replayed(make_outputs, inputs, change):
@@ -334,3 +336,30 @@ def test_other_streams():
     torch.cuda.synchronize()
     for run in got:
         assert all(torch.equal(a, b) for a, b in zip(run, want))
+
+
+def test_a_second_derivative_is_refused():
+    from metis_hip import residual_norm, swiglu, token_logprobs
+    x, y, w, p, g, gh, gn = make(17, (4, 64), BF, BF, True, None)
+    hidden, head, t = torch.randn(4, 64, device="cuda").to(BF), torch.randn(40, 64, device="cuda").to(BF), torch.arange(4, device="cuda")
+    for leaf, run in ((x, lambda v: residual_norm(v, y, w, post_weight=p)[1].float().square().sum()), (x, lambda v: swiglu(v, y).float().square().sum()),
+                      (hidden, lambda v: token_logprobs(v, head, t).square().sum())):
+        leaf = leaf.clone().requires_grad_()
+        plain, = torch.autograd.grad(run(leaf), leaf)
+        first, = torch.autograd.grad(run(leaf), leaf, create_graph=True)
+        assert torch.equal(first, plain)
+        with pytest.raises(RuntimeError, match="twice"):
+            first.float().sum().backward()
+
+
+def test_backward_into_leaves_and_hooks():
+    """.backward() accumulates, twice; the two equal gradients of a plain sum are tensors of their own in .grad."""
+    from metis_hip import residual_norm
+    x, y, w, _, _, gh, gn = make(18, (5, 128), BF, BF, False, None)
+    x, y, w = (t.requires_grad_() for t in (x, y, w))
+    seen = []
+    x.register_hook(lambda g: seen.append(g.clone()))
+    for k in (1, 2):
+        h, n = residual_norm(x, y, w)
+        torch.autograd.backward((h, n), (gh, gn))
+    assert torch.equal(x.grad, y.grad) and x.grad.data_ptr() != y.grad.data_ptr() and torch.equal(seen[0] + seen[1], x.grad)
