@@ -7,6 +7,7 @@ result rounded once; their autograd nodes are compiled (csrc/host_autograd.cpp).
 from __future__ import annotations
 
 import torch
+from torch import nn
 
 from . import _lib, ops
 
@@ -39,3 +40,36 @@ def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
         ops._check_swiglu(gate, up)
         return _lib.host().recorded_swiglu(gate, up)
     return ops.swiglu(gate, up)
+
+
+class GatedMLP(nn.Module):
+    """A gated MLP with SiLU on its own projections: down_proj(swiglu(gate_proj(x), up_proj(x))).  The projections keep their names, so the
+    parameters do too."""
+
+    def __init__(self, gate_proj: nn.Module, up_proj: nn.Module, down_proj: nn.Module):
+        super().__init__()
+        self.gate_proj, self.up_proj, self.down_proj = gate_proj, up_proj, down_proj
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        gate, up = self.gate_proj(x), self.up_proj(x)
+        if gate.is_cuda and gate.dtype == up.dtype and gate.dtype in ops._FLOATS:
+            return self.down_proj(swiglu(gate, up))
+        return self.down_proj(nn.functional.silu(gate) * up)
+
+
+def fuse_gated_mlps(model: nn.Module) -> int:
+    """Replace every MLP that holds gate_proj, up_proj and down_proj around a SiLU (`act_fn`), and nothing else with parameters, by GatedMLP on
+    the same projections.  Returns the number replaced."""
+    replaced = 0
+    for parent in list(model.modules()):
+        for name, mlp in list(parent.named_children()):
+            parts = dict(mlp.named_children())
+            act = getattr(mlp, "act_fn", None)
+            silu = isinstance(act, nn.SiLU) or act is nn.functional.silu or type(act).__name__ == "SiLUActivation"
+            if isinstance(mlp, GatedMLP) or not silu or not {"gate_proj", "up_proj", "down_proj"} <= parts.keys() <= {"gate_proj", "up_proj", "down_proj", "act_fn"}:
+                continue
+            fused = GatedMLP(parts["gate_proj"], parts["up_proj"], parts["down_proj"])
+            fused.train(mlp.training)
+            setattr(parent, name, fused)
+            replaced += 1
+    return replaced

@@ -59,3 +59,25 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     if reduction == "none":
         return loss
     return loss.sum() if reduction == "sum" else loss.sum() / (targets != ignore_index).sum()
+
+
+def model_token_logprobs(model, input_ids: torch.Tensor, attention_mask: torch.Tensor | None = None, labels: torch.Tensor | None = None, *,
+                         temperature: float = 1.0, ignore_index: int = -100, entropy: bool = False, **inputs):
+    """token_logprobs of a causal language model's next tokens, [B, S - 1] for input_ids [B, S], without its logits: the model's decoder
+    (`base_model`) gives the last hidden states, its output embedding's weight is the head.  What a DPO or GRPO step takes of the policy and of the
+    reference model.
+
+    labels defaults to input_ids; positions with ignore_index, or that attention_mask leaves out, have 0 and no gradient (and are not
+    computed).  inputs: further arguments of the decoder."""
+    head = model.get_output_embeddings()
+    if getattr(head, "bias", None) is not None:
+        raise ValueError("model_token_logprobs: a head without bias")
+    cap = getattr(getattr(model, "config", None), "final_logit_softcapping", None)
+    if cap:
+        raise ValueError("model_token_logprobs: a head whose logits are used as they are, not capped")
+    out = model.base_model(input_ids=input_ids, attention_mask=attention_mask, **inputs)
+    hidden = out[0] if isinstance(out, tuple) else out.last_hidden_state
+    targets = (input_ids if labels is None else labels)[:, 1:]
+    if attention_mask is not None:
+        targets = targets.masked_fill(attention_mask[:, 1:] == 0, ignore_index)
+    return token_logprobs(hidden[:, :-1], head.weight, targets, temperature=temperature, ignore_index=ignore_index, entropy=entropy)

@@ -17,6 +17,7 @@ from torch import nn
 
 from . import ops
 from ._lib import MODE_P32, MODE_PB16
+from .block import residual_norm
 from .ops import CenteredNVFP4
 from .bitlinear import BitLinear, LinearLowbitFunction, _param, _version_of
 from .quant import is_hip_nvfp4
@@ -106,7 +107,20 @@ class FusedRMSNormQuant(nn.Module):
         packed = CenteredNVFP4(F.q_forward_input.pack(normed, arith=cd, center=me, **more), me, me32)
         return normed, packed
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def _behind(self, y: torch.Tensor, residual: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """(h, n): the residual stream behind a block whose output is y, and its norm, from one kernel.  The group packs n as it would any input."""
+        weight, cols = _param(self, "weight"), y.shape[-1]
+        if (y.is_cuda and residual.device == y.device and residual.shape == y.shape and weight.dtype == y.dtype and y.dtype in ops._FLOATS
+                and residual.dtype in (y.dtype, torch.float32) and cols % 8 == 0 and 0 < cols <= ops.RESIDUAL_NORM_MAX_COLS):
+            return residual_norm(residual, y, weight, eps=self.variance_epsilon)
+        h = residual + y
+        return h, self._plain(h)
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+        """The norm of x; with the residual stream of a block whose output is x the pair (residual + x, its norm), see residual_norm (whose norm
+        is rounded once, where this module's rounds x * rstd first as the reference's does)."""
+        if residual is not None:
+            return self._behind(x, residual)
         F = LinearLowbitFunction
         cols = x.shape[-1]
         weight = _param(self, "weight")

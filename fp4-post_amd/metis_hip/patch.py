@@ -103,9 +103,10 @@ def replace_linear_with_metis(model, dtype, metis_args, target_modules=None, com
     return model
 
 
-def replace_model_with_metis(model, metis_args=None, fuse_norms: bool = False):
+def replace_model_with_metis(model, metis_args=None, fuse_norms: bool = False, fuse_mlps: bool = False):
     """bf16 storage and compute, default targets (reference grpo.py:199-215).  fuse_norms additionally
-    replaces the RMSNorm in front of every q/k/v and gate/up group by the fused norm+quant module."""
+    replaces the RMSNorm in front of every q/k/v and gate/up group by the fused norm+quant module, fuse_mlps the
+    gated MLPs by ones whose silu(gate) * up is one kernel."""
     if metis_args is None:
         metis_args = MetisArgs()
     model = replace_linear_with_metis(model=model, dtype=torch.bfloat16, metis_args=metis_args,
@@ -113,4 +114,7 @@ def replace_model_with_metis(model, metis_args=None, fuse_norms: bool = False):
     if fuse_norms:
         from .norm import fuse_rmsnorm_into_groups
         fuse_rmsnorm_into_groups(model)
+    if fuse_mlps:
+        from .block import fuse_gated_mlps
+        fuse_gated_mlps(model)
     return model
