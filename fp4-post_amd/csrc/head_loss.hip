@@ -47,6 +47,15 @@ typedef hl_short4_t __attribute__((address_space(3))) * hl_lds_ptr_t;
 __device__ __forceinline__ int hl_swz(int q) { return ((q >> 2) & 1) | ((((q >> 1) ^ (q >> 3)) & 1) << 1); }
 template <int ROW_BYTES> __device__ __forceinline__ int hl_turn(int k) { return ROW_BYTES >= 256 ? (k & 3) << 6 : ((k >> 1) & 1) << 6; }
 
+// The thread's number, as a value of its own at each place: what follows from it is formed again for every tile and not kept in registers across its products
+// (kept, the kernels that go through several tiles need more than there are).
+__device__ __forceinline__ int hl_thread()
+{
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
 struct Operand {
     const uint16_t* base;        // first element of the tile's rows (plain) or of the first k's row (turned)
     int64_t ld;                  // elements between rows (plain) or between k (turned)
@@ -56,181 +65,194 @@ struct Operand {
     int64_t panel;               // A in panels: elements between panels of 64 columns of the stored matrix, whose rows are then 64 long (ld 64)
 };
 
-// Stages [0, steps) of 32 along the contraction; half: only the first sixteen k of the last one count.  Where fewer count otherwise, one operand holds zeros
-// beyond them.  PANELS: A is stored in panels.
-template <int TM, bool AT, bool BT, bool PANELS>
-__device__ __forceinline__ void hl_main_loop(float16_t (&acc)[TM][HL_TN], uint8_t* lds, const Operand& a, const Operand& b, int steps, bool half)
-{
-    constexpr int BM = 64 * TM, NA = BM / 16, TOTAL = NA + HL_BN / 16, LPW = (TOTAL + 7) / 8, STAGE = hl_stage_bytes(TM), NS = HL_NS, B_AT = NA * 1024;
-    constexpr int A_RB = BM * 2, B_RB = HL_BN * 2;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave >> 2, wn = wave & 3;
+// One wave's view of it.  aim() at a tile: stages [0, steps) along the contraction; half: only the first sixteen k of the last one count.  Where fewer
+// count otherwise, one operand holds zeros beyond them.  PANELS: A is stored in panels.  Then request(0), request(2) and multiply(): the first pair of stages
+// goes to slots 0 and 1, the second to 2 and 3, so that the next tile's first pair can be under way while this one's results leave through the
+// rest of the ring.
+template <int TM, bool AT, bool BT, bool PANELS> struct Pipe {
+    static constexpr int BM = 64 * TM, NA = BM / 16, TOTAL = NA + HL_BN / 16, LPW = (TOTAL + 7) / 8, STAGE = hl_stage_bytes(TM), NS = HL_NS, B_AT = NA * 1024;
+    static constexpr int A_RB = BM * 2, B_RB = HL_BN * 2;
+    uint8_t* lds;
+    const uint8_t* src[LPW];     // this wave's load instructions of a stage: where the lane reads next,
+    int64_t inc[LPW], inc_odd[LPW];   // how far it goes behind even and odd stages (64 bytes where both operands are plain),
+    uint32_t back[LPW];          // and how far back in the last one
+    int steps;
+    bool half;
 
-    // ---- this wave's load instructions of a stage: where its lanes read in the first one, how far they go per stage, and back in the last
-    const uint8_t* src[LPW];
-    int64_t inc[LPW], inc_odd[LPW];                            // behind even and odd stages (64 where both operands are plain)
-    uint32_t back[LPW];
-    int place[LPW];
+    __device__ __forceinline__ void aim(const Operand& a, const Operand& b, int count, bool half_last)
+    {
+        const int thread = hl_thread(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
+        steps = count;
+        half = half_last;
 #pragma unroll
-    for (int j = 0; j < LPW; ++j) {
-        int ot = j * 8 + wave;
-        if (ot >= TOTAL) ot -= 8;                              // (a piece that another wave loads too: the same bytes to the same place)
-        place[j] = ot * 1024;
-        const bool is_a = ot < NA;
-        const Operand& o = is_a ? a : b;
-        const int q = is_a ? ot : ot - NA;
-        if (is_a ? AT : BT) {
-            const int rb = is_a ? A_RB : B_RB, k = q * (1024 / rb) + lane * 16 / rb, at = lane * 16 % rb;
-            int col = (at ^ (is_a ? hl_turn<A_RB>(k) : hl_turn<B_RB>(k))) >> 1;
-            if (col >= o.limit) col = 0;                       // (columns in eights: all there or none)
-            src[j] = reinterpret_cast<const uint8_t*>(o.base + (int64_t)k * o.ld + (PANELS && is_a ? (col >> 6) * o.panel + (col & 63) : col));
-            inc[j] = inc_odd[j] = o.ld * 64;
-            back[j] = k >= o.rest ? (uint32_t)((k - (o.rest - 1)) * (o.ld * 2)) : 0u;
-        } else {
-            const int row = q * 16 + (lane >> 2), chunk = (lane & 3) ^ hl_swz(row & 15);
-            int r = row < o.limit ? row : o.limit - 1;
-            const int64_t at = o.index ? o.index[r] : r;
-            src[j] = reinterpret_cast<const uint8_t*>(o.base + at * o.ld + chunk * 8);
-            inc[j] = 64;
-            inc_odd[j] = PANELS && is_a ? o.panel * 2 - 64 : 64;
-            back[j] = chunk * 8 >= o.rest ? 32u : 0u;
+        for (int j = 0; j < LPW; ++j) {
+            int ot = j * 8 + wave;
+            if (ot >= TOTAL) ot -= 8;                              // (a piece that another wave loads too: the same bytes to the same place)
+            const bool is_a = ot < NA;
+            const Operand& o = is_a ? a : b;
+            const int q = is_a ? ot : ot - NA;
+            if (is_a ? AT : BT) {
+                const int rb = is_a ? A_RB : B_RB, k = q * (1024 / rb) + lane * 16 / rb, at = lane * 16 % rb;
+                int col = (at ^ (is_a ? hl_turn<A_RB>(k) : hl_turn<B_RB>(k))) >> 1;
+                if (col >= o.limit) col = 0;                       // (columns in eights: all there or none)
+                src[j] = reinterpret_cast<const uint8_t*>(o.base + (int64_t)k * o.ld + (PANELS && is_a ? (col >> 6) * o.panel + (col & 63) : col));
+                inc[j] = inc_odd[j] = o.ld * 64;
+                back[j] = k >= o.rest ? (uint32_t)((k - (o.rest - 1)) * (o.ld * 2)) : 0u;
+            } else {
+                const int row = q * 16 + (lane >> 2), chunk = (lane & 3) ^ hl_swz(row & 15);
+                int r = row < o.limit ? row : o.limit - 1;
+                const int64_t at = o.index ? o.index[r] : r;
+                src[j] = reinterpret_cast<const uint8_t*>(o.base + at * o.ld + chunk * 8);
+                inc[j] = 64;
+                inc_odd[j] = PANELS && is_a ? o.panel * 2 - 64 : 64;
+                back[j] = chunk * 8 >= o.rest ? 32u : 0u;
+            }
         }
     }
-    auto issue_one = [&](int slot, int j, bool odd, bool last) {
+    __device__ __forceinline__ void issue_one(int slot, int j, bool odd, bool last)
+    {
         const uint8_t* g = src[j] - (last ? back[j] : 0u);
-        const uint32_t dst = (uint32_t)(slot * STAGE + place[j]);
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), at = j * 8 + wave, ot = at < TOTAL ? at : at - 8;
+        const uint32_t dst = __builtin_amdgcn_readfirstlane((uint32_t)(slot * STAGE + ot * 1024));
         asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(g), "s"(dst) : "memory");
         if constexpr (!AT && !BT && !PANELS) src[j] += 64;
         else if constexpr (!AT && PANELS) src[j] += odd ? inc_odd[j] : inc[j];
         else src[j] += inc[j];
-    };
-
-    // ---- fragments: lane -> row l % 32 of a 32-row tile, k 8 (l / 32) .. + 7 of a half stage
-    const int lr = lane & 31, hi = lane >> 5;
-    const int plain = (lr >> 4) * 1024 + (lr & 15) * 64 + ((hi ^ hl_swz(lr & 15)) * 16);
-    int a_off[AT ? TM : 2], b_off[BT ? HL_TN : 2];
-    const int tk = 8 * hi + ((lane & 15) >> 2), tc = ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
-    if constexpr (AT) {
-#pragma unroll
-        for (int i = 0; i < TM; ++i) a_off[i] = tk * A_RB + (((wm * TM + i) * 64) ^ hl_turn<A_RB>(tk)) + tc;
-    } else {
-        a_off[0] = wm * TM * 2048 + plain;
-        a_off[1] = wm * TM * 2048 + (plain ^ 32);
     }
-    if constexpr (BT) {
-#pragma unroll
-        for (int j = 0; j < HL_TN; ++j) b_off[j] = B_AT + tk * B_RB + (((wn * HL_TN + j) * 64) ^ hl_turn<B_RB>(tk)) + tc;
-    } else {
-        b_off[0] = B_AT + wn * HL_TN * 2048 + plain;
-        b_off[1] = B_AT + wn * HL_TN * 2048 + (plain ^ 32);
-    }
-    uint4 fa[2][TM], fb[2][HL_TN];
-    auto turned = [&](const uint8_t* p, int rb) -> uint4 {
-        const hl_short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((hl_lds_ptr_t)p);
-        const hl_short4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((hl_lds_ptr_t)(p + 4 * rb));
-        const hl_short8_t v = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
-        return __builtin_bit_cast(uint4, v);
-    };
-    auto load_frags = [&](int slot, int ks) {
-        const uint8_t* x = lds + slot * STAGE;
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            if constexpr (AT) fa[ks][i] = turned(x + a_off[i] + ks * 16 * A_RB, A_RB);
-            else fa[ks][i] = *reinterpret_cast<const uint4*>(x + a_off[ks] + i * 2048);
-        }
-#pragma unroll
-        for (int j = 0; j < HL_TN; ++j) {
-            if constexpr (BT) fb[ks][j] = turned(x + b_off[j] + ks * 16 * B_RB, B_RB);
-            else fb[ks][j] = *reinterpret_cast<const uint4*>(x + b_off[ks] + j * 2048);
-        }
-    };
-    auto mfma_one = [&](int ks, int i, int j) {
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, fb[ks][j]), __builtin_bit_cast(bf16x8_t, fa[ks][i]), acc[i][j], 0, 0, 0);
-    };
-    auto mfmas = [&](int ks) {
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < HL_TN; ++j) mfma_one(ks, i, j);
-    };
-    constexpr int NM = TM * HL_TN, NF = TM * (AT ? 2 : 1) + HL_TN * (BT ? 2 : 1);
-
-    if (steps <= 0) return;
     // Two stages are requested together, piece by piece: a plain operand's two pieces are the halves of the same 128-byte lines.
-    auto issue_pair = [&](int slot0, int slot1, int j, int stage0) {
+    __device__ __forceinline__ void issue_pair(int slot0, int slot1, int j, int stage0)
+    {
         if (stage0 < steps) issue_one(slot0, j, false, stage0 == steps - 1);
         if (stage0 + 1 < steps) issue_one(slot1, j, true, stage0 + 1 == steps - 1);
-    };
+    }
+    __device__ __forceinline__ void request(int stage0)
+    {
 #pragma unroll
-    for (int p = 0; p < 4; p += 2)
+        for (int j = 0; j < LPW; ++j) issue_pair(stage0, stage0 + 1, j, stage0);
+    }
+
+    // adds the tile's products; behind it every slot is free
+    __device__ __forceinline__ void multiply(float16_t (&acc)[TM][HL_TN])
+    {
+        if (steps <= 0) return;
+        const int thread = hl_thread(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), wm = wave >> 2, wn = wave & 3;
+        // ---- fragments: lane -> row l % 32 of a 32-row tile, k 8 (l / 32) .. + 7 of a half stage
+        const int lr = lane & 31, hi = lane >> 5;
+        const int plain = (lr >> 4) * 1024 + (lr & 15) * 64 + ((hi ^ hl_swz(lr & 15)) * 16);
+        int a_off[AT ? TM : 2], b_off[BT ? HL_TN : 2];
+        const int tk = 8 * hi + ((lane & 15) >> 2), tc = ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+        if constexpr (AT) {
 #pragma unroll
-        for (int j = 0; j < LPW; ++j) issue_pair(p, p + 1, j, p);
-    if (steps >= 4) HL_WAIT(2 * LPW + 1, 15);
-    else HL_WAIT(0, 15);
-    __syncthreads();
-    load_frags(0, 0);
-    int s = 0, slot = 0;
-    auto next_of = [](int k) { return k + 1 == NS ? 0 : k + 1; };
-    auto before = [](int k) { return k == 0 ? NS - 1 : k - 1; };
-    // Stage s in `slot`.  FIRST (s even): half of the load instructions of stages s + 4 and s + 5, into the slots before `slot` and `slot` itself, whose
-    // stages every wave has in registers behind this barrier; the iteration after it the other half, EARLY pairs of them before its own barrier: with turned
-    // operands, whose fragments take twice the reads, the queue is evener so (both products of 4096 x 3584 against 32768 columns 1.74 -> 1.70 ms; grad_hidden
-    // alone likes two early, grad_weight alone one).  At a barrier at most `most` loads are outstanding.
-    constexpr int EARLY = !BT ? 0 : AT ? 1 : 2;
-    auto iterate = [&](auto first, auto most) {
-        constexpr bool FIRST = decltype(first)::value;
-        constexpr int H0 = LPW / 2, E = FIRST ? 0 : EARLY < LPW - H0 ? EARLY : LPW - H0, J0 = FIRST ? 0 : H0 + E, COUNT = FIRST ? H0 : LPW - H0 - E;
-        const int slot1 = FIRST ? slot : before(slot), slot0 = before(slot1);
-        const bool last = (FIRST ? s + 5 : s + 4) == steps - 1;
-        auto loads = [&](int m, int from, int count) {         // between the products: instruction m of NM
+            for (int i = 0; i < TM; ++i) a_off[i] = tk * A_RB + (((wm * TM + i) * 64) ^ hl_turn<A_RB>(tk)) + tc;
+        } else {
+            a_off[0] = wm * TM * 2048 + plain;
+            a_off[1] = wm * TM * 2048 + (plain ^ 32);
+        }
+        if constexpr (BT) {
 #pragma unroll
-            for (int j = from; j < from + count; ++j)
-                if ((j - from) * NM / count == m) {
-                    issue_one(slot0, j, false, false);
-                    issue_one(slot1, j, true, last);
-                }
+            for (int j = 0; j < HL_TN; ++j) b_off[j] = B_AT + tk * B_RB + (((wn * HL_TN + j) * 64) ^ hl_turn<B_RB>(tk)) + tc;
+        } else {
+            b_off[0] = B_AT + wn * HL_TN * 2048 + plain;
+            b_off[1] = B_AT + wn * HL_TN * 2048 + (plain ^ 32);
+        }
+        uint4 fa[2][TM], fb[2][HL_TN];
+        auto turned = [&](const uint8_t* p, int rb) -> uint4 {
+            const hl_short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((hl_lds_ptr_t)p);
+            const hl_short4_t up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((hl_lds_ptr_t)(p + 4 * rb));
+            const hl_short8_t v = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
+            return __builtin_bit_cast(uint4, v);
         };
-        load_frags(slot, 1);
+        auto load_frags = [&](int slot, int ks) {
+            const uint8_t* x = lds + slot * STAGE;
 #pragma unroll
-        for (int m = 0; m < NM; ++m) {
-            if constexpr (E > 0) loads(m, H0, E);
-            mfma_one(0, m / HL_TN, m % HL_TN);
-        }
-        if constexpr (E == 0) sched_substep<NM, 0, NF, 0>();
-        HL_WAIT(decltype(most)::value, 0);                     // own loads of stage s + 1 are there, own reads of stage s done
+            for (int i = 0; i < TM; ++i) {
+                if constexpr (AT) fa[ks][i] = turned(x + a_off[i] + ks * 16 * A_RB, A_RB);
+                else fa[ks][i] = *reinterpret_cast<const uint4*>(x + a_off[ks] + i * 2048);
+            }
+#pragma unroll
+            for (int j = 0; j < HL_TN; ++j) {
+                if constexpr (BT) fb[ks][j] = turned(x + b_off[j] + ks * 16 * B_RB, B_RB);
+                else fb[ks][j] = *reinterpret_cast<const uint4*>(x + b_off[ks] + j * 2048);
+            }
+        };
+        auto mfma_one = [&](int ks, int i, int j) {
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, fb[ks][j]), __builtin_bit_cast(bf16x8_t, fa[ks][i]), acc[i][j], 0, 0, 0);
+        };
+        auto mfmas = [&](int ks) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < HL_TN; ++j) mfma_one(ks, i, j);
+        };
+        constexpr int NM = TM * HL_TN, NF = TM * (AT ? 2 : 1) + HL_TN * (BT ? 2 : 1);
+
+        if (steps >= 4) HL_WAIT(2 * LPW + 1, 15);
+        else HL_WAIT(0, 15);
         __syncthreads();
-        load_frags(next_of(slot), 0);
+        load_frags(0, 0);
+        int s = 0, slot = 0;
+        auto next_of = [](int k) { return k + 1 == NS ? 0 : k + 1; };
+        auto before = [](int k) { return k == 0 ? NS - 1 : k - 1; };
+        // Stage s in `slot`.  FIRST (s even): half of the load instructions of stages s + 4 and s + 5, into the slots before `slot` and `slot` itself, whose
+        // stages every wave has in registers behind this barrier; the iteration after it the other half, EARLY pairs of them before its own barrier: with turned
+        // operands, whose fragments take twice the reads, the queue is evener so (both products of 4096 x 3584 against 32768 columns 1.74 -> 1.70 ms; grad_hidden
+        // alone likes two early, grad_weight alone one).  At a barrier at most `most` loads are outstanding.
+        constexpr int EARLY = !BT ? 0 : AT ? 1 : 2;
+        auto iterate = [&](auto first, auto most) {
+            constexpr bool FIRST = decltype(first)::value;
+            constexpr int H0 = LPW / 2, E = FIRST ? 0 : EARLY < LPW - H0 ? EARLY : LPW - H0, J0 = FIRST ? 0 : H0 + E, COUNT = FIRST ? H0 : LPW - H0 - E;
+            const int slot1 = FIRST ? slot : before(slot), slot0 = before(slot1);
+            const bool last = (FIRST ? s + 5 : s + 4) == steps - 1;
+            auto loads = [&](int m, int from, int count) {         // between the products: instruction m of NM
 #pragma unroll
-        for (int m = 0; m < NM; ++m) {
-            if constexpr (COUNT > 0) loads(m, J0, COUNT);
-            mfma_one(1, m / HL_TN, m % HL_TN);
-        }
-        slot = next_of(slot);
-        ++s;
-    };
-    // when stage s + 1 has to be there: s even, all of its pair (all but the next pair); s odd, the even half of its pair (all but the last load of it,
-    // the first half of the next pair and what went out early)
-    constexpr int SENT = LPW / 2 + (EARLY < LPW - LPW / 2 ? EARLY : LPW - LPW / 2);
-    while (s + 5 < steps) {
-        iterate(std::true_type{}, std::integral_constant<int, 2 * LPW>{});
-        iterate(std::false_type{}, std::integral_constant<int, 2 * SENT + 1>{});
-    }
-    for (; s < steps; ++s) {
-        const bool both = s + 1 < steps || !half;
-        if (both) load_frags(slot, 1);
-        mfmas(0);
-        HL_WAIT(0, 0);
-        __syncthreads();
-        if (s + 1 < steps) load_frags(next_of(slot), 0);
-        if ((s & 1) == 0) {
+                for (int j = from; j < from + count; ++j)
+                    if ((j - from) * NM / count == m) {
+                        issue_one(slot0, j, false, false);
+                        issue_one(slot1, j, true, last);
+                    }
+            };
+            load_frags(slot, 1);
 #pragma unroll
-            for (int j = 0; j < LPW; ++j) issue_pair(before(slot), slot, j, s + 4);
+            for (int m = 0; m < NM; ++m) {
+                if constexpr (E > 0) loads(m, H0, E);
+                mfma_one(0, m / HL_TN, m % HL_TN);
+            }
+            if constexpr (E == 0) sched_substep<NM, 0, NF, 0>();
+            HL_WAIT(decltype(most)::value, 0);                     // own loads of stage s + 1 are there, own reads of stage s done
+            __syncthreads();
+            load_frags(next_of(slot), 0);
+#pragma unroll
+            for (int m = 0; m < NM; ++m) {
+                if constexpr (COUNT > 0) loads(m, J0, COUNT);
+                mfma_one(1, m / HL_TN, m % HL_TN);
+            }
+            slot = next_of(slot);
+            ++s;
+        };
+        // when stage s + 1 has to be there: s even, all of its pair (all but the next pair); s odd, the even half of its pair (all but the last load of it,
+        // the first half of the next pair and what went out early)
+        constexpr int SENT = LPW / 2 + (EARLY < LPW - LPW / 2 ? EARLY : LPW - LPW / 2);
+        while (s + 5 < steps) {
+            iterate(std::true_type{}, std::integral_constant<int, 2 * LPW>{});
+            iterate(std::false_type{}, std::integral_constant<int, 2 * SENT + 1>{});
         }
-        if (both) mfmas(1);
-        slot = next_of(slot);
+        for (; s < steps; ++s) {
+            const bool both = s + 1 < steps || !half;
+            if (both) load_frags(slot, 1);
+            mfmas(0);
+            HL_WAIT(0, 0);
+            __syncthreads();
+            if (s + 1 < steps) load_frags(next_of(slot), 0);
+            if ((s & 1) == 0) {
+#pragma unroll
+                for (int j = 0; j < LPW; ++j) issue_pair(before(slot), slot, j, s + 4);
+            }
+            if (both) mfmas(1);
+            slot = next_of(slot);
+        }
+        __syncthreads();                                           // the ring is free
     }
-    __syncthreads();                                           // the ring is free
-}
+};
 
 // acc[i][j][e] of lane l: row 32 (TM wm + i) + l % 32, column 64 wn + 32 j + 8 (e / 4) + 4 (l / 32) + e % 4 of the tile.
 // The tile as bf16, the wave's 64 columns in rows of `ld` elements from `out` on: through the wave's own part of LDS, 32 rows at a time, so that a store
@@ -239,7 +261,7 @@ template <int TM>
 __device__ __forceinline__ void hl_store_bf16(const float16_t (&acc)[TM][HL_TN], uint8_t* lds, uint16_t* out, int64_t ld, int rows, int cols)
 {
     constexpr int CROW = 72;                                   // 144 bytes
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 2, lr = lane & 31, hi = lane >> 5;
+    const int thread = hl_thread(), lane = thread & 63, wave = thread >> 6, wm = wave >> 2, lr = lane & 31, hi = lane >> 5;
     uint16_t* cw = reinterpret_cast<uint16_t*>(lds) + wave * (32 * CROW);
     const int n = (lane & 7) * 8;
 #pragma unroll
@@ -277,11 +299,11 @@ struct Tokens {
 };
 __device__ __forceinline__ const int* live_rows(const int* index) { return index + 64; }
 
-// workgroup -> tile, a contiguous range of the tiles per XCD
-__device__ __forceinline__ int hl_logical(int total)
+// the k-th tile of this workgroup's XCD, which has a contiguous range of the tiles; -1 behind it
+__device__ __forceinline__ int hl_logical(int total, int k)
 {
-    const int per = (total + 7) >> 3, logical = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    return (int)(blockIdx.x >> 3) < per && logical < total ? logical : -1;
+    const int per = (total + 7) >> 3, logical = (blockIdx.x & 7) * per + k;
+    return k < per && logical < total ? logical : -1;
 }
 // groups of up to five tile rows, as even as they come, walked column by column: 32 compute units of an XCD share the operands of a few rows and columns.
 // (Groups of up to 6, 8, 16 rows: 16 rows of tiles, all three products, 1 to 6 % slower.)
@@ -331,26 +353,16 @@ template <int TM> __device__ __forceinline__ void hl_clear(float16_t (&acc)[TM][
 // Forward: per tile and live token the maximum of its logits (in powers of two), the sum of 2^(l - maximum) and, for the entropy, of
 // 2^(l - maximum) (l - maximum); the target's logit from the tile that has it.
 // ---------------------------------------------------------------------------------------------
+// What a tile leaves, from its accumulators; `red`: LDS.
 template <int TM, bool ENT>
-__device__ __forceinline__ void hl_stats_tile(uint8_t* hl_lds, const Tokens& tk, int count, const int* live, const uint16_t* weight, int64_t ldw, int stride, float2* part, float* part_e,
-                                              float* hit)
+__device__ __forceinline__ void hl_stats_out(float16_t (&acc)[TM][HL_TN], float* red, const Tokens& tk, int count, const int* live, int m0, int tn, int stride, float2* part, float* part_e,
+                                             float* hit)
 {
     constexpr int BM = 64 * TM;
-    const int tiles_m = (count + BM - 1) / BM, tiles_n = (tk.V + HL_BN - 1) / HL_BN;
-    const int logical = hl_logical(tiles_m * tiles_n);
-    if (logical < 0) return;
-    int tm, tn;
-    hl_origin(logical, tiles_m, tiles_n, tm, tn);
-    const int m0 = tm * BM, n0 = tn * HL_BN;
-    float16_t acc[TM][HL_TN];
-    hl_clear<TM>(acc);
-    const int rest = tk.H % 32 ? 16 : 32;
-    const Operand a = {tk.hidden, tk.ld, count - m0, live + m0, rest, 0}, b = {weight + (int64_t)n0 * ldw, ldw, tk.V - n0, nullptr, rest, 0};
-    hl_main_loop<TM, false, false, false>(acc, hl_lds, a, b, (tk.H + 31) / 32, rest == 16);
-
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3, lr = lane & 31, hi = lane >> 5;
+    const int n0 = tn * HL_BN;
+    const int thread = hl_thread(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), wm = wave >> 2, wn = wave & 3, lr = lane & 31, hi = lane >> 5;
     const int there = tk.V - (n0 + wn * 64);                   // columns of this wave that exist
-    float* red = reinterpret_cast<float*>(hl_lds);             // [row][wave column][3]
+    // red: [row][wave column][3]
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         const int row = (wm * TM + i) * 32 + lr, m = m0 + row;
@@ -395,7 +407,7 @@ __device__ __forceinline__ void hl_stats_tile(uint8_t* hl_lds, const Tokens& tk,
         }
     }
     __syncthreads();
-    const int row = threadIdx.x;
+    const int row = thread;
     if (row >= BM || m0 + row >= count) return;
     float top = red[row * 12], sum = red[row * 12 + 1], ent = red[row * 12 + 2];   // (the first wave has columns that exist)
 #pragma unroll
@@ -409,6 +421,41 @@ __device__ __forceinline__ void hl_stats_tile(uint8_t* hl_lds, const Tokens& tk,
     }
     part[(size_t)tn * stride + m0 + row] = make_float2(top, sum);
     if constexpr (ENT) part_e[(size_t)tn * stride + m0 + row] = ent;
+}
+
+// A workgroup per compute unit (their LDS holds no second) goes through its tiles, the next one's first stages under way while one's results leave: 64 tokens
+// x 3584 against 131072 rows 180 -> 172 us, of many tokens 0 to 2 %.  (dl's tiles and those of grad_weight gain nothing by it: their stores have to be done
+// before the next tile's stages can be waited for.)
+template <int TM, bool ENT>
+__device__ __forceinline__ void hl_stats_tiles(uint8_t* hl_lds, const Tokens& tk, int count, const int* live, const uint16_t* weight, int64_t ldw, int stride, float2* part, float* part_e,
+                                               float* hit)
+{
+    constexpr int BM = 64 * TM;
+    const int tiles_m = (count + BM - 1) / BM, tiles_n = (tk.V + HL_BN - 1) / HL_BN, total = tiles_m * tiles_n, rest = tk.H % 32 ? 16 : 32;
+    int k = blockIdx.x >> 3, logical = hl_logical(total, k), tm, tn;
+    if (logical < 0) return;
+    Pipe<TM, false, false, false> pipe;
+    pipe.lds = hl_lds;
+    auto begin = [&]() {
+        hl_origin(logical, tiles_m, tiles_n, tm, tn);
+        const int m0 = tm * BM, n0 = tn * HL_BN;
+        pipe.aim(Operand{tk.hidden, tk.ld, count - m0, live + m0, rest, 0}, Operand{weight + (int64_t)n0 * ldw, ldw, tk.V - n0, nullptr, rest, 0}, (tk.H + 31) / 32, rest == 16);
+        pipe.request(0);
+    };
+    begin();
+    while (true) {
+        pipe.request(2);
+        float16_t acc[TM][HL_TN];
+        hl_clear<TM>(acc);
+        pipe.multiply(acc);
+        const int m0 = tm * BM, at_n = tn;
+        k += gridDim.x >> 3;
+        logical = hl_logical(total, k);
+        if (logical >= 0) begin();
+        hl_stats_out<TM, ENT>(acc, reinterpret_cast<float*>(hl_lds + 2 * hl_stage_bytes(TM)), tk, count, live, m0, at_n, stride, part, part_e, hit);
+        if (logical < 0) return;
+        __syncthreads();
+    }
 }
 
 // kList: every workgroup lists the live tokens for itself, in LDS behind the ring, and the first writes the list down for the launches to come: a launch less
@@ -442,7 +489,7 @@ __global__ __launch_bounds__(HL_THREADS, 2) void head_stats_kernel(const Tokens 
         count = tk.index[0];
         live = live_rows(tk.index);
     }
-    with_row_tiles<ROWS>(count, [&](auto tm) { hl_stats_tile<decltype(tm)::value, ENT>(hl_lds, tk, count, live, weight, ldw, stride, part, part_e, hit); });
+    with_row_tiles<ROWS>(count, [&](auto tm) { hl_stats_tiles<decltype(tm)::value, ENT>(hl_lds, tk, count, live, weight, ldw, stride, part, part_e, hit); });
 }
 
 // A maximum with its sum of 2^(l - maximum) and, for the entropy, of 2^(l - maximum) (l - maximum); empty: -infinity, 0, 0.
@@ -547,26 +594,15 @@ __global__ __launch_bounds__(1024) void head_index_kernel(const int64_t* __restr
 struct RowGrads {
     const float *lse, *entropy, *g_logp, *g_entropy;           // by token; entropy and g_entropy may be nullptr
 };
+// dl of a tile from its accumulators; `area`: LDS.
 template <int TM>
-__device__ __forceinline__ void hl_dlogits_tile(uint8_t* hl_lds, const Tokens& tk, int count, const uint16_t* weight, int64_t ldw, int v0, int width, const RowGrads& rg, uint16_t* dl,
-                                                int64_t panel)
+__device__ __forceinline__ void hl_dlogits_out(float16_t (&acc)[TM][HL_TN], uint8_t* area, const Tokens& tk, int count, int m0, int n0, int v0, int width, const RowGrads& rg, uint16_t* dl,
+                                               int64_t panel)
 {
     constexpr int BM = 64 * TM;
     constexpr float kLn2 = 0.693147180559945f, kLog2e = 1.44269504088896f;
-    const int tiles_m = (count + BM - 1) / BM, tiles_n = (width + HL_BN - 1) / HL_BN;
-    const int logical = hl_logical(tiles_m * tiles_n);
-    if (logical < 0) return;
-    int tm, tn;
-    hl_origin(logical, tiles_m, tiles_n, tm, tn);
-    const int m0 = tm * BM, n0 = tn * HL_BN;
-    float16_t acc[TM][HL_TN];
-    hl_clear<TM>(acc);
     const int* live = live_rows(tk.index);
-    const int rest = tk.H % 32 ? 16 : 32;
-    const Operand a = {tk.hidden, tk.ld, count - m0, live + m0, rest, 0}, b = {weight + (int64_t)(v0 + n0) * ldw, ldw, width - n0, nullptr, rest, 0};
-    hl_main_loop<TM, false, false, false>(acc, hl_lds, a, b, (tk.H + 31) / 32, rest == 16);
-
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3, lr = lane & 31, hi = lane >> 5;
+    const int thread = hl_thread(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), wm = wave >> 2, wn = wave & 3, lr = lane & 31, hi = lane >> 5;
     const int there = width - (n0 + wn * 64);
     const float inv_t = tk.scale2 * kLn2;                      // 1 / temperature
 #pragma unroll
@@ -618,7 +654,29 @@ __device__ __forceinline__ void hl_dlogits_tile(uint8_t* hl_lds, const Tokens& t
                     if (!on || j * 32 + 8 * (e >> 2) + 4 * hi + (e & 3) >= there) acc[i][j][e] = 0.0f;
         }
     }
-    hl_store_bf16<TM>(acc, hl_lds, dl + (int64_t)(n0 / 64 + wn) * panel + m0 * 64, 64, BM, 64);
+    hl_store_bf16<TM>(acc, area, dl + (int64_t)(n0 / 64 + wn) * panel + m0 * 64, 64, BM, 64);
+}
+
+template <int TM>
+__device__ __forceinline__ void hl_dlogits_tile(uint8_t* hl_lds, const Tokens& tk, int count, const uint16_t* weight, int64_t ldw, int v0, int width, const RowGrads& rg, uint16_t* dl,
+                                                int64_t panel)
+{
+    constexpr int BM = 64 * TM;
+    const int tiles_m = (count + BM - 1) / BM, tiles_n = (width + HL_BN - 1) / HL_BN, rest = tk.H % 32 ? 16 : 32, logical = hl_logical(tiles_m * tiles_n, blockIdx.x >> 3);
+    if (logical < 0) return;
+    int tm, tn;
+    hl_origin(logical, tiles_m, tiles_n, tm, tn);
+    const int m0 = tm * BM, n0 = tn * HL_BN;
+    float16_t acc[TM][HL_TN];
+    hl_clear<TM>(acc);
+    Pipe<TM, false, false, false> pipe;
+    pipe.lds = hl_lds;
+    pipe.aim(Operand{tk.hidden, tk.ld, count - m0, live_rows(tk.index) + m0, rest, 0}, Operand{weight + (int64_t)(v0 + n0) * ldw, ldw, width - n0, nullptr, rest, 0}, (tk.H + 31) / 32,
+             rest == 16);
+    pipe.request(0);
+    pipe.request(2);
+    pipe.multiply(acc);
+    hl_dlogits_out<TM>(acc, hl_lds, tk, count, m0, n0, v0, width, rg, dl, panel);
 }
 
 template <int ROWS>
@@ -692,7 +750,12 @@ __device__ __forceinline__ void hl_hidden_tile(uint8_t* hl_lds, const Products& 
         });
     const Operand a = {p.dl + (int64_t)(begin / 2) * p.rows * 64 + m0 * 64, 64, 64 * TMX, nullptr, 32, p.rows * 64};
     const Operand b = {p.weight + (int64_t)begin * 32 * p.ldw + n0, p.ldw, p.H - n0, nullptr, end == kt && p.width % 32 ? p.width % 32 : 32, 0};
-    hl_main_loop<TMX, false, true, true>(acc, hl_lds, a, b, end - begin, false);
+    Pipe<TMX, false, true, true> pipe;
+    pipe.lds = hl_lds;
+    pipe.aim(a, b, end - begin, false);
+    pipe.request(0);
+    pipe.request(2);
+    pipe.multiply(acc);
     each([](const float16_t& v, int e, float4* q) { *q = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]); });
 }
 
@@ -717,12 +780,15 @@ __global__ __launch_bounds__(HL_THREADS, 2) void head_products_kernel(const Prod
     if (li >= per || job >= jobs) return;
     int tm, tn;
     hl_origin(job, tiles_v, tiles_h, tm, tn);
-    const int m0 = tm * 256, n0 = tn * HL_BN;
+    const int m0 = tm * 256, n0 = tn * HL_BN, wn = (threadIdx.x >> 6) & 3;
     float16_t acc[4][HL_TN];
     hl_clear<4>(acc);
-    const Operand a = {p.dl + (int64_t)(m0 / 64) * p.rows * 64, 64, 256, nullptr, 32, p.rows * 64}, b = {p.gathered + n0, p.H, p.H - n0, nullptr, 32, 0};
-    hl_main_loop<4, true, true, true>(acc, hl_lds, a, b, (count + 31) / 32, false);
-    const int wn = (threadIdx.x >> 6) & 3;
+    Pipe<4, true, true, true> pipe;
+    pipe.lds = hl_lds;
+    pipe.aim(Operand{p.dl + (int64_t)(m0 / 64) * p.rows * 64, 64, 256, nullptr, 32, p.rows * 64}, Operand{p.gathered + n0, p.H, p.H - n0, nullptr, 32, 0}, (count + 31) / 32, false);
+    pipe.request(0);
+    pipe.request(2);
+    pipe.multiply(acc);
     hl_store_bf16<4>(acc, hl_lds, p.grad_weight + (int64_t)m0 * p.H + n0 + wn * 64, p.H, p.width - m0, p.H - (n0 + wn * 64));
 }
 
@@ -793,6 +859,8 @@ template <class F> int with_rows(int64_t tokens, F&& f)
         default: return f(std::integral_constant<int, kMany>{});
     }
 }
+// a workgroup for each tile, alike on all XCDs
+unsigned tile_grid(int64_t tiles) { return (unsigned)((tiles + 7) / 8 * 8); }
 // LDS of a kernel whose tiles have at most 64 TM rows
 constexpr size_t ring_bytes(int TM) { return (size_t)HL_NS * hl_stage_bytes(TM); }
 
@@ -802,8 +870,8 @@ int launch_stats(const Tokens& tk, const void* weight, int64_t ldw, int stride, 
     static bool done[64] = {};
     const size_t lds = ROWS == kList ? ring_bytes(1) + kListTokens * sizeof(int) : ring_bytes(4);
     if (const int rc = allow_dynamic_lds((const void*)head_stats_kernel<ROWS, ENT>, lds, done)) return rc;
-    const int64_t tiles = most_row_tiles(tk.tokens) * ((tk.V + HL_BN - 1) / HL_BN);
-    hipLaunchKernelGGL((head_stats_kernel<ROWS, ENT>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(HL_THREADS), lds, st, tk, (const uint16_t*)weight, ldw, stride, part, part_e, hit,
+    const unsigned tiles = tile_grid(most_row_tiles(tk.tokens) * ((tk.V + HL_BN - 1) / HL_BN)), cus = (unsigned)(device_cus() + 7) / 8 * 8;
+    hipLaunchKernelGGL((head_stats_kernel<ROWS, ENT>), dim3(tiles < cus ? tiles : cus), dim3(HL_THREADS), lds, st, tk, (const uint16_t*)weight, ldw, stride, part, part_e, hit,
                        ignore, list);
     return hipGetLastError() == hipSuccess ? METIS_OK : METIS_E_LAUNCH;
 }
@@ -814,8 +882,7 @@ int launch_dlogits(const Tokens& tk, const void* weight, int64_t ldw, int v0, in
     static bool done[64] = {};
     const size_t lds = ring_bytes(ROWS == kList ? 1 : 4);
     if (const int rc = allow_dynamic_lds((const void*)head_dlogits_kernel<ROWS>, lds, done)) return rc;
-    const int64_t tiles = most_row_tiles(tk.tokens) * ((width + HL_BN - 1) / HL_BN);
-    hipLaunchKernelGGL((head_dlogits_kernel<ROWS>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(HL_THREADS), lds, st, tk, (const uint16_t*)weight, ldw, v0, width, rg, dl, panel);
+    hipLaunchKernelGGL((head_dlogits_kernel<ROWS>), dim3(tile_grid(most_row_tiles(tk.tokens) * ((width + HL_BN - 1) / HL_BN))), dim3(HL_THREADS), lds, st, tk, (const uint16_t*)weight, ldw, v0, width, rg, dl, panel);
     return hipGetLastError() == hipSuccess ? METIS_OK : METIS_E_LAUNCH;
 }
 
