@@ -594,10 +594,17 @@ __global__ __launch_bounds__(1024) void head_index_kernel(const int64_t* __restr
 struct RowGrads {
     const float *lse, *entropy, *g_logp, *g_entropy;           // by token; entropy and g_entropy may be nullptr
 };
+// dl at the targets, by place among the live tokens: the value as bf16, what that leaves out, the target (-1: not in the vocabulary).  This one element makes
+// most of a token's gradient, so its rounding (up to 2^-8) would be a common factor of a whole row: the products take `rounded`, and `left` goes into both
+// gradients in binary32.  (Gradients against 64 bits, 411 x 1536 against 32003: 0.0025 of their norm with the rounding left as it is.)
+struct AtTarget {
+    float *rounded, *left;
+    int* column;
+};
 // dl of a tile from its accumulators; `area`: LDS.
 template <int TM>
-__device__ __forceinline__ void hl_dlogits_out(float16_t (&acc)[TM][HL_TN], uint8_t* area, const Tokens& tk, int count, int m0, int n0, int v0, int width, const RowGrads& rg, uint16_t* dl,
-                                               int64_t panel)
+__device__ __forceinline__ void hl_dlogits_out(float16_t (&acc)[TM][HL_TN], uint8_t* area, const Tokens& tk, int count, int m0, int n0, int v0, int width, const RowGrads& rg, const AtTarget& target,
+                                               uint16_t* dl, int64_t panel)
 {
     constexpr int BM = 64 * TM;
     constexpr float kLn2 = 0.693147180559945f, kLog2e = 1.44269504088896f;
@@ -608,7 +615,7 @@ __device__ __forceinline__ void hl_dlogits_out(float16_t (&acc)[TM][HL_TN], uint
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         const int m = m0 + (wm * TM + i) * 32 + lr;
-        float lse2 = 0.0f, g = 0.0f, ge = 0.0f, h = 0.0f;
+        float lse2 = 0.0f, g = 0.0f, ge = 0.0f, h = 0.0f, at_target = 0.0f;
         int want = -1;
         const bool on = m < count;
         if (on) {
@@ -619,10 +626,13 @@ __device__ __forceinline__ void hl_dlogits_out(float16_t (&acc)[TM][HL_TN], uint
                 ge = rg.g_entropy[t] * inv_t;
                 h = rg.entropy[t];
             }
-            const int64_t w = tk.targets[t] - (v0 + n0 + wn * 64);
-            want = w >= 0 && w < 64 ? (int)w : -1;
+            const int w = target.column[m] - (v0 + n0 + wn * 64);
+            if (w >= 0 && w < 64) {
+                want = w;
+                at_target = target.rounded[m];
+            }
         }
-        // -p f everywhere, then g more at the target, then zero where nothing is: the last two in few tiles
+        // -p f everywhere, then the target's, then zero where nothing is: the last two in few tiles
         const float ge2 = ge * kLn2;
         if (rg.g_entropy) {
             g = fmaf(ge, h, g);                                // f = g + ge (d ln 2 + h)
@@ -633,7 +643,6 @@ __device__ __forceinline__ void hl_dlogits_out(float16_t (&acc)[TM][HL_TN], uint
                     const float d = fmaf(acc[i][j][e], tk.scale2, -lse2);
                     acc[i][j][e] = -__builtin_amdgcn_exp2f(d) * fmaf(ge2, d, g);
                 }
-            g = on && rg.g_logp ? rg.g_logp[live[m]] * inv_t : 0.0f;
         } else {
 #pragma unroll
             for (int j = 0; j < HL_TN; ++j)
@@ -644,7 +653,7 @@ __device__ __forceinline__ void hl_dlogits_out(float16_t (&acc)[TM][HL_TN], uint
 #pragma unroll
             for (int j = 0; j < HL_TN; ++j)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) acc[i][j][e] += j * 32 + 8 * (e >> 2) + 4 * hi + (e & 3) == want ? g : 0.0f;
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = j * 32 + 8 * (e >> 2) + 4 * hi + (e & 3) == want ? at_target : acc[i][j][e];
         }
         if (__any(!on) || there < 64) {
 #pragma unroll
@@ -658,8 +667,8 @@ __device__ __forceinline__ void hl_dlogits_out(float16_t (&acc)[TM][HL_TN], uint
 }
 
 template <int TM>
-__device__ __forceinline__ void hl_dlogits_tile(uint8_t* hl_lds, const Tokens& tk, int count, const uint16_t* weight, int64_t ldw, int v0, int width, const RowGrads& rg, uint16_t* dl,
-                                                int64_t panel)
+__device__ __forceinline__ void hl_dlogits_tile(uint8_t* hl_lds, const Tokens& tk, int count, const uint16_t* weight, int64_t ldw, int v0, int width, const RowGrads& rg,
+                                                const AtTarget& target, uint16_t* dl, int64_t panel)
 {
     constexpr int BM = 64 * TM;
     const int tiles_m = (count + BM - 1) / BM, tiles_n = (width + HL_BN - 1) / HL_BN, rest = tk.H % 32 ? 16 : 32, logical = hl_logical(tiles_m * tiles_n, blockIdx.x >> 3);
@@ -676,25 +685,114 @@ __device__ __forceinline__ void hl_dlogits_tile(uint8_t* hl_lds, const Tokens& t
     pipe.request(0);
     pipe.request(2);
     pipe.multiply(acc);
-    hl_dlogits_out<TM>(acc, hl_lds, tk, count, m0, n0, v0, width, rg, dl, panel);
+    hl_dlogits_out<TM>(acc, hl_lds, tk, count, m0, n0, v0, width, rg, target, dl, panel);
 }
 
 template <int ROWS>
 __global__ __launch_bounds__(HL_THREADS, 2) void head_dlogits_kernel(const Tokens tk, const uint16_t* __restrict__ weight, int64_t ldw, int v0, int width, const RowGrads rg,
-                                                                     uint16_t* __restrict__ dl, int64_t panel)
+                                                                     const AtTarget target, uint16_t* __restrict__ dl, int64_t panel)
 {
     extern __shared__ __attribute__((aligned(1024))) uint8_t hl_lds[];
     const int count = tk.index[0];
-    with_row_tiles<ROWS>(count, [&](auto tm) { hl_dlogits_tile<decltype(tm)::value>(hl_lds, tk, count, weight, ldw, v0, width, rg, dl, panel); });
+    with_row_tiles<ROWS>(count, [&](auto tm) { hl_dlogits_tile<decltype(tm)::value>(hl_lds, tk, count, weight, ldw, v0, width, rg, target, dl, panel); });
 }
 
-// The live rows of hidden side by side, then zero rows up to a multiple of 32.
-__global__ __launch_bounds__(256) void head_gather_kernel(const Tokens tk, uint4* __restrict__ out)
+// Before the pieces: dl at the targets, and for grad_weight (`out`) the live rows of hidden side by side, then zero rows up to a multiple of 32.
+__global__ __launch_bounds__(256) void head_gather_kernel(const Tokens tk, const uint16_t* __restrict__ weight, int64_t ldw, const RowGrads rg, const AtTarget target, uint4* __restrict__ out)
 {
-    const int count = tk.index[0], rows = (count + 31) & ~31, cpr = tk.H / 8;
-    for (int m = blockIdx.x; m < rows; m += gridDim.x) {
-        const uint4* src = m < count ? reinterpret_cast<const uint4*>(tk.hidden + (int64_t)live_rows(tk.index)[m] * tk.ld) : nullptr;
-        for (int c = threadIdx.x; c < cpr; c += 256) out[(int64_t)m * cpr + c] = src ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+    constexpr float kLn2 = 0.693147180559945f, kLog2e = 1.44269504088896f;
+    __shared__ float red[2][4];
+    const int count = tk.index[0], rows = out ? (count + 31) & ~31 : count, cpr = tk.H / 8;
+    int turn = 0;
+    for (int m = blockIdx.x; m < rows; m += gridDim.x, turn ^= 1) {
+        if (m >= count) {
+            for (int c = threadIdx.x; c < cpr; c += 256) out[(int64_t)m * cpr + c] = make_uint4(0u, 0u, 0u, 0u);
+            continue;
+        }
+        const int t = live_rows(tk.index)[m];
+        const int64_t want = tk.targets[t];
+        const bool there = want >= 0 && want < tk.V;
+        const uint4* x = reinterpret_cast<const uint4*>(tk.hidden + (int64_t)t * tk.ld);
+        const uint4* w = reinterpret_cast<const uint4*>(weight + (there ? want : 0) * ldw);
+        float dot = 0.0f;
+        for (int c = threadIdx.x; c < cpr; c += 256) {
+            const uint4 a = x[c], b = w[c];
+            if (out) out[(int64_t)m * cpr + c] = a;
+            const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                dot = fmaf(__uint_as_float(aw[k] << 16), __uint_as_float(bw[k] << 16), dot);
+                dot = fmaf(__uint_as_float(aw[k] & 0xffff0000u), __uint_as_float(bw[k] & 0xffff0000u), dot);
+            }
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) dot += __shfl_xor(dot, o, 64);
+        if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = dot;
+        __syncthreads();
+        if (threadIdx.x) continue;
+        dot = (red[turn][0] + red[turn][1]) + (red[turn][2] + red[turn][3]);
+        const float inv_t = tk.scale2 * kLn2, g = rg.g_logp ? rg.g_logp[t] * inv_t : 0.0f, d = fmaf(dot, tk.scale2, -rg.lse[t] * kLog2e);
+        const float f = rg.g_entropy ? fmaf(rg.g_entropy[t] * inv_t, fmaf(d, kLn2, rg.entropy[t]), g) : g;
+        const float v = fmaf(-__builtin_amdgcn_exp2f(d), f, g), r = __uint_as_float(rb_pair(v, 0.0f) << 16);
+        target.rounded[m] = r;
+        target.left[m] = there && fabsf(r) < INFINITY ? v - r : 0.0f;
+        target.column[m] = there ? (int)want : -1;
+    }
+}
+
+// Per 256 rows of the vocabulary (and 512 columns): which rows of grad_weight are targets' (`row_of`: the first live token with that target, or -1) and, as the row
+// of that token, what `left` of all tokens with that target gives, in their order.  (Its own rounding to bf16 is 2^-8 of at most 2^-8 of the gradient.)
+__global__ __launch_bounds__(256) void head_targets_kernel(const int* __restrict__ index, const AtTarget target, const uint16_t* __restrict__ gathered, int H, int* __restrict__ row_of,
+                                                           uint16_t* __restrict__ rest)
+{
+    __shared__ int first[256], times[256];
+    const int count = index[0], v0 = blockIdx.x * 256, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.y * 512 + lane * 8;
+    first[threadIdx.x] = INT32_MAX;
+    times[threadIdx.x] = 0;
+    __syncthreads();
+    for (int m = threadIdx.x; m < count; m += 256) {
+        const int row = target.column[m] - v0;
+        if (row >= 0 && row < 256) {
+            atomicMin(&first[row], m);
+            atomicAdd(&times[row], 1);
+        }
+    }
+    __syncthreads();
+    if (blockIdx.y == 0) row_of[v0 + threadIdx.x] = times[threadIdx.x] ? first[threadIdx.x] : -1;
+    const int mine = threadIdx.x;                              // a wave's 64 rows, by lane
+    uint64_t rows = __ballot(times[mine] > 0);
+    while (rows) {
+        const int row = wave * 64 + __builtin_ctzll(rows), begin = __builtin_amdgcn_readfirstlane(first[row]);
+        int to_come = __builtin_amdgcn_readfirstlane(times[row]);
+        rows &= rows - 1;
+        float sum[8] = {};
+        for (int m0 = begin; m0 < count && to_come > 0; m0 += 64) {
+            uint64_t same = to_come == 1 && m0 == begin ? 1ull : __ballot(m0 + lane < count && target.column[m0 + lane] == v0 + row);
+            to_come -= __popcll(same);
+            while (same) {                                     // eight rows requested together
+                uint4 x[8];
+                float left[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int m = m0 + (same ? __builtin_ctzll(same) : 0);
+                    left[k] = same ? target.left[m] : 0.0f;
+                    x[k] = make_uint4(0u, 0u, 0u, 0u);
+                    if (same && c < H) x[k] = *reinterpret_cast<const uint4*>(gathered + (int64_t)m * H + c);
+                    same &= same - 1;
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        sum[2 * e] = fmaf(left[k], __uint_as_float(w[e] << 16), sum[2 * e]);
+                        sum[2 * e + 1] = fmaf(left[k], __uint_as_float(w[e] & 0xffff0000u), sum[2 * e + 1]);
+                    }
+                }
+            }
+        }
+        if (c < H)
+            *reinterpret_cast<uint4*>(rest + (int64_t)begin * H + c) = make_uint4(rb_pair(sum[0], sum[1]), rb_pair(sum[2], sum[3]), rb_pair(sum[4], sum[5]), rb_pair(sum[6], sum[7]));
     }
 }
 
@@ -713,6 +811,8 @@ struct Products {
     float* slabs;                // nullptr: grad_hidden is not wanted
     uint16_t* grad_weight;       // nullptr: grad_weight is not wanted
     const int* index;
+    const int* row_of;           // by the piece's rows, and
+    const uint16_t* rest;        // what they are to have added (head_targets_kernel)
     int width, H, splits, first; // first: the slabs hold nothing yet
 };
 // Tile `job` of grad_hidden.
@@ -789,22 +889,53 @@ __global__ __launch_bounds__(HL_THREADS, 2) void head_products_kernel(const Prod
     pipe.request(0);
     pipe.request(2);
     pipe.multiply(acc);
+    const int thread = hl_thread(), lane = thread & 63, wm = thread >> 8, lr = lane & 31, hi = lane >> 5;
+    int from[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) from[i] = p.row_of[m0 + (wm * 4 + i) * 32 + lr];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (!__any(from[i] >= 0)) continue;
+        if (from[i] >= 0) {
+            const uint16_t* rest = p.rest + (int64_t)from[i] * p.H + n0 + wn * 64 + 4 * hi;
+#pragma unroll
+            for (int j = 0; j < HL_TN; ++j)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    if (n0 + wn * 64 + j * 32 + 8 * g + 4 * hi >= p.H) continue;
+                    const uint2 r = *reinterpret_cast<const uint2*>(rest + j * 32 + 8 * g);
+                    acc[i][j][4 * g] += __uint_as_float(r.x << 16);
+                    acc[i][j][4 * g + 1] += __uint_as_float(r.x & 0xffff0000u);
+                    acc[i][j][4 * g + 2] += __uint_as_float(r.y << 16);
+                    acc[i][j][4 * g + 3] += __uint_as_float(r.y & 0xffff0000u);
+                }
+        }
+    }
     hl_store_bf16<4>(acc, hl_lds, p.grad_weight + (int64_t)m0 * p.H + n0 + wn * 64, p.H, p.width - m0, p.H - (n0 + wn * 64));
 }
 
-// grad_hidden of every token: the slabs of a live one added in order, zero for the others.
+// grad_hidden of every token: the slabs of a live one added in order, then what its dl at the target left, zero for the others.
 __global__ __launch_bounds__(256) void head_hidden_kernel(const float* __restrict__ slabs, int splits, int64_t slab_rows, const int* __restrict__ index, int tokens, int H,
-                                                          uint16_t* __restrict__ out)
+                                                          const uint16_t* __restrict__ weight, int64_t ldw, const AtTarget target, uint16_t* __restrict__ out)
 {
     const int quads = H / 4;
     for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < (int64_t)tokens * quads; at += (int64_t)gridDim.x * 256) {
         const int t = (int)(at / quads), c = (int)(at - (int64_t)t * quads), pos = live_rows(index)[tokens + t];
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (pos >= 0)
+        if (pos >= 0) {
+            const int column = target.column[pos];
+            const float left = target.left[pos];
+            uint2 w = make_uint2(0u, 0u);
+            if (column >= 0) w = *reinterpret_cast<const uint2*>(weight + (int64_t)column * ldw + c * 4);
             for (int s = 0; s < splits; ++s) {
                 const float4 q = *reinterpret_cast<const float4*>(slabs + ((int64_t)s * slab_rows + pos) * H + c * 4);
                 v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
             }
+            v.x = fmaf(left, __uint_as_float(w.x << 16), v.x);
+            v.y = fmaf(left, __uint_as_float(w.x & 0xffff0000u), v.y);
+            v.z = fmaf(left, __uint_as_float(w.y << 16), v.z);
+            v.w = fmaf(left, __uint_as_float(w.y & 0xffff0000u), v.w);
+        }
         *reinterpret_cast<uint2*>(out + (int64_t)t * H + c * 4) = make_uint2(rb_pair(v.x, v.y), rb_pair(v.z, v.w));
     }
 }
@@ -877,12 +1008,13 @@ int launch_stats(const Tokens& tk, const void* weight, int64_t ldw, int stride, 
 }
 
 template <int ROWS>
-int launch_dlogits(const Tokens& tk, const void* weight, int64_t ldw, int v0, int width, const RowGrads& rg, uint16_t* dl, int64_t panel, hipStream_t st)
+int launch_dlogits(const Tokens& tk, const void* weight, int64_t ldw, int v0, int width, const RowGrads& rg, const AtTarget& target, uint16_t* dl, int64_t panel, hipStream_t st)
 {
     static bool done[64] = {};
     const size_t lds = ring_bytes(ROWS == kList ? 1 : 4);
     if (const int rc = allow_dynamic_lds((const void*)head_dlogits_kernel<ROWS>, lds, done)) return rc;
-    hipLaunchKernelGGL((head_dlogits_kernel<ROWS>), dim3(tile_grid(most_row_tiles(tk.tokens) * ((width + HL_BN - 1) / HL_BN))), dim3(HL_THREADS), lds, st, tk, (const uint16_t*)weight, ldw, v0, width, rg, dl, panel);
+    hipLaunchKernelGGL((head_dlogits_kernel<ROWS>), dim3(tile_grid(most_row_tiles(tk.tokens) * ((width + HL_BN - 1) / HL_BN))), dim3(HL_THREADS), lds, st, tk, (const uint16_t*)weight, ldw, v0,
+                       width, rg, target, dl, panel);
     return hipGetLastError() == hipSuccess ? METIS_OK : METIS_E_LAUNCH;
 }
 
@@ -952,7 +1084,7 @@ size_t head_logprobs_backward_workspace_bytes(int64_t tokens, int64_t H, int64_t
 {
     if (tokens <= 0 || !sizes_ok(tokens, H, V)) return 0;
     const BackwardPlan p = backward_plan(tokens, H, V, want_weight != 0);
-    return align256((size_t)p.rows * p.width * 2) + (want_weight ? align256((size_t)p.rows * H * 2) : 0) + (want_hidden ? align256((size_t)p.splits * p.rows * H * 4) : 0);
+    return align256((size_t)p.rows * p.width * 2) + 3 * align256((size_t)p.rows * 4) + (want_weight ? 2 * align256((size_t)p.rows * H * 2) + (size_t)padded(V, 256) * 4 : 0) + (want_hidden ? align256((size_t)p.splits * p.rows * H * 4) : 0);
 }
 
 int head_logprobs_backward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, const void* targets, int64_t tokens, int64_t H, int64_t V, float temperature,
@@ -969,26 +1101,42 @@ int head_logprobs_backward(const void* hidden, int64_t ldh, const void* weight, 
     char* at = static_cast<char*>(workspace);
     uint16_t* dl = reinterpret_cast<uint16_t*>(at);
     at += align256((size_t)p.rows * p.width * 2);
-    uint16_t* gathered = nullptr;
+    auto take = [&](size_t bytes) {
+        char* here = at;
+        at += align256(bytes);
+        return here;
+    };
+    const size_t by_row = (size_t)p.rows * 4;
+    AtTarget target;
+    target.rounded = reinterpret_cast<float*>(take(by_row));
+    target.left = reinterpret_cast<float*>(take(by_row));
+    target.column = reinterpret_cast<int*>(take(by_row));
+    uint16_t *gathered = nullptr, *rest = nullptr;
+    int* row_of = nullptr;
     if (grad_weight) {
-        gathered = reinterpret_cast<uint16_t*>(at);
-        at += align256((size_t)p.rows * H * 2);
+        gathered = reinterpret_cast<uint16_t*>(take((size_t)p.rows * H * 2));
+        rest = reinterpret_cast<uint16_t*>(take((size_t)p.rows * H * 2));
+        row_of = reinterpret_cast<int*>(take((size_t)padded(V, 256) * 4));
     }
     float* slabs = grad_hidden ? reinterpret_cast<float*>(at) : nullptr;
     const Tokens tk = tokens_of(hidden, ldh, targets, index, tokens, H, V, temperature);
     const RowGrads rg = {lse, entropy, g_logp, g_entropy};
     const int cus = device_cus();
+    hipLaunchKernelGGL(head_gather_kernel, dim3((unsigned)(tokens + 31 < 8 * (int64_t)cus ? tokens + 31 : 8 * (int64_t)cus)), dim3(256), 0, st, tk, (const uint16_t*)weight, ldw, rg, target,
+                       (uint4*)gathered);
+    if (hipGetLastError() != hipSuccess) return METIS_E_LAUNCH;
     if (grad_weight) {
-        hipLaunchKernelGGL(head_gather_kernel, dim3((unsigned)(tokens + 31 < 8 * (int64_t)cus ? tokens + 31 : 8 * (int64_t)cus)), dim3(256), 0, st, tk, (uint4*)gathered);
+        hipLaunchKernelGGL(head_targets_kernel, dim3((unsigned)((V + 255) / 256), (unsigned)((H + 511) / 512)), dim3(256), 0, st, (const int*)index, target, (const uint16_t*)gathered, (int)H,
+                           row_of, rest);
         if (hipGetLastError() != hipSuccess) return METIS_E_LAUNCH;
     }
     const int64_t tiles_h = (H + 255) / 256;
     for (int64_t v0 = 0; v0 < V; v0 += p.width) {
         const int width = (int)(V - v0 < p.width ? V - v0 : p.width);
-        int rc = with_rows(tokens, [&](auto rows) { return launch_dlogits<decltype(rows)::value>(tk, weight, ldw, (int)v0, width, rg, dl, p.rows * 64, st); });
+        int rc = with_rows(tokens, [&](auto rows) { return launch_dlogits<decltype(rows)::value>(tk, weight, ldw, (int)v0, width, rg, target, dl, p.rows * 64, st); });
         if (rc != METIS_OK) return rc;
-        const Products pr = {dl, p.rows, (const uint16_t*)weight + v0 * ldw, ldw, gathered, slabs, grad_weight ? (uint16_t*)grad_weight + v0 * H : nullptr, (const int*)index, width,
-                             (int)H, p.splits, v0 == 0};
+        const Products pr = {dl, p.rows, (const uint16_t*)weight + v0 * ldw, ldw, gathered, slabs, grad_weight ? (uint16_t*)grad_weight + v0 * H : nullptr, (const int*)index,
+                             row_of ? row_of + v0 : nullptr, rest, width, (int)H, p.splits, v0 == 0};
         const int64_t hidden_jobs = slabs ? most_row_tiles(tokens) * tiles_h * p.splits : 0, weight_jobs = grad_weight ? (width + 255) / 256 * tiles_h : 0;
         const unsigned grid = 8u * (unsigned)((hidden_jobs + 7) / 8 + (weight_jobs + 7) / 8);
         rc = with_rows(tokens, [&](auto rows) { return launch_products<decltype(rows)::value>(pr, grid, st); });
@@ -997,7 +1145,7 @@ int head_logprobs_backward(const void* hidden, int64_t ldh, const void* weight, 
     if (grad_hidden) {
         const int64_t need = (tokens * (H / 4) + 255) / 256, cap = (int64_t)cus * 16;
         hipLaunchKernelGGL(head_hidden_kernel, dim3((unsigned)(need < cap ? need : cap)), dim3(256), 0, st, (const float*)slabs, p.splits, p.rows, (const int*)index, (int)tokens, (int)H,
-                           (uint16_t*)grad_hidden);
+                           (const uint16_t*)weight, ldw, target, (uint16_t*)grad_hidden);
         if (hipGetLastError() != hipSuccess) return METIS_E_LAUNCH;
     }
     return METIS_OK;

@@ -3,9 +3,10 @@
 Tolerances.  A logit is a binary32 sum of H exact products of bf16 values: off by at most H 2^-24 sum |x w| (times 1 / temperature).  With E the largest
 such error of a token's logits, log-sum-exp is off by no more than E and what the exponentials, their sums (chains of under 2^9 additions, 2^-15 of a
 positive sum) and the logarithm lose: 2^-14 in all, and 2^-21 of the magnitudes that are subtracted.  The entropy moves by at most E sum p |log p + H|.
-dl: p is off by a factor of exp of those errors (r below); then one rounding to bf16, half a step (2^-8 of dl).  The products' own sums lose at most
-(number of terms) 2^-24 of the sum of magnitudes, and the result is rounded to bf16 once.  The same bounds in the 2-norm, where the roundings' part is 2^-8 |dl| |w| with
-the spectral norm of w: much nearer, and what a missing or doubled piece cannot meet."""
+dl: p is off by a factor of exp of those errors (r below); then one rounding to bf16, half a step (2^-8 of dl), but at the target, whose rounding is made
+good to 2^-16 of it (half a step of half a step, bf16 again).  The products' own sums lose at most (number of terms) 2^-24 of the sum of magnitudes, and the
+result is rounded to bf16 once.  The same bounds in the 2-norm, where the roundings' part is 2^-8 |dl| |w| with the spectral norm of w: much nearer, and what a
+missing or doubled piece cannot meet."""
 import pytest
 import torch
 
@@ -63,8 +64,9 @@ class Exact:
         d = (g * (self.onehot - self.p) - e * self.p * inside) / self.temp
         r = (torch.expm1(2 * self.tol))[:, None]
         loss = r * self.p * (g.abs() + e.abs() * (inside.abs() + 1)) / self.temp         # before the rounding
-        off = HALF * d.abs() + (1 + HALF) * loss
-        for got, left, a, b, terms in ((gx, d, off, self.w, self.w.shape[0]), (gw, d.t(), off.t(), self.x, self.x.shape[0])):
+        rounded = (HALF * (1 - self.onehot) + HALF ** 2 * self.onehot) * d.abs()
+        off = rounded + (1 + HALF) * loss
+        for got, left, a, rnd, b, terms in ((gx, d, off, rounded, self.w, self.w.shape[0]), (gw, d.t(), off.t(), rounded.t(), self.x, self.x.shape[0])):
             if got is None:
                 continue
             live = b if b is self.w else torch.where(self.live[:, None], b, 0.0)
@@ -74,7 +76,7 @@ class Exact:
             err = (got.double() - want).abs()
             assert bool((err <= bound).all()), float((err / bound).max())
             norm = torch.linalg.matrix_norm(live, 2)
-            most = HALF * (want.norm() + left.norm() * norm) + ((a - HALF * left.abs()).clamp_min(0).norm() + terms * 2.0 ** -24 * left.norm()) * norm * 1.01
+            most = HALF * want.norm() + rnd.norm() * norm + ((a - rnd).clamp_min(0).norm() + terms * 2.0 ** -24 * left.norm()) * norm * 1.01
             assert float(err.norm()) <= float(most) + 1e-30, float(err.norm() / most)
 
 
@@ -115,6 +117,27 @@ def test_token_logprobs(case):
         ex.check(*out)
         ex.check_gradients(g, e if entropy else None, gx, gw)
         assert not bool(gx[t == -100].any())
+
+
+@pytest.mark.parametrize("T", [1, 40, 300, 2500])
+def test_the_targets_rounding(T):
+    """Nearly all of these gradients comes from dl at the targets, which all but a few tokens share: their roundings would go one way in a row of either.
+    In the 2-norm what remains is the results' own rounding, and a bf16 step of the others and of the shared target's remainder."""
+    from metis_hip import token_logprobs
+    H, V = 528, 20011
+    x, w, t, _, _ = make(9, T, H, V, scale=0.05, ignored=0.1 if T > 1 else 0.0, sharp=False)
+    t = torch.where((t != -100) & (torch.arange(T, device=t.device) % 7 < 5), 12345, t)
+    g = torch.full((T,), 1.003, device="cuda")                 # of bf16's 1 and 1.0078: 0.003 off
+    gx, gw = torch.autograd.grad(token_logprobs(x.requires_grad_(), w.requires_grad_(), t), (x, w), g)
+    with torch.no_grad():
+        ex = Exact(x, w, t, 1.0)
+        ex.check_gradients(g, None, gx, gw)
+        d = torch.where(ex.live, g.double(), 0.0)[:, None] * (ex.onehot - ex.p)
+        # of the rows alone: the share of a gradient along itself, to which independent roundings of its elements (half a step at most, of either sign) add nothing
+        # but by chance: six times their root mean square, 2^-8 / 3^0.5 sum(v^4)^0.5 / sum(v^2)
+        for got, want in ((gx[ex.live][-1], (d @ ex.w)[ex.live][-1]), (gw[12345], d[:, 12345] @ ex.x)):
+            share = float(got.double() @ want / (want @ want)) - 1
+            assert abs(share) <= 6 * HALF / 3 ** 0.5 * float((want ** 4).sum().sqrt() / (want @ want)) + 2.0 ** -14, share
 
 
 @pytest.mark.parametrize("want", ["hidden", "weight"])
