@@ -740,17 +740,20 @@ __global__ __launch_bounds__(256) void head_gather_kernel(const Tokens tk, const
     }
 }
 
-// Per 256 rows of the vocabulary (and 512 columns): which rows of grad_weight are targets' (`row_of`: the first live token with that target, or -1) and, as the row
-// of that token, what `left` of all tokens with that target gives, in their order.  (Its own rounding to bf16 is 2^-8 of at most 2^-8 of the gradient.)
-__global__ __launch_bounds__(256) void head_targets_kernel(const int* __restrict__ index, const AtTarget target, const uint16_t* __restrict__ gathered, int H, int* __restrict__ row_of,
-                                                           uint16_t* __restrict__ rest)
+// Per 256 rows of the vocabulary: which rows of grad_weight are targets' (`row_of`: the first live token with that target, or -1) and, as the row of that
+// token, what `left` of all tokens with that target gives, in their order.  (Its own rounding to bf16 is 2^-8 of at most 2^-8 of the gradient.)  A wave takes
+// 512 columns of one such row; where the vocabulary has few rows, gridDim.y workgroups share its columns.
+__global__ __launch_bounds__(1024) void head_targets_kernel(const int* __restrict__ index, const AtTarget target, const uint16_t* __restrict__ gathered, int H, int* __restrict__ row_of,
+                                                            uint16_t* __restrict__ rest)
 {
-    __shared__ int first[256], times[256];
-    const int count = index[0], v0 = blockIdx.x * 256, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.y * 512 + lane * 8;
-    first[threadIdx.x] = INT32_MAX;
-    times[threadIdx.x] = 0;
+    __shared__ int first[256], times[256], list[256], listed[4];
+    const int count = index[0], v0 = blockIdx.x * 256, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (threadIdx.x < 256) {
+        first[threadIdx.x] = INT32_MAX;
+        times[threadIdx.x] = 0;
+    }
     __syncthreads();
-    for (int m = threadIdx.x; m < count; m += 256) {
+    for (int m = threadIdx.x; m < count; m += 1024) {
         const int row = target.column[m] - v0;
         if (row >= 0 && row < 256) {
             atomicMin(&first[row], m);
@@ -758,13 +761,20 @@ __global__ __launch_bounds__(256) void head_targets_kernel(const int* __restrict
         }
     }
     __syncthreads();
-    if (blockIdx.y == 0) row_of[v0 + threadIdx.x] = times[threadIdx.x] ? first[threadIdx.x] : -1;
-    const int mine = threadIdx.x;                              // a wave's 64 rows, by lane
-    uint64_t rows = __ballot(times[mine] > 0);
-    while (rows) {
-        const int row = wave * 64 + __builtin_ctzll(rows), begin = __builtin_amdgcn_readfirstlane(first[row]);
+    const bool has = threadIdx.x < 256 && times[threadIdx.x & 255] > 0;
+    const uint64_t mask = __ballot(has);
+    if (wave < 4 && lane == 0) listed[wave] = __popcll(mask);
+    if (blockIdx.y == 0 && threadIdx.x < 256) row_of[v0 + threadIdx.x] = has ? first[threadIdx.x] : -1;
+    __syncthreads();
+    int at = __popcll(mask & ((1ull << lane) - 1ull));
+#pragma unroll
+    for (int w = 0; w < 3; ++w) at += w < wave ? listed[w] : 0;
+    if (has) list[at] = threadIdx.x;
+    __syncthreads();
+    const int chunks = ((H + 511) / 512 - (int)blockIdx.y + (int)gridDim.y - 1) / (int)gridDim.y, jobs = (listed[0] + listed[1] + listed[2] + listed[3]) * chunks;
+    for (int job = wave; job < jobs; job += 16) {
+        const int row = list[job / chunks], c = ((int)blockIdx.y + job % chunks * (int)gridDim.y) * 512 + lane * 8, begin = __builtin_amdgcn_readfirstlane(first[row]);
         int to_come = __builtin_amdgcn_readfirstlane(times[row]);
-        rows &= rows - 1;
         float sum[8] = {};
         for (int m0 = begin; m0 < count && to_come > 0; m0 += 64) {
             uint64_t same = to_come == 1 && m0 == begin ? 1ull : __ballot(m0 + lane < count && target.column[m0 + lane] == v0 + row);
@@ -881,36 +891,36 @@ __global__ __launch_bounds__(HL_THREADS, 2) void head_products_kernel(const Prod
     int tm, tn;
     hl_origin(job, tiles_v, tiles_h, tm, tn);
     const int m0 = tm * 256, n0 = tn * HL_BN, wn = (threadIdx.x >> 6) & 3;
+    const int thread = hl_thread(), lane = thread & 63, wm = thread >> 8, lr = lane & 31, hi = lane >> 5;
+    // Sums begin with what the targets' rows are to have added: which rows, asked for before the ring's stages (5 x 1536 against 131072, both gradients: 305 us;
+    // behind the products 313, and 297 without the targets' remainders), the values behind them.
     float16_t acc[4][HL_TN];
     hl_clear<4>(acc);
+    int from[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) from[i] = p.row_of[m0 + (wm * 4 + i) * 32 + lr];
     Pipe<4, true, true, true> pipe;
     pipe.lds = hl_lds;
     pipe.aim(Operand{p.dl + (int64_t)(m0 / 64) * p.rows * 64, 64, 256, nullptr, 32, p.rows * 64}, Operand{p.gathered + n0, p.H, p.H - n0, nullptr, 32, 0}, (count + 31) / 32, false);
     pipe.request(0);
     pipe.request(2);
-    pipe.multiply(acc);
-    const int thread = hl_thread(), lane = thread & 63, wm = thread >> 8, lr = lane & 31, hi = lane >> 5;
-    int from[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) from[i] = p.row_of[m0 + (wm * 4 + i) * 32 + lr];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if (!__any(from[i] >= 0)) continue;
-        if (from[i] >= 0) {
-            const uint16_t* rest = p.rest + (int64_t)from[i] * p.H + n0 + wn * 64 + 4 * hi;
+        if (from[i] < 0) continue;
+        const uint16_t* rest = p.rest + (int64_t)from[i] * p.H + n0 + wn * 64 + 4 * hi;
 #pragma unroll
-            for (int j = 0; j < HL_TN; ++j)
+        for (int j = 0; j < HL_TN; ++j)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    if (n0 + wn * 64 + j * 32 + 8 * g + 4 * hi >= p.H) continue;
-                    const uint2 r = *reinterpret_cast<const uint2*>(rest + j * 32 + 8 * g);
-                    acc[i][j][4 * g] += __uint_as_float(r.x << 16);
-                    acc[i][j][4 * g + 1] += __uint_as_float(r.x & 0xffff0000u);
-                    acc[i][j][4 * g + 2] += __uint_as_float(r.y << 16);
-                    acc[i][j][4 * g + 3] += __uint_as_float(r.y & 0xffff0000u);
-                }
-        }
+            for (int g = 0; g < 4; ++g) {
+                if (n0 + wn * 64 + j * 32 + 8 * g + 4 * hi >= p.H) continue;
+                const uint2 r = *reinterpret_cast<const uint2*>(rest + j * 32 + 8 * g);
+                acc[i][j][4 * g] = __uint_as_float(r.x << 16);
+                acc[i][j][4 * g + 1] = __uint_as_float(r.x & 0xffff0000u);
+                acc[i][j][4 * g + 2] = __uint_as_float(r.y << 16);
+                acc[i][j][4 * g + 3] = __uint_as_float(r.y & 0xffff0000u);
+            }
     }
+    pipe.multiply(acc);
     hl_store_bf16<4>(acc, hl_lds, p.grad_weight + (int64_t)m0 * p.H + n0 + wn * 64, p.H, p.width - m0, p.H - (n0 + wn * 64));
 }
 
@@ -1126,7 +1136,9 @@ int head_logprobs_backward(const void* hidden, int64_t ldh, const void* weight, 
                        (uint4*)gathered);
     if (hipGetLastError() != hipSuccess) return METIS_E_LAUNCH;
     if (grad_weight) {
-        hipLaunchKernelGGL(head_targets_kernel, dim3((unsigned)((V + 255) / 256), (unsigned)((H + 511) / 512)), dim3(256), 0, st, (const int*)index, target, (const uint16_t*)gathered, (int)H,
+        const int64_t fit = 2 * (int64_t)cus / ((V + 255) / 256), chunks = (H + 511) / 512;
+        const unsigned share = (unsigned)(fit < 1 ? 1 : fit < chunks ? fit : chunks);
+        hipLaunchKernelGGL(head_targets_kernel, dim3((unsigned)((V + 255) / 256), share), dim3(1024), 0, st, (const int*)index, target, (const uint16_t*)gathered, (int)H,
                            row_of, rest);
         if (hipGetLastError() != hipSuccess) return METIS_E_LAUNCH;
     }
