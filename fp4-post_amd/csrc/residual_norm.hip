@@ -13,7 +13,8 @@
 //
 // A row belongs to W waves (one per 512 columns up to 2048, then four or eight), lane l of wave w holding the chunks of eight elements
 // (i W + w) 64 + l: every access instruction of a wave covers consecutive bytes, the row is read once, its sums are folded across the lanes with
-// DPP moves and across the waves through LDS.  Bound by memory.
+// DPP moves and across the waves through LDS.  Bound by memory: 8192 x 3584 bf16 forward 40 us (5.9 TB/s of the 8 bytes an element), backward
+// 40 and 4 for the columns' sums (4.4 TB/s of 6 bytes: its reads, one after the other's folds, do not fill the queue as a copy's do).
 #include "chunk8.h"
 #include "metis_host.h"
 
@@ -151,9 +152,10 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void residual_norm_kernel(con
 // partial rows of the workspace, [sum][gate row][slab][column], which residual_norm_sums_kernel adds in order.  No gate: one gate row for all rows.
 // Where there are more gate rows than workgroups a workgroup takes several, one after the other, and writes the gate's gradient itself.
 //
-// The sums' registers leave room for two waves per SIMD, one workgroup of eight per compute unit (two of four would leave twice the partial rows: 2103 x 4096
-// with a norm behind the block and gates, binary32 stream, 42 us, now 37), so a row's reads have to be under way while the one before is
-// worked on: the next row is requested before the folds (AHEAD; where the registers hold it).  weight, post_weight and the gate stay in LDS, every lane reading what it put there itself.
+// The sums' registers leave room for two waves per SIMD, one workgroup of eight per compute unit: two of four leave twice the partial rows (512 x 3584 bf16 12.8 us,
+// now 10.6, 2048 x 3584 17.3 and 16.1, 4099 x 3584 39.6 and 38.8; 2103 x 4096 with a norm behind the block and gates, binary32 stream, is the one that loses,
+// 42.1 and 43.7 with the sums).  A row's reads have to be under way while the one before is worked on: the next row is requested before the folds (AHEAD; where
+// the registers hold it).  weight, post_weight and the gate stay in LDS, every lane reading what it put there itself.
 template <class R, class B> struct RowIn {                    // one chunk of the lane's share of a row
     R h, gh;
     B gn, y;

@@ -72,9 +72,9 @@ def model_token_logprobs(model, input_ids: torch.Tensor, attention_mask: torch.T
     head = model.get_output_embeddings()
     if getattr(head, "bias", None) is not None:
         raise ValueError("model_token_logprobs: a head without bias")
-    cap = getattr(getattr(model, "config", None), "final_logit_softcapping", None)
-    if cap:
-        raise ValueError("model_token_logprobs: a head whose logits are used as they are, not capped")
+    config = getattr(model, "config", None)
+    if getattr(config, "final_logit_softcapping", None) or any(getattr(config, k, None) not in (None, 1, 1.0) for k in ("logit_scale", "logits_scaling")):
+        raise ValueError("model_token_logprobs: a head whose logits are used as they are, not capped or scaled")
     out = model.base_model(input_ids=input_ids, attention_mask=attention_mask, **inputs)
     hidden = out[0] if isinstance(out, tuple) else out.last_hidden_state
     targets = (input_ids if labels is None else labels)[:, 1:]

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from metis_hip import MetisHipError, _lib, linear_cross_entropy, token_logprobs
+from metis_hip import MetisHipError, _lib, linear_cross_entropy, model_token_logprobs, token_logprobs
 
 
 def test_host_tensors_are_refused():
@@ -13,6 +13,14 @@ def test_host_tensors_are_refused():
         linear_cross_entropy(x, w, t)
     with pytest.raises(ValueError, match="reduction"):
         linear_cross_entropy(x, w, t, reduction="max")
+
+
+@pytest.mark.parametrize("setting", [dict(final_logit_softcapping=30.0), dict(logit_scale=0.0625), dict(logits_scaling=8.0)])
+def test_heads_that_do_more_than_a_product_are_refused(setting):
+    from types import SimpleNamespace
+    model = SimpleNamespace(config=SimpleNamespace(**setting), get_output_embeddings=lambda: SimpleNamespace(weight=None, bias=None))
+    with pytest.raises(ValueError, match="not capped or scaled"):
+        model_token_logprobs(model, torch.zeros(1, 4, dtype=torch.int64))
 
 
 def _forward(**changes):
@@ -43,10 +51,10 @@ def test_workspaces():
     assert _forward(tokens=0, hidden=None, workspace=None) == _lib.OK
     back = L.metis_head_logprobs_backward_workspace_bytes
     assert back(4, 64, 100, 1, 1) >= back(4, 64, 100, 0, 1) > 0 and back(4, 64, 100, 1, 0) > 0 and back(0, 64, 100, 1, 1) == 0
-    # a piece of the gradient of the logits, not the whole: 4096 x 131072 of it would be 1 GiB
-    assert back(4096, 3584, 131072, 0, 0) <= 256 << 20
+    # a piece of the gradient of the logits, not the whole: 4096 x 131072 of it would be 1 GiB (and three numbers a token)
+    assert back(4096, 3584, 131072, 0, 0) <= (256 << 20) + 12 * 4096
     # and with many tokens at most twice the binary32 gradient of hidden
-    assert back(1 << 20, 4096, 131072, 0, 0) <= 8 * (1 << 20) * 4096
+    assert back(1 << 20, 4096, 131072, 0, 0) <= 8 * (1 << 20) * 4096 + 12 * (1 << 20)
 
 
 def _backward(**changes):
