@@ -1051,7 +1051,7 @@ bool operands_ok(const void* hidden, int64_t ldh, const void* weight, int64_t ld
 {
     if (!hidden || !weight || !targets || !index || ldh < H || ldw < H || ldh % 8 || ldw % 8 || ldw > INT32_MAX / 128) return false;
     if ((uintptr_t)hidden % 16 || (uintptr_t)weight % 16 || (uintptr_t)targets % 8 || (uintptr_t)index % 256) return false;
-    return temperature > 0.0f && temperature < INFINITY;
+    return temperature > 0.0f && temperature < INFINITY && 1.44269504088896f / temperature < INFINITY;
 }
 
 }  // namespace

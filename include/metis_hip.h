@@ -991,11 +991,12 @@ int metis_swiglu_backward(const void *gate, int64_t ld_gate, const void *up, int
  *   logp, lse, entropy  float [tokens]; entropy may be NULL
  *   index    metis_head_index_bytes(tokens) bytes, 256-byte aligned: written by the forward, read by the backward
  * Backward, for gradients of logp and entropy (float [tokens], NULL: zero; with grad_entropy also entropy):
- *   dl = (grad_logp (1[v = target] - p) - grad_entropy p (l - lse + entropy)) / temperature, rounded to bf16 once
+ *   dl = (grad_logp (1[v = target] - p) - grad_entropy p (l - lse + entropy)) / temperature, rounded to bf16 once; what the
+ *   rounding leaves out at the target is added to both gradients
  *   grad_hidden = dl weight, grad_weight = dl^T hidden, dense bf16, sums in binary32 in a fixed order; NULL: not wanted
  * The logits are formed again in pieces of the vocabulary.  Workspaces need no initialisation; the backward's holds one
  * piece of dl (at most the larger of 256 MiB and twice the binary32 gradient of hidden, at least 256 columns) beside the
- * binary32 gradient of hidden.
+ * binary32 gradient of hidden and, for grad_weight, two bf16 copies of hidden's size and 4 bytes a row of the vocabulary.
  */
 size_t metis_head_index_bytes(int64_t tokens);
 size_t metis_head_logprobs_workspace_bytes(int64_t tokens, int64_t H, int64_t V, int entropy);

@@ -182,3 +182,48 @@ def test_refusals_of_heads():
     model.lm_head = nn.Linear(64, 515, bias=True, device="cuda", dtype=BF)
     with pytest.raises(ValueError, match="bias"):
         model_token_logprobs(model, ids, mask)
+
+
+def test_forward_and_backward_in_a_graph():
+    """The three operators with their recorded backward, captured on leaves of their own and replayed on changed values, eager steps on copies between the
+    replays; every replay has the eager step's bits."""
+    from metis_hip import residual_norm, swiglu, token_logprobs
+    gen = torch.Generator().manual_seed(31)
+
+    def values():
+        def normal(*shape, scale=1.0):
+            return (torch.randn(*shape, generator=gen) * scale).to(BF).cuda()
+        x, y, weight, up, head = normal(2, 65, 256), normal(2, 65, 256), 1 + normal(256, scale=0.1), normal(2, 65, 256), normal(1003, 256, scale=0.1)
+        targets = torch.randint(1003, (2, 65), generator=gen)
+        targets[0, :9] = -100
+        return [x, y, weight, up, head], targets.cuda(), torch.randn(2, 65, generator=gen).cuda()
+
+    def step(leaves, targets, g):
+        x, y, weight, up, head = leaves
+        h, n = residual_norm(x, y, weight)
+        logp, ent = token_logprobs(swiglu(n, up) + h, head, targets, entropy=True)
+        return [logp.detach(), *torch.autograd.grad((logp, ent), leaves, (g, 0.1 * g))]
+
+    def eager(tensors, targets, g):
+        return step([t.detach().clone().requires_grad_() for t in tensors], targets, g)
+
+    tensors, targets, g = values()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        eager(tensors, targets, g)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    leaves = [t.requires_grad_() for t in tensors]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(leaves, targets, g)
+    for _ in range(3):
+        more, new_targets, new_g = values()
+        with torch.no_grad():
+            for a, b in zip((*leaves, targets, g), (*more, new_targets, new_g)):
+                a.copy_(b)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, eager(leaves, targets, g)))

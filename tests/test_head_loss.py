@@ -32,7 +32,7 @@ def _forward(**changes):
 
 BAD = [dict(H=60), dict(H=0), dict(H=65552, ldh=65552, ldw=65552), dict(V=0), dict(V=(1 << 22) + 1), dict(tokens=-1), dict(tokens=(1 << 24) + 1), dict(hidden=None), dict(weight=None),
        dict(targets=None), dict(index=None), dict(ldh=56), dict(ldw=56), dict(ldh=68), dict(ldw=68), dict(hidden=4104), dict(weight=4104), dict(targets=4100), dict(index=4112),
-       dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("inf")), dict(temperature=float("nan"))]
+       dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("inf")), dict(temperature=float("nan")), dict(temperature=4e-39)]
 
 
 @pytest.mark.parametrize("changes", BAD + [dict(logp=None), dict(lse=None), dict(lse=4098), dict(entropy=4098)])
