@@ -973,8 +973,10 @@ struct BackwardPlan {
     int splits;
 };
 // Pieces: as many columns as 256 MiB of dl hold, or twice the bytes of the binary32 gradient of hidden where that is more (what a piece costs apart from its
-// products is one pass over that gradient).  Splits of grad_hidden's contraction: as many as leave none of its tiles longer than a compute unit's
-// share of the launch.
+// products is one pass over that gradient).  Splits of grad_hidden's contraction: beside grad_weight, whose tiles fill the launch up, as many as leave none of
+// its tiles longer than a compute unit's share; by itself those with the fewest stages in a row, a tile's beginning and end counted as eight and a pass over the
+// slabs as its bytes (in a stage's 0.8 us 4 MB go), for tokens that are all live.  (By itself with the share's rule 540 x 2048 against 65536 had 11 splits of 24
+// tiles, a second round of eight: 442 us, now 352; 5 x 1536 against 131072 222 and 174, 64 x 3584 499 and 373, 4096 x 3584 7.0 and 6.7 ms.)
 BackwardPlan backward_plan(int64_t tokens, int64_t H, int64_t V, bool want_weight)
 {
     BackwardPlan p;
@@ -992,6 +994,16 @@ BackwardPlan backward_plan(int64_t tokens, int64_t H, int64_t V, bool want_weigh
     int64_t s = (stages + share - 1) / share;
     if (s > 64) s = 64;
     p.splits = (int)(s < 1 ? 1 : s);
+    if (want_weight) return p;
+    const int64_t rows = tokens <= kListTokens ? 64 : 64 * (tokens <= kFewTokens ? hl_row_tiles((int)tokens) : 4), live_tiles = (tokens + rows - 1) / rows * tiles_h;
+    double least = 0.0;
+    for (int n = 1; n <= 64 && (n == 1 || n * 16 <= stages); ++n) {
+        const double rounds = (double)((live_tiles * n + cus - 1) / cus), cost = rounds * ((double)stages / n + 8.0) + (double)n * (double)p.rows * (double)H * 8.0 / 4e6;
+        if (n == 1 || cost < least) {
+            least = cost;
+            p.splits = n;
+        }
+    }
     return p;
 }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
