@@ -987,7 +987,8 @@ BackwardPlan backward_plan(int64_t tokens, int64_t H, int64_t V, bool want_weigh
     if (most < 256) most = 256;
     const int64_t pieces = (V + most - 1) / most;
     p.width = padded((V + pieces - 1) / pieces, 256);
-    const int64_t tiles_h = (H + 255) / 256, tiles = most_row_tiles(tokens) * tiles_h, stages = p.width / 32;
+    const int64_t tiles_h = (H + 255) / 256, stages = p.width / 32;
+    const int64_t rows = tokens <= kListTokens ? 64 : 64 * (tokens <= kFewTokens ? hl_row_tiles((int)tokens) : 4), tiles = (tokens + rows - 1) / rows * tiles_h;
     const int64_t all = tiles * stages + (want_weight ? p.width / 256 * tiles_h * ((tokens + 31) / 32) : 0), cus = device_cus();
     int64_t share = (all + cus - 1) / cus;
     if (share < 16) share = 16;
@@ -995,10 +996,9 @@ BackwardPlan backward_plan(int64_t tokens, int64_t H, int64_t V, bool want_weigh
     if (s > 64) s = 64;
     p.splits = (int)(s < 1 ? 1 : s);
     if (want_weight) return p;
-    const int64_t rows = tokens <= kListTokens ? 64 : 64 * (tokens <= kFewTokens ? hl_row_tiles((int)tokens) : 4), live_tiles = (tokens + rows - 1) / rows * tiles_h;
     double least = 0.0;
     for (int n = 1; n <= 64 && (n == 1 || n * 16 <= stages); ++n) {
-        const double rounds = (double)((live_tiles * n + cus - 1) / cus), cost = rounds * ((double)stages / n + 8.0) + (double)n * (double)p.rows * (double)H * 8.0 / 4e6;
+        const double rounds = (double)((tiles * n + cus - 1) / cus), cost = rounds * ((double)stages / n + 8.0) + (double)n * (double)p.rows * (double)H * 8.0 / 4e6;
         if (n == 1 || cost < least) {
             least = cost;
             p.splits = n;
