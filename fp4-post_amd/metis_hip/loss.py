@@ -75,9 +75,12 @@ def model_token_logprobs(model, input_ids: torch.Tensor, attention_mask: torch.T
     config = getattr(model, "config", None)
     if getattr(config, "final_logit_softcapping", None) or any(getattr(config, k, None) not in (None, 1, 1.0) for k in ("logit_scale", "logits_scaling")):
         raise ValueError("model_token_logprobs: a head whose logits are used as they are, not capped or scaled")
+    weight = getattr(head, "weight", None)
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise ValueError(f"model_token_logprobs: an output embedding with one weight [V, H], not {type(head).__name__}")
     out = model.base_model(input_ids=input_ids, attention_mask=attention_mask, **inputs)
     hidden = out[0] if isinstance(out, tuple) else out.last_hidden_state
     targets = (input_ids if labels is None else labels)[:, 1:]
     if attention_mask is not None:
         targets = targets.masked_fill(attention_mask[:, 1:] == 0, ignore_index)
-    return token_logprobs(hidden[:, :-1], head.weight, targets, temperature=temperature, ignore_index=ignore_index, entropy=entropy)
+    return token_logprobs(hidden[:, :-1], weight, targets, temperature=temperature, ignore_index=ignore_index, entropy=entropy)

@@ -23,6 +23,13 @@ def test_heads_that_do_more_than_a_product_are_refused(setting):
         model_token_logprobs(model, torch.zeros(1, 4, dtype=torch.int64))
 
 
+@pytest.mark.parametrize("head", [None, torch.nn.Identity(), torch.nn.LayerNorm(8, bias=False)])
+def test_heads_without_one_matrix_are_refused(head):
+    from types import SimpleNamespace
+    with pytest.raises(ValueError, match="one weight"):
+        model_token_logprobs(SimpleNamespace(get_output_embeddings=lambda: head), torch.zeros(1, 4, dtype=torch.int64))
+
+
 def _forward(**changes):
     a = dict(hidden=4096, ldh=64, weight=4096, ldw=64, targets=4096, ignore=-100, tokens=4, H=64, V=100, temperature=1.0, logp=4096, lse=4096, entropy=None, index=4096,
              workspace=4096, bytes=1 << 30, stream=None)
