@@ -67,8 +67,9 @@ def model_token_logprobs(model, input_ids: torch.Tensor, attention_mask: torch.T
     (`base_model`) gives the last hidden states, its output embedding's weight is the head.  What a DPO or GRPO step takes of the policy and of the
     reference model.
 
-    labels defaults to input_ids; positions with ignore_index, or that attention_mask leaves out, have 0 and no gradient (and are not
-    computed).  inputs: further arguments of the decoder."""
+    labels defaults to input_ids; positions with ignore_index have 0 and no gradient (and are not computed), and so do those that
+    attention_mask leaves out: where the token is masked, or the position before it, whose hidden state would predict it (padding on the left: a
+    row's first token has nothing to be predicted from).  inputs: further arguments of the decoder."""
     head = model.get_output_embeddings()
     if getattr(head, "bias", None) is not None:
         raise ValueError("model_token_logprobs: a head without bias")
@@ -82,5 +83,5 @@ def model_token_logprobs(model, input_ids: torch.Tensor, attention_mask: torch.T
     hidden = out[0] if isinstance(out, tuple) else out.last_hidden_state
     targets = (input_ids if labels is None else labels)[:, 1:]
     if attention_mask is not None:
-        targets = targets.masked_fill(attention_mask[:, 1:] == 0, ignore_index)
+        targets = targets.masked_fill((attention_mask[:, 1:] == 0) | (attention_mask[:, :-1] == 0), ignore_index)
     return token_logprobs(hidden[:, :-1], weight, targets, temperature=temperature, ignore_index=ignore_index, entropy=entropy)

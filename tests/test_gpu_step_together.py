@@ -175,6 +175,41 @@ def test_mlps_of_a_model_are_replaced():
         assert bool(((after.float() - before.float()).abs() <= 2.0 ** -8 * (4 * terms + 2 * before.float().abs())).all())
 
 
+def test_padding_on_the_left_reaches_nothing():
+    """Hidden states of padding that are NaN, on the left and on the right: the log-probabilities are those of the rows without padding (the same
+    products of the same rows, in tiles of other neighbours: a logit is a binary32 sum of 64 products whose magnitudes make less than 8 together, off by at
+    most 64 2^-24 8 = 2^-15, and so is the lse; both on two sides: 2^-13), and no gradient is touched."""
+    from metis_hip import model_token_logprobs, token_logprobs
+    torch.manual_seed(9)
+    vocab, H, B, S = 515, 64, 3, 40
+    hidden = torch.randn(B, S, H).to(BF).cuda()
+    mask = torch.ones(B, S, dtype=torch.int64)
+    mask[0, :13] = 0
+    mask[1, :39] = 0
+    mask[2, 30:] = 0
+    mask = mask.cuda()
+    ids = torch.randint(vocab, (B, S)).cuda()
+    padded = hidden.masked_fill(mask[:, :, None] == 0, float("nan")).requires_grad_()
+
+    class Known(nn.Module):
+        def forward(self, input_ids, attention_mask=None):
+            return (padded,)
+
+    model = Model(vocab=vocab, hidden=H, inter=64, layers=1).to(BF).cuda()
+    model.base_model = Known()
+    logp = model_token_logprobs(model, ids, mask)
+    logp.sum().backward()
+    live = (mask[:, 1:] != 0) & (mask[:, :-1] != 0)
+    assert not bool(logp[~live].any()) and bool(logp.isfinite().all())
+    for b, (first, end) in enumerate(((13, S), (39, S), (0, 30))):
+        assert int(live[b].sum()) == end - first - 1
+        with torch.no_grad():
+            alone = token_logprobs(hidden[b, first:end - 1], model.lm_head.weight, ids[b, first + 1:end])
+        assert bool(((logp[b, first:end - 1] - alone).abs() <= 2.0 ** -13).all())
+    assert bool(padded.grad.isfinite().all()) and not bool(padded.grad[:, :-1][~live].any())
+    assert bool(model.lm_head.weight.grad.isfinite().all()) and bool(model.lm_head.weight.grad.any())
+
+
 def test_refusals_of_heads():
     from metis_hip import model_token_logprobs
     model = Model(hidden=64, inter=64, layers=1).to(BF).cuda()

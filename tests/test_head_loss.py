@@ -81,3 +81,36 @@ def test_the_backward_wants_its_workspace():
     for changes in (dict(workspace=None), dict(bytes=need - 1), dict(workspace=4096 + 16)):
         assert _backward(**changes) == _lib.E_WORKSPACE
     assert _backward(gh=None, gw=None, workspace=None) == _lib.OK
+
+
+def _seen_targets(monkeypatch, ids, mask, **more):
+    """The targets and hidden states that model_token_logprobs hands on, without a device."""
+    from types import SimpleNamespace
+    from metis_hip import loss
+    got = {}
+
+    def take(hidden, weight, targets, **_):
+        got.update(hidden=hidden, targets=targets)
+        return targets
+    monkeypatch.setattr(loss, "token_logprobs", take)
+    hidden = torch.zeros(*ids.shape, 8)
+    model = SimpleNamespace(get_output_embeddings=lambda: torch.nn.Linear(8, 32, bias=False), base_model=lambda **_: (hidden,))
+    model_token_logprobs(model, ids, mask, **more)
+    return got["targets"].tolist()
+
+
+@pytest.mark.parametrize("mask,want", [([0, 0, 1, 1, 1], [-100, -100, 6, 7]),        # padded on the left: the first real token has no context
+                                       ([1, 1, 1, 0, 0], [4, 5, -100, -100]),        # on the right
+                                       ([1, 0, 1, 1, 0], [-100, -100, 6, -100]),     # a hole: neither into it nor out of it
+                                       ([0, 0, 0, 0, 0], [-100] * 4), ([0, 0, 0, 0, 1], [-100] * 4), ([1] * 5, [4, 5, 6, 7]), (None, [4, 5, 6, 7])])
+def test_tokens_count_where_they_and_the_position_before_them_are_there(monkeypatch, mask, want):
+    ids = torch.tensor([[3, 4, 5, 6, 7]])
+    for dtype in (torch.int64, torch.bool):
+        assert _seen_targets(monkeypatch, ids, None if mask is None else torch.tensor([mask], dtype=dtype)) == [want]
+
+
+def test_labels_and_the_mask_both_leave_tokens_out(monkeypatch):
+    ids, labels = torch.tensor([[3, 4, 5, 6, 7]]), torch.tensor([[-100, -100, -100, 9, 10]])
+    assert _seen_targets(monkeypatch, ids, torch.tensor([[0, 1, 1, 1, 1]]), labels=labels) == [[-100, -100, 9, 10]]
+    assert _seen_targets(monkeypatch, ids, torch.tensor([[0, 0, 0, 1, 1]]), labels=labels) == [[-100, -100, -100, 10]]
+    assert _seen_targets(monkeypatch, ids, torch.tensor([[1, 1, 1, 1, 0]]), labels=labels, ignore_index=10) == [[-100, -100, 9, 10]]
