@@ -6,6 +6,8 @@ result rounded once; their autograd nodes are compiled (csrc/host_autograd.cpp).
 """
 from __future__ import annotations
 
+import inspect
+
 import torch
 from torch import nn
 
@@ -57,9 +59,51 @@ class GatedMLP(nn.Module):
         return self.down_proj(nn.functional.silu(gate) * up)
 
 
+# what a module may have registered that its replacement would not run, by nn.Module's names
+_REGISTERED = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks", "_state_dict_hooks", "_state_dict_pre_hooks",
+               "_load_state_dict_pre_hooks", "_load_state_dict_post_hooks")
+
+
+@torch.no_grad()
+def _is_gated_mlp(mlp: nn.Module) -> bool:
+    """Whether the module computes down_proj(silu(gate_proj(x)) * up_proj(x)) of its one argument and holds nothing else that counts.  Its class's
+    forward is asked, on a twin with the module's attributes and small projections in 64 bits on the CPU, in training and in evaluation: factors, clamps and
+    dropout kept in plain attributes show there, and the module's own projections are not run."""
+    kind = type(mlp)
+    if (any(t is not None for t in (*mlp._parameters.values(), *mlp._buffers.values())) or any(getattr(mlp, name, None) for name in _REGISTERED)
+            or "forward" in vars(mlp) or kind.__call__ is not nn.Module.__call__):
+        return False
+    try:
+        (argument,) = list(inspect.signature(kind.forward).parameters.values())[1:]
+        if argument.kind not in (argument.POSITIONAL_ONLY, argument.POSITIONAL_OR_KEYWORD):
+            return False
+        with torch.device("cpu"):
+            small = {}
+            for k, (name, n, m) in enumerate((("gate_proj", 4, 6), ("up_proj", 4, 6), ("down_proj", 6, 4))):
+                small[name] = nn.Linear(n, m, bias=False, dtype=torch.float64, device="meta").to_empty(device="cpu")
+                small[name].weight.copy_(torch.sin(torch.arange(1.0 + 7 * k, 1 + 7 * k + n * m, dtype=torch.float64) ** 2).reshape(m, n))
+            # from rows of zeros to rows far beyond any clamp
+            scale = torch.tensor([0.0, 1e-2, 1.0, 3e1, 1e3, 1e6], dtype=torch.float64).reshape(1, 6, 1)
+            x = torch.cos(torch.arange(48, dtype=torch.float64) ** 2).reshape(2, 6, 4) * scale
+            want = small["down_proj"](nn.functional.silu(small["gate_proj"](x)) * small["up_proj"](x))
+            twin = object.__new__(kind)
+            twin.__dict__.update(vars(mlp), _modules={**mlp._modules, **small})
+            for training in (True, False):
+                twin.__dict__["training"] = training
+                with torch.random.fork_rng(devices=[]):
+                    got = kind.forward(twin, x.clone())
+                # (a forward that goes through binary32 on its way is the formula too)
+                if not isinstance(got, torch.Tensor) or got.shape != want.shape or not bool(((got - want).abs() <= 1e-5 * want.abs().amax(-1, keepdim=True)).all()):
+                    return False
+    except Exception:                                              # (asks its projections for more than a product, or its caller for more than x)
+        return False
+    return True
+
+
 def fuse_gated_mlps(model: nn.Module) -> int:
-    """Replace every MLP that holds gate_proj, up_proj and down_proj around a SiLU (`act_fn`), and nothing else with parameters, by GatedMLP on
-    the same projections.  Returns the number replaced."""
+    """Replace every MLP that holds gate_proj, up_proj and down_proj around a SiLU (`act_fn`) by GatedMLP on the same projections, where that is all
+    it does: one with parameters, buffers, hooks or a forward of its own beside them, or whose forward computes anything else, stays as it is.  Returns the number
+    replaced."""
     replaced = 0
     for parent in list(model.modules()):
         for name, mlp in list(parent.named_children()):
@@ -67,6 +111,8 @@ def fuse_gated_mlps(model: nn.Module) -> int:
             act = getattr(mlp, "act_fn", None)
             silu = isinstance(act, nn.SiLU) or act is nn.functional.silu or type(act).__name__ == "SiLUActivation"
             if isinstance(mlp, GatedMLP) or not silu or not {"gate_proj", "up_proj", "down_proj"} <= parts.keys() <= {"gate_proj", "up_proj", "down_proj", "act_fn"}:
+                continue
+            if not _is_gated_mlp(mlp):
                 continue
             fused = GatedMLP(parts["gate_proj"], parts["up_proj"], parts["down_proj"])
             fused.train(mlp.training)

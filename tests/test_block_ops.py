@@ -1,10 +1,10 @@
-"""residual_norm and swiglu: what is refused, without a device."""
+"""residual_norm, swiglu and the modules that call them: what is refused or left as it is, without a device."""
 import ctypes
 
 import pytest
 import torch
 
-from metis_hip import MetisHipError, _lib, ops, residual_norm, swiglu
+from metis_hip import GatedMLP, MetisHipError, _lib, fuse_gated_mlps, ops, residual_norm, swiglu
 
 
 def test_host_tensors_are_refused():
@@ -82,3 +82,142 @@ def test_swiglu_refuses_before_a_launch(changes):
 def test_swiglu_refuses_more_pieces_than_it_counts():
     rows = (1 << 31) // 8
     assert _lib.load().metis_swiglu(4096, 64, 4096, 64, rows, 64, 0, 4096, None) == _lib.E_TOO_LARGE
+
+
+class _Mlp(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        Linear = torch.nn.Linear
+        self.gate_proj, self.up_proj, self.down_proj, self.act_fn = Linear(16, 24, bias=False), Linear(16, 24), Linear(24, 16, bias=False), torch.nn.SiLU()
+
+    def forward(self, x):
+        return self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
+
+
+class _Cast(_Mlp):                                                       # the same formula, written in another way
+    def forward(self, hidden_states):
+        shape = hidden_states.shape
+        x = hidden_states.reshape(-1, shape[-1])
+        gate = torch.nn.functional.silu(self.gate_proj(x).float()).to(x.dtype)
+        return self.down_proj(self.up_proj(x) * gate).view(shape)
+
+
+class _GateMultiplier(_Mlp):
+    multiplier = 1.5
+
+    def forward(self, x):
+        return self.down_proj(self.act_fn(self.gate_proj(x) * self.multiplier) * self.up_proj(x))
+
+
+class _DownMultiplier(_Mlp):
+    def __init__(self):
+        super().__init__()
+        self.multipliers = [1.0, 0.5]
+
+    def forward(self, x):
+        return self.down_proj(self.act_fn(self.gate_proj(x) * self.multipliers[0]) * self.up_proj(x)) * self.multipliers[1]
+
+
+class _Clamped(_Mlp):
+    def forward(self, x):
+        return self.down_proj(self.act_fn(self.gate_proj(x).clamp(max=200.0)) * self.up_proj(x))
+
+
+class _Dropout(_Mlp):
+    def forward(self, x):
+        return self.down_proj(torch.nn.functional.dropout(self.act_fn(self.gate_proj(x)) * self.up_proj(x), 0.1, self.training))
+
+
+class _Swapped(_Mlp):
+    def forward(self, x):
+        return self.down_proj(self.act_fn(self.up_proj(x)) * self.gate_proj(x))
+
+
+class _Residual(_Mlp):
+    def forward(self, x):
+        return x + super().forward(x)
+
+
+class _Optional(_Mlp):
+    def forward(self, x, scale=None):
+        x = super().forward(x)
+        return x if scale is None else x * scale
+
+
+class _Pair(_Mlp):
+    def forward(self, x):
+        return super().forward(x), None
+
+
+class _OwnParameter(_Mlp):                                               # (not used: it would vanish from the model all the same)
+    def __init__(self):
+        super().__init__()
+        self.scale = torch.nn.Parameter(torch.ones(()))
+
+
+class _OwnBuffer(_Mlp):
+    def __init__(self):
+        super().__init__()
+        self.register_buffer("scale", torch.ones(()))
+
+
+def _hooked(register):
+    def make():
+        mlp = _Mlp()
+        getattr(mlp, register)(lambda *_: None)
+        return mlp
+    return make
+
+
+def _with_its_own_forward():
+    mlp = _Mlp()
+    mlp.forward = lambda x: x
+    return mlp
+
+
+def _in_a_model(mlp, train):
+    model = torch.nn.Module()
+    model.layer = torch.nn.Module()
+    model.layer.mlp = mlp
+    return model.train(train)
+
+
+@pytest.mark.parametrize("train", [True, False])
+@pytest.mark.parametrize("make", [_Mlp, _Cast])
+def test_mlps_that_are_the_formula_are_replaced(make, train):
+    mlp = make()
+    model = _in_a_model(mlp, train)
+    names, calls = [n for n, _ in model.named_parameters()], []
+    for p in (mlp.gate_proj, mlp.up_proj, mlp.down_proj):
+        p.register_forward_hook(lambda *_: calls.append(1))
+    before = torch.get_rng_state()
+    assert fuse_gated_mlps(model) == 1 and isinstance(model.layer.mlp, GatedMLP) and model.layer.mlp.training == train
+    assert not calls and torch.equal(torch.get_rng_state(), before)      # (the projections themselves were not asked)
+    assert [n for n, _ in model.named_parameters()] == names and model.layer.mlp.gate_proj is mlp.gate_proj
+
+
+@pytest.mark.parametrize("train", [True, False])
+@pytest.mark.parametrize("make", [_GateMultiplier, _DownMultiplier, _Clamped, _Dropout, _Swapped, _Residual, _Optional, _Pair, _OwnParameter, _OwnBuffer, _with_its_own_forward,
+                                  *(_hooked(r) for r in ("register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook", "register_full_backward_pre_hook",
+                                                         "register_state_dict_pre_hook"))])
+def test_mlps_that_do_more_stay_as_they_are(make, train):
+    torch.manual_seed(1)
+    mlp = make()
+    model = _in_a_model(mlp, train)
+    names, x = sorted(model.state_dict()), torch.randn(3, 5, 16)
+    attributes = dict(vars(mlp))
+    assert fuse_gated_mlps(model) == 0 and model.layer.mlp is mlp
+    assert sorted(model.state_dict()) == names and dict(vars(mlp)) == attributes
+    if make not in (_Dropout, _Pair):
+        with torch.no_grad():
+            assert torch.equal(model.layer.mlp(x), mlp(x))
+
+
+def test_mlps_of_a_library_are_told_apart():
+    """The same children and activation in both: one multiplies in its forward."""
+    transformers = pytest.importorskip("transformers")
+    from transformers.models.falcon_h1.modeling_falcon_h1 import FalconH1MLP
+    from transformers.models.llama.modeling_llama import LlamaMLP
+    small = dict(hidden_size=16, intermediate_size=24, num_attention_heads=2, num_key_value_heads=2)
+    assert fuse_gated_mlps(_in_a_model(LlamaMLP(transformers.LlamaConfig(**small)), True)) == 1
+    assert fuse_gated_mlps(_in_a_model(FalconH1MLP(transformers.FalconH1Config(**small, mlp_multipliers=[2.0, 0.5])), True)) == 0
