@@ -7,7 +7,11 @@ operator on the last hidden states and the head's weight.
 """
 from __future__ import annotations
 
+import inspect
+from collections.abc import Mapping
+
 import torch
+from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -61,6 +65,59 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     return loss.sum() if reduction == "sum" else loss.sum() / (targets != ignore_index).sum()
 
 
+class _Known(nn.Module):
+    """A decoder's stand-in that returns `out`: in place of the whole of it and of any module inside; whatever else is asked of it is the decoder's own."""
+
+    def __init__(self, out, decoder):
+        super().__init__()
+        self.__dict__["__known"] = out, decoder                    # (a name that no decoder's attribute has; not registered as its module)
+
+    def __getattr__(self, name):
+        value = getattr(self.__dict__["__known"][1], name)
+        return self if isinstance(value, nn.Module) else value
+
+    def forward(self, *args, **kwargs):
+        return self.__dict__["__known"][0]
+
+
+@torch.no_grad()
+def _logits_are_the_product(model, head, weight: torch.Tensor, out, masked: bool, inputs: dict) -> bool:
+    """Whether the model's logits are its last hidden states times the head's weight, with no factor, cap, shift or cut on the way.  Its class's forward is
+    asked, on a twin with the model's attributes whose decoder returns known hidden states (as `out`, its output, holds them) and whose head is a small one, on the
+    CPU: no setting has to be known by its name.  A model without a forward of its own has nothing to say against it."""
+    model = getattr(model, "_orig_mod", model)                     # (compiled)
+    kind = type(model)
+    if not isinstance(model, nn.Module) or kind.forward is nn.Module.forward:
+        return True
+    rows, H, V = 3, 2, weight.shape[0]
+    try:
+        with torch.device("cpu"):
+            # a row of zeros (a shift), rows of usual size and beyond any cap; as many columns as the head has
+            hidden = torch.cos(torch.arange(rows * H, dtype=torch.float64) ** 2).reshape(1, rows, H) * torch.tensor([0.0, 1e1, 1e5], dtype=torch.float64)[:, None]
+            small = nn.Linear(H, V, bias=False, dtype=torch.float64, device="meta")
+            small.weight = nn.Parameter(torch.linspace(-1.0, 1.0, V * H, dtype=torch.float64).reshape(V, H), requires_grad=False)
+            known = _Known((hidden, *out[1:]) if isinstance(out, tuple) else type(out)(last_hidden_state=hidden), model.base_model)
+            modules = {name: known if m is model.base_model else small if m is head else m for name, m in model._modules.items()}
+            if known not in modules.values() or small not in modules.values():
+                return False
+            twin = object.__new__(kind)
+            twin.__dict__.update(vars(model), _modules=modules)
+            given = {"input_ids": torch.zeros(1, rows, dtype=torch.int64), **({"attention_mask": torch.ones(1, rows, dtype=torch.int64)} if masked else {}), **inputs}
+            takes = inspect.signature(kind.forward).parameters
+            every = any(p.kind is p.VAR_KEYWORD for p in takes.values())
+            got = kind.forward(twin, **{name: v for name, v in given.items() if every or name in takes})
+            if isinstance(got, tuple):
+                got = got[0]
+            elif isinstance(got, Mapping):
+                got = got.get("logits")
+            got = got if isinstance(got, torch.Tensor) else getattr(got, "logits", None)
+            want = small(hidden)
+            # (a forward that rounds its logits to bf16 returns the product too: half a step of it is 2^-8, and binary32's is lost in that)
+            return isinstance(got, torch.Tensor) and got.shape == want.shape and bool(((got - want).abs_().amax(-1) <= 2.0 ** -7 * want.abs().amax(-1)).all())
+    except Exception:                                              # (takes its decoder apart, or wants more than a decoder's call)
+        return False
+
+
 def model_token_logprobs(model, input_ids: torch.Tensor, attention_mask: torch.Tensor | None = None, labels: torch.Tensor | None = None, *,
                          temperature: float = 1.0, ignore_index: int = -100, entropy: bool = False, **inputs):
     """token_logprobs of a causal language model's next tokens, [B, S - 1] for input_ids [B, S], without its logits: the model's decoder
@@ -69,7 +126,10 @@ def model_token_logprobs(model, input_ids: torch.Tensor, attention_mask: torch.T
 
     labels defaults to input_ids; positions with ignore_index have 0 and no gradient (and are not computed), and so do those that
     attention_mask leaves out: where the token is masked, or the position before it, whose hidden state would predict it (padding on the left: a
-    row's first token has nothing to be predicted from).  inputs: further arguments of the decoder."""
+    row's first token has nothing to be predicted from).  inputs: further arguments of the decoder.
+
+    Only for models whose logits are that product and nothing more: their own forward is asked each time, on stand-ins of the decoder and the head
+    (on the CPU, beside the decoder's work on the device), and models that scale, cap, shift or cut their logits are refused."""
     head = model.get_output_embeddings()
     if getattr(head, "bias", None) is not None:
         raise ValueError("model_token_logprobs: a head without bias")
@@ -81,6 +141,9 @@ def model_token_logprobs(model, input_ids: torch.Tensor, attention_mask: torch.T
         raise ValueError(f"model_token_logprobs: an output embedding with one weight [V, H], not {type(head).__name__}")
     out = model.base_model(input_ids=input_ids, attention_mask=attention_mask, **inputs)
     hidden = out[0] if isinstance(out, tuple) else out.last_hidden_state
+    if not _logits_are_the_product(model, head, weight, out, attention_mask is not None, inputs):
+        raise ValueError(f"model_token_logprobs: {type(model).__name__} does not return its decoder's last hidden states times its head's weight as logits; "
+                         "use token_logprobs on the hidden states that its head is given")
     targets = (input_ids if labels is None else labels)[:, 1:]
     if attention_mask is not None:
         targets = targets.masked_fill((attention_mask[:, 1:] == 0) | (attention_mask[:, :-1] == 0), ignore_index)

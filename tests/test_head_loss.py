@@ -114,3 +114,133 @@ def test_labels_and_the_mask_both_leave_tokens_out(monkeypatch):
     assert _seen_targets(monkeypatch, ids, torch.tensor([[0, 1, 1, 1, 1]]), labels=labels) == [[-100, -100, 9, 10]]
     assert _seen_targets(monkeypatch, ids, torch.tensor([[0, 0, 0, 1, 1]]), labels=labels) == [[-100, -100, -100, 10]]
     assert _seen_targets(monkeypatch, ids, torch.tensor([[1, 1, 1, 1, 0]]), labels=labels, ignore_index=10) == [[-100, -100, 9, 10]]
+
+
+class _Decoder(torch.nn.Module):
+    def __init__(self, output):
+        super().__init__()
+        self.embed, self.output, self.lm_head_multiplier = torch.nn.Embedding(20, 8), output, 0.25
+        if output == "inside":                                           # as models whose decoder lies one level further down
+            self.decoder = _Decoder("object")
+
+    def forward(self, input_ids, attention_mask=None):
+        from types import SimpleNamespace
+        hidden = self.embed(input_ids)
+        return (hidden, None) if self.output == "tuple" else SimpleNamespace(last_hidden_state=hidden)
+
+
+class _Causal(torch.nn.Module):
+    """A causal language model whose logits are its head's product, returned in one of the usual ways."""
+
+    def __init__(self, output="object", returned="object"):
+        super().__init__()
+        self.base_model, self.lm_head, self.returned, self.calls = _Decoder(output), torch.nn.Linear(8, 20, bias=False), returned, []
+        self.factor = 2.0
+
+    def get_output_embeddings(self):
+        return self.lm_head
+
+    def hidden(self, input_ids, attention_mask):
+        out = (self.base_model.decoder if self.base_model.output == "inside" else self.base_model)(input_ids, attention_mask=attention_mask)
+        return out[0] if isinstance(out, tuple) else out.last_hidden_state
+
+    def logits(self, hidden):
+        return self.lm_head(hidden)
+
+    def forward(self, input_ids, attention_mask=None, labels=None):
+        from types import SimpleNamespace
+        logits = self.logits(self.hidden(input_ids, attention_mask)).float()
+        return {"object": SimpleNamespace(logits=logits), "tuple": (logits, None), "tensor": logits, "dict": {"logits": logits}, "nothing": None}[self.returned]
+
+
+class _TimesHead(_Causal):
+    def logits(self, hidden):
+        return self.lm_head(hidden) * self.factor
+
+
+class _TimesDecoders(_Causal):
+    def logits(self, hidden):
+        return self.lm_head(hidden) * self.base_model.lm_head_multiplier
+
+
+class _TimesHidden(_Causal):
+    def logits(self, hidden):
+        return self.lm_head(hidden / 3.0)
+
+
+class _Capped(_Causal):
+    def logits(self, hidden):
+        return 50.0 * torch.tanh(self.lm_head(hidden) / 50.0)
+
+
+class _Shifted(_Causal):
+    def __init__(self):
+        super().__init__()
+        self.shift = torch.full((20,), 1e-3)
+
+    def logits(self, hidden):
+        return self.lm_head(hidden) + self.shift
+
+
+class _Cut(_Causal):
+    def logits(self, hidden):
+        return self.lm_head(hidden)[..., :17]
+
+
+class _Normed(_Causal):
+    def logits(self, hidden):
+        return self.lm_head(torch.nn.functional.layer_norm(hidden, hidden.shape[-1:]))
+
+
+class _ByHand(_Causal):                                                  # asks its decoder for its parts
+    def hidden(self, input_ids, attention_mask):
+        return self.base_model.embed.weight[input_ids]
+
+
+def _asked(model, mask=True):
+    """model_token_logprobs without a device: it ends in token_logprobs' refusal of host tensors."""
+    ids = torch.tensor([[3, 4, 5, 6, 7, 8], [1, 2, 3, 4, 5, 6]])
+    with pytest.raises(MetisHipError, match="no CPU path"):
+        model_token_logprobs(model, ids, torch.ones_like(ids) if mask else None)
+
+
+@pytest.mark.parametrize("mask", [True, False])
+@pytest.mark.parametrize("output", ["object", "tuple", "inside"])
+@pytest.mark.parametrize("returned", ["object", "tuple", "tensor", "dict"])
+def test_models_whose_logits_are_the_product_are_taken(output, returned, mask):
+    model = _Causal(output, returned)
+    attributes = dict(vars(model))
+    _asked(model, mask)
+    assert dict(vars(model)) == attributes and set(model._modules) == {"base_model", "lm_head"}
+
+
+@pytest.mark.parametrize("kind", [_TimesHead, _TimesDecoders, _TimesHidden, _Capped, _Shifted, _Cut, _Normed, _ByHand])
+def test_models_whose_logits_are_something_else_are_refused(kind):
+    with pytest.raises(ValueError, match="logits"):
+        model_token_logprobs(kind(), torch.tensor([[3, 4, 5, 6]]))
+
+
+def test_models_that_return_no_logits_are_refused():
+    with pytest.raises(ValueError, match="logits"):
+        model_token_logprobs(_Causal(returned="nothing"), torch.tensor([[3, 4, 5, 6]]))
+
+
+def test_a_factor_of_one_is_no_factor():
+    model = _TimesHead()
+    model.factor = 1.0
+    _asked(model)
+
+
+@pytest.mark.parametrize("name,setting,taken", [("Llama", {}, True), ("Qwen2", {}, True), ("OPT", {"word_embed_proj_dim": 32, "ffn_dim": 48}, True),
+                                                ("Mixtral", {"num_local_experts": 2}, True), ("Gemma2", {"head_dim": 8, "final_logit_softcapping": None}, True),
+                                                ("Gemma2", {"head_dim": 8}, False), ("Granite", {"logits_scaling": 8.0}, False), ("Cohere", {}, False)])
+def test_models_of_a_library(name, setting, taken):
+    transformers = pytest.importorskip("transformers")
+    config = getattr(transformers, f"{name}Config")(vocab_size=20, hidden_size=32, intermediate_size=48, num_hidden_layers=1, num_attention_heads=4, num_key_value_heads=2,
+                                                    pad_token_id=0, bos_token_id=0, eos_token_id=0, tie_word_embeddings=False, **setting)
+    model = getattr(transformers, f"{name}ForCausalLM")(config)
+    if taken:
+        _asked(model)
+    else:
+        with pytest.raises(ValueError, match="logits"):
+            model_token_logprobs(model, torch.tensor([[3, 4, 5, 6]]))
