@@ -139,6 +139,8 @@ def model_token_logprobs(model, input_ids: torch.Tensor, attention_mask: torch.T
     weight = getattr(head, "weight", None)
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError(f"model_token_logprobs: an output embedding with one weight [V, H], not {type(head).__name__}")
+    if type(head).forward is not nn.Linear.forward or "forward" in vars(head) or head._forward_hooks or head._forward_pre_hooks:
+        raise ValueError(f"model_token_logprobs: a plain linear head without hooks, whose forward multiplies by its weight and does nothing else, not {type(head).__name__}")
     out = model.base_model(input_ids=input_ids, attention_mask=attention_mask, **inputs)
     hidden = out[0] if isinstance(out, tuple) else out.last_hidden_state
     if not _logits_are_the_product(model, head, weight, out, attention_mask is not None, inputs):

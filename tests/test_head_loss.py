@@ -244,3 +244,55 @@ def test_models_of_a_library(name, setting, taken):
     else:
         with pytest.raises(ValueError, match="logits"):
             model_token_logprobs(model, torch.tensor([[3, 4, 5, 6]]))
+
+
+class _Adapted(torch.nn.Module):
+    """A head in an adapter's wrapper that hands out the weight of what it wraps."""
+
+    def __init__(self, head):
+        super().__init__()
+        self.head, self.a, self.b = head, torch.nn.Linear(8, 2, bias=False), torch.nn.Linear(2, 20, bias=False)
+
+    weight = property(lambda self: self.head.weight)
+    bias = property(lambda self: self.head.bias)
+
+    def forward(self, x):
+        return self.head(x) + self.b(self.a(x))
+
+
+class _Doubled(torch.nn.Linear):
+    def forward(self, x):
+        return 2.0 * super().forward(x)
+
+
+def _lowbit_head():
+    from metis_hip import LinearLowbit, MetisArgs
+    return LinearLowbit(8, 20, bias=False, args=MetisArgs(), device="cpu")
+
+
+def _changed(change):
+    head = torch.nn.Linear(8, 20, bias=False)
+    change(head)
+    return head
+
+
+@pytest.mark.parametrize("make", [lambda: _Adapted(torch.nn.Linear(8, 20, bias=False)), lambda: _Doubled(8, 20, bias=False), _lowbit_head,
+                                  lambda: _changed(lambda h: h.register_forward_hook(lambda m, a, y: 2 * y)),
+                                  lambda: _changed(lambda h: h.register_forward_pre_hook(lambda m, a: (2 * a[0],))),
+                                  lambda: _changed(lambda h: setattr(h, "forward", lambda x: torch.nn.functional.linear(x, 2 * h.weight)))],
+                         ids=["adapter", "subclass", "quantized", "hook", "pre_hook", "forward"])
+def test_heads_that_compute_something_else_with_their_weight_are_refused(make):
+    model = _Causal()
+    model.lm_head = make()
+    with pytest.raises(ValueError, match="plain linear"):
+        model_token_logprobs(model, torch.tensor([[3, 4, 5, 6]]))
+
+
+def test_parametrized_heads_are_taken():
+    """The weight of a parametrization is what its forward multiplies by."""
+    class Scaled(torch.nn.Module):
+        def forward(self, w):
+            return 2 * w
+    model = _Causal()
+    torch.nn.utils.parametrize.register_parametrization(model.lm_head, "weight", Scaled())
+    _asked(model)
