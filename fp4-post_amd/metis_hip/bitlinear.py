@@ -832,12 +832,17 @@ class LinearLowbit(nn.Module):
         return super()._apply(fn, recurse=recurse)
 
 
+def _transformed() -> bool:
+    """Whether forward-mode differentiation, one of torch.func's transforms or a tracer sees this call: they need not leave a mark on the tensors that
+    reverse mode leaves (requires_grad), and have to meet an autograd function, or its refusal."""
+    return torch.autograd.forward_ad._current_level >= 0 or torch._C._functorch.maybe_current_level() is not None or torch.jit.is_tracing()
+
+
 def _autograd_may_see() -> bool:
     """Whether something may want to record or transform what an autograd function computes: autograd itself, forward-mode
     differentiation, torch.func's transforms, a tracer.  Without any of them the function's values are computed without the function
     (a decode step pays 8 us for each apply)."""
-    return (torch.is_grad_enabled() or torch.autograd.forward_ad._current_level >= 0
-            or torch._C._functorch.maybe_current_level() is not None or torch.jit.is_tracing() or torch.compiler.is_compiling())
+    return torch.is_grad_enabled() or _transformed() or torch.compiler.is_compiling()
 
 
 class _MetisFusedFunction(torch.autograd.Function):

@@ -10,8 +10,46 @@ import inspect
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
+from .bitlinear import _transformed
+
+
+class _ResidualNorm(torch.autograd.Function):
+    """residual_norm where a tracer or a transform sees the call: the compiled node (csrc/host_autograd.cpp) would be a constant to the first and is not
+    met at all by a tensor that carries a tangent and no requires_grad.  The tracer records this one, the others have its refusal."""
+
+    @staticmethod
+    def forward(ctx, x, y, weight, post_weight, gate, scale, eps):
+        h, n = ops.residual_norm(x, y, weight, post_weight, gate, scale, eps)
+        ctx.save_for_backward(h, y if post_weight is not None or gate is not None else None, weight, post_weight, gate)
+        ctx.more = scale, eps, y.dtype
+        ctx.set_materialize_grads(False)
+        return h, n
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_h, grad_n):
+        if grad_h is None and grad_n is None:
+            return (None,) * 7
+        h, y, weight, post_weight, gate = ctx.saved_tensors
+        scale, eps, y_dtype = ctx.more
+        return (*ops.residual_norm_backward(h, y, weight, post_weight, gate, scale, eps, grad_h, grad_n, y_dtype, ctx.needs_input_grad[:5]), None, None)
+
+
+class _SwiGLU(torch.autograd.Function):
+    """swiglu where a tracer or a transform sees the call, as _ResidualNorm."""
+
+    @staticmethod
+    def forward(ctx, gate, up):
+        ctx.save_for_backward(gate, up)
+        return ops.swiglu(gate, up)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        return ops.swiglu_backward(*ctx.saved_tensors, grad)
 
 
 def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, *, post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None,
@@ -26,8 +64,10 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, *, pos
     weight, post_weight   [C] in y's type
     gate      in y's type: [C], or x's leading sizes followed by ones ([B, 1, C]: one for each sequence of [B, S, C])
 
-    Returns (h in x's type, n in y's type); n is the norm of h as it is stored.  Differentiable (once) in all tensors."""
+    Returns (h in x's type, n in y's type); n is the norm of h as it is stored.  Differentiable (once, in reverse) in all tensors."""
     scale, eps = float(residual_scale), float(eps)
+    if _transformed():
+        return _ResidualNorm.apply(x, y, weight, post_weight, gate, scale, eps)
     if torch.is_grad_enabled() and (x.requires_grad or y.requires_grad or weight.requires_grad or (post_weight is not None and post_weight.requires_grad)
                                     or (gate is not None and gate.requires_grad)):
         ops._check_residual_norm(x, y, weight, post_weight, gate, y.dtype)
@@ -37,7 +77,9 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, *, pos
 
 def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     """silu(gate) * up, the activation of a gated MLP: [..., C] bf16 or float32 of one shape and type, rows of any stride (the halves of
-    one product are taken as they are).  The result is dense.  Differentiable (once) in both."""
+    one product are taken as they are).  The result is dense.  Differentiable (once, in reverse) in both."""
+    if _transformed():
+        return _SwiGLU.apply(gate, up)
     if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
         ops._check_swiglu(gate, up)
         return _lib.host().recorded_swiglu(gate, up)

@@ -15,6 +15,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import ops
+from .bitlinear import _transformed
 
 
 class _TokenLogprobs(torch.autograd.Function):
@@ -46,8 +47,8 @@ def token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Te
     targets   int64 [...]; a token whose target is ignore_index has 0 and no gradient, and its hidden state is not looked at.  Any other
               target outside the vocabulary makes its results NaN.
 
-    Differentiable (once) in hidden and weight; the logits are formed in pieces, in both directions, and never kept."""
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+    Differentiable (once, in reverse) in hidden and weight; the logits are formed in pieces, in both directions, and never kept."""
+    if _transformed() or (torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)):
         return _TokenLogprobs.apply(hidden, weight, targets, int(ignore_index), float(temperature), bool(entropy))
     logp, _, ent, _ = ops.head_logprobs(hidden, weight, targets, ignore_index, temperature, entropy)
     return (logp, ent) if entropy else logp

@@ -262,3 +262,48 @@ def test_forward_and_backward_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, eager(leaves, targets, g)))
+
+
+def test_traced_calls_run_again():
+    """What torch.jit.trace records of the three operators runs them on the inputs that it is given: the bits of the calls themselves, values and gradients."""
+    from metis_hip import residual_norm, swiglu, token_logprobs
+    torch.manual_seed(41)
+    weight, post, head = ((1 + 0.1 * torch.randn(256)).to(BF).cuda(), (1 + 0.1 * torch.randn(256)).to(BF).cuda(), torch.randn(515, 256).to(BF).cuda())
+
+    def step(x, y, gate, targets):
+        h, n = residual_norm(x, y, weight, post_weight=post, gate=gate, residual_scale=0.5)
+        h, n = residual_norm(h, swiglu(n, h), weight)
+        logp, ent = token_logprobs(n, head, targets, entropy=True)
+        return logp + 0.1 * ent, h
+
+    def values():
+        return *(torch.randn(2, n, 256).to(BF).cuda().requires_grad_() for n in (35, 35, 1)), torch.randint(515, (2, 35)).cuda()
+
+    traced = torch.jit.trace(step, values(), check_trace=False)
+    for _ in range(2):
+        x, y, gate, targets = values()
+        results = []
+        for run in (traced, step):
+            loss, h = run(x, y, gate, targets)
+            results.append([loss.detach(), h.detach(), *torch.autograd.grad((loss.sum(), h), (x, y, gate), (torch.ones((), device="cuda"), torch.ones_like(h)))])
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+    with torch.no_grad():
+        traced = torch.jit.trace(step, values(), check_trace=False)
+        new = values()
+        assert all(torch.equal(a, b) for a, b in zip(traced(*new), step(*new)))
+
+
+def test_tangents_are_refused_on_the_device():
+    """Forward mode meets a refusal, with and without reverse mode beside it, and a level that none of the tensors is part of changes nothing."""
+    import torch.autograd.forward_ad as fwd
+    from metis_hip import residual_norm, swiglu, token_logprobs
+    x, y, head = torch.randn(5, 64).to(BF).cuda(), torch.randn(5, 64).to(BF).cuda(), torch.randn(70, 64).to(BF).cuda()
+    w, targets = torch.ones(64, dtype=BF, device="cuda"), torch.randint(70, (5,)).cuda()
+    calls = {"norm": lambda x: residual_norm(x, y, w)[1], "gate": lambda x: swiglu(x, y), "loss": lambda x: token_logprobs(x, head, targets)}
+    for call in calls.values():
+        for leaf in (x, x.clone().requires_grad_()):
+            want = call(leaf)
+            with fwd.dual_level():
+                assert torch.equal(call(leaf), want)
+                with pytest.raises(NotImplementedError, match="jvp"):
+                    call(fwd.make_dual(leaf, torch.ones_like(leaf)))

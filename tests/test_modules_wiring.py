@@ -524,3 +524,55 @@ def test_sizes_that_follow_a_device_are_kept_for_each_device(monkeypatch, size, 
         assert ask(*shape, 0) == first and ask(*shape, 1) != first
     finally:
         ask.cache_clear()
+
+
+def _plain_operators(monkeypatch):
+    """The operators' three calls with torch's operations in place of the kernels, and what each is called on."""
+    from metis_hip import linear_cross_entropy, ops, residual_norm, swiglu, token_logprobs
+    monkeypatch.setattr(ops, "residual_norm", lambda x, y, w, post, gate, scale, eps: (x + scale * y, (x + scale * y) * w))
+    monkeypatch.setattr(ops, "swiglu", lambda gate, up: torch.nn.functional.silu(gate) * up)
+
+    def logprobs(hidden, weight, targets, ignore_index, temperature, entropy):
+        logp = torch.log_softmax(hidden @ weight.t() / temperature, -1)
+        return logp.gather(-1, targets.unsqueeze(-1)).squeeze(-1), logp[..., 0], -(logp.exp() * logp).sum(-1) if entropy else None, targets
+    monkeypatch.setattr(ops, "head_logprobs", logprobs)
+    w, head, targets = torch.ones(4), torch.randn(6, 4), torch.tensor([1, 5, 2])
+    return {"residual_norm": lambda a, b: residual_norm(a, b, w)[1], "swiglu": swiglu,
+            "token_logprobs": lambda a, b: token_logprobs(a + b, head, targets), "entropy": lambda a, b: token_logprobs(a + b, head, targets, entropy=True)[1],
+            "linear_cross_entropy": lambda a, b: linear_cross_entropy(a + b, head, targets)}
+
+
+OPERATORS = ["residual_norm", "swiglu", "token_logprobs", "entropy", "linear_cross_entropy"]
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("name", OPERATORS)
+def test_a_tangent_does_not_get_lost_in_an_operator(monkeypatch, name, grad):
+    """Forward-mode differentiation and torch.func's transforms are refused, not answered with a derivative of zero or a constant."""
+    import torch.autograd.forward_ad as fwd
+    run = _plain_operators(monkeypatch)[name]
+    a, b = torch.randn(3, 4), torch.randn(3, 4)
+    with torch.set_grad_enabled(grad):
+        with fwd.dual_level():
+            with pytest.raises(NotImplementedError, match="jvp"):
+                run(fwd.make_dual(a, torch.ones_like(a)), b)
+        with pytest.raises(RuntimeError, match="setup_context"):
+            torch.func.jvp(lambda a: run(a, b), (a,), (a,))
+        with pytest.raises(RuntimeError, match="setup_context"):
+            torch.func.vmap(lambda a: run(a, b))(torch.randn(2, 3, 4))
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("name", OPERATORS)
+def test_a_traced_operator_is_no_constant(monkeypatch, name, grad):
+    run = _plain_operators(monkeypatch)[name]
+    a, b = torch.randn(3, 4), torch.randn(3, 4)
+    with torch.set_grad_enabled(grad):
+        traced = torch.jit.trace(run, (a, b), check_trace=False)
+        if grad:
+            a.requires_grad_()
+            with_grad = torch.jit.trace(run, (a, b), check_trace=False)
+            assert torch.equal(with_grad(b, a), run(b, a.detach()))
+            a = a.detach()
+        new = torch.randn(3, 4), torch.randn(3, 4)
+        assert torch.equal(traced(*new), run(*new)) and not torch.equal(traced(*new), run(a, b))
