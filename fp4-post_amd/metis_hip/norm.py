@@ -114,7 +114,7 @@ class FusedRMSNormQuant(nn.Module):
                 and residual.dtype in (y.dtype, torch.float32) and cols % 8 == 0 and 0 < cols <= ops.RESIDUAL_NORM_MAX_COLS):
             return residual_norm(residual, y, weight, eps=self.variance_epsilon)
         h = residual + y
-        return h, self._plain(h)
+        return h, self._plain(h).to(y.dtype)                       # (the types that the kernel gives, whatever was taken here)
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
         """The norm of x; with the residual stream of a block whose output is x the pair (residual + x, its norm), see residual_norm (whose norm

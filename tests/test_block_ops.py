@@ -221,3 +221,22 @@ def test_mlps_of_a_library_are_told_apart():
     small = dict(hidden_size=16, intermediate_size=24, num_attention_heads=2, num_key_value_heads=2)
     assert fuse_gated_mlps(_in_a_model(LlamaMLP(transformers.LlamaConfig(**small)), True)) == 1
     assert fuse_gated_mlps(_in_a_model(FalconH1MLP(transformers.FalconH1Config(**small, mlp_multipliers=[2.0, 0.5])), True)) == 0
+
+
+@pytest.mark.parametrize("cols", [64, 60])
+@pytest.mark.parametrize("stream,branch,weight", [(torch.bfloat16, torch.bfloat16, torch.bfloat16), (torch.float32, torch.bfloat16, torch.bfloat16),
+                                                  (torch.float32, torch.float32, torch.float32), (torch.float32, torch.bfloat16, torch.float32)])
+def test_the_norm_modules_pair_has_its_types_without_the_kernel_too(stream, branch, weight, cols):
+    """FusedRMSNormQuant(y, residual) where the kernel does not take the tensors: the stream in its own type and the norm in the branch's, as the kernel
+    gives them; each value that of binary64 but for its roundings: the sum's, x * rstd's where the module rounds it, and the result's, and binary32's own."""
+    from metis_hip import FusedRMSNormQuant
+    g = torch.Generator().manual_seed(7)
+    x, y = torch.randn(3, 5, cols, generator=g).to(stream), torch.randn(3, 5, cols, generator=g).to(branch)
+    w = torch.nn.Parameter((1 + 0.1 * torch.randn(cols, generator=g)).to(weight))
+    with torch.no_grad():
+        h, n = FusedRMSNormQuant(w, 1e-6, {"name": "mlp.gate_up"})(y, x)
+    assert h.dtype == stream and n.dtype == branch and h.shape == n.shape == x.shape
+    total = x.double() + y.double()
+    assert bool(((h.double() - total).abs() <= torch.finfo(stream).eps / 2 * total.abs()).all())
+    want = h.double() / (h.double().square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
+    assert bool(((n.double() - want).abs() <= (1.01 * torch.finfo(branch).eps + 2.0 ** -20) * want.abs()).all())
