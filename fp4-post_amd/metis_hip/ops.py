@@ -1475,13 +1475,15 @@ def _head_backward_bytes(tokens: int, H: int, V: int, want_hidden: bool, want_we
     return int(load().metis_head_logprobs_backward_workspace_bytes(tokens, H, V, want_hidden, want_weight))      # depends on the device's CU count only
 
 
-def _head_operand(t: torch.Tensor) -> torch.Tensor:
-    """[rows, H] bf16 whose rows are dense and 16-byte aligned, at any stride that keeps them so; a copy only where it has to be one."""
-    t = t.reshape(-1, t.shape[-1])
-    if t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) < t.shape[1] or t.stride(0) % 8)) or t.data_ptr() % 16:
+def _head_operand(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """[rows, H] bf16 whose rows are dense and 16-byte aligned, at any stride that keeps them so, and that stride (of a single row H: it has none that
+    counts); a copy only where it has to be one."""
+    H = t.shape[-1]
+    t = t.reshape(-1, H)
+    if t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) < H or t.stride(0) % 8)) or t.data_ptr() % 16:
         t = t.contiguous()
         t = t if t.data_ptr() % 16 == 0 else t.clone()
-    return t
+    return t, t.stride(0) if t.shape[0] > 1 else H
 
 
 def _check_head(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, temperature: float) -> None:
@@ -1506,7 +1508,7 @@ def head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Ten
     """(logp, lse, entropy or None, index): log-probability of every target under softmax(hidden weight^T / temperature), the logits' log-sum-exp and
     the entropy, float32 of targets' shape, without the logits; `index` is for head_logprobs_backward.  hidden bf16 [..., H], weight bf16 [V, H]."""
     _check_head(hidden, weight, targets, temperature)
-    x, w, t = _head_operand(hidden), _head_operand(weight), targets.reshape(-1).contiguous()
+    (x, ldx), (w, ldw), t = _head_operand(hidden), _head_operand(weight), targets.reshape(-1).contiguous()
     (V, H), tokens = weight.shape, t.numel()
     if tokens == 0:
         zero = torch.zeros(targets.shape, dtype=torch.float32, device=hidden.device)
@@ -1514,7 +1516,7 @@ def head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Ten
     index, need = _head_bytes(tokens, H, V, entropy)
     shape = (F32, *targets.shape)
     new = _lib.call("metis_head_logprobs", hidden.device.index, (shape, shape, (U8, index), (U8, need), shape if entropy else (F32, 0)),
-                    (x, max(x.stride(0), H), w, max(w.stride(0), H), t, int(ignore_index), tokens, H, V, float(temperature), "0", "1", "4" if entropy else None, "2", "3", need, _stream()))
+                    (x, ldx, w, ldw, t, int(ignore_index), tokens, H, V, float(temperature), "0", "1", "4" if entropy else None, "2", "3", need, _stream()))
     if new.__class__ is int:
         check(new, "metis_head_logprobs", hidden.shape)
     return new[0], new[1], new[4] if entropy else None, new[2]
@@ -1531,7 +1533,7 @@ def head_logprobs_backward(hidden: torch.Tensor, weight: torch.Tensor, targets: 
             raise ValueError(f"head_logprobs_backward: {name} is float32 {tuple(targets.shape)}, not {g.dtype} {tuple(g.shape)}")
     if lse is None or (grad_entropy is not None and entropy is None):
         raise ValueError("head_logprobs_backward: lse, and for grad_entropy also entropy, of the forward call")
-    x, w, t = _head_operand(hidden), _head_operand(weight), targets.reshape(-1).contiguous()
+    (x, ldx), (w, ldw), t = _head_operand(hidden), _head_operand(weight), targets.reshape(-1).contiguous()
     (V, H), tokens = weight.shape, t.numel()
     if tokens == 0 or (grad_logp is None and grad_entropy is None):
         return torch.zeros(hidden.shape, dtype=hidden.dtype, device=hidden.device) if want_hidden else None, torch.zeros((V, H), dtype=weight.dtype, device=hidden.device) if want_weight else None
@@ -1545,7 +1547,7 @@ def head_logprobs_backward(hidden: torch.Tensor, weight: torch.Tensor, targets: 
             place[k] = str(len(specs))
             specs.append((B16, *shape))
     new = _lib.call("metis_head_logprobs_backward", hidden.device.index, tuple(specs),
-                    (x, max(x.stride(0), H), w, max(w.stride(0), H), t, tokens, H, V, float(temperature), lse, entropy, grad_logp, grad_entropy, index, *place, "0", need, _stream()))
+                    (x, ldx, w, ldw, t, tokens, H, V, float(temperature), lse, entropy, grad_logp, grad_entropy, index, *place, "0", need, _stream()))
     if new.__class__ is int:
         check(new, "metis_head_logprobs_backward", hidden.shape)
     return tuple(None if k is None else new[int(k)] for k in place)

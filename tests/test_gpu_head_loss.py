@@ -346,3 +346,22 @@ def test_other_streams():
             got.append(run())
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for r in got for a, b in zip(r, want))
+
+
+def test_a_single_row_of_any_stride():
+    """One token cut out of a wider row (stride 68, no multiple of eight), and a head of one such row: the bits of dense copies."""
+    from metis_hip import token_logprobs
+    g = torch.Generator().manual_seed(77)
+    wide = torch.randn(4, 68, generator=g).to(BF).cuda()
+    heads = torch.randn(300, 64, generator=g).to(BF).cuda(), wide[2:3, :64]
+    for x in (wide[:1, :64], wide[:1].view(1, 1, 68)[..., :64]):
+        for w in heads:
+            t = torch.zeros(x.shape[:-1], dtype=torch.int64, device="cuda")
+            results = []
+            for change in (lambda v: v, lambda v: v.reshape(-1).clone().view(v.shape)):
+                leaves = [change(v.detach()).requires_grad_() for v in (x, w)]
+                logp = token_logprobs(*leaves, t)
+                results.append([logp.detach(), *torch.autograd.grad(logp.sum(), leaves)])
+            assert all(torch.equal(a, b) for a, b in zip(*results))
+            # (E = 64 2^-24 sum |x w| < 2^-18 100, two of it and 2^-14: under 1e-3)
+            assert abs(float(results[0][0].sum()) - float(torch.log_softmax(x.reshape(-1, 64).double() @ w.double().t(), 1)[0, 0])) < 1e-3

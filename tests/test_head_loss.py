@@ -296,3 +296,16 @@ def test_parametrized_heads_are_taken():
     model = _Causal()
     torch.nn.utils.parametrize.register_parametrization(model.lm_head, "weight", Scaled())
     _asked(model)
+
+
+def test_a_single_row_has_no_stride_that_counts():
+    """A row cut out of a wider one, or the last position of one sequence: the entry point wants strides in eights, and of one row there is none."""
+    from metis_hip import ops
+    wide = torch.zeros(3, 68, dtype=torch.bfloat16)
+    for t in (wide[:1, :64], wide.flatten()[:68].view(1, 1, 68)[..., :64], torch.zeros(1, 7, 61, 64, dtype=torch.bfloat16)[:, 2:3, 5:6]):
+        taken, ld = ops._head_operand(t)
+        assert ld == 64 and taken.shape == (1, 64) and taken.data_ptr() % 16 == 0
+    taken, ld = ops._head_operand(wide[:, :64])                          # (more rows are copied for it)
+    assert ld == 64 and taken.is_contiguous()
+    taken, ld = ops._head_operand(torch.zeros(3, 72, dtype=torch.bfloat16)[:, :64])
+    assert ld == 72 and taken.stride() == (72, 1)
