@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import inspect
 from dataclasses import dataclass
 
 import torch
@@ -1269,12 +1270,15 @@ def rmsnorm_backward(x: torch.Tensor, g: torch.Tensor, gamma: torch.Tensor, eps:
 
 def _on_own_device(fn):
     """The call runs on the current stream of its first tensor's device, whichever device is current."""
+    name = next(iter(inspect.signature(fn).parameters))
+
     @functools.wraps(fn)
-    def run(first: torch.Tensor, *args, **kwargs):
-        if first.is_cuda and first.get_device() != (_raw_device or torch.cuda.current_device)():
+    def run(*args, **kwargs):
+        first = args[0] if args else kwargs.get(name)
+        if first is not None and first.is_cuda and first.get_device() != (_raw_device or torch.cuda.current_device)():
             with torch.cuda.device(first.device):
-                return fn(first, *args, **kwargs)
-        return fn(first, *args, **kwargs)
+                return fn(*args, **kwargs)
+        return fn(*args, **kwargs)
     return run
 
 

@@ -240,3 +240,18 @@ def test_the_norm_modules_pair_has_its_types_without_the_kernel_too(stream, bran
     assert bool(((h.double() - total).abs() <= torch.finfo(stream).eps / 2 * total.abs()).all())
     want = h.double() / (h.double().square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
     assert bool(((n.double() - want).abs() <= (1.01 * torch.finfo(branch).eps + 2.0 ** -20) * want.abs()).all())
+
+
+@pytest.mark.parametrize("name", ["residual_norm", "residual_norm_backward", "swiglu", "swiglu_backward", "head_logprobs", "head_logprobs_backward"])
+def test_operators_take_all_their_arguments_by_name(name):
+    """Their first one too, which says on which device the call runs."""
+    x, w = torch.zeros(2, 64, dtype=torch.bfloat16), torch.ones(64, dtype=torch.bfloat16)
+    t, f = torch.zeros(2, dtype=torch.int64), torch.zeros(2)
+    given = {"residual_norm": dict(y=x, weight=w, x=x), "swiglu": dict(up=x, gate=x), "swiglu_backward": dict(grad=x, up=x, gate=x),
+             "residual_norm_backward": dict(y=None, weight=w, post_weight=None, gate=None, scale=1.0, eps=1e-6, grad_h=x, grad_n=x, y_dtype=x.dtype, h=x),
+             "head_logprobs": dict(weight=x, targets=t, hidden=x),
+             "head_logprobs_backward": dict(weight=x, targets=t, temperature=1.0, lse=f, entropy=None, index=t, grad_logp=f, grad_entropy=None, hidden=x)}[name]
+    with pytest.raises(MetisHipError, match="no CPU path"):
+        getattr(ops, name)(**given)
+    with pytest.raises(TypeError):
+        getattr(ops, name)()
