@@ -363,3 +363,60 @@ def test_backward_into_leaves_and_hooks():
         h, n = residual_norm(x, y, w)
         torch.autograd.backward((h, n), (gh, gn))
     assert torch.equal(x.grad, y.grad) and x.grad.data_ptr() != y.grad.data_ptr() and torch.equal(seen[0] + seen[1], x.grad)
+
+
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("rows,cols,xd,yd", [(8195, 512, BF, BF), (4103, 1024, BF, BF), (2103, 2048, F32, BF), (4099, 3584, BF, BF), (1030, 4096, F32, F32), (2103, 8192, F32, BF)])
+def test_more_rows_than_a_launch_has_teams(rows, cols, xd, yd, post):
+    """Each number of waves to a row, with rows left for a second or third turn of the forward's workgroups and teams that have none in the last."""
+    from metis_hip import residual_norm
+    x, y, w, p, g, gh, gn = make(rows + cols, (rows, cols), xd, yd, post, (cols,) if post else None)
+    leaves = [t.requires_grad_() for t in (x, y, w, p, g) if t is not None]
+    h, n = residual_norm(x, y, w, post_weight=p, gate=g, eps=EPS)
+    got = list(torch.autograd.grad((h, n), leaves, (gh, gn)))
+    full = [got.pop(0) if t is not None else None for t in (x, y, w, p, g)]
+    with torch.no_grad():
+        check_forward(x, y, w, p, g, 1.0, h, n)
+        check_backward(x, y, w, p, g, 1.0, h, gh, gn, full)
+
+
+@pytest.mark.parametrize("dtype,rows", [(BF, 2521), (F32, 1261)])
+def test_swiglu_beyond_the_memory_side_cache(dtype, rows):
+    """More than 256 MiB forward and backward, an odd number of eight-element chunks: the last lanes have one chunk where the others have two, or none."""
+    from metis_hip import swiglu
+    cols = 18952
+    chunks = rows * cols // 8
+    assert rows * cols * dtype.itemsize * 3 > 256 << 20 and chunks % 2 and 0 < chunks % 512 < 512
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    both = (torch.randn(rows, 2 * cols, generator=gen, device="cuda") * 3).to(dtype)
+    da = torch.randn(rows, cols, generator=gen, device="cuda").to(dtype)
+    g, u = both[:, :cols].requires_grad_(), both[:, cols:].requires_grad_()
+    a = swiglu(g, u)
+    dg, du = torch.autograd.grad(a, (g, u), da)
+    with torch.no_grad():
+        check_swiglu(g, u, da, a, dg, du)
+
+
+def test_recomputed_and_packed_away():
+    """Gradients under checkpointing of both kinds, and with the saved tensors kept on the host in between: the bits of those without."""
+    from torch.utils.checkpoint import checkpoint
+    from metis_hip import residual_norm, swiglu
+    x, y, w, p, g, gh, gn = make(23, (2, 37, 520), BF, BF, True, (2, 1, 520))
+    leaves = [t.requires_grad_() for t in (x, y, w, p, g)]
+
+    def step(x, y, w, p, g):
+        h, n = residual_norm(x, y, w, post_weight=p, gate=g, residual_scale=0.5, eps=EPS)
+        h, n = residual_norm(h, swiglu(n, h), w, eps=EPS)
+        return h, n
+
+    def kept_on_the_host(*args):
+        with torch.autograd.graph.save_on_cpu():
+            return step(*args)
+
+    want = torch.autograd.grad(step(*leaves), leaves, (gh, gn))
+    for run in (lambda *a: checkpoint(step, *a, use_reentrant=False), kept_on_the_host):
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(run(*leaves), leaves, (gh, gn)), want))
+    for t in leaves:
+        t.grad = None
+    torch.autograd.backward(checkpoint(step, *leaves, use_reentrant=True), (gh, gn))
+    assert all(torch.equal(t.grad, b) for t, b in zip(leaves, want))

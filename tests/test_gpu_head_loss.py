@@ -365,3 +365,34 @@ def test_a_single_row_of_any_stride():
             assert all(torch.equal(a, b) for a, b in zip(*results))
             # (E = 64 2^-24 sum |x w| < 2^-18 100, two of it and 2^-14: under 1e-3)
             assert abs(float(results[0][0].sum()) - float(torch.log_softmax(x.reshape(-1, 64).double() @ w.double().t(), 1)[0, 0])) < 1e-3
+
+
+@pytest.mark.parametrize("T,H,V,temp", [(5, 528, 131075, 1.0), (61, 208, 70001, 0.7), (700, 208, 65537, 1.0), (2500, 208, 20003, 0.8)])
+def test_several_tiles_to_a_workgroup(T, H, V, temp):
+    """More tiles of the logits than workgroups, each of seven stages or more with half a one at the end: the next tile's first stages are under way while the
+    statistics of one leave."""
+    from metis_hip import token_logprobs
+    x, w, t, _, _ = make(T + V, T, H, V)
+    with torch.no_grad():
+        Exact(x, w, t, temp).check(*token_logprobs(x, w, t, temperature=temp, entropy=True))
+
+
+def test_recomputed_and_packed_away():
+    """Gradients under checkpointing of both kinds, and with the saved tensors kept on the host in between: the bits of those without."""
+    from torch.utils.checkpoint import checkpoint
+    from metis_hip import token_logprobs
+    x, w, t, g, e = make(91, 150, 80, 1001)
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+
+    def step(x, w):
+        return token_logprobs(x, w, t, temperature=0.8, entropy=True)
+
+    def kept_on_the_host(x, w):
+        with torch.autograd.graph.save_on_cpu():
+            return step(x, w)
+
+    want = torch.autograd.grad(step(x, w), leaves, (g, e))
+    for run in (lambda *a: checkpoint(step, *a, use_reentrant=False), kept_on_the_host):
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(run(x, w), leaves, (g, e)), want))
+    torch.autograd.backward(checkpoint(step, x, w, use_reentrant=True), (g, e))
+    assert all(torch.equal(t.grad, b) for t, b in zip(leaves, want))
