@@ -994,9 +994,14 @@ int metis_swiglu_backward(const void *gate, int64_t ld_gate, const void *up, int
  *   dl = (grad_logp (1[v = target] - p) - grad_entropy p (l - lse + entropy)) / temperature, rounded to bf16 once; what the
  *   rounding leaves out at the target is added to both gradients
  *   grad_hidden = dl weight, grad_weight = dl^T hidden, dense bf16, sums in binary32 in a fixed order; NULL: not wanted
- * The logits are formed again in pieces of the vocabulary.  Workspaces need no initialisation; the backward's holds one
- * piece of dl (at most the larger of 256 MiB and twice the binary32 gradient of hidden, at least 256 columns) beside the
- * binary32 gradient of hidden and, for grad_weight, two bf16 copies of hidden's size and 4 bytes a row of the vocabulary.
+ * The logits are formed again in pieces of the vocabulary.  Workspaces need no initialisation; the backward's holds
+ *   one piece of dl (at most the larger of 256 MiB and twice the binary32 gradient of hidden, at least 256 columns), and
+ *   three numbers of 4 bytes a token,
+ *   for grad_hidden  its partial sums, S binary32 copies of hidden's size: one for every range of a piece's columns that
+ *                    workgroups go through at the same time, at most 64 and at most one for each 512 columns of a piece
+ *                    (4096 x 3584 against 131072 rows: 1, 56 MiB; 540 x 2048 against 65536, alone: 10, 60 MiB),
+ *   for grad_weight  two bf16 copies of hidden's size and 4 bytes a row of the vocabulary,
+ * all of them for padded tokens: a multiple of 64, with 192 more where they are 65 to 2048, or of 256 beyond that.
  */
 size_t metis_head_index_bytes(int64_t tokens);
 size_t metis_head_logprobs_workspace_bytes(int64_t tokens, int64_t H, int64_t V, int entropy);

@@ -309,3 +309,18 @@ def test_a_single_row_has_no_stride_that_counts():
     assert ld == 64 and taken.is_contiguous()
     taken, ld = ops._head_operand(torch.zeros(3, 72, dtype=torch.bfloat16)[:, :64])
     assert ld == 72 and taken.stride() == (72, 1)
+
+
+@pytest.mark.parametrize("T,H,V", [(1, 16, 1), (5, 1536, 131072), (64, 3584, 131072), (65, 2048, 131072), (540, 2048, 65536), (600, 2048, 128003), (2048, 4096, 131072), (2049, 512, 4000),
+                                   (4096, 3584, 131072), (1 << 17, 4096, 152064)])
+def test_the_backwards_workspace_is_what_the_header_says(T, H, V):
+    """With the partial sums of grad_hidden, which want_hidden adds: at most 64 copies, and at most one for each 512 columns of a piece."""
+    ask = _lib.load().metis_head_logprobs_backward_workspace_bytes
+    rows = -(-T // 64) * 64 + (192 if T > 64 else 0) if T <= 2048 else -(-T // 256) * 256
+    piece = max(256 << 20, 8 * rows * H) // (2 * rows) // 256 * 256 or 256
+    width = min(piece, -(-V // 256) * 256)
+    copies = max(1, min(64, width // 512))
+    for weight in (0, 1):
+        without = 2 * rows * width + 12 * rows + weight * (4 * rows * H + 4 * (-(-V // 256) * 256)) + 6 * 256
+        assert 0 < ask(T, H, V, 0, weight) <= without
+        assert 4 * rows * H <= ask(T, H, V, 1, weight) - ask(T, H, V, 0, weight) <= 4 * rows * H * copies
