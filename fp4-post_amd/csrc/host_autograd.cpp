@@ -41,7 +41,25 @@ Tensor flat(const Tensor& t)
 const void* in(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* out(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 
-void checked(int rc, const char* what) { TORCH_CHECK(rc == METIS_OK, what, ": ", metis_error_string(rc), " (code ", rc, ")"); }
+// A return code as the package's own exception, in the forward and through the engine in the backward (the type is asked for with the interpreter held).
+struct EntryError : torch::PyTorchError {
+    using PyTorchError::PyTorchError;
+    PyObject* python_type() override
+    {
+        static PyObject* const type = [] {
+            PyObject* lib = PyImport_ImportModule("metis_hip._lib");
+            PyObject* found = lib ? PyObject_GetAttrString(lib, "MetisHipError") : nullptr;
+            Py_XDECREF(lib);
+            if (!found) PyErr_Clear();
+            return found ? found : PyExc_RuntimeError;
+        }();
+        return type;
+    }
+};
+void checked(int rc, const char* what)
+{
+    if (rc != METIS_OK) throw EntryError(std::string(what) + ": " + metis_error_string(rc) + " (code " + std::to_string(rc) + ")");
+}
 
 // Gradients that may be differentiated no further: where a second time is prepared, using them says so.
 variable_list once(variable_list grads)

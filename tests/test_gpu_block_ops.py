@@ -420,3 +420,14 @@ def test_recomputed_and_packed_away():
         t.grad = None
     torch.autograd.backward(checkpoint(step, *leaves, use_reentrant=True), (gh, gn))
     assert all(torch.equal(t.grad, b) for t, b in zip(leaves, want))
+
+
+def test_an_entry_points_refusal_is_the_packages_exception():
+    """More pieces than the kernel counts (2^28 rows of 64: refused before a launch, nothing reads or writes the 32 GiB), recorded and not."""
+    from metis_hip import MetisHipError, swiglu
+    big = torch.empty(1 << 28, 64, dtype=BF, device="cuda")
+    for grad in (False, True):
+        with pytest.raises(MetisHipError, match="metis_swiglu"):
+            swiglu(big.requires_grad_(grad), big)
+    del big
+    torch.cuda.empty_cache()
