@@ -832,10 +832,14 @@ class LinearLowbit(nn.Module):
         return super()._apply(fn, recurse=recurse)
 
 
+# (looked up once: every call of an operator asks, some of them cost 8 us of host time in all)
+_forward_ad, _transform_level, _is_tracing = torch.autograd.forward_ad, torch._C._functorch.maybe_current_level, torch.jit.is_tracing
+
+
 def _transformed() -> bool:
     """Whether forward-mode differentiation, one of torch.func's transforms or a tracer sees this call: they need not leave a mark on the tensors that
     reverse mode leaves (requires_grad), and have to meet an autograd function, or its refusal."""
-    return torch.autograd.forward_ad._current_level >= 0 or torch._C._functorch.maybe_current_level() is not None or torch.jit.is_tracing()
+    return _forward_ad._current_level >= 0 or _transform_level() is not None or _is_tracing()
 
 
 def _autograd_may_see() -> bool:
