@@ -8,9 +8,14 @@
 //
 // All three products run on one tile engine (below).  Forward: every 256-column tile of the logits leaves, per token, its maximum and its sum of
 // exponentials (and of p l) from the accumulators; a second launch folds the tiles.  Backward: pieces of the vocabulary one after the other; a piece's
-// logits are formed again, turned into dl in the accumulators, rounded to bf16 once (the type in which both products take it; the one element that makes
-// most of a row, the target's, is made good: AtTarget) and kept only until the piece's two products have read it.  The gradient of hidden is summed in
-// binary32 over the pieces.
+// logits are formed again, turned into dl in the accumulators, rounded to bf16 once and kept only until the piece's two products have read it.  The gradient of
+// hidden is summed in binary32 over the pieces.
+//
+// That rounding is a choice: bf16 is the type in which the matrix units take both products at their full rate (dl in two parts would be two more products,
+// 6 ms beside 12.5 at 4096 x 3584 against 131072), and the one in which a bf16 model's gradient of its logits is held anyway.  It is made good where it would not average
+// out, at the target, whose element makes most of a token's row (AtTarget).  Errors against 64 bits, relative to the norm (411 x 1536 against 32003, 600 x 2048 against
+// 65537; the results' own rounding to bf16 alone is 0.0017): both gradients 0.0017 where the targets' elements are most of them; where the mass lies on other
+// tokens, 0.0018; the entropy's alone under peaked distributions, and the rows of the weight's gradient that are no token's target, 0.0024.
 //
 // Tokens whose target is ignored take no part: a first launch lists the others ("live"), the products run over the listed rows, and what an ignored
 // row of hidden holds (padding: anything) is never read into a sum.

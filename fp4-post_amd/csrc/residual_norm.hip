@@ -13,8 +13,8 @@
 //
 // A row belongs to W waves (one per 512 columns up to 2048, then four or eight), lane l of wave w holding the chunks of eight elements
 // (i W + w) 64 + l: every access instruction of a wave covers consecutive bytes, the row is read once, its sums are folded across the lanes with
-// DPP moves and across the waves through LDS.  Bound by memory: 8192 x 3584 bf16 forward 40 us (5.9 TB/s of the 8 bytes an element), backward
-// 40 and 4 for the columns' sums (4.4 TB/s of 6 bytes: its reads, one after the other's folds, do not fill the queue as a copy's do).
+// DPP moves and across the waves through LDS.  Bound by memory: 8192 x 3584 bf16 forward 40 us and backward 40, both 5.9 TB/s of 8 bytes an element (x, y
+// read, h, n written; h, gh, gn read, gx written, which is gy too where nothing lies between the sum and y), and 4 us for the columns' sums.
 #include "chunk8.h"
 #include "metis_host.h"
 

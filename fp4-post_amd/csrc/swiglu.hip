@@ -1,7 +1,7 @@
 // silu(gate) * up between two projections of an MLP, and its gradients:
 //   a = g s u,   s = 1 / (1 + exp(-g));     du = da g s,   dg = da u s (1 + g (1 - s))
 // in binary32, each result rounded once.  Elementwise and bound by memory: 6 (10) bytes an element in bf16.  gate and up are rows of their own strides
-// (the halves of one product's rows as they are; 4096 x 18944 bf16 in halves 70 us forward and 121 backward, 6.7 and 6.4 TB/s); a lane takes eight elements where rows, strides and addresses allow whole 16-byte accesses, else one.
+// (the halves of one product's rows as they are; 4096 x 18944 bf16 in halves 72 us forward and 123 backward, 6.4 and 6.3 TB/s); a lane takes eight elements where rows, strides and addresses allow whole 16-byte accesses, else one.
 #include "chunk8.h"
 #include "metis_host.h"
 
@@ -27,7 +27,7 @@ template <bool F32> __device__ __forceinline__ void gated_back(float g, float u,
 template <class I> __device__ __forceinline__ size_t strided(I at, uint32_t per, uint64_t ld) { return ld == per ? at : at / per * ld + at % per; }
 
 // STREAM: more bytes than the memory-side cache holds (kStreamBytes) go by it with the non-temporal hint, and the backward takes two chunks a lane at once.
-// 4096 x 18944 bf16, halves of one product: 87 -> 69 us and 148 -> 122 (6.8 and 6.3 TB/s); of 1024 rows, which stay in the cache, 19 and 31 us with or without
+// 4096 x 18944 bf16, halves of one product: 87 us forward and 148 backward without either, 72 and 123 with both; of 1024 rows, which stay in the cache, 19 and 31 us with or without
 // the hint, 512 x 8960 8.4 us without and 9.4 with it.
 template <class C, bool STREAM>
 __global__ __launch_bounds__(256) void swiglu_kernel(const void* __restrict__ gate, uint64_t ldg, const void* __restrict__ up, uint64_t ldu, uint32_t total,
