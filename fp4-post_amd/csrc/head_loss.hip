@@ -298,7 +298,7 @@ __device__ __forceinline__ void hl_store_bf16(const float16_t (&acc)[TM][HL_TN],
 }
 
 // What the launches share about the tokens: index[0] the number of live ones, index[64 ..] their rows in order, index[64 + tokens ..] each row's place
-// among them or -1.
+// among them or -1, index[64 + 2 tokens ..] by place the target's log-probability in powers of two, as the forward's own sums give it.
 struct Tokens {
     const uint16_t* hidden;
     int64_t ld;
@@ -308,6 +308,7 @@ struct Tokens {
     float scale2;                // log2(e) / temperature: logits in powers of two
 };
 __device__ __forceinline__ const int* live_rows(const int* index) { return index + 64; }
+__host__ __device__ constexpr int64_t index_words(int64_t tokens) { return 64 + 3 * tokens; }
 
 // the k-th tile of this workgroup's XCD, which has a contiguous range of the tiles; -1 behind it
 __device__ __forceinline__ int hl_logical(int total, int k)
@@ -361,7 +362,7 @@ template <int TM> __device__ __forceinline__ void hl_clear(float16_t (&acc)[TM][
 
 // ---------------------------------------------------------------------------------------------
 // Forward: per tile and live token the maximum of its logits (in powers of two), the sum of 2^(l - maximum) and, for the entropy, of
-// 2^(l - maximum) (l - maximum); the target's logit from the tile that has it.
+// 2^(l - maximum) (l - maximum); the target's sum of products from the tile that has it.
 // ---------------------------------------------------------------------------------------------
 // What a tile leaves, from its accumulators; `red`: LDS.
 template <int TM, bool ENT>
@@ -407,7 +408,7 @@ __device__ __forceinline__ void hl_stats_out(float16_t (&acc)[TM][HL_TN], float*
                 for (int j = 0; j < HL_TN; ++j)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (want == j * 32 + 8 * (e >> 2) + 4 * hi + (e & 3)) hit[m] = acc[i][j][e] * tk.scale2;
+                        if (want == j * 32 + 8 * (e >> 2) + 4 * hi + (e & 3)) hit[m] = acc[i][j][e];
             }
         }
         if (hi == 0) {
@@ -520,7 +521,7 @@ template <bool ENT> __device__ __forceinline__ Fold fold(const Fold& a, const Fo
 // The tiles of a token folded, 16 tokens per workgroup: 64 chains of every 64th tile, eight requested together, then the four chains of a wave by lanes and
 // the sixteen waves in order.
 template <bool ENT>
-__global__ __launch_bounds__(1024) void head_finish_kernel(const int64_t* __restrict__ targets, const int* __restrict__ index, int tokens, int V, int tiles_n, int stride,
+__global__ __launch_bounds__(1024) void head_finish_kernel(const int64_t* __restrict__ targets, int* __restrict__ index, int tokens, int V, int tiles_n, int stride, float scale2,
                                                            const float2* __restrict__ part, const float* __restrict__ part_e, const float* __restrict__ hit,
                                                            float* __restrict__ logp, float* __restrict__ lse, float* __restrict__ entropy)
 {
@@ -565,8 +566,13 @@ __global__ __launch_bounds__(1024) void head_finish_kernel(const int64_t* __rest
     const int64_t want = targets[t];
     const bool there = want >= 0 && want < V;                  // (a target outside of the vocabulary shows: everything of its row is NaN)
     const float l2 = __log2f(mine.sum), nan = __uint_as_float(0x7fc00000u);
+    // The target's logit is compared with the maximum as the sums compared each of theirs: one fma from its sum of products.  Where it is the maximum, what is left
+    // is the sum's distance from one, with nothing of the size of the logits in it.
+    float lp2 = there ? fmaf(hit[pos], scale2, -mine.top) - l2 : nan;
+    lp2 = lp2 > 0.0f ? 0.0f : lp2;                             // (a rounding above zero; NaN stays)
     lse[t] = there ? (mine.top + l2) * kLn2 : nan;
-    logp[t] = there ? ((hit[pos] - mine.top) - l2) * kLn2 : nan;
+    logp[t] = lp2 * kLn2;
+    reinterpret_cast<float*>(index)[64 + 2 * tokens + pos] = lp2;
     if constexpr (ENT) entropy[t] = there ? (l2 - mine.ent / mine.sum) * kLn2 : nan;
 }
 
@@ -708,45 +714,31 @@ __global__ __launch_bounds__(HL_THREADS, 2) void head_dlogits_kernel(const Token
 }
 
 // Before the pieces: dl at the targets, and for grad_weight (`out`) the live rows of hidden side by side, then zero rows up to a multiple of 32.
-__global__ __launch_bounds__(256) void head_gather_kernel(const Tokens tk, const uint16_t* __restrict__ weight, int64_t ldw, const RowGrads rg, const AtTarget target, uint4* __restrict__ out)
+//   dl = g (1 - p) - e p (log p + H)  at the target, with the forward's log p: 1 - p is what the other tokens' p add up to but for the rounding of sums of about one.
+// (With p from a product of its own and the log-sum-exp 1 - p was off by their roundings, 2^-24 of the logits: where a model is sure, 1 - p under 1e-3, by
+// a tenth and more of these tokens' gradients.)
+__global__ __launch_bounds__(256) void head_gather_kernel(const Tokens tk, const RowGrads rg, const AtTarget target, uint4* __restrict__ out)
 {
-    constexpr float kLn2 = 0.693147180559945f, kLog2e = 1.44269504088896f;
-    __shared__ float red[2][4];
-    const int count = tk.index[0], rows = out ? (count + 31) & ~31 : count, cpr = tk.H / 8;
-    int turn = 0;
-    for (int m = blockIdx.x; m < rows; m += gridDim.x, turn ^= 1) {
-        if (m >= count) {
-            for (int c = threadIdx.x; c < cpr; c += 256) out[(int64_t)m * cpr + c] = make_uint4(0u, 0u, 0u, 0u);
-            continue;
-        }
+    constexpr float kLn2 = 0.693147180559945f;
+    const int count = tk.index[0], cpr = tk.H / 8;
+    const float inv_t = tk.scale2 * kLn2;                      // 1 / temperature
+    for (int m = blockIdx.x * 256 + threadIdx.x; m < count; m += gridDim.x * 256) {
         const int t = live_rows(tk.index)[m];
         const int64_t want = tk.targets[t];
         const bool there = want >= 0 && want < tk.V;
-        const uint4* x = reinterpret_cast<const uint4*>(tk.hidden + (int64_t)t * tk.ld);
-        const uint4* w = reinterpret_cast<const uint4*>(weight + (there ? want : 0) * ldw);
-        float dot = 0.0f;
-        for (int c = threadIdx.x; c < cpr; c += 256) {
-            const uint4 a = x[c], b = w[c];
-            if (out) out[(int64_t)m * cpr + c] = a;
-            const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                dot = fmaf(__uint_as_float(aw[k] << 16), __uint_as_float(bw[k] << 16), dot);
-                dot = fmaf(__uint_as_float(aw[k] & 0xffff0000u), __uint_as_float(bw[k] & 0xffff0000u), dot);
-            }
-        }
-#pragma unroll
-        for (int o = 32; o; o >>= 1) dot += __shfl_xor(dot, o, 64);
-        if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = dot;
-        __syncthreads();
-        if (threadIdx.x) continue;
-        dot = (red[turn][0] + red[turn][1]) + (red[turn][2] + red[turn][3]);
-        const float inv_t = tk.scale2 * kLn2, g = rg.g_logp ? rg.g_logp[t] * inv_t : 0.0f, d = fmaf(dot, tk.scale2, -rg.lse[t] * kLog2e);
-        const float f = rg.g_entropy ? fmaf(rg.g_entropy[t] * inv_t, fmaf(d, kLn2, rg.entropy[t]), g) : g;
-        const float v = fmaf(-__builtin_amdgcn_exp2f(d), f, g), r = __uint_as_float(rb_pair(v, 0.0f) << 16);
+        const float lp = reinterpret_cast<const float*>(tk.index)[64 + 2 * tk.tokens + m] * kLn2;
+        float v = rg.g_logp ? rg.g_logp[t] * inv_t * -expm1f(lp) : 0.0f;
+        if (rg.g_entropy) v = fmaf(-expf(lp), rg.g_entropy[t] * inv_t * (lp + rg.entropy[t]), v);
+        const float r = __uint_as_float(rb_pair(v, 0.0f) << 16);
         target.rounded[m] = r;
         target.left[m] = there && fabsf(r) < INFINITY ? v - r : 0.0f;
         target.column[m] = there ? (int)want : -1;
+    }
+    if (!out) return;
+    const int rows = (count + 31) & ~31;
+    for (int m = blockIdx.x; m < rows; m += gridDim.x) {
+        const uint4* x = reinterpret_cast<const uint4*>(tk.hidden + (int64_t)live_rows(tk.index)[m < count ? m : 0] * tk.ld);
+        for (int c = threadIdx.x; c < cpr; c += 256) out[(int64_t)m * cpr + c] = m < count ? x[c] : make_uint4(0u, 0u, 0u, 0u);
     }
 }
 
@@ -1073,7 +1065,7 @@ bool operands_ok(const void* hidden, int64_t ldh, const void* weight, int64_t ld
 
 }  // namespace
 
-size_t head_index_bytes(int64_t tokens) { return tokens < 0 || tokens > (1 << 24) ? 0 : align256((size_t)(64 + 2 * tokens) * sizeof(int)); }
+size_t head_index_bytes(int64_t tokens) { return tokens < 0 || tokens > (1 << 24) ? 0 : align256((size_t)index_words(tokens) * sizeof(int)); }
 
 size_t head_logprobs_workspace_bytes(int64_t tokens, int64_t H, int64_t V, int entropy)
 {
@@ -1106,9 +1098,9 @@ int head_logprobs(const void* hidden, int64_t ldh, const void* weight, int64_t l
     if (rc != METIS_OK) return rc;
     const dim3 grid((unsigned)((tokens + 15) / 16));
     if (entropy)
-        hipLaunchKernelGGL((head_finish_kernel<true>), grid, dim3(1024), 0, st, (const int64_t*)targets, (const int*)index, (int)tokens, (int)V, tiles_n, stride, part, part_e, hit, logp, lse, entropy);
+        hipLaunchKernelGGL((head_finish_kernel<true>), grid, dim3(1024), 0, st, (const int64_t*)targets, (int*)index, (int)tokens, (int)V, tiles_n, stride, tk.scale2, part, part_e, hit, logp, lse, entropy);
     else
-        hipLaunchKernelGGL((head_finish_kernel<false>), grid, dim3(1024), 0, st, (const int64_t*)targets, (const int*)index, (int)tokens, (int)V, tiles_n, stride, part, part_e, hit, logp, lse, entropy);
+        hipLaunchKernelGGL((head_finish_kernel<false>), grid, dim3(1024), 0, st, (const int64_t*)targets, (int*)index, (int)tokens, (int)V, tiles_n, stride, tk.scale2, part, part_e, hit, logp, lse, entropy);
     return hipGetLastError() == hipSuccess ? METIS_OK : METIS_E_LAUNCH;
 }
 
@@ -1154,7 +1146,7 @@ int head_logprobs_backward(const void* hidden, int64_t ldh, const void* weight, 
     const Tokens tk = tokens_of(hidden, ldh, targets, index, tokens, H, V, temperature);
     const RowGrads rg = {lse, entropy, g_logp, g_entropy};
     const int cus = device_cus();
-    hipLaunchKernelGGL(head_gather_kernel, dim3((unsigned)(tokens + 31 < 8 * (int64_t)cus ? tokens + 31 : 8 * (int64_t)cus)), dim3(256), 0, st, tk, (const uint16_t*)weight, ldw, rg, target,
+    hipLaunchKernelGGL(head_gather_kernel, dim3((unsigned)(tokens + 31 < 8 * (int64_t)cus ? tokens + 31 : 8 * (int64_t)cus)), dim3(256), 0, st, tk, rg, target,
                        (uint4*)gathered);
     if (hipGetLastError() != hipSuccess) return METIS_E_LAUNCH;
     if (grad_weight) {

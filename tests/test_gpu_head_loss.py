@@ -396,3 +396,43 @@ def test_recomputed_and_packed_away():
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(run(x, w), leaves, (g, e)), want))
     torch.autograd.backward(checkpoint(step, x, w, use_reentrant=True), (g, e))
     assert all(torch.equal(t.grad, b) for t, b in zip(leaves, want))
+
+
+@pytest.mark.parametrize("temp", [1.0, 0.5, 2.0])
+@pytest.mark.parametrize("T", [7, 90, 2100])
+def test_tokens_that_the_model_is_all_but_sure_of(T, temp):
+    """Logits far from zero that lie close together, of whole numbers, so that every sum of products is exact: 6144 from what all rows of the head share, and
+    twelve signs of each row's own, of which every one that differs from the target's takes 2 s off, s = 3 .. 10.  What is left of 1 - p is 0.03 to 1e-8.
+
+    logp: the target's term and the maximum are the same number, so what is lost is lost in a sum that is a little over one, of at most 64 additions on any
+    way (2^-24 each), and its logarithm: 2^-17 in all.  (As the difference of a logit and a log-sum-exp in binary32 it would be off by 2^-24 6144 / temperature, up to 1e-3.)
+    dl at the target, g (1 - p): the same 2^-17 of g, and the remainder's rounding; elsewhere a rounding to bf16 and what the log-sum-exp's roundings make of p, three
+    of 2^-24 and two constants' of 2^-25 of 6144 / temperature: under 2^-8 of it.  And the products' binary32 sums."""
+    from metis_hip import token_logprobs
+    g = torch.Generator().manual_seed(T)
+    V, H = 1500, 64
+    codes = torch.randperm(4096, generator=g)[:V]
+    signs = ((codes[:, None] >> torch.arange(12)) & 1) * 2 - 1
+    w = torch.cat([torch.full((V, 48), 8.0), signs.float(), torch.zeros(V, 4)], 1).to(BF).cuda()
+    t = torch.randint(V, (T,), generator=g)
+    s = torch.randint(3, 11, (T, 1), generator=g).float()
+    x = torch.cat([torch.full((T, 48), 16.0), s * signs[t], torch.randn(T, 4, generator=g).to(BF).float()], 1).to(BF).cuda()
+    t, grad = t.cuda(), torch.randn(T, generator=g).cuda()
+    t[::5] = -100
+    x.requires_grad_()
+    w.requires_grad_()
+    logp = token_logprobs(x, w, t, temperature=temp)
+    gx, gw = torch.autograd.grad(logp, (x, w), grad)
+    with torch.no_grad():
+        live, at = t != -100, torch.where(t == -100, 0, t)[:, None]
+        l = x.double() @ w.double().t() / temp
+        others = torch.exp(l - l.gather(1, at)).scatter_(1, at, 0.0)                      # relative to the target's
+        rest = others.sum(1, keepdim=True)
+        want = torch.where(live, -torch.log1p(rest).squeeze(1), 0.0)
+        assert bool(((logp.double() - want).abs() <= 2.0 ** -17 + 2.0 ** -23 * want.abs()).all()), float((logp.double() - want).abs().max())
+        gd = torch.where(live, grad.double(), 0.0)[:, None] / temp
+        d = (-gd * others / (1 + rest)).scatter_(1, at, gd * rest / (1 + rest))
+        off = ((HALF + 2.0 ** -8) * d.abs()).scatter_(1, at, HALF ** 2 * d.abs().gather(1, at) + 2.0 ** -17 * gd.abs()) + max(T, V) * 2.0 ** -24 * d.abs()
+        for got, exact, bound in ((gx, d @ w.double(), off @ w.double().abs()), (gw, d.t() @ x.double(), off.t() @ x.double().abs())):
+            bound = bound + HALF * (exact.abs() + bound) + 1e-30
+            assert bool(((got.double() - exact).abs() <= bound).all()), float(((got.double() - exact).abs() / bound).max())
