@@ -1146,8 +1146,8 @@ int head_logprobs_backward(const void* hidden, int64_t ldh, const void* weight, 
     const Tokens tk = tokens_of(hidden, ldh, targets, index, tokens, H, V, temperature);
     const RowGrads rg = {lse, entropy, g_logp, g_entropy};
     const int cus = device_cus();
-    hipLaunchKernelGGL(head_gather_kernel, dim3((unsigned)(tokens + 31 < 8 * (int64_t)cus ? tokens + 31 : 8 * (int64_t)cus)), dim3(256), 0, st, tk, rg, target,
-                       (uint4*)gathered);
+    const int64_t teams = gathered ? tokens + 31 : (tokens + 255) / 256;
+    hipLaunchKernelGGL(head_gather_kernel, dim3((unsigned)(teams < 8 * (int64_t)cus ? teams : 8 * (int64_t)cus)), dim3(256), 0, st, tk, rg, target, (uint4*)gathered);
     if (hipGetLastError() != hipSuccess) return METIS_E_LAUNCH;
     if (grad_weight) {
         const int64_t fit = 2 * (int64_t)cus / ((V + 255) / 256), chunks = (H + 511) / 512;
