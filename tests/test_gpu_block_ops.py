@@ -431,3 +431,38 @@ def test_an_entry_points_refusal_is_the_packages_exception():
             swiglu(big.requires_grad_(grad), big)
     del big
     torch.cuda.empty_cache()
+
+
+def _repeated(rows, cols, times, seed, dtype=BF):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(rows, cols, generator=gen, device="cuda").to(dtype).repeat(times, 1)
+
+
+def test_residual_norm_beyond_32_bits_of_elements():
+    """2^32 elements and 8192 rows more, the same 4096 rows again and again: every repetition has the first one's bits, forward and backward."""
+    from metis_hip import ops
+    rows, cols, times = 4096, 8192, 130
+    assert rows * cols * times > 1 << 32
+    x, y, gn = (_repeated(rows, cols, times, k) for k in (1, 2, 3))
+    w = _repeated(1, cols, 1, 4)[0]
+    h, n = ops.residual_norm(x, y, w)
+    gx, gy, gw, _, _ = ops.residual_norm_backward(h, y, w, None, None, 1.0, 1e-6, None, gn, BF)
+    small = ops.residual_norm(x[:rows], y[:rows], w)
+    want = (*small, ops.residual_norm_backward(small[0], y[:rows], w, None, None, 1.0, 1e-6, None, gn[:rows], BF)[0])
+    for got, first in zip((h, n, gx), want):
+        assert all(torch.equal(got[k * rows:(k + 1) * rows], first) for k in range(times))
+    assert bool(gw.isfinite().all())
+    del x, y, gn, h, n, gx, gy
+    torch.cuda.empty_cache()
+
+
+def test_swiglu_beyond_32_bits_of_elements():
+    from metis_hip import ops
+    rows, cols, times = 2048, 18952, 111
+    assert rows * cols * times > 1 << 32
+    g, u, da = (_repeated(rows, cols, times, k) for k in (5, 6, 7))
+    want = (ops.swiglu(g[:rows], u[:rows]), *ops.swiglu_backward(g[:rows], u[:rows], da[:rows]))
+    for got, first in zip((ops.swiglu(g, u), *ops.swiglu_backward(g, u, da)), want):
+        assert all(torch.equal(got[k * rows:(k + 1) * rows], first) for k in range(times))
+    del g, u, da, got
+    torch.cuda.empty_cache()

@@ -436,3 +436,27 @@ def test_tokens_that_the_model_is_all_but_sure_of(T, temp):
         for got, exact, bound in ((gx, d @ w.double(), off @ w.double().abs()), (gw, d.t() @ x.double(), off.t() @ x.double().abs())):
             bound = bound + HALF * (exact.abs() + bound) + 1e-30
             assert bool(((got.double() - exact).abs() <= bound).all()), float(((got.double() - exact).abs() / bound).max())
+
+
+def test_hidden_beyond_32_bits_of_elements():
+    """2^32 elements of hidden and more, the same 3000 tokens again and again: every repetition has the first one's bits where the sums are the same ones, the
+    log-probabilities, and but for the order of binary32 sums those of a call on 3000, hidden's gradient."""
+    from metis_hip import ops
+    T, H, V, times = 3000, 4096, 300, 350
+    assert T * H * times > 1 << 32
+    x, w, t, g, _ = make(5, T, H, V)
+    many, ts, gs = x.repeat(times, 1), t.repeat(times), g.repeat(times)
+    logp, lse, _, index = ops.head_logprobs(many, w, ts)
+    gx, gw = ops.head_logprobs_backward(many, w, ts, 1.0, lse, None, index, gs, None)
+    first = ops.head_logprobs(x, w, t)
+    gx1, gw1 = ops.head_logprobs_backward(x, w, t, 1.0, first[1], None, first[3], g, None)
+    assert all(torch.equal(logp[k * T:(k + 1) * T], first[0]) for k in range(times))
+    # (dl is the same, its products with the head are sums of 300 terms in one order or another: a step of bf16 where they round apart)
+    for k in range(times):
+        assert bool(((gx[k * T:(k + 1) * T].float() - gx1.float()).abs() <= 2 * HALF * gx1.float().abs() + 300 * 2.0 ** -24 * (w.float().norm(dim=1).max() * g.abs().max())).all())
+    # each element of the weight's gradient is `times` times the small call's, both rounded once and their binary32 sums in between: of a million terms in chains
+    # of the tokens' order, sqrt(2^20) 2^-24 of their magnitudes
+    scale = float(gw1.double().norm())
+    assert float((gw.double() / times - gw1.double()).norm()) <= (2 * HALF + 2.0 ** -14 * 8) * scale
+    del many, gx
+    torch.cuda.empty_cache()
