@@ -7,6 +7,7 @@ operator on the last hidden states and the head's weight.
 """
 from __future__ import annotations
 
+import copy
 import inspect
 from collections.abc import Mapping
 
@@ -81,6 +82,18 @@ class _Known(nn.Module):
         return self.__dict__["__known"][0]
 
 
+def _with_hidden(out, hidden: torch.Tensor):
+    """A decoder's output like `out` that holds these last hidden states, and nothing else where its class can be made of them alone."""
+    if isinstance(out, tuple):
+        return out._replace(**{out._fields[0]: hidden}) if hasattr(out, "_fields") else (hidden, *out[1:])
+    try:
+        return type(out)(last_hidden_state=hidden)
+    except TypeError:
+        other = copy.copy(out)
+        other.last_hidden_state = hidden
+        return other
+
+
 @torch.no_grad()
 def _logits_are_the_product(model, head, weight: torch.Tensor, out, masked: bool, inputs: dict) -> bool:
     """Whether the model's logits are its last hidden states times the head's weight, with no factor, cap, shift or cut on the way.  Its class's forward is
@@ -97,7 +110,7 @@ def _logits_are_the_product(model, head, weight: torch.Tensor, out, masked: bool
             hidden = torch.cos(torch.arange(rows * H, dtype=torch.float64) ** 2).reshape(1, rows, H) * torch.tensor([0.0, 1e1, 1e5], dtype=torch.float64)[:, None]
             small = nn.Linear(H, V, bias=False, dtype=torch.float64, device="meta")
             small.weight = nn.Parameter(torch.linspace(-1.0, 1.0, V * H, dtype=torch.float64).reshape(V, H), requires_grad=False)
-            known = _Known((hidden, *out[1:]) if isinstance(out, tuple) else type(out)(last_hidden_state=hidden), model.base_model)
+            known = _Known(_with_hidden(out, hidden), model.base_model)
             modules = {name: known if m is model.base_model else small if m is head else m for name, m in model._modules.items()}
             if known not in modules.values() or small not in modules.values():
                 return False

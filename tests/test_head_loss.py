@@ -324,3 +324,30 @@ def test_the_backwards_workspace_is_what_the_header_says(T, H, V):
         without = 2 * rows * width + 12 * rows + weight * (4 * rows * H + 4 * (-(-V // 256) * 256)) + 6 * 256
         assert 0 < ask(T, H, V, 0, weight) <= without
         assert 4 * rows * H <= ask(T, H, V, 1, weight) - ask(T, H, V, 0, weight) <= 4 * rows * H * copies
+
+
+def test_decoder_outputs_of_a_class_of_their_own_are_taken():
+    """One that cannot be made of the hidden states alone, and a tuple with names."""
+    from collections import namedtuple
+
+    class Output:
+        def __init__(self, last_hidden_state, aux):
+            self.last_hidden_state, self.aux = last_hidden_state, aux
+
+    for output in (Output, namedtuple("Named", ["last_hidden_state", "aux"])):
+        class Decoder(_Decoder):
+            def forward(self, input_ids, attention_mask=None, output=output):
+                return output(self.embed(input_ids), 3)
+
+        for kind, taken in ((_Causal, True), (_TimesHead, False)):
+            class Model(kind):
+                def hidden(self, input_ids, attention_mask):
+                    return self.base_model(input_ids, attention_mask=attention_mask).last_hidden_state
+
+            model = Model()
+            model.base_model = Decoder("object")
+            if taken:
+                _asked(model)
+            else:
+                with pytest.raises(ValueError, match="logits"):
+                    model_token_logprobs(model, torch.tensor([[3, 4, 5, 6]]))
