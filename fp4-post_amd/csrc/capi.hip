@@ -682,4 +682,46 @@ int metis_head_logprobs_backward(const void* hidden, int64_t ld_hidden, const vo
                                   grad_weight, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
+int metis_rotary(const void* q, int64_t q_token, int64_t q_head, int64_t q_heads, const void* k, int64_t k_token, int64_t k_head, int64_t k_heads, const int64_t* positions,
+                 int64_t npos, const void* inv_freq, int freq_dtype, int64_t tokens, int64_t dim, int64_t turned, int interleaved, int back, float factor, int dtype, void* q_out,
+                 void* k_out, void* stream)
+{
+    return rotary(q, q_token, q_head, q_heads, k, k_token, k_head, k_heads, nullptr, 0, 0, positions, npos, inv_freq, freq_dtype, nullptr, tokens, dim, turned, interleaved, back,
+                  factor, dtype, 0, 1, METIS_DTYPE_BF16, 1.0f, 1.0f, q_out, k_out, nullptr, false, (hipStream_t)stream);
+}
+
+int metis_rotary_append(const void* q, int64_t q_token, int64_t q_head, int64_t q_heads, const void* k, int64_t k_token, int64_t k_head, int64_t kv_heads, const void* v,
+                        int64_t v_token, int64_t v_head, const int64_t* positions, const void* inv_freq, int freq_dtype, const int64_t* slots, int64_t tokens, int64_t dim,
+                        int64_t turned, int interleaved, float factor, int64_t pages, int64_t page, int cache_dtype, float key_scale, float value_scale, void* keys, void* values,
+                        void* q_out, void* stream)
+{
+    return rotary(q, q_token, q_head, q_heads, k, k_token, k_head, kv_heads, v, v_token, v_head, positions, tokens, inv_freq, freq_dtype, slots, tokens, dim, turned, interleaved, 0,
+                  factor, METIS_DTYPE_BF16, pages, page, cache_dtype, key_scale, value_scale, q_out, keys, values, true, (hipStream_t)stream);
+}
+
+size_t metis_paged_attention_workspace_bytes(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t capacity)
+{
+    return paged_attention_workspace_bytes(seqs, q_heads, kv_heads, dim, capacity);
+}
+
+int metis_paged_attention(const void* q, int64_t q_seq, int64_t q_head, int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, const void* keys, const void* values,
+                          int64_t pages, int64_t page, int cache_dtype, const int32_t* tables, int64_t table_stride, int64_t width, const int32_t* lengths, float scale,
+                          float key_scale, float value_scale, void* out, void* workspace, size_t workspace_bytes, void* stream)
+{
+    return paged_attention(q, q_seq, q_head, seqs, q_heads, kv_heads, dim, keys, values, pages, page, cache_dtype, tables, table_stride, width, lengths, scale, key_scale,
+                           value_scale, out, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int metis_cache_copy_pages(void* keys, void* values, int64_t layers, int64_t pages, int64_t page_bytes, const int64_t* sources, const int64_t* destinations, int64_t count,
+                           void* stream)
+{
+    return copy_pages(keys, values, layers, pages, page_bytes, sources, destinations, count, (hipStream_t)stream);
+}
+
+int metis_sample_tokens(const void* logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const float* uniforms, const double* parameters, const double* row_parameters,
+                        int64_t* tokens, float* logprobs, void* stream)
+{
+    return sample_tokens(logits, ld, dtype, rows, vocab, uniforms, parameters, row_parameters, tokens, logprobs, (hipStream_t)stream);
+}
+
 }  // extern "C"

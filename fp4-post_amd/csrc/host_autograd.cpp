@@ -1,7 +1,7 @@
-// residual_norm and swiglu as nodes of torch's autograd, in compiled code.  Host code only: the arithmetic is libmetis_hip.so's, the checks of arguments are
+// residual_norm, swiglu and rotary as nodes of torch's autograd, in compiled code.  Host code only: the arithmetic is libmetis_hip.so's, the checks of arguments are
 // made by the Python functions that call these (metis_hip/block.py, metis_hip/ops.py).
 //
-// Both are kernels of some tens of microseconds in a training step, and a node written in Python costs more than that: recorded, run backward in the
+// All are kernels of some tens of microseconds in a training step, and a node written in Python costs more than that: recorded, run backward in the
 // engine's own thread (which has to get the interpreter first) and allocated for.  One token x 1536, forward and all gradients: 101 us through
 // torch.autograd.Function in Python, 49 of them an empty one's, and 123 with a norm behind the block and a gate; here 73 and 93.
 #define PY_SSIZE_T_CLEAN
@@ -168,6 +168,62 @@ struct SwiGLU : torch::autograd::Function<SwiGLU> {
     }
 };
 
+// [..., heads, dim] as [tokens, heads, dim] with dense dimensions, and the strides of its tokens and heads (of a single one: none that counts)
+struct HeadRows {
+    Tensor t;
+    int64_t token = 0, head = 0, heads = 0;
+    HeadRows(const Tensor& given, int64_t tokens)
+    {
+        if (!given.defined()) return;
+        heads = given.size(-2);
+        const int64_t dim = given.size(-1);
+        t = given.reshape({tokens, heads, dim});
+        if (t.stride(2) != 1) t = t.contiguous();
+        token = tokens > 1 ? t.stride(0) : heads * dim;
+        head = heads > 1 ? t.stride(1) : dim;
+    }
+};
+
+struct Rotary : torch::autograd::Function<Rotary> {
+    // both results, undefined where there is nothing to turn
+    static variable_list turn(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq, bool interleaved, double factor, bool back)
+    {
+        const Tensor& any = q.defined() ? q : k;
+        const c10::DeviceGuard on(any.device());
+        const int64_t dim = any.size(-1), heads = any.size(-2), tokens = any.numel() > 0 ? any.numel() / (heads * dim) : 0;
+        const at::TensorOptions type = any.options().memory_format(at::MemoryFormat::Contiguous);
+        const Tensor to_q = q.defined() ? at::empty(q.sizes(), type) : Tensor(), to_k = k.defined() ? at::empty(k.sizes(), type) : Tensor();
+        if (tokens > 0) {
+            const HeadRows a(q, tokens), b(k, tokens);
+            checked(metis_rotary(in(a.t), a.token, a.head, a.heads, in(b.t), b.token, b.head, b.heads, positions.const_data_ptr<int64_t>(), positions.numel(), in(inv_freq),
+                                 inv_freq.scalar_type() == at::kDouble ? METIS_DTYPE_F64 : METIS_DTYPE_F32, tokens, dim, 2 * inv_freq.numel(), interleaved, back,
+                                 static_cast<float>(factor), dtype_of(any.scalar_type()), out(to_q), out(to_k), stream_of(any)), "metis_rotary");
+        }
+        return {to_q, to_k};
+    }
+
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq, bool interleaved, double factor)
+    {
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({positions, inv_freq});
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["factor"] = factor;
+        return turn(q, k, positions, inv_freq, interleaved, factor, false);
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        variable_list given(6);
+        const Tensor gq = ctx->needs_input_grad(0) ? grads[0] : Tensor(), gk = ctx->needs_input_grad(1) ? grads[1] : Tensor();
+        if (!gq.defined() && !gk.defined()) return given;
+        const variable_list saved = ctx->get_saved_variables();
+        const variable_list turned = turn(gq, gk, saved[0], saved[1], ctx->saved_data["interleaved"].toBool(), ctx->saved_data["factor"].toDouble(), true);
+        given[0] = turned[0];
+        given[1] = turned[1];
+        return once(std::move(given));
+    }
+};
+
 // The interpreter's lock given up: an allocation may wait for the device.
 struct Unlocked {
     PyThreadState* state = PyEval_SaveThread();
@@ -239,5 +295,37 @@ PyObject* metis_recorded_swiglu(PyObject*, PyObject* const* a, Py_ssize_t n)
         r = SwiGLU::apply(gate, up);
     }
     return THPVariable_Wrap(std::move(r));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* metis_recorded_rotary(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    Tensor t[4];
+    if (n != 6) {
+        PyErr_SetString(PyExc_TypeError, "recorded_rotary(q, k, positions, inv_freq, interleaved, factor)");
+        return nullptr;
+    }
+    for (int i = 0; i < 4; ++i) {
+        if (!tensor_of(a[i], &t[i])) return nullptr;
+        if (!t[i].defined()) {
+            PyErr_SetString(PyExc_TypeError, "recorded_rotary: q, k, positions and inv_freq are tensors");
+            return nullptr;
+        }
+    }
+    const int interleaved = PyObject_IsTrue(a[4]);
+    const double factor = PyFloat_AsDouble(a[5]);
+    if (PyErr_Occurred()) return nullptr;
+    variable_list r;
+    {
+        Unlocked unlocked;
+        r = Rotary::apply(t[0], t[1], t[2], t[3], interleaved != 0, factor);
+    }
+    PyObject* q = THPVariable_Wrap(std::move(r[0]));
+    PyObject* k = q ? THPVariable_Wrap(std::move(r[1])) : nullptr;
+    PyObject* both = k ? PyTuple_Pack(2, q, k) : nullptr;
+    Py_XDECREF(q);
+    Py_XDECREF(k);
+    return both;
     END_HANDLE_TH_ERRORS
 }

@@ -5,3 +5,4 @@
 
 PyObject* metis_recorded_residual_norm(PyObject*, PyObject* const* args, Py_ssize_t count);
 PyObject* metis_recorded_swiglu(PyObject*, PyObject* const* args, Py_ssize_t count);
+PyObject* metis_recorded_rotary(PyObject*, PyObject* const* args, Py_ssize_t n);

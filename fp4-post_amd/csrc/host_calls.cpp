@@ -3,7 +3,7 @@
 //
 //   call(name, device_index, specs, args) -> tuple of tensors, or the entry point's return code if it is not METIS_OK
 //
-// specs: one (type, size, ...) per tensor to allocate on the device, type 0 uint8, 1 bfloat16, 2 float32.  args: the entry point's arguments in order,
+// specs: one (type, size, ...) per tensor to allocate on the device, type 0 uint8, 1 bfloat16, 2 float32, 3 int64.  args: the entry point's arguments in order,
 // each taken as the declaration in metis_hip.h says: for an integer whatever Python takes for an index (its low bits, as ctypes passes it), for a float
 // whatever has a float value, for an address None, a tensor, an integer or the new tensor at a text of one character's distance from "0", for an array of
 // structures (metis_linear_member, metis_lowrank_factor) a list of tuples of their 64-bit words, as many as the argument behind it says.  Anything else
@@ -136,6 +136,11 @@ constexpr Entry kEntries[] = {
     METIS_ENTRY(metis_swiglu_backward),
     METIS_ENTRY(metis_head_logprobs),
     METIS_ENTRY(metis_head_logprobs_backward),
+    METIS_ENTRY(metis_rotary),
+    METIS_ENTRY(metis_rotary_append),
+    METIS_ENTRY(metis_paged_attention),
+    METIS_ENTRY(metis_cache_copy_pages),
+    METIS_ENTRY(metis_sample_tokens),
 };
 constexpr size_t kMaxArgs = 32, kMaxOuts = 32;
 constexpr bool all_counted()
@@ -208,7 +213,7 @@ PyObject* call(PyObject*, PyObject* const* a, Py_ssize_t n)
     const long device = PyLong_AsLong(a[1]);
     if (device == -1 && PyErr_Occurred()) return nullptr;
 
-    static const at::ScalarType types[] = {at::kByte, at::kBFloat16, at::kFloat};
+    static const at::ScalarType types[] = {at::kByte, at::kBFloat16, at::kFloat, at::kLong};
     struct { at::ScalarType type; size_t begin, dims; } spec[kMaxOuts];
     c10::SmallVector<int64_t, 64> sizes;
     Outputs outs;
@@ -218,8 +223,8 @@ PyObject* call(PyObject*, PyObject* const* a, Py_ssize_t n)
         PyObject* s = PyTuple_GET_ITEM(a[2], i);
         const Py_ssize_t dims = PyTuple_Check(s) ? PyTuple_GET_SIZE(s) - 1 : -1;
         const long type = dims >= 0 ? PyLong_AsLong(PyTuple_GET_ITEM(s, 0)) : -1;
-        if (dims < 0 || type < 0 || type > 2) {
-            if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "call: a spec is (0 | 1 | 2, size, ...)");
+        if (dims < 0 || type < 0 || type > 3) {
+            if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "call: a spec is (0 | 1 | 2 | 3, size, ...)");
             return nullptr;
         }
         spec[i] = {types[type], sizes.size(), static_cast<size_t>(dims)};
@@ -295,6 +300,8 @@ PyMethodDef methods[] = {{"call", reinterpret_cast<PyCFunction>(reinterpret_cast
                           "recorded_residual_norm(x, y, weight, post_weight, gate, gate_rows, scale, eps): residual_norm of checked arguments as a node of autograd"},
                          {"recorded_swiglu", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&metis_recorded_swiglu)), METH_FASTCALL,
                           "recorded_swiglu(gate, up): swiglu of checked arguments as a node of autograd"},
+                         {"recorded_rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&metis_recorded_rotary)), METH_FASTCALL,
+                          "recorded_rotary(q, k, positions, inv_freq, interleaved, factor): rotary of checked arguments as a node of autograd"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_metis_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -133,6 +133,20 @@ size_t head_logprobs_backward_workspace_bytes(int64_t tokens, int64_t H, int64_t
 int head_logprobs_backward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, const void* targets, int64_t tokens, int64_t H, int64_t V, float temperature,
                            const float* lse, const float* entropy, const float* g_logp, const float* g_entropy, const void* index, void* grad_hidden, void* grad_weight,
                            void* workspace, size_t workspace_bytes, hipStream_t st);
+// queries and keys turned by their positions' angles; cached: keys and values into a cache's pages (k_out, v_out); rotary.hip
+int rotary(const void* q, int64_t q_token, int64_t q_head, int64_t q_heads, const void* k, int64_t k_token, int64_t k_head, int64_t k_heads, const void* v, int64_t v_token,
+           int64_t v_head, const int64_t* positions, int64_t npos, const void* inv_freq, int freq_dtype, const int64_t* slots, int64_t tokens, int64_t dim, int64_t turned,
+           int interleaved, int back, float factor, int dtype, int64_t pages, int64_t page, int cache_dtype, float key_scale, float value_scale, void* q_out, void* k_out,
+           void* v_out, bool cached, hipStream_t st);
+// one new token of each sequence over its pages, and copies of pages; paged_attention.hip
+size_t paged_attention_workspace_bytes(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t capacity);
+int paged_attention(const void* q, int64_t q_seq, int64_t q_head, int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, const void* keys, const void* values, int64_t pages,
+                    int64_t page, int cache_dtype, const int32_t* tables, int64_t table_stride, int64_t width, const int32_t* lengths, float scale, float key_scale,
+                    float value_scale, void* out, void* workspace, size_t workspace_bytes, hipStream_t st);
+int copy_pages(void* keys, void* values, int64_t layers, int64_t pages, int64_t page_bytes, const int64_t* from, const int64_t* to, int64_t count, hipStream_t st);
+// a token of each row's distribution by a given random number; sample.hip
+int sample_tokens(const void* logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const float* uniforms, const double* parameters, const double* row_parameters,
+                  int64_t* tokens, float* logprobs, hipStream_t st);
 int gemm_nvfp4(const void* a_codes, const void* a_scales, const float* a_unit, const void* b_codes, const void* b_scales,
                const float* b_unit, int64_t M, int64_t N, int64_t K, const void* t, const void* u, int64_t r,
                const void* bias, void* out, int out_dtype, hipStream_t st, void* workspace = nullptr,

@@ -1,0 +1,423 @@
+// Attention of one new token of each sequence over the pages of its keys and values, and copies of whole pages:
+//   o = sum_t p_t v_t / sum_t p_t,   p_t = exp(scale q . k_t - m),   m the largest of the scores so far (one pass, the sums rescaled when it grows)
+// Bound by reading the cache.  All query heads that share a head of the cache (up to 16 in a tile) go through it together on the matrix cores, each key and value
+// read once, from memory straight into the registers that the products take them from:
+//   scores^T [tokens, heads] = K q^T        K is the first operand as it lies in its page (a row is a token)
+//   o^T [dim, heads] = V^T p^T              V is kept transposed in its page (a row is a dimension, its tokens side by side)
+// and the tokens are dealt to the rows of the first product in an order that leaves a lane with exactly the eight (two times eight) neighbouring tokens of one head
+// that the second product wants from it: no value crosses lanes but the maximum.  The probabilities enter the second product as two bf16 terms (2^-16 of them is lost),
+// which costs nothing: the matrix cores are idle most of the time.
+#include "metis_device.h"
+#include "metis_host.h"
+
+namespace metis {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;                                          // waves of a workgroup, each with its own blocks of tokens
+constexpr int kHeadTile = 16;
+
+struct AttendArgs {
+    const void *q, *keys, *values;
+    const int *tables, *lengths;
+    void* out;
+    float* partial;                                                // [pair, tile, split][16 heads][dim + 2]: sums, then maximum and sum of the weights
+    int64_t q_seq, q_head, table_stride;
+    int q_heads, kv_heads, group, pages, page_shift, width, splits, chunk, tiles;
+    float scale, value_scale;                                      // scale: of the scores, with log2 e
+};
+
+// eight e4m3 bytes as bf16, exactly
+__device__ __forceinline__ bf16x8_t widen(uint32_t lo, uint32_t hi)
+{
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true),
+                   c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+    return (bf16x8_t){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// DT: dimensions / 32.  F8: the cache is e4m3.  TOK: tokens of a block, 64, or 32 where 64 tokens' keys and values do not fit the registers.
+template <int DT, bool F8, int TOK>
+__global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(const AttendArgs a)
+{
+    constexpr int D = 32 * DT, S = TOK / 32, T = TOK / 16, NV = D / 16;
+    constexpr bool WIDE = F8 && TOK == 64;                         // sixteen neighbouring tokens to a lane, one 16-byte load of values for both steps; else eight a step
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const int split = blockIdx.x % a.splits;
+    int rest = blockIdx.x / a.splits;
+    const int tile = rest % a.tiles;
+    rest /= a.tiles;
+    const int kv = rest % a.kv_heads, seq = rest / a.kv_heads;
+    const int capacity = a.width << a.page_shift, said = a.lengths[seq], length = said < 0 ? 0 : said > capacity ? capacity : said;
+    const bool lie = said != length;                               // a length that the table cannot have: the result is NaN
+    const int begin = split * a.chunk, end = min(length, begin + a.chunk);
+    if (split > 0 && begin >= length) return;
+    const int heads = min(a.group - tile * kHeadTile, kHeadTile);  // heads of this tile
+    const int* table = a.tables + (size_t)seq * a.table_stride;
+
+    // q^T, the second operand: head n, dimensions as the keys' pieces have them
+    bf16x8_t q[DT];
+    const uint16_t* qrow = static_cast<const uint16_t*>(a.q) + (size_t)seq * a.q_seq + (size_t)(kv * a.group + tile * kHeadTile + n) * a.q_head;
+#pragma unroll
+    for (int c = 0; c < DT; ++c) {
+        const int d = F8 ? 64 * (c / 2) + 16 * g + 8 * (c & 1) : 32 * c + 8 * g;
+        const uint4 w = n < heads ? *reinterpret_cast<const uint4*>(qrow + d) : make_uint4(0u, 0u, 0u, 0u);
+        q[c] = __builtin_bit_cast(bf16x8_t, w);
+    }
+
+    f32x4_t o[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) o[i] = (f32x4_t){0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, sum = 0.0f;
+
+    const size_t unit = F8 ? 1 : 2, head_bytes = ((size_t)D << a.page_shift) * unit, page_bytes = head_bytes * a.kv_heads;
+    const char* keys = static_cast<const char*>(a.keys) + kv * head_bytes;
+    const char* values = static_cast<const char*>(a.values) + kv * head_bytes;
+    const int mask = (1 << a.page_shift) - 1;
+
+    for (int t0 = begin + wave * TOK; t0 < end; t0 += kWaves * TOK) {
+        uint32_t bad = 0;                                          // bit t: the page of this lane's key of tile t is none
+        uint4 kx[T][F8 ? DT / 2 : DT];
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const int r = n >> 2, j = n & 3;
+            const int tok = t0 + (WIDE ? 16 * r + 4 * t + j : 32 * (t >> 1) + 8 * r + 4 * (t & 1) + j);
+            int page = tok < end ? table[tok >> a.page_shift] : 0;
+            if ((uint32_t)page >= (uint32_t)a.pages) { page = 0; bad |= 1u << t; }
+            const char* row = keys + (size_t)page * page_bytes + (size_t)(tok & mask) * (D * unit);
+#pragma unroll
+            for (int c = 0; c < (F8 ? DT / 2 : DT); ++c) kx[t][c] = *reinterpret_cast<const uint4*>(row + 64 * c + 16 * g);
+        }
+        constexpr int VL = WIDE ? 1 : S, VW = F8 && !WIDE ? 2 : 4; // loads of a dimension, and their words
+        uint32_t vx[NV][VL][VW];
+#pragma unroll
+        for (int s = 0; s < VL; ++s) {
+            const int tok = t0 + (WIDE ? 16 * g : 32 * s + 8 * g);
+            int page = tok < end ? table[tok >> a.page_shift] : 0;
+            if ((uint32_t)page >= (uint32_t)a.pages) page = 0;
+            const char* col = values + (size_t)page * page_bytes + (size_t)(tok & mask) * unit;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const char* at = col + (((size_t)(16 * i + n) << a.page_shift) * unit);
+                if constexpr (VW == 4) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(at);
+                    vx[i][s][0] = w.x; vx[i][s][1] = w.y; vx[i][s][2] = w.z; vx[i][s][3] = w.w;
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2*>(at);
+                    vx[i][s][0] = w.x; vx[i][s][1] = w.y;
+                }
+            }
+        }
+
+        float p[TOK / 4];                                          // scores, then weights, of the lane's tokens in their order
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < DT; ++c) {
+                bf16x8_t k;
+                if constexpr (F8) k = (c & 1) ? widen(kx[t][c / 2].z, kx[t][c / 2].w) : widen(kx[t][c / 2].x, kx[t][c / 2].y);
+                else k = __builtin_bit_cast(bf16x8_t, kx[t][c]);
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[c], acc, 0, 0, 0);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[4 * t + j] = acc[j] * a.scale;
+        }
+        // tokens behind the end have no weight; a token whose page is none makes the result NaN
+        const bool tail = t0 + TOK > end;
+        if (tail || __any(bad != 0)) {
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int tok = t0 + (WIDE ? 16 * g + 4 * t + j : 32 * (t >> 1) + 8 * g + 4 * (t & 1) + j);
+                    const int from = 4 * g + j;                    // the lane that loaded this row's key
+                    const bool none = (__shfl((int)bad, from, 64) >> t) & 1;
+                    if (tok >= end) p[4 * t + j] = -INFINITY;
+                    else if (none) p[4 * t + j] = __builtin_nanf("");
+                }
+            }
+            if (tail) {                                            // (what lies behind the end may be anything: 0 times it has to be 0)
+#pragma unroll
+                for (int s = 0; s < VL; ++s) {
+                    const int left = end - (t0 + (WIDE ? 16 * g : 32 * s + 8 * g));        // tokens of this load that count
+                    constexpr int PER = F8 ? 4 : 2;                                        // of a word
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) {
+                        const int k = min(max(left - PER * w, 0), PER);
+                        const uint32_t keep = k == PER ? ~0u : (1u << (32 / PER * k)) - 1u;
+#pragma unroll
+                        for (int i = 0; i < NV; ++i) vx[i][s][w] &= keep;
+                    }
+                }
+            }
+        }
+        float top = p[0];
+#pragma unroll
+        for (int i = 1; i < TOK / 4; ++i) top = fmaxf(top, p[i]);
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float next = fmaxf(m, top), shift = next == -INFINITY ? 0.0f : next;
+        const float shrink = __builtin_amdgcn_exp2f(m - shift);
+        m = next;
+        sum *= shrink;
+#pragma unroll
+        for (int i = 0; i < TOK / 4; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(p[i] - shift);
+            sum += p[i];
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) o[i] *= shrink;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float x = p[8 * s + 2 * w], y = p[8 * s + 2 * w + 1];
+                hi[w] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);      // both cut off
+                // what is left of them is positive: an infinite value keeps its sign in both products (2^-100 is lost in any weight that counts)
+                lo[w] = rb_pair(fmaxf(x - bf16_lo(hi[w]), 0x1p-100f), fmaxf(y - bf16_hi(hi[w]), 0x1p-100f));
+            }
+            const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, make_uint4(hi[0], hi[1], hi[2], hi[3])), pl = __builtin_bit_cast(bf16x8_t, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                bf16x8_t v;
+                if constexpr (WIDE) v = widen(vx[i][0][2 * s], vx[i][0][2 * s + 1]);
+                else if constexpr (F8) v = widen(vx[i][s][0], vx[i][s][1]);
+                else v = __builtin_bit_cast(bf16x8_t, make_uint4(vx[i][s][0], vx[i][s][1], vx[i][s][2], vx[i][s][3]));
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ph, o[i], 0, 0, 0);
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pl, o[i], 0, 0, 0);
+            }
+        }
+    }
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+
+    // the waves' sums together: [wave][head][dim], heads a bank apart
+    __shared__ float part[kWaves][kHeadTile][D + 1];
+    __shared__ float tops[kWaves][kHeadTile], sums[kWaves][kHeadTile];
+    if (g == 0) {
+        tops[wave][n] = m;
+        sums[wave][n] = sum;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) part[wave][n][16 * i + 4 * g + j] = o[i][j];
+    __syncthreads();
+    for (int e = threadIdx.x; e < heads * D; e += 64 * kWaves) {
+        const int head = e / D, d = e - head * D;
+        float top = tops[0][head];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, tops[w][head]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float num = 0.0f, den = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(tops[w][head] - base);
+            num = fmaf(part[w][head][d], f, num);
+            den = fmaf(sums[w][head], f, den);
+        }
+        if (a.splits == 1) {
+            // (no token: zero)
+            const float v = lie ? __builtin_nanf("") : length == 0 ? 0.0f : num / den * a.value_scale;
+            static_cast<uint16_t*>(a.out)[((size_t)seq * a.q_heads + kv * a.group + tile * kHeadTile + head) * D + d] = (uint16_t)bf16_bits(v);
+        } else {
+            float* to = a.partial + (((size_t)seq * a.q_heads + kv * a.group + tile * kHeadTile + head) * a.splits + split) * (D + 2);
+            to[d] = num;
+            if (d == 0) {
+                to[D] = top;
+                to[D + 1] = den;
+            }
+        }
+    }
+}
+
+// The splits' sums of one head together.
+template <int DT>
+__global__ __launch_bounds__(256) void attend_join_kernel(const AttendArgs a)
+{
+    constexpr int D = 32 * DT, G = 256 / D > 0 ? 256 / D : 1;      // splits at a time
+    const int row = blockIdx.x, seq = row / a.q_heads;
+    const int capacity = a.width << a.page_shift, said = a.lengths[seq], length = said < 0 ? 0 : said > capacity ? capacity : said;
+    const int splits = max(1, (length + a.chunk - 1) / a.chunk);
+    const float* from = a.partial + (size_t)row * a.splits * (D + 2);
+    float top = -INFINITY;
+    for (int s = threadIdx.x & 63; s < splits; s += 64) top = fmaxf(top, from[(size_t)s * (D + 2) + D]);
+    top = wave_max(top);
+    const float base = top == -INFINITY ? 0.0f : top;
+    const int d = threadIdx.x % D, k = threadIdx.x / D;
+    float num = 0.0f, den = 0.0f;
+    if (k < G)
+        for (int s = k; s < splits; s += G) {
+            const float* part = from + (size_t)s * (D + 2);
+            const float f = __builtin_amdgcn_exp2f(part[D] - base);
+            num = fmaf(part[d], f, num);
+            den = fmaf(part[D + 1], f, den);
+        }
+    __shared__ float nums[G][D], dens[G];
+    if (k < G) {
+        nums[k][d] = num;
+        if (d == 0) dens[k] = den;
+    }
+    __syncthreads();
+    if (k != 0) return;
+#pragma unroll
+    for (int i = 1; i < G; ++i) {
+        num += nums[i][d];
+        den += dens[i];
+    }
+    const float v = said != length ? __builtin_nanf("") : length == 0 ? 0.0f : num / den * a.value_scale;
+    static_cast<uint16_t*>(a.out)[(size_t)row * D + d] = (uint16_t)bf16_bits(v);
+}
+
+// Tokens of a split.  One sequence of few tokens is left whole (no second launch); else as many splits as give every compute unit two workgroups, of 256 tokens at least
+// (one block for each wave), so that long sequences of a ragged batch have many workgroups and short ones few.
+static int64_t split_tokens(int64_t pairs, int64_t capacity)
+{
+    const int64_t block = 64 * kWaves, want = 2 * (int64_t)device_cus();
+    int64_t splits = (want + pairs - 1) / pairs;
+    int64_t chunk = (capacity + splits - 1) / splits;
+    if (chunk > 1024) chunk = 1024;                                // a ragged batch: at most 1024 tokens of one sequence in a workgroup
+    chunk = (chunk + block - 1) / block * block;
+    return capacity <= 2 * block ? 2 * block : chunk;
+}
+
+size_t paged_attention_workspace_bytes(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t capacity)
+{
+    if (seqs <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || dim <= 0 || capacity <= 0 || capacity > INT32_MAX || seqs > INT32_MAX || q_heads > 65536) return 16;
+    const int64_t tiles = (q_heads / kv_heads + kHeadTile - 1) / kHeadTile, chunk = split_tokens(seqs * kv_heads * tiles, capacity), splits = (capacity + chunk - 1) / chunk;
+    return splits <= 1 ? 16 : (size_t)seqs * (size_t)q_heads * (size_t)splits * (size_t)(dim + 2) * 4;
+}
+
+int paged_attention(const void* q, int64_t q_seq, int64_t q_head, int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, const void* keys, const void* values, int64_t pages,
+                    int64_t page, int cache_dtype, const int* tables, int64_t table_stride, int64_t width, const int* lengths, float scale, float key_scale, float value_scale,
+                    void* out, void* workspace, size_t workspace_bytes, hipStream_t st)
+{
+    const bool f8 = cache_dtype == METIS_DTYPE_E4M3;
+    if (seqs < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads > 65536 || q_heads % kv_heads || pages < 0 || pages > INT32_MAX || width < 0 || q_seq < 0 || q_head < 0 || table_stride < 0 ||
+        (cache_dtype != METIS_DTYPE_BF16 && !f8))
+        return METIS_E_ARG;
+    if (dim <= 0 || dim > 256 || dim % (f8 ? 64 : 32) || page < 16 || page > 4096 || (page & (page - 1))) return METIS_E_ARG;
+    if (seqs == 0) return METIS_OK;
+    if (!out || (uintptr_t)out % 2 || !lengths || (uintptr_t)lengths % 4 || (width > 0 && (!tables || (uintptr_t)tables % 4)) || !q || (uintptr_t)q % 16 || q_seq % 8 || q_head % 8)
+        return METIS_E_ARG;
+    if (pages > 0 ? (!keys || !values || ((uintptr_t)keys | (uintptr_t)values) % 16) : width > 0) return METIS_E_ARG;
+    if (width > INT32_MAX / page || seqs > ((int64_t)1 << 46) / q_heads / dim) return METIS_E_ARG;
+    const int64_t capacity = width * page, tiles = (q_heads / kv_heads + kHeadTile - 1) / kHeadTile, pairs = seqs * kv_heads * tiles;
+    const int64_t chunk = split_tokens(pairs, capacity > 0 ? capacity : 1), splits = capacity > 0 ? (capacity + chunk - 1) / chunk : 1;
+    if (pairs > INT32_MAX / splits || seqs * q_heads > INT32_MAX) return METIS_E_TOO_LARGE;
+    if (splits > 1 && (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < (size_t)seqs * (size_t)q_heads * (size_t)splits * (size_t)(dim + 2) * 4)) return METIS_E_WORKSPACE;
+    AttendArgs a = {};
+    a.q = q; a.keys = keys; a.values = values; a.tables = tables; a.lengths = lengths; a.out = out; a.partial = static_cast<float*>(workspace);
+    a.q_seq = q_seq; a.q_head = q_head; a.table_stride = table_stride;
+    a.q_heads = (int)q_heads; a.kv_heads = (int)kv_heads; a.group = (int)(q_heads / kv_heads); a.pages = (int)pages; a.page_shift = __builtin_ctzll((unsigned long long)page);
+    a.width = (int)width; a.splits = (int)splits; a.chunk = (int)chunk; a.tiles = (int)tiles;
+    a.scale = (float)((double)scale * (double)key_scale * 1.4426950408889634);
+    a.value_scale = value_scale;
+    const dim3 grid((unsigned)(pairs * splits)), block(64 * kWaves), rows((unsigned)(seqs * q_heads));
+#define METIS_ATT(DT, F, TOK) hipLaunchKernelGGL((attend_kernel<DT, F, TOK>), grid, block, 0, st, a)
+    if (f8) {
+        switch (dim / 32) {
+            case 2: METIS_ATT(2, true, 64); break;
+            case 4: METIS_ATT(4, true, 64); break;
+            case 6: METIS_ATT(6, true, 32); break;
+            default: METIS_ATT(8, true, 32);
+        }
+    } else {
+        switch (dim / 32) {
+            case 1: METIS_ATT(1, false, 64); break;
+            case 2: METIS_ATT(2, false, 64); break;
+            case 3: METIS_ATT(3, false, 64); break;
+            case 4: METIS_ATT(4, false, 64); break;
+            case 5: METIS_ATT(5, false, 32); break;
+            case 6: METIS_ATT(6, false, 32); break;
+            case 7: METIS_ATT(7, false, 32); break;
+            default: METIS_ATT(8, false, 32);
+        }
+    }
+#undef METIS_ATT
+    if (splits > 1) {
+        switch (dim / 32) {
+#define METIS_JOIN(DT) case DT: hipLaunchKernelGGL((attend_join_kernel<DT>), rows, dim3(256), 0, st, a); break
+            METIS_JOIN(1); METIS_JOIN(2); METIS_JOIN(3); METIS_JOIN(4); METIS_JOIN(5); METIS_JOIN(6); METIS_JOIN(7); METIS_JOIN(8);
+#undef METIS_JOIN
+        }
+    }
+    return hipGetLastError() == hipSuccess ? METIS_OK : METIS_E_LAUNCH;
+}
+
+// ---------------------------------------------------------------------------------------------- copies of pages
+// The pairs travel with the launch: nothing has to be brought to the device first.
+constexpr int kCopyPairs = 240;
+struct CopyArgs {
+    char *keys, *values;
+    uint64_t page_bytes, layer_bytes;
+    int layers, pieces, count;
+    int from[kCopyPairs], to[kCopyPairs];
+};
+constexpr int kCopyPiece = 16384;                                  // bytes of a workgroup, 64 a lane
+
+__global__ __launch_bounds__(256) void copy_pages_kernel(const CopyArgs a)
+{
+    uint32_t b = blockIdx.x;
+    const uint32_t piece = b % a.pieces;
+    b /= a.pieces;
+    const uint32_t layer = b % a.layers;
+    b /= a.layers;
+    const uint32_t which = b & 1, pair = b >> 1;
+    char* base = (which ? a.values : a.keys) + (size_t)layer * a.layer_bytes;
+    const char* from = base + (size_t)a.from[pair] * a.page_bytes;
+    char* to = base + (size_t)a.to[pair] * a.page_bytes;
+    const uint64_t at = (uint64_t)piece * kCopyPiece + threadIdx.x * 16;
+    if ((uint64_t)(piece + 1) * kCopyPiece <= a.page_bytes) {
+        uint4 w[kCopyPiece / 4096];
+#pragma unroll
+        for (int i = 0; i < kCopyPiece / 4096; ++i) w[i] = *reinterpret_cast<const uint4*>(from + at + 4096 * i);
+#pragma unroll
+        for (int i = 0; i < kCopyPiece / 4096; ++i) *reinterpret_cast<uint4*>(to + at + 4096 * i) = w[i];
+    } else {
+        for (int i = 0; i < kCopyPiece / 4096; ++i)
+            if (at + 4096 * i < a.page_bytes) *reinterpret_cast<uint4*>(to + at + 4096 * i) = *reinterpret_cast<const uint4*>(from + at + 4096 * i);
+    }
+}
+
+int copy_pages(void* keys, void* values, int64_t layers, int64_t pages, int64_t page_bytes, const int64_t* from, const int64_t* to, int64_t count, hipStream_t st)
+{
+    if (layers < 0 || pages < 0 || pages > INT32_MAX || page_bytes <= 0 || page_bytes % 16 || page_bytes > ((int64_t)1 << 31) || count < 0 || count > pages) return METIS_E_ARG;
+    if (count == 0 || layers == 0) return METIS_OK;
+    if (!keys || !values || ((uintptr_t)keys | (uintptr_t)values) % 16 || !from || !to) return METIS_E_ARG;
+    for (int64_t i = 0; i < count; ++i)
+        if (from[i] < 0 || from[i] >= pages || to[i] < 0 || to[i] >= pages) return METIS_E_ARG;
+    // copies of one launch run side by side: no page is written twice, and none that is written is read
+    unsigned char* written = static_cast<unsigned char*>(calloc((size_t)(pages + 7) / 8, 1));
+    if (!written) return METIS_E_TOO_LARGE;
+    bool apart = true;
+    for (int64_t i = 0; i < count && apart; ++i) {
+        apart = !(written[to[i] >> 3] >> (to[i] & 7) & 1);
+        written[to[i] >> 3] |= (unsigned char)(1u << (to[i] & 7));
+    }
+    for (int64_t i = 0; i < count && apart; ++i) apart = !(written[from[i] >> 3] >> (from[i] & 7) & 1);
+    free(written);
+    if (!apart) return METIS_E_ARG;
+    CopyArgs a = {};
+    a.keys = static_cast<char*>(keys); a.values = static_cast<char*>(values);
+    a.page_bytes = (uint64_t)page_bytes; a.layer_bytes = (uint64_t)page_bytes * (uint64_t)pages;
+    a.pieces = (int)((page_bytes + kCopyPiece - 1) / kCopyPiece);
+    const int64_t one = 2 * layers * a.pieces;
+    if (layers > INT32_MAX / 2 / a.pieces || one > INT32_MAX / kCopyPairs) return METIS_E_TOO_LARGE;
+    a.layers = (int)layers;
+    for (int64_t done = 0; done < count; done += kCopyPairs) {
+        a.count = (int)(count - done < kCopyPairs ? count - done : kCopyPairs);
+        for (int i = 0; i < a.count; ++i) {
+            a.from[i] = (int)from[done + i];
+            a.to[i] = (int)to[done + i];
+        }
+        hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(one * a.count)), dim3(256), 0, st, a);
+        if (hipGetLastError() != hipSuccess) return METIS_E_LAUNCH;
+    }
+    return METIS_OK;
+}
+
+}  // namespace metis

@@ -22,7 +22,7 @@ class LinearMember(ctypes.Structure):
 
 MODE_P32, MODE_PB16 = 0, 1
 MODE_P32_F32 = 2      # quantizer entry points only: binary32 arithmetic on a binary32 tensor
-DTYPE_BF16, DTYPE_F32 = 0, 1
+DTYPE_BF16, DTYPE_F32, DTYPE_F64, DTYPE_E4M3 = 0, 1, 2, 3
 
 _vp, _i64, _i32, _u64, _f32, _sz = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_uint64,
                                     ctypes.c_float, ctypes.c_size_t)
@@ -136,6 +136,13 @@ SIGNATURES = {
     "metis_head_logprobs": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "metis_head_logprobs_backward_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
     "metis_head_logprobs_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "metis_rotary": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _i32, _i64, _i64, _i64, _i32, _i32, _f32, _i32, _vp, _vp, _vp]),
+    "metis_rotary_append": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i32, _f32, _i64, _i64, _i32, _f32,
+                                   _f32, _vp, _vp, _vp, _vp]),
+    "metis_paged_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "metis_paged_attention": (_i32, [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _f32, _f32, _f32, _vp, _vp, _sz, _vp]),
+    "metis_cache_copy_pages": (_i32, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "metis_sample_tokens": (_i32, [_vp, _i64, _i32, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
 }
 
 _lib = None
@@ -166,7 +173,7 @@ def load():
 
 
 HOST_PATH = os.path.join(_HERE, "_metis_host.so")
-U8, B16, F32 = 0, 1, 2          # types of call()'s new tensors
+U8, B16, F32, I64 = 0, 1, 2, 3  # types of call()'s new tensors
 
 
 def call(name: str, device_index: int, specs: tuple, args: tuple):

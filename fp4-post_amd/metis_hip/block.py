@@ -1,12 +1,13 @@
-"""What a decoder layer runs between its packed projections: the residual sum with its norms, and the product of gate and up.
+"""What a decoder layer runs between its packed projections: the residual sum with its norms, the product of gate and up, and the turn of queries and keys.
 
 The reference leaves both to the model: `residual + hidden` and the RMSNorm of src/Metis/models/llama.py:23-31, and
-`act_fn(gate_proj(x)) * up_proj(x)` of its MLP.  Here each is one kernel, forward and backward, in binary32 arithmetic with every
+`act_fn(gate_proj(x)) * up_proj(x)` of its MLP, and the rotary embedding between its q / k projections and attention.  Here each is one kernel, forward and backward, in binary32 arithmetic with every
 result rounded once; their autograd nodes are compiled (csrc/host_autograd.cpp).
 """
 from __future__ import annotations
 
 import inspect
+import math
 
 import torch
 from torch import nn
@@ -52,6 +53,22 @@ class _SwiGLU(torch.autograd.Function):
         return ops.swiglu_backward(*ctx.saved_tensors, grad)
 
 
+class _Rotary(torch.autograd.Function):
+    """rotary where a tracer or a transform sees the call, as _ResidualNorm."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, interleaved, factor):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.more = interleaved, factor
+        return ops.rotary(q, k, positions, inv_freq, interleaved, factor)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_q, grad_k):
+        positions, inv_freq = ctx.saved_tensors
+        return (*ops.rotary(grad_q, grad_k, positions, inv_freq, *ctx.more, True), None, None, None, None)
+
+
 def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, *, post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None,
                   residual_scale: float = 1.0, eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
     """The residual stream behind a block and the input of the next one, from one pass:
@@ -84,6 +101,81 @@ def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
         ops._check_swiglu(gate, up)
         return _lib.host().recorded_swiglu(gate, up)
     return ops.swiglu(gate, up)
+
+
+def rotary_frequencies(turned: int, base: float = 10000.0, scaling: dict | None = None, *, device=None) -> tuple[torch.Tensor, float]:
+    """(inv_freq, factor) for rotary: the frequencies base^(-2 i / turned), float64 [turned / 2], and what multiplies the turned vectors (1.0, but for
+    "yarn").  `scaling` stretches them for contexts beyond the trained length, by its "type" (or "rope_type", as model settings have it):
+
+        "linear"  every frequency divided by "factor"
+        "llama3"  frequencies of wavelengths beyond original / low_freq_factor divided by "factor", those below original / high_freq_factor left, between
+                  them a mixture, linear in original / wavelength; original = "original_max_position_embeddings"
+        "yarn"    the pairs that turn more than "beta_fast" (32) times within the original length left, those that turn less than "beta_slow" (1) times
+                  divided by "factor", between them a mixture, linear in the pair's number; the factor of the vectors is "attention_factor", or
+                  0.1 log(factor) + 1"""
+    if turned <= 0 or turned % 2 or not base > 0.0:
+        raise ValueError(f"rotary_frequencies: a positive even number of columns and a positive base, not {turned} and {base}")
+    freq = [float(base) ** (-2 * i / turned) for i in range(turned // 2)]
+    factor = 1.0
+    kind = None if scaling is None else scaling.get("rope_type", scaling.get("type"))
+    if kind not in (None, "default"):
+        if kind not in ("linear", "llama3", "yarn"):
+            raise ValueError(f"rotary_frequencies: scaling is 'linear', 'llama3' or 'yarn', not {kind!r}")
+        need = {"linear": ("factor",), "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"),
+                "yarn": ("factor", "original_max_position_embeddings")}[kind]
+        missing = [name for name in need if scaling.get(name) is None]
+        if missing:
+            raise ValueError(f"rotary_frequencies: {kind!r} needs {', '.join(missing)}")
+        stretch = float(scaling["factor"])
+        if not stretch >= 1.0:
+            raise ValueError(f"rotary_frequencies: a factor of at least 1, not {stretch}")
+        if kind == "linear":
+            keep = [0.0] * len(freq)
+        elif kind == "llama3":
+            low, high, original = (float(scaling[name]) for name in need[1:])
+            if not high > low:
+                raise ValueError(f"rotary_frequencies: high_freq_factor above low_freq_factor, not {high} and {low}")
+            keep = [min(max((original * f / (2 * math.pi) - low) / (high - low), 0.0), 1.0) for f in freq]
+        else:
+            original = float(scaling["original_max_position_embeddings"])
+            fast, slow = float(scaling.get("beta_fast") or 32.0), float(scaling.get("beta_slow") or 1.0)
+
+            def pair(turns):                                       # the pair that turns so often within the original length
+                return turned * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+            first, last = pair(fast), pair(slow)
+            if scaling.get("truncate", True):
+                first, last = math.floor(first), math.ceil(last)
+            first, last = max(first, 0), min(last, turned - 1)
+            last = last + 0.001 if first == last else last
+            keep = [1.0 - min(max((i - first) / (last - first), 0.0), 1.0) for i in range(len(freq))]
+            given = scaling.get("attention_factor")
+            if given is None and (scaling.get("mscale") or scaling.get("mscale_all_dim")):
+                raise ValueError("rotary_frequencies: settings with mscale say what they mean by it: attention_factor")
+            factor = float(given) if given is not None else (0.1 * math.log(stretch) + 1.0 if stretch > 1.0 else 1.0)
+        freq = [f * w + f / stretch * (1.0 - w) for f, w in zip(freq, keep)]
+    return torch.tensor(freq, dtype=torch.float64, device=device), factor
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False, factor: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Queries and keys turned by the angles of their positions:
+
+        (y1, y2) = factor * (x1 cos a - x2 sin a, x2 cos a + x1 sin a),     a = position * inv_freq[i]
+
+    q, k       [..., heads, dim] of one type, bf16 or float32, alike but for their heads (parts of one product's rows are taken as they are); dim even, up to 512
+    positions  int64, of the leading sizes of q ([B, S] for [B, S, heads, dim]) or of the last of them ([S], [1, S])
+    inv_freq   float32 or float64 [n], n at most dim / 2: the first 2 n columns of each head are turned, the pairs (i, i + n) or, interleaved, (2 i, 2 i + 1);
+               the columns behind them are copied.  rotary_frequencies gives it, with `factor`; a model's own buffer is taken too
+
+    The angles are formed in 64 bits.  The results are dense.  Differentiable (once, in reverse) in q and k."""
+    factor = float(factor)
+    if inv_freq.requires_grad:
+        raise ValueError("rotary: no gradient of inv_freq")
+    if _transformed():
+        return _Rotary.apply(q, k, positions, inv_freq, bool(interleaved), factor)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        ops._check_rotary("rotary", q, k, positions, inv_freq)
+        return _lib.host().recorded_rotary(q, k, ops._flat_positions("rotary", positions, q.shape[:-2]), inv_freq, interleaved, factor)
+    return ops.rotary(q, k, positions, inv_freq, interleaved, factor)
 
 
 class GatedMLP(nn.Module):

@@ -13,7 +13,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import B16, DTYPE_BF16, DTYPE_F32, F32, MODE_P32, MODE_PB16, U8, check, load
+from ._lib import B16, DTYPE_BF16, DTYPE_E4M3, DTYPE_F32, DTYPE_F64, F32, I64, MODE_P32, MODE_PB16, U8, check, load
 
 BLOCK = 16
 _workspaces: dict = {}
@@ -1555,6 +1555,220 @@ def head_logprobs_backward(hidden: torch.Tensor, weight: torch.Tensor, targets: 
     if new.__class__ is int:
         check(new, "metis_head_logprobs_backward", hidden.shape)
     return tuple(None if k is None else new[int(k)] for k in place)
+
+
+def _head_rows(t: torch.Tensor, tokens: int) -> tuple[torch.Tensor, int, int]:
+    """[..., heads, dim] as [tokens, heads, dim] with dense dimensions, and the strides of its tokens and heads (of a single one: none that counts)."""
+    heads, dim = t.shape[-2:]
+    if t.is_contiguous():
+        return t, heads * dim, dim
+    t = t.reshape(tokens, heads, dim)
+    if t.stride(2) != 1:
+        t = t.contiguous()
+    return t, t.stride(0) if tokens > 1 else heads * dim, t.stride(1) if heads > 1 else dim
+
+
+_FREQUENCIES = {torch.float32: DTYPE_F32, torch.float64: DTYPE_F64}
+
+
+def _check_rotary(what: str, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor) -> None:
+    _same_device(what, q, k, positions, inv_freq)
+    if q.dim() < 3 or k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1] or k.dtype != q.dtype or q.dtype not in _FLOATS:
+        raise ValueError(f"{what}: q and k are [..., heads, dim] of one type, bf16 or float32, alike but for their heads: {tuple(q.shape)} of {q.dtype}, {tuple(k.shape)} of {k.dtype}")
+    dim = q.shape[-1]
+    if dim % 2 or not 0 < dim <= 512 or not 0 < q.shape[-2] <= 65536 or not 0 < k.shape[-2] <= 65536:
+        raise ValueError(f"{what}: an even dim up to 512 and 1 to 65536 heads, not {dim}, {q.shape[-2]} and {k.shape[-2]}")
+    if inv_freq.dim() != 1 or inv_freq.dtype not in _FREQUENCIES or not 0 < 2 * inv_freq.shape[0] <= dim or not inv_freq.is_contiguous():
+        raise ValueError(f"{what}: inv_freq is a dense vector of float32 or float64, a frequency for each pair of the columns that are turned (at most {dim // 2}), not "
+                         f"{tuple(inv_freq.shape)} of {inv_freq.dtype}")
+    if positions.dtype != torch.int64:
+        raise ValueError(f"{what}: positions are int64, not {positions.dtype}")
+
+
+def _flat_positions(what: str, positions: torch.Tensor, lead: torch.Size) -> torch.Tensor:
+    """positions as a dense vector that goes through the tokens, once or over and over: of the shape `lead`, or of its last sizes (behind ones)."""
+    own = list(positions.shape)
+    while own and own[0] == 1:
+        own.pop(0)
+    if own != list(lead[len(lead) - len(own):]):
+        raise ValueError(f"{what}: positions have the tokens' sizes {tuple(lead)}, or the last of them, not {tuple(positions.shape)}")
+    return positions.reshape(-1).contiguous()
+
+
+@_on_own_device
+def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False, factor: float = 1.0,
+           back: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """(q, k) turned by position * inv_freq (back: by its negative), both dense; bf16 or float32, angles in 64 bits, each result rounded once."""
+    _check_rotary("rotary", q, k, positions, inv_freq)
+    lead, dim = q.shape[:-2], q.shape[-1]
+    pos = _flat_positions("rotary", positions, lead)
+    if q.numel() == 0:
+        return torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(k, memory_format=torch.contiguous_format)
+    tokens, (dt, spec) = q.numel() // (q.shape[-2] * dim), _FLOATS[q.dtype]
+    (a, at, ah), (b, bt, bh) = _head_rows(q, tokens), _head_rows(k, tokens)
+    new = _lib.call("metis_rotary", q.get_device(), ((spec, *q.shape), (spec, *k.shape)),
+                    (a, at, ah, q.shape[-2], b, bt, bh, k.shape[-2], pos, pos.numel(), inv_freq, _FREQUENCIES[inv_freq.dtype], tokens, dim, 2 * inv_freq.shape[0], bool(interleaved),
+                     bool(back), factor, dt, "0", "1", _stream()))
+    if new.__class__ is int:
+        check(new, "metis_rotary", q.shape)
+    return new
+
+
+_CACHES = {torch.bfloat16: DTYPE_BF16, torch.float8_e4m3fn: DTYPE_E4M3}
+
+
+def _check_cache(what: str, keys: torch.Tensor, values: torch.Tensor, layers: bool = False) -> None:
+    lead = 1 if layers else 0
+    if keys.dtype not in _CACHES or values.dtype != keys.dtype or keys.dim() != 4 + lead or values.dim() != 4 + lead or not keys.is_contiguous() or not values.is_contiguous():
+        raise ValueError(f"{what}: keys and values are the dense {'layers, ' if layers else ''}pages, heads, page, dim and .. dim, page of a cache, bf16 or float8_e4m3fn: "
+                         f"{tuple(keys.shape)} of {keys.dtype}, {tuple(values.shape)} of {values.dtype}")
+    if keys.shape[:-2] != values.shape[:-2] or keys.shape[-2] != values.shape[-1] or keys.shape[-1] != values.shape[-2]:
+        raise ValueError(f"{what}: values have their dimensions in front of their tokens, [.., dim, page] beside keys of [.., page, dim]: {tuple(keys.shape)}, {tuple(values.shape)}")
+
+
+def _check_scales(what: str, key_scale: float, value_scale: float) -> None:
+    if not 0.0 < key_scale < float("inf") or not 0.0 < value_scale < float("inf"):
+        raise ValueError(f"{what}: positive scales of keys and values, not {key_scale} and {value_scale}")
+
+
+@_on_own_device
+def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, slots: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
+                  interleaved: bool = False, factor: float = 1.0, key_scale: float = 1.0, value_scale: float = 1.0) -> torch.Tensor:
+    """q [tokens, heads, dim] turned; k, turned, and v written to their places in keys and values."""
+    _check_rotary("rotary_append", q, k, positions, inv_freq)
+    _same_device("rotary_append", q, v, slots, keys, values)
+    _check_cache("rotary_append", keys, values)
+    tokens, heads, dim = q.shape if q.dim() == 3 else (-1, -1, -1)
+    if tokens < 0 or q.dtype != torch.bfloat16 or v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError(f"rotary_append: q, k and v are [tokens, heads, dim] of bf16, k and v alike, not {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)} of {q.dtype} and {v.dtype}")
+    pages, kv, page = keys.shape[:3]
+    if kv != k.shape[1] or keys.shape[3] != dim:
+        raise ValueError(f"rotary_append: a cache of {k.shape[1]} heads of {dim}, not {kv} of {keys.shape[3]}")
+    for name, t in (("positions", positions), ("slots", slots)):
+        if t.shape != (tokens,) or t.dtype != torch.int64:
+            raise ValueError(f"rotary_append: {name} are int64 [{tokens}], not {t.dtype} {tuple(t.shape)}")
+    _check_scales("rotary_append", key_scale, value_scale)
+    if tokens == 0:
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    if pages == 0 or not 0 < page <= 4096:
+        raise ValueError(f"rotary_append: a cache with pages of 1 to 4096 tokens, not {tuple(keys.shape)}")
+    (a, at, ah), (b, bt, bh), (c, ct, ch) = _head_rows(q, tokens), _head_rows(k, tokens), _head_rows(v, tokens)
+    new = _lib.call("metis_rotary_append", q.get_device(), ((B16, tokens, heads, dim),),
+                    (a, at, ah, heads, b, bt, bh, kv, c, ct, ch, positions.contiguous(), inv_freq, _FREQUENCIES[inv_freq.dtype], slots.contiguous(), tokens, dim, 2 * inv_freq.shape[0],
+                     bool(interleaved), factor, pages, page, _CACHES[keys.dtype], key_scale, value_scale, keys, values, "0", _stream()))
+    if new.__class__ is int:
+        check(new, "metis_rotary_append", q.shape)
+    return new[0]
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_attention_bytes(seqs: int, heads: int, kv: int, dim: int, capacity: int, device_index: int) -> int:
+    return int(load().metis_paged_attention_workspace_bytes(seqs, heads, kv, dim, capacity))      # depends on the device's CU count only
+
+
+@_on_own_device
+def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, scale: float | None = None, key_scale: float = 1.0,
+                    value_scale: float = 1.0) -> torch.Tensor:
+    """softmax(scale q K^T) V of one token of each sequence over its pages; q bf16 [seqs, heads, dim], the result dense."""
+    _same_device("paged_attention", q, keys, values, tables, lengths)
+    _check_cache("paged_attention", keys, values)
+    if q.dim() != 3 or q.dtype != torch.bfloat16:
+        raise ValueError(f"paged_attention: q is [seqs, heads, dim] of bf16, not {tuple(q.shape)} of {q.dtype}")
+    (seqs, heads, dim), (pages, kv, page, kdim) = q.shape, keys.shape
+    whole = 64 if keys.dtype == torch.float8_e4m3fn else 32
+    if kdim != dim or kv == 0 or heads == 0 or heads > 65536 or heads % kv or dim % whole or not 0 < dim <= 256:
+        raise ValueError(f"paged_attention: heads that share those of the cache evenly, of dim a multiple of {whole} up to 256: {heads} of {dim} over {kv} of {kdim}")
+    if page < 16 or page > 4096 or page & (page - 1):
+        raise ValueError(f"paged_attention: pages of a power of two from 16 to 4096 tokens, not {page}")
+    if tables.dim() != 2 or tables.shape[0] != seqs or tables.dtype != torch.int32 or lengths.shape != (seqs,) or lengths.dtype != torch.int32:
+        raise ValueError(f"paged_attention: tables int32 [{seqs}, pages] and lengths int32 [{seqs}], not {tables.dtype} {tuple(tables.shape)} and {lengths.dtype} {tuple(lengths.shape)}")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not abs(scale) < float("inf"):
+        raise ValueError(f"paged_attention: a finite scale, not {scale}")
+    _check_scales("paged_attention", key_scale, value_scale)
+    if seqs == 0:
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    width = tables.shape[1]
+    if width > 0 and pages == 0 or width * page >= 1 << 31:
+        raise ValueError(f"paged_attention: tables of a cache with pages, of less than 2^31 tokens a sequence, not {tuple(tables.shape)} of pages of {page}")
+    if width > 1 and tables.stride(1) != 1:
+        tables = tables.contiguous()
+    if q.stride(2) != 1 or (heads > 1 and q.stride(1) % 8) or (seqs > 1 and q.stride(0) % 8) or q.data_ptr() % 16:
+        q = _flat(q.contiguous())
+    need = _paged_attention_bytes(seqs, heads, kv, dim, width * page, q.get_device())
+    new = _lib.call("metis_paged_attention", q.get_device(), ((B16, seqs, heads, dim), (U8, need)) if need > 16 else ((B16, seqs, heads, dim),),
+                    (q, q.stride(0) if seqs > 1 else heads * dim, q.stride(1) if heads > 1 else dim, seqs, heads, kv, dim, keys, values, pages, page, _CACHES[keys.dtype], tables,
+                     tables.stride(0), width, lengths.contiguous(), scale, key_scale, value_scale, "0", "1" if need > 16 else None, need, _stream()))
+    if new.__class__ is int:
+        check(new, "metis_paged_attention", q.shape)
+    return new[0]
+
+
+@_on_own_device
+def copy_pages(keys: torch.Tensor, values: torch.Tensor, sources, destinations) -> None:
+    """Pages of all layers of a cache (keys [layers, pages, heads, page, dim], values alike) to other places; sources and destinations are numbers on the host."""
+    _same_device("copy_pages", keys, values)
+    _check_cache("copy_pages", keys, values, layers=True)
+    pairs = torch.tensor([list(sources), list(destinations)] if len(sources) == len(destinations) else [], dtype=torch.int64)
+    if pairs.dim() != 2:
+        raise ValueError(f"copy_pages: a destination for each source, not {len(destinations)} for {len(sources)}")
+    layers, pages = keys.shape[:2]
+    count = pairs.shape[1]
+    if count == 0 or layers == 0:
+        return
+    size = keys.shape[2] * keys.shape[3] * keys.shape[4] * keys.element_size()
+    if size == 0 or size % 16 or size > 1 << 31:
+        raise ValueError(f"copy_pages: pages of a multiple of 16 bytes up to 2^31, not {size}")
+    from_, to = pairs
+    if int(pairs.min()) < 0 or int(pairs.max()) >= pages:
+        raise ValueError(f"copy_pages: pages 0 to {pages - 1}")
+    written = set(destinations)
+    if len(written) < count or not written.isdisjoint(sources):
+        raise ValueError("copy_pages: no page is written twice, and none that is written is read")
+    rc = _lib.call("metis_cache_copy_pages", keys.get_device(), (), (keys, values, layers, pages, size, from_, to, count, _stream()))
+    if rc.__class__ is int:
+        check(rc, "metis_cache_copy_pages", keys.shape)
+
+
+@functools.lru_cache(maxsize=4096)
+def _sample_parameters(*settings: float) -> ctypes.Array:
+    return (ctypes.c_double * 4)(*settings)
+
+
+@_on_own_device
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """(token int64, log-probability float32) of every row of logits [..., V]; the settings numbers, or tensors with one for each row."""
+    _same_device("sample_tokens", logits, uniforms)
+    if logits.dim() < 1 or logits.dtype not in _FLOATS or not 0 < logits.shape[-1] <= 1 << 22:
+        raise ValueError(f"sample_tokens: logits are [..., V] of bf16 or float32, V from 1 to 2^22, not {tuple(logits.shape)} of {logits.dtype}")
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    if uniforms.shape != lead or uniforms.dtype != torch.float32:
+        raise ValueError(f"sample_tokens: uniforms are float32 {tuple(lead)}, not {uniforms.dtype} {tuple(uniforms.shape)}")
+    settings = (temperature, top_k, top_p, min_p)
+    each = any(isinstance(s, torch.Tensor) for s in settings)
+    for name, s, ok in zip(("temperature", "top_k", "top_p", "min_p"), settings, (lambda s: 0.0 < s < float("inf"), lambda s: s >= 0, lambda s: s > 0.0, lambda s: 0.0 <= s <= 1.0)):
+        if isinstance(s, torch.Tensor):
+            if s.shape != lead or s.device != logits.device or s.is_complex():
+                raise ValueError(f"sample_tokens: {name} is a number, or a tensor {tuple(lead)} on the logits' device, not {tuple(s.shape)} on {s.device}")
+        elif not ok(s):
+            raise ValueError(f"sample_tokens: temperature is positive, top_k at least 0 (all), top_p positive, min_p from 0 to 1: not {name} = {s}")
+    rows = uniforms.numel()
+    if rows == 0:
+        return torch.empty(lead, dtype=torch.int64, device=logits.device), torch.empty(lead, dtype=torch.float32, device=logits.device)
+    dt, _ = _FLOATS[logits.dtype]
+    x = logits.reshape(rows, V)
+    if (V > 1 and x.stride(1) != 1) or (rows > 1 and x.stride(0) < V):
+        x = x.contiguous()
+    if each:
+        own, common = torch.stack([s.to(torch.float64).expand(lead) if isinstance(s, torch.Tensor) else torch.full(lead, float(s), dtype=torch.float64, device=logits.device)
+                                   for s in settings], -1).contiguous(), None
+    else:
+        own, common = None, _sample_parameters(*map(float, settings))
+    new = _lib.call("metis_sample_tokens", logits.get_device(), ((I64, *lead), (F32, *lead)),
+                    (x, x.stride(0) if rows > 1 else V, dt, rows, V, uniforms.contiguous(), common and ctypes.addressof(common), own, "0", "1", _stream()))
+    if new.__class__ is int:
+        check(new, "metis_sample_tokens", logits.shape)
+    return new
 
 
 @functools.lru_cache(maxsize=16)

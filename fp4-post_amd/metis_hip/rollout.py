@@ -1,0 +1,252 @@
+"""What a rollout runs besides the projections: a paged cache of keys and values, attention of new tokens over it, and the draw of the next ones.
+
+The reference's GRPO entry rolls completions out through its library's generate() (src/grpo/grpo.py:671-693, with the merged weights of a rollout), which keeps
+a cache for each completion and sorts the vocabulary for each token.  Here a prompt's pages are shared by the completions that start from it, attention reads
+each cached key and value once, and nothing is sorted.  None of it has gradients: the step that trains on the tokens recomputes them.
+"""
+from __future__ import annotations
+
+from collections.abc import Sequence
+from dataclasses import dataclass
+
+import torch
+from torch import nn
+
+from . import ops
+from .bitlinear import _transformed
+
+
+class _Recorded(torch.autograd.Function):
+    """A call that a tracer records and that transforms and forward-mode differentiation refuse: they need not leave a mark on the tensors."""
+
+    @staticmethod
+    def forward(ctx, fn, *args):
+        out = fn(*args)
+        ctx.mark_non_differentiable(*(out if isinstance(out, tuple) else (out,)))
+        return out
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("metis_hip: a call without gradients")
+
+
+def _no_gradients(what: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise ValueError(f"{what}: no gradients; call it under torch.no_grad()")
+
+
+def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, slots: torch.Tensor, keys: torch.Tensor,
+                  values: torch.Tensor, *, interleaved: bool = False, factor: float = 1.0, key_scale: float = 1.0, value_scale: float = 1.0) -> torch.Tensor:
+    """New tokens' queries and keys turned as by rotary, the turned keys and the values written to the cache in the same launch.  Returns the queries.
+
+    q          bf16 [tokens, heads, dim]; k, v bf16 [tokens, kv_heads, dim] (parts of one product's rows are taken as they are)
+    positions  int64 [tokens]; inv_freq, interleaved and factor as in rotary
+    slots      int64 [tokens]: each token's place, page * page size + offset; a negative one: not cached (padding).  A place that the cache does not have is not
+               written and makes the token's query NaN; no two tokens may have one place
+    keys       [pages, kv_heads, page, dim], values [pages, kv_heads, dim, page] of one layer, bf16 or float8_e4m3fn: there the numbers are value / scale,
+               rounded to nearest, 448 for everything beyond it"""
+    _no_gradients("rotary_append", q, k, v)
+    args = q, k, v, positions, inv_freq, slots, keys, values, bool(interleaved), float(factor), float(key_scale), float(value_scale)
+    return _Recorded.apply(ops.rotary_append, *args) if _transformed() else ops.rotary_append(*args)
+
+
+def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, *, scale: float | None = None,
+                    key_scale: float = 1.0, value_scale: float = 1.0) -> torch.Tensor:
+    """Attention of one new token of each sequence over the tokens that the cache holds of it (its own among them): softmax(scale q K^T) V, bf16 [seqs, heads, dim].
+
+    q        bf16 [seqs, heads, dim]; query head h reads head h // (heads // kv_heads) of the cache; scale defaults to dim^-0.5
+    keys, values   as in rotary_append, turned keys; dim a multiple of 32 up to 256 (float8_e4m3fn: of 64), pages of a power of two from 16 to 4096 tokens
+    tables   int32 [seqs, n]: the pages of each sequence in order; lengths int32 [seqs]: its tokens.  What stands in a table behind them, or in a page, counts
+             for nothing.  A length of 0 gives 0; a negative one, one that the table has no pages for, and a page that the cache does not have give NaN"""
+    _no_gradients("paged_attention", q, keys, values)
+    args = q, keys, values, tables, lengths, scale, float(key_scale), float(value_scale)
+    return _Recorded.apply(ops.paged_attention, *args) if _transformed() else ops.paged_attention(*args)
+
+
+def copy_pages(keys: torch.Tensor, values: torch.Tensor, sources: Sequence[int], destinations: Sequence[int]) -> None:
+    """Copies whole pages, sources[i] to destinations[i], in all layers of a cache: keys [layers, pages, kv_heads, page, dim], values [layers, pages, kv_heads, dim,
+    page].  The numbers are the host's.  No page may be written twice, or written and read."""
+    ops.copy_pages(keys, values, sources, destinations)
+
+
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: float | torch.Tensor = 1.0, top_k: int | torch.Tensor = 0,
+                  top_p: float | torch.Tensor = 1.0, min_p: float | torch.Tensor = 0.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """A token of each row's distribution, drawn by the row's random number, and its log-probability: (int64, float32), both of uniforms' shape.
+
+    logits    [..., V] bf16 or float32; -inf is never drawn
+    uniforms  float32 [...] in [0, 1): the same numbers give the same tokens
+    Of the tokens by falling logits, of equal ones the lower index first, the first top_k are kept (0: all), of those the ones with less than top_p of their
+    weight before them, of those the ones at least min_p times as likely as the likeliest.  The number then falls into the kept tokens' weights, added up in the
+    order of the tokens.  Each setting is a number, or a tensor with one for each row.
+
+    The log-probability is that under softmax(logits / temperature), before anything is left out: what token_logprobs gives for it, and a GRPO step takes its
+    ratios to.  A row of nothing but -inf, one with a NaN, or one whose settings or number are out of range has token -1 and NaN."""
+    _no_gradients("sample_tokens", logits)
+    args = logits, uniforms, temperature, top_k, top_p, min_p
+    return _Recorded.apply(ops.sample_tokens, *args) if _transformed() else ops.sample_tokens(*args)
+
+
+@dataclass
+class CacheStep:
+    """New tokens of some sequences, as rotary_append and paged_attention take them.  Tokens lie sequence by sequence."""
+    positions: torch.Tensor     # int64 [tokens]
+    slots: torch.Tensor         # int64 [tokens]
+    tables: torch.Tensor        # int32 [seqs, pages of the longest]
+    lengths: torch.Tensor       # int32 [seqs], the new tokens among them
+
+
+class PagedCache:
+    """Keys and values of all layers in pages, and the sequences whose tokens they hold.  Sequences that are forked from one share its pages until they write to
+    them: only a last page that is not full is copied, when the first of them goes on.
+
+    The pages of a sequence may be handed on as soon as it is freed or the cache made dense: steps taken before that are not to be used after it, and everything
+    runs on one stream (or on streams that wait for each other)."""
+
+    def __init__(self, layers: int, pages: int, kv_heads: int, head_dim: int, *, page: int = 16, dtype: torch.dtype = torch.bfloat16, device="cuda", key_scale: float = 1.0,
+                 value_scale: float = 1.0):
+        if dtype not in ops._CACHES:
+            raise ValueError(f"PagedCache: bf16 or float8_e4m3fn, not {dtype}")
+        if min(layers, pages, kv_heads) < 1 or page < 16 or page > 4096 or page & (page - 1) or not 0 < head_dim <= 256 or head_dim % (32 if dtype == torch.bfloat16 else 64):
+            raise ValueError("PagedCache: at least one layer, page and head, pages of a power of two from 16 to 4096 tokens, head_dim a multiple of 32 up to 256 "
+                             f"(float8_e4m3fn: of 64), not {layers}, {pages}, {kv_heads}, {page} and {head_dim}")
+        ops._check_scales("PagedCache", key_scale, value_scale)
+        self.page, self.key_scale, self.value_scale = page, float(key_scale), float(value_scale)
+        self.keys = torch.empty(layers, pages, kv_heads, page, head_dim, dtype=dtype, device=device)
+        self.values = torch.empty(layers, pages, kv_heads, head_dim, page, dtype=dtype, device=device)
+        self._free = list(range(pages - 1, -1, -1))                # taken from the end: low numbers first
+        self._users = [0] * pages                                  # sequences that hold the page
+        self._pages: dict[int, list[int]] = {}
+        self._length: dict[int, int] = {}
+        self._next = 0
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def length(self, seq: int) -> int:
+        return self._length[seq]
+
+    def pages(self, seq: int) -> tuple[int, ...]:
+        return tuple(self._pages[seq])
+
+    def new(self, count: int = 1) -> list[int]:
+        """So many empty sequences."""
+        ids = list(range(self._next, self._next + count))
+        self._next += count
+        for i in ids:
+            self._pages[i], self._length[i] = [], 0
+        return ids
+
+    def fork(self, seq: int, count: int = 1) -> list[int]:
+        """So many more sequences that begin with this one's tokens; nothing is copied yet."""
+        held, length = self._pages[seq], self._length[seq]
+        ids = self.new(count)
+        for i in ids:
+            self._pages[i], self._length[i] = list(held), length
+        for p in held:
+            self._users[p] += count
+        return ids
+
+    def free(self, seqs: Sequence[int]) -> None:
+        if len(set(seqs)) != len(seqs) or any(s not in self._pages for s in seqs):
+            raise ValueError(f"PagedCache: sequences of this cache, each once, not {list(seqs)}")
+        for s in seqs:
+            for p in reversed(self._pages.pop(s)):
+                self._users[p] -= 1
+                if self._users[p] == 0:
+                    self._free.append(p)
+            del self._length[s]
+
+    def extend(self, seqs: Sequence[int], counts: Sequence[int] | int = 1) -> CacheStep:
+        """Room for new tokens of these sequences, so many of each, and where they go.  Raises MemoryError, and changes nothing, where the pages do not suffice."""
+        counts = [counts] * len(seqs) if isinstance(counts, int) else list(counts)
+        if len(counts) != len(seqs) or len(set(seqs)) != len(seqs) or any(s not in self._pages for s in seqs) or any(n < 0 for n in counts):
+            raise ValueError(f"PagedCache: sequences of this cache, each once, and a number of new tokens for each: {list(seqs)}, {counts}")
+        page, need, writers = self.page, 0, {}
+        for s, n in zip(seqs, counts):
+            length, held = self._length[s], self._pages[s]
+            need += -(-(length + n) // page) - len(held)
+            if n > 0 and length % page and self._users[held[-1]] > 1:
+                writers[held[-1]] = writers.get(held[-1], 0) + 1
+        # of the holders of a shared page the last one to write keeps it, if nobody else reads it
+        copies = sum(min(w, self._users[p] - 1) for p, w in writers.items())
+        if need + copies > len(self._free):
+            raise MemoryError(f"PagedCache: {need + copies} pages are needed and {len(self._free)} free")
+        sources, destinations = [], []
+        positions, slots, lengths, tables = [], [], [], []
+        for s, n in zip(seqs, counts):
+            length, held = self._length[s], self._pages[s]
+            if n > 0 and length % page and self._users[held[-1]] > 1:
+                fresh = self._free.pop()
+                sources.append(held[-1])
+                destinations.append(fresh)
+                self._users[held[-1]] -= 1
+                self._users[fresh] = 1
+                held[-1] = fresh
+            while len(held) * page < length + n:
+                fresh = self._free.pop()
+                self._users[fresh] = 1
+                held.append(fresh)
+            positions.extend(range(length, length + n))
+            slots.extend(held[t // page] * page + t % page for t in range(length, length + n))
+            self._length[s] = length + n
+            lengths.append(length + n)
+            tables.append(held)
+        if sources:
+            copy_pages(self.keys, self.values, sources, destinations)
+        width = max((len(t) for t in tables), default=0)
+        filled = [t + [0] * (width - len(t)) for t in tables]
+        return CacheStep(self._there(positions, torch.int64), self._there(slots, torch.int64), self._there(filled, torch.int32).reshape(len(filled), width),
+                         self._there(lengths, torch.int32))
+
+    def compact(self) -> int:
+        """Moves pages so that those in use are the first ones; returns how many were moved."""
+        used = len(self._users) - len(self._free)
+        holes = sorted(p for p in self._free if p < used)
+        moved = dict(zip((p for p in range(used, len(self._users)) if self._users[p]), holes))
+        if moved:
+            copy_pages(self.keys, self.values, list(moved), list(moved.values()))
+            for p, to in moved.items():
+                self._users[to], self._users[p] = self._users[p], 0
+            for held in self._pages.values():
+                held[:] = [moved.get(p, p) for p in held]
+        self._free = list(range(len(self._users) - 1, used - 1, -1))
+        return len(moved)
+
+    def _there(self, values: list, dtype: torch.dtype) -> torch.Tensor:
+        host = torch.tensor(values, dtype=dtype)
+        device = self.keys.device
+        return host.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else host.to(device)
+
+
+class CachedAttention(nn.Module):
+    """Self-attention of one new token of each sequence on its own projections: o_proj(paged_attention(..)) of q_proj, k_proj and v_proj of x, over a PagedCache.
+    The projections keep their names, so the parameters do too (a model's attention and this one may share them)."""
+
+    def __init__(self, q_proj: nn.Module, k_proj: nn.Module, v_proj: nn.Module, o_proj: nn.Module, head_dim: int, inv_freq: torch.Tensor, *, interleaved: bool = False,
+                 factor: float = 1.0, scale: float | None = None):
+        super().__init__()
+        self.q_proj, self.k_proj, self.v_proj, self.o_proj = q_proj, k_proj, v_proj, o_proj
+        self.head_dim, self.interleaved, self.factor, self.scale = head_dim, interleaved, factor, scale
+        self.register_buffer("inv_freq", inv_freq, persistent=False)
+
+    def _apply(self, fn, *args, **kwargs):
+        kept = self.inv_freq
+        super()._apply(fn, *args, **kwargs)
+        self.inv_freq = kept.to(self.inv_freq.device)              # (frequencies move with the module; they are not rounded with its parameters)
+        return self
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor, cache: PagedCache, layer: int, step: CacheStep) -> torch.Tensor:
+        """x [seqs, hidden], the newest token of each of the step's sequences."""
+        if x.dim() != 2 or x.shape[0] != step.lengths.shape[0] or step.slots.shape != step.lengths.shape:
+            raise ValueError(f"CachedAttention: one new token of each sequence, [{step.lengths.shape[0]}, hidden] for a step of as many tokens, not {tuple(x.shape)} and "
+                             f"{step.slots.shape[0]}")
+        q, k, v = (proj(x).to(torch.bfloat16).unflatten(-1, (-1, self.head_dim)) for proj in (self.q_proj, self.k_proj, self.v_proj))
+        keys, values = cache.keys[layer], cache.values[layer]
+        q = rotary_append(q, k, v, step.positions, self.inv_freq, step.slots, keys, values, interleaved=self.interleaved, factor=self.factor, key_scale=cache.key_scale,
+                          value_scale=cache.value_scale)
+        o = paged_attention(q, keys, values, step.tables, step.lengths, scale=self.scale, key_scale=cache.key_scale, value_scale=cache.value_scale)
+        return self.o_proj(o.flatten(1).to(x.dtype))

@@ -59,6 +59,8 @@ extern "C" {
 
 #define METIS_DTYPE_BF16 0
 #define METIS_DTYPE_F32 1
+#define METIS_DTYPE_F64 2      /* frequencies of rotary positions only */
+#define METIS_DTYPE_E4M3 3     /* caches of keys and values only: float8_e4m3fn */
 
 /* Library version, (major << 16) | (minor << 8) | patch.  No reference counterpart. */
 int metis_version(void);
@@ -1017,6 +1019,95 @@ int metis_head_logprobs_backward(const void *hidden, int64_t ld_hidden, const vo
                                  const float *grad_logp, const float *grad_entropy, const void *index,
                                  void *grad_hidden, void *grad_weight, void *workspace,
                                  size_t workspace_bytes, void *stream);
+
+/*
+ * Queries and keys turned by the angles of their positions (rotary position embedding; the reference's models apply it
+ * between their q / k projections and attention, in separate operations), in binary32 with each result rounded once:
+ *   (y1, y2) = factor (x1 cos a - x2 sin a, x2 cos a + x1 sin a),   a = position * inv_freq[i], formed in 64 bits,
+ * for the pairs (i, i + turned/2) of a head's first `turned` columns, or with interleaved (2i, 2i + 1); the columns
+ * behind them are copied.  With back the turn by -a: the gradients of q and k for those of the results.
+ *   q, k       [tokens, heads, dim] bf16 or float (dtype); strides of tokens and heads in elements, any; either may have no
+ *              heads (then its pointers are not looked at).  q_out, k_out dense [tokens, heads, dim], not the inputs
+ *   positions  int64 [npos]: token t has positions[t % npos]; npos divides tokens
+ *   inv_freq   [turned / 2], float or double (freq_dtype METIS_DTYPE_F32 / _F64)
+ *   dim        even, up to 512; turned even, 0 to dim.  16-byte aligned pointers and strides with turned and dim - turned
+ *              multiples of 16 are read in whole pieces
+ */
+int metis_rotary(const void *q, int64_t q_token, int64_t q_head, int64_t q_heads, const void *k,
+                 int64_t k_token, int64_t k_head, int64_t k_heads, const int64_t *positions,
+                 int64_t npos, const void *inv_freq, int freq_dtype, int64_t tokens, int64_t dim,
+                 int64_t turned, int interleaved, int back, float factor, int dtype, void *q_out,
+                 void *k_out, void *stream);
+
+/*
+ * A paged cache of one layer: keys [pages, heads, page, dim] and values [pages, heads, dim, page] (a value's dimensions lie
+ * `page` elements apart, its neighbours in time side by side), bf16 or e4m3 with one scale for all keys and one for all
+ * values (a cached number times the scale is the value).  A place is page number * page + offset.
+ *
+ * metis_rotary_append: metis_rotary of new tokens' q and k (bf16), the turned keys and the values written to the cache at
+ * each token's place, e4m3 rounded to nearest with 448 for everything beyond it.
+ *   slots      int64 [tokens]: the places; a negative one: the token is not cached (padding).  A place behind the cache is
+ *              not written and makes the token's query NaN.  Of two tokens with one place either may stay
+ *   q_out      dense [tokens, q_heads, dim]
+ */
+int metis_rotary_append(const void *q, int64_t q_token, int64_t q_head, int64_t q_heads, const void *k,
+                        int64_t k_token, int64_t k_head, int64_t kv_heads, const void *v,
+                        int64_t v_token, int64_t v_head, const int64_t *positions,
+                        const void *inv_freq, int freq_dtype, const int64_t *slots, int64_t tokens,
+                        int64_t dim, int64_t turned, int interleaved, float factor, int64_t pages,
+                        int64_t page, int cache_dtype, float key_scale, float value_scale, void *keys,
+                        void *values, void *q_out, void *stream);
+
+/*
+ * softmax(scale q K^T) V of one new token of each sequence over the cached tokens of the sequence (its own among them):
+ * scores and sums in binary32, the result rounded once to bf16.  Query head h reads head h / (q_heads / kv_heads) of the cache.
+ *   q        bf16 [seqs, q_heads, dim], strides of sequences and heads in elements, multiples of 8; 16-byte aligned
+ *   tables   int32 [seqs, width], row stride table_stride: the pages of each sequence in order; lengths int32 [seqs]: its
+ *            tokens.  What lies behind a length, in the table or in the last page, is not read into any result.  A length
+ *            of 0 gives 0; one that is negative or larger than the table's pages, or a page that the cache does not
+ *            have, makes the sequence's results NaN
+ *   page     a power of two from 16 to 4096; dim a multiple of 32 up to 256 (e4m3: of 64); kv_heads divides q_heads
+ *   out      dense [seqs, q_heads, dim]
+ *   workspace metis_paged_attention_workspace_bytes(.., width * page) bytes, no initialisation needed
+ */
+size_t metis_paged_attention_workspace_bytes(int64_t seqs, int64_t q_heads, int64_t kv_heads,
+                                             int64_t dim, int64_t capacity);
+int metis_paged_attention(const void *q, int64_t q_seq, int64_t q_head, int64_t seqs, int64_t q_heads,
+                          int64_t kv_heads, int64_t dim, const void *keys, const void *values,
+                          int64_t pages, int64_t page, int cache_dtype, const int32_t *tables,
+                          int64_t table_stride, int64_t width, const int32_t *lengths, float scale,
+                          float key_scale, float value_scale, void *out, void *workspace,
+                          size_t workspace_bytes, void *stream);
+
+/*
+ * Copies of whole pages, in all layers of a cache (keys and values each [layers, pages, page_bytes]).
+ *   sources, destinations  HOST pointers, int64 [count], read before the call returns; count up to `pages`.  No page may
+ *                          be written twice, or written and read: METIS_E_ARG
+ *   page_bytes             a multiple of 16
+ */
+int metis_cache_copy_pages(void *keys, void *values, int64_t layers, int64_t pages, int64_t page_bytes,
+                           const int64_t *sources, const int64_t *destinations, int64_t count,
+                           void *stream);
+
+/*
+ * A token of each row's distribution, drawn by a given random number (the reference's rollouts sample through their library's
+ * generate()).  With w_i = exp((x_i - max x) / temperature), tokens in the order of falling logits and of equal ones by
+ * rising index:
+ *   K1  the first top_k of them (0: all);  K2  those of K1 with less than top_p sum(K1) of weight before them;
+ *   K3  those of K2 with w >= min_p
+ *   token = the lowest index i in K3 with sum_{j <= i, j in K3} w_j > u sum(K3),
+ *   logprob = log w_token - log sum_i w_i, over all tokens: its log-probability under softmax(x / temperature)
+ * Weights and sums in 64 bits; the same inputs give the same token always.
+ *   logits      bf16 or float [rows, vocab], row stride ld; vocab up to 2^22.  -inf: never drawn
+ *   uniforms    float [rows] in [0, 1)
+ *   parameters  HOST double[4]: temperature > 0, top_k >= 0, top_p > 0, min_p in [0, 1]; or row_parameters, device
+ *               double [rows, 4], which is then used in its place
+ *   A row without a finite or infinite largest logit (all -inf, or a NaN), or with parameters or a number outside their
+ *   ranges, has token -1 and logprob NaN.
+ */
+int metis_sample_tokens(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab,
+                        const float *uniforms, const double *parameters,
+                        const double *row_parameters, int64_t *tokens, float *logprobs, void *stream);
 
 #ifdef __cplusplus
 }

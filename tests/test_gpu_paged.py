@@ -1,0 +1,406 @@
+"""The paged cache on the device: what rotary_append writes, paged_attention against its formula in 64 bits, copies of pages.
+
+paged_attention's tolerance: the result is the formula's value rounded once to bf16, half a step (2^-9 for values up to the next power of two: eps / 2), and before that off by a part of
+sum p |v|.  Scores: products of two bf16 (or exact e4m3) numbers in binary32 chains of dim terms, (dim + 4) 2^-24 of scale sum |q k|; that is the relative error of
+a weight, in numerator and denominator, beside 2^-21 for the exponential and its argument.  The weights enter the product as two bf16 terms (2^-16) and
+are summed over chains of at most 2^9 terms of a workgroup's waves and splits (2^-15): 2 delta + 2^-14 covers all."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF, E4 = torch.bfloat16, torch.float8_e4m3fn
+
+
+def cache(g, pages, kv, page, dim, dtype=BF, scale=1.0):
+    def normal(*shape):
+        return (torch.randn(*shape, generator=g) * scale).to(dtype).cuda()
+    return normal(pages, kv, page, dim), normal(pages, kv, dim, page)
+
+
+def tables_of(g, lengths, page, pages, behind=0, extra=0):
+    """Pages in any order, none twice; behind them whatever `behind` says."""
+    order = torch.randperm(pages, generator=g).tolist()
+    width = max(-(-n // page) for n in lengths) + extra
+    rows = []
+    for n in lengths:
+        need = -(-n // page)
+        rows.append([order.pop() for _ in range(need)] + [behind] * (width - need))
+    return torch.tensor(rows, dtype=torch.int32).reshape(len(lengths), width).cuda()
+
+
+def check(got, q, keys, values, tables, lengths, scale=None, key_scale=1.0, value_scale=1.0):
+    seqs, heads, dim = q.shape
+    kv, page = keys.shape[1], keys.shape[2]
+    scale = dim ** -0.5 if scale is None else scale
+    assert got.shape == q.shape and got.dtype == BF and got.is_contiguous()
+    for i, n in enumerate(lengths):
+        if n == 0:
+            assert not bool(got[i].any())
+            continue
+        used = tables[i, :-(-n // page)].long()
+        for h in range(kv):
+            mine = slice(h * heads // kv, (h + 1) * heads // kv)
+            k = keys[used, h].reshape(-1, dim)[:n].double() * key_scale
+            v = values[used, h].transpose(1, 2).reshape(-1, dim)[:n].double() * value_scale
+            x = q[i, mine].double()
+            p = torch.softmax(x @ k.t() * scale, 1)
+            want, mag = p @ v, p @ v.abs()
+            delta = (dim + 4) * 2.0 ** -24 * abs(scale) * (x.abs() @ k.abs().t()).amax(1, keepdim=True)
+            lost = (2 * delta + 2.0 ** -14) * mag
+            bad = (got[i, mine].double() - want).abs() > 2.0 ** -8 * (want.abs() + lost) + lost
+            assert not bool(bad.any()), f"sequence {i} of {n} tokens, cache head {h}: {int(bad.sum())} of {bad.numel()} off"
+
+
+# lengths, heads, heads of the cache, dim, page, cache
+CASES = [([1], 1, 1, 128, 16, BF), ([411], 12, 2, 128, 16, BF), ([512], 12, 2, 128, 16, BF), ([513], 12, 2, 128, 16, BF), ([1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 255, 256, 257], 28, 4, 128, 16, BF),
+         ([0, 5, 0, 700], 4, 4, 64, 32, BF), ([3000, 1, 1999], 8, 1, 96, 64, BF), ([777, 4096], 16, 2, 256, 16, BF), ([2500], 40, 8, 32, 128, BF), ([1100, 90], 34, 2, 160, 16, BF),
+         ([5000], 48, 1, 128, 16, BF), ([9000, 300, 1025, 1024], 28, 4, 128, 256, BF), ([130, 620], 3, 1, 192, 16, BF), ([130, 1620], 6, 2, 224, 64, BF), ([5, 700], 2, 2, 128, 4096, BF),
+         ([1, 16, 17, 64, 65, 130, 411], 8, 2, 128, 16, E4), ([8000, 1, 2049], 32, 8, 128, 64, E4), ([1500, 63], 5, 1, 64, 16, E4), ([900, 2222], 8, 4, 256, 32, E4), ([70, 1300], 20, 1, 192, 16, E4),
+         ([33000], 14, 2, 128, 16, BF), ([7] * 300, 4, 2, 64, 16, BF)]
+
+
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_attention_against_64_bits(case):
+    from metis_hip import paged_attention
+    lengths, heads, kv, dim, page, dt = CASES[case]
+    g = torch.Generator().manual_seed(case)
+    pages = sum(-(-n // page) for n in lengths) + 3
+    keys, values = cache(g, pages, kv, page, dim, dt, 1.5)
+    q = torch.randn(len(lengths), heads, dim, generator=g).to(BF).cuda()
+    tables = tables_of(g, lengths, page, pages)
+    scales = dict(key_scale=0.7, value_scale=1.3) if dt == E4 else {}
+    got = paged_attention(q, keys, values, tables, torch.tensor(lengths, dtype=torch.int32).cuda(), **scales)
+    check(got, q, keys, values, tables, lengths, **scales)
+    assert torch.equal(got, paged_attention(q, keys, values, tables, torch.tensor(lengths, dtype=torch.int32).cuda(), **scales))
+
+
+@pytest.mark.parametrize("dt", [BF, E4])
+@pytest.mark.parametrize("junk", [float("nan"), float("inf"), -float("inf")])
+def test_what_lies_behind_the_lengths_counts_for_nothing(dt, junk):
+    """The rest of a last page, whole pages behind it and their table entries: the bits of clean ones."""
+    from metis_hip import paged_attention
+    g = torch.Generator().manual_seed(1)
+    if dt == E4 and junk != junk or dt == BF:
+        bad = junk
+    else:
+        bad = 448.0 if junk > 0 else -448.0
+    lengths, page = [1, 15, 17, 63, 64, 300, 1030, 0], 16
+    pages = sum(-(-n // page) for n in lengths)
+    keys, values = cache(g, pages, 2, page, 128, dt)
+    q = torch.randn(len(lengths), 6, 128, generator=g).to(BF).cuda()
+    tables = tables_of(g, lengths, page, pages, extra=2)
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    want = paged_attention(q, keys, values, tables, n)
+    check(want, q, keys, values, tables, lengths)
+    dirty = torch.cat((keys.float(), torch.full_like(keys[:1], bad).float())), torch.cat((values.float(), torch.full_like(values[:1], bad).float()))
+    for i, length in enumerate(lengths):
+        used = -(-length // page)
+        if length % page:
+            dirty[0][tables[i, used - 1].long(), :, length % page:] = bad
+            dirty[1][tables[i, used - 1].long(), :, :, length % page:] = bad
+        tables[i, used:] = torch.tensor([pages, -5, 1 << 30, pages + 7])[torch.arange(tables.shape[1] - used) % 4].int()
+    got = paged_attention(q, *(t.to(dt) for t in dirty), tables, n)
+    assert torch.equal(got, want)
+
+
+def test_pages_and_lengths_that_are_none_show():
+    """NaN for the sequence that names them, the others as they were.  (The kernel reads no page outside of the cache and no entry outside of its table.)"""
+    from metis_hip import paged_attention
+    g = torch.Generator().manual_seed(2)
+    for lengths, capacity in (([100, 40, 64, 90], 7), ([3000, 40, 2000, 90], 190)):
+        keys, values = cache(g, 400, 2, 16, 128)
+        q = torch.randn(4, 4, 128, generator=g).to(BF).cuda()
+        tables = tables_of(g, lengths, 16, 400)
+        tables = torch.nn.functional.pad(tables, (0, capacity - tables.shape[1]))
+        n = torch.tensor(lengths, dtype=torch.int32).cuda()
+        want = paged_attention(q, keys, values, tables, n)
+        for bad in (-1, 400, 1 << 30, -(1 << 31)):
+            for at in (0, 1, 5):
+                broken = tables.clone()
+                broken[0, at] = bad
+                got = paged_attention(q, keys, values, broken, n)
+                assert bool(got[0].isnan().all()) and torch.equal(got[1:], want[1:])
+        for bad in (-1, -(1 << 31), capacity * 16 + 1, (1 << 31) - 1):
+            lie = n.clone()
+            lie[2] = bad
+            got = paged_attention(q, keys, values, tables, lie)
+            assert bool(got[2].isnan().all()) and torch.equal(got[:2], want[:2]) and torch.equal(got[3], want[3])
+
+
+def test_far_scores_and_extreme_values():
+    """Scores of thousands (one token has all the weight), scores that are all alike, an infinite value under a weight, a NaN key."""
+    from metis_hip import paged_attention
+    g = torch.Generator().manual_seed(3)
+    lengths, page = [700, 1500], 16
+    pages = sum(-(-n // page) for n in lengths)
+    keys, values = cache(g, pages, 2, page, 128)
+    q = torch.randn(2, 8, 128, generator=g).to(BF).cuda()
+    tables = tables_of(g, lengths, page, pages)
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    for scale in (0.0, 1e-3, -0.3):
+        check(paged_attention(q, keys, values, tables, n, scale=scale), q, keys, values, tables, lengths, scale=scale)
+    big = (q.float() * 400).to(BF)
+    got = paged_attention(big, keys, values, tables, n)
+    for i, length in enumerate(lengths):
+        used = tables[i, :-(-length // page)].long()
+        for h in range(8):
+            s = big[i, h].double() @ keys[used, h // 4].reshape(-1, 128)[:length].double().t() * 128 ** -0.5
+            best = s.topk(2)
+            if float(best.values[0] - best.values[1]) > 40:
+                assert torch.equal(got[i, h], values[used, h // 4].transpose(1, 2).reshape(-1, 128)[best.indices[0]])
+    values2, keys2 = values.clone(), keys.clone()
+    values2[tables[0, 3].long(), 1, 5, 2] = float("inf")
+    got = paged_attention(q, keys, values2, tables, n)
+    assert bool((got[0, 4:, 5] == float("inf")).all()) and bool(got[0, :4].isfinite().all()) and bool(got[1].isfinite().all())
+    keys2[tables[1, 0].long(), 0, 3] = float("nan")
+    got = paged_attention(q, keys2, values, tables, n)
+    assert bool(got[1, :4].isnan().all()) and bool(got[1, 4:].isfinite().all()) and bool(got[0].isfinite().all())
+
+
+def test_strides_and_shared_pages():
+    """Queries that are parts of wider rows, tables cut out of wider ones, one page in many tables."""
+    from metis_hip import paged_attention
+    g = torch.Generator().manual_seed(4)
+    lengths = [48, 48, 700]
+    keys, values = cache(g, 60, 2, 16, 64)
+    tables = tables_of(g, lengths, 16, 60)
+    tables[1] = tables[0]
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    for width, first in ((4 * 64 + 96, 0), (4 * 64 + 96, 40), (4 * 64 + 5, 1), (4 * 64 + 16, 3)):
+        q = torch.randn(3, width, generator=g).to(BF).cuda()[:, first:first + 256].unflatten(-1, (4, 64))
+        got = paged_attention(q, keys, values, tables, n)
+        check(got, q, keys, values, tables, lengths)
+        wide = torch.nn.functional.pad(tables, (3, 9), value=-1)[:, 3:3 + tables.shape[1]]
+        assert torch.equal(paged_attention(q, keys, values, wide, n), got)
+        assert torch.equal(paged_attention(q, keys, values, tables.t().contiguous().t(), n), got)
+    q = torch.randn(4, 3, 64, generator=g).to(BF).cuda().transpose(0, 1)
+    check(paged_attention(q, keys, values, tables, n), q, keys, values, tables, lengths)
+    one = torch.randn(1, 64, generator=g).to(BF).cuda().expand(4, 64).expand(3, 4, 64)
+    check(paged_attention(one, keys, values, tables, n), one, keys, values, tables, lengths)
+
+
+def test_attention_refusals():
+    from metis_hip import MetisHipError, paged_attention
+    g = torch.Generator().manual_seed(5)
+    keys, values = cache(g, 8, 2, 16, 64)
+    q, tables, n = torch.zeros(3, 4, 64, dtype=BF, device="cuda"), torch.zeros(3, 2, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    bad = [(q.float(), keys, values, tables, n), (q[:, :3], keys, values, tables, n), (q[..., :32], keys, values, tables, n), (q, keys, keys, tables, n), (q, keys.float(), values.float(), tables, n),
+           (q, keys.transpose(0, 1), values.transpose(0, 1), tables, n), (q, keys[:, :, :, ::2], values, tables, n), (q, keys, values.to(E4), tables, n), (q, keys, values, tables.long(), n),
+           (q, keys, values, tables, n.long()), (q, keys, values, tables[:2], n), (q, keys, values, tables, n[:2]), (q[0], keys, values, tables, n), (q, keys, values, tables.cpu(), n),
+           (q, keys[:0], values[:0], tables, n), (q[:, :0], keys, values, tables, n)]
+    for args in bad:
+        with pytest.raises(ValueError):
+            paged_attention(*args)
+    for page in (8, 24, 8192):
+        k, v = torch.zeros(2, 2, page, 64, dtype=BF, device="cuda"), torch.zeros(2, 2, 64, page, dtype=BF, device="cuda")
+        with pytest.raises(ValueError, match="power of two"):
+            paged_attention(q, k, v, tables, n)
+    for dim, dt in ((48, BF), (288, BF), (32, E4), (96, E4)):
+        k, v = torch.zeros(2, 2, 16, dim, device="cuda").to(dt), torch.zeros(2, 2, dim, 16, device="cuda").to(dt)
+        with pytest.raises(ValueError, match="multiple"):
+            paged_attention(torch.zeros(3, 4, dim, dtype=BF, device="cuda"), k, v, tables, n)
+    for more in (dict(scale=float("nan")), dict(key_scale=0.0), dict(value_scale=-1.0), dict(value_scale=float("inf"))):
+        with pytest.raises(ValueError):
+            paged_attention(q, keys, values, tables, n, **more)
+    with pytest.raises(ValueError, match="no gradients"):
+        paged_attention(q.requires_grad_(), keys, values, tables, n)
+    with pytest.raises(MetisHipError, match="no CPU path"):
+        paged_attention(q.detach().cpu(), keys, values, tables, n)
+    q = q.detach()
+    assert paged_attention(q[:0], keys, values, tables[:0], n[:0]).shape == (0, 4, 64)
+    assert not bool(paged_attention(q, keys, values, tables[:, :0], 0 * n).any())
+    assert bool(paged_attention(q, keys, values, tables[:, :0], n).isnan().all())
+
+
+def test_attention_on_other_streams_and_replayed():
+    """Calls side by side on streams, with workspaces of their own; two graphs captured from one shape, replayed in turn on changed lengths, tables and queries."""
+    from metis_hip import paged_attention
+    g = torch.Generator().manual_seed(6)
+    keys, values = cache(g, 700, 4, 16, 128)
+
+    def given(lengths):
+        tables = tables_of(g, lengths, 16, 700)
+        return [torch.randn(3, 28, 128, generator=g).to(BF).cuda(), torch.nn.functional.pad(tables, (0, 400 - tables.shape[1])).contiguous(), torch.tensor(lengths, dtype=torch.int32).cuda()]
+
+    calls = [given(n) for n in ([6000, 1, 700], [90, 3000, 2048], [0, 17, 6400])]
+    want = [paged_attention(q, keys, values, t, n) for q, t, n in calls]
+    for (q, t, n), w in zip(calls, want):
+        check(w, q, keys, values, t, n.tolist())
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in calls], []
+    for _ in range(3):
+        for s, (q, t, n) in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append(paged_attention(q, keys, values, t, n))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want[i % 3]) for i, a in enumerate(got))
+    held, graphs = [[t.clone() for t in calls[0]] for _ in range(2)], []
+    for h in held:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = paged_attention(h[0], keys, values, h[1], h[2])
+        graphs.append((graph, out))
+    for k in range(4):
+        for j, h in enumerate(held):
+            for a, b in zip(h, calls[(k + j) % 3]):
+                a.copy_(b)
+        for graph, _ in graphs:
+            graph.replay()
+        eager = paged_attention(calls[k % 3][0], keys, values, *calls[k % 3][1:])
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[k % 3]) and all(torch.equal(out, want[(k + j) % 3]) for j, (_, out) in enumerate(graphs))
+
+
+def test_attention_beyond_32_bits_of_elements():
+    """Keys and values of 2^32 elements and more each; the sequences' pages lie at both ends."""
+    from metis_hip import paged_attention
+    g = torch.Generator(device="cuda").manual_seed(7)
+    pages = (1 << 32) // (4 * 16 * 128) + 64
+    keys, values = torch.zeros(pages, 4, 16, 128, dtype=BF, device="cuda"), torch.zeros(pages, 4, 128, 16, dtype=BF, device="cuda")
+    for t in (keys, values):
+        t[-64:] = torch.randn(t[-64:].shape, generator=g, device="cuda").to(BF)
+        t[:8] = torch.randn(t[:8].shape, generator=g, device="cuda").to(BF)
+    assert keys.numel() > 1 << 32
+    tables = torch.cat((torch.arange(pages - 60, pages), torch.arange(0, 8))).int().cuda()[None]
+    q = torch.randn(1, 28, 128, generator=g, device="cuda").to(BF)
+    check(paged_attention(q, keys, values, tables, torch.tensor([68 * 16 - 3], dtype=torch.int32).cuda()), q, keys, values, tables, [68 * 16 - 3])
+    del keys, values
+    torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------------------------------------- appends
+def frequencies(n):
+    return (1e4 ** (-torch.arange(n, dtype=torch.float64) / n)).cuda()
+
+
+# tokens, heads, heads of the cache, dim, turned, page, interleaved, columns in front of the rows (alignment)
+APPENDS = [(1, 12, 2, 128, 128, 16, False, 0), (5, 7, 1, 64, 64, 32, True, 0), (300, 28, 4, 128, 128, 16, False, 0), (77, 4, 4, 96, 48, 16, False, 0), (33, 6, 3, 32, 30, 16, False, 3),
+           (1030, 8, 8, 256, 128, 64, True, 0), (9, 2, 2, 6, 4, 4, False, 1), (4099, 6, 2, 128, 128, 16, False, 0)]
+
+
+@pytest.mark.parametrize("dt", [BF, E4])
+@pytest.mark.parametrize("case", range(len(APPENDS)))
+def test_appends(case, dt):
+    """The queries and keys are rotary's bits (e4m3: within half a step, 2^-4 relative or 2^-10, of the turned key over the scale, which differs from rotary's by its
+    rounding to bf16 alone), the values the given ones; every other place is as it was, padding leaves none."""
+    from metis_hip import ops, rotary, rotary_append
+    T, hq, kv, dim, part, page, inter, front = APPENDS[case]
+    g = torch.Generator().manual_seed(case)
+    rows = torch.randn(T, front + (hq + 2 * kv) * dim, generator=g).to(BF).cuda()[:, front:]
+    q, k, v = (t.unflatten(-1, (-1, dim)) for t in rows.split([hq * dim, kv * dim, kv * dim], -1))
+    positions, inv = (torch.arange(T) + 1000).cuda(), frequencies(part // 2)
+    pages = T // page + 9
+    order = torch.randperm(pages * page, generator=g)[:T] if case % 2 else (torch.randperm(pages, generator=g)[(torch.arange(T) + 5) // page] * page + (torch.arange(T) + 5) % page)
+    order[1::7] = -1 - order[1::7]
+    slots = order.cuda()
+    keys, values = (t.float().clamp(-200, 200).to(dt) for t in cache(g, pages, kv, page, dim))
+    before = keys.clone(), values.clone()
+    scales = dict(key_scale=0.01, value_scale=2.0) if dt == E4 else {}
+    got = rotary_append(q, k, v, positions, inv, slots, keys, values, interleaved=inter, factor=1.25, **scales)
+    want_q, want_k = rotary(q, k, positions, inv, interleaved=inter, factor=1.25)
+    assert torch.equal(got, want_q) and got.is_contiguous()
+    kept = slots >= 0
+    at_page, at = slots[kept] // page, slots[kept] % page
+    new_k, new_v = keys[at_page, :, at], values[at_page, :, :, at]
+    if dt == BF:
+        assert torch.equal(new_k, want_k[kept]) and torch.equal(new_v, v[kept])
+    else:
+        for new, exact, scale, off in ((new_k, want_k[kept], 0.01, 2.0 ** -8), (new_v, v[kept], 2.0, 0.0)):
+            exact = (exact.double() / scale).clamp(-448, 448)
+            bound = (2.0 ** -4 + off) * exact.abs() * (1 + off) + 2.0 ** -10 * (1 + 2.0 ** -20)
+            assert bool(((new.double() - exact).abs() <= bound).all())
+        assert torch.equal(new_v.float(), (v[kept].float() / 2.0).to(E4).float())
+    left = torch.ones(pages * page, dtype=torch.bool, device="cuda")
+    left[slots[kept]] = False
+    left = left.view(pages, page)
+    raw = torch.uint8 if dt == E4 else torch.int16
+    assert torch.equal(keys.view(raw).transpose(1, 2)[left], before[0].view(raw).transpose(1, 2)[left])
+    assert torch.equal(values.view(raw).permute(0, 3, 1, 2)[left], before[1].view(raw).permute(0, 3, 1, 2)[left])
+
+
+def test_places_that_are_none_show_and_values_beyond_e4m3():
+    from metis_hip import rotary, rotary_append
+    g = torch.Generator().manual_seed(11)
+    keys, values = cache(g, 4, 2, 16, 64)
+    before = keys.clone(), values.clone()
+    q, k, v = (torch.randn(5, h, 64, generator=g).to(BF).cuda() for h in (4, 2, 2))
+    at, inv = torch.arange(5).cuda(), frequencies(32)
+    got = rotary_append(q, k, v, at, inv, torch.tensor([64, -1, 1 << 40, -(1 << 62), 1 << 62]).cuda(), keys, values)
+    want, _ = rotary(q, k, at, inv)
+    assert bool(got[[0, 2, 4]].isnan().all()) and torch.equal(got[[1, 3]], want[[1, 3]])
+    assert torch.equal(keys, before[0]) and torch.equal(values, before[1])
+    keys, values = (t.to(E4) for t in before)
+    v[0, 0, 0], v[0, 0, 1], v[0, 0, 2], v[0, 0, 3] = 1e30, -float("inf"), float("nan"), 465.0
+    rotary_append(q, 1e4 * k, v, 0 * at, inv, at, keys, values)
+    assert values[0, 0, :4, 0].float().tolist()[:2] == [448.0, -448.0] and bool(values[0, 0, 2, 0].float().isnan()) and float(values[0, 0, 3, 0]) == 448.0
+    assert torch.equal(keys[0, :, :5].float().transpose(0, 1), (1e4 * k).float().clamp(-448, 448).to(E4).float())
+
+
+def test_append_refusals():
+    from metis_hip import rotary_append
+    g = torch.Generator().manual_seed(12)
+    keys, values = cache(g, 4, 2, 16, 64)
+    q, k, v = (torch.zeros(5, h, 64, dtype=BF, device="cuda") for h in (4, 2, 2))
+    at, inv = torch.arange(5).cuda(), frequencies(32)
+    bad = [(q.float(), k.float(), v.float(), at, inv, at, keys, values), (q[None], k[None], v[None], at[None], inv, at[None], keys, values), (q, k, v[:, :1], at, inv, at, keys, values),
+           (q, k[:, :1], v[:, :1], at, inv, at, keys, values), (q, k, v, at[:1], inv, at, keys, values), (q, k, v, at, inv, at[:4], keys, values), (q, k, v, at, inv, at.int(), keys, values),
+           (q, k, v, at, inv, at, keys, keys), (q, k, v, at, inv, at, keys.float(), values.float()), (q, k, v, at, inv, at, keys[:0], values[:0]), (q, k, v, at, inv, at.cpu(), keys, values),
+           (q, k, v.float(), at, inv, at, keys, values)]
+    for args in bad:
+        with pytest.raises(ValueError):
+            rotary_append(*args)
+    with pytest.raises(ValueError, match="scales"):
+        rotary_append(q, k, v, at, inv, at, keys, values, key_scale=0.0)
+    with pytest.raises(ValueError, match="no gradients"):
+        rotary_append(q, k.requires_grad_(), v, at, inv, at, keys, values)
+    k = k.detach()
+    assert rotary_append(q[:0], k[:0], v[:0], at[:0], inv, at[:0], keys, values).shape == (0, 4, 64)
+
+
+# ---------------------------------------------------------------------------------------------- pages
+@pytest.mark.parametrize("layers,pages,kv,page,dim,dt,count", [(1, 2, 1, 16, 32, BF, 1), (3, 700, 2, 16, 64, BF, 300), (2, 40, 8, 64, 128, BF, 20), (5, 33, 3, 32, 64, E4, 11),
+                                                               (2, 9, 1, 16, 8, E4, 4), (1, 1000, 1, 16, 96, BF, 481), (2, 30, 5, 16, 72, BF, 14)])
+def test_copies(layers, pages, kv, page, dim, dt, count):
+    from metis_hip import copy_pages
+    g = torch.Generator().manual_seed(pages)
+    keys = torch.randn(layers, pages, kv, page, dim, generator=g).to(dt).cuda()
+    values = torch.randn(layers, pages, kv, dim, page, generator=g).to(dt).cuda()
+    order = torch.randperm(pages, generator=g).tolist()
+    to, rest = order[:count], order[count:]
+    for sources in ([rest[i % len(rest)] for i in range(count)], [rest[0]] * count):
+        want = []
+        for t in (keys, values):
+            t = t.view(torch.uint8 if dt == E4 else torch.int16).clone()
+            t[:, to] = t[:, sources]
+            want.append(t)
+        copy_pages(keys, values, sources, to)
+        assert torch.equal(keys.view(want[0].dtype), want[0]) and torch.equal(values.view(want[1].dtype), want[1])
+
+
+def test_copy_refusals_leave_the_cache():
+    from metis_hip import copy_pages
+    g = torch.Generator().manual_seed(13)
+    keys, values = torch.randn(2, 6, 1, 16, 32, generator=g).to(BF).cuda(), torch.randn(2, 6, 1, 32, 16, generator=g).to(BF).cuda()
+    before = keys.clone(), values.clone()
+    for a, b in (([0], [6]), ([-1], [2]), ([0], [1, 2]), ([0, 1], [2, 2]), ([0, 1], [1, 2]), ([3], [3]), ([0, 1, 2], [3, 4, 0])):
+        with pytest.raises(ValueError):
+            copy_pages(keys, values, a, b)
+    for args in ((keys[0], values[0], [0], [1]), (keys, keys, [0], [1]), (keys[:, ::2], values[:, ::2], [0], [1])):
+        with pytest.raises(ValueError):
+            copy_pages(*args)
+    copy_pages(keys, values, [], [])
+    assert torch.equal(keys, before[0]) and torch.equal(values, before[1])
+
+
+def test_copies_beyond_32_bits_of_bytes():
+    from metis_hip import copy_pages
+    g = torch.Generator(device="cuda").manual_seed(14)
+    pages = 140000
+    keys, values = torch.zeros(2, pages, 4, 16, 128, dtype=BF, device="cuda"), torch.zeros(2, pages, 4, 128, 16, dtype=BF, device="cuda")
+    keys[:, -3:], values[:, -3:] = torch.randn(2, 3, 4, 16, 128, generator=g, device="cuda").to(BF), torch.randn(2, 3, 4, 128, 16, generator=g, device="cuda").to(BF)
+    assert keys[0].numel() * 2 > 1 << 31 and keys.numel() * 2 > 1 << 32
+    copy_pages(keys, values, [pages - 1, pages - 2], [0, pages - 5])
+    for t in (keys, values):
+        assert torch.equal(t[:, 0], t[:, -1]) and torch.equal(t[:, -5], t[:, -2]) and not bool(t[:, 1].any()) and bool(t[:, -1].any())
+    del keys, values, t
+    torch.cuda.empty_cache()

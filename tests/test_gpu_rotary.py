@@ -1,0 +1,258 @@
+"""rotary on the device against its formula in 64 bits.
+
+Tolerances: a result is the formula's value in binary32, rounded once, so it is off by at most half a step of its type (eps / 2, relative) and by what the
+sine, the cosine and two products lose, all relative to |x1| + |x2|.  For binary32 the library's sine and cosine of a part of a turn are within 4 units (2^-21), the
+part's own rounding to binary32 moves the angle by 2 pi 2^-26, the products and the sum by 2^-23: under 2^-19.  For bf16 the hardware's sine and cosine
+are taken, which are off by at most 2^-18 (over all multiples of 2^-24 of a turn 2^-20.5 was seen): under 2^-16.  The angles are formed in 64 bits here and there:
+positions up to 2^24 times frequencies up to one leave 2^-29 of an angle."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+LOST = {BF: 2.0 ** -16, F32: 2.0 ** -19}
+
+
+def turned(x, positions, inv_freq, interleaved, factor, back=False):
+    """(x turned, the magnitudes that enter each value) in 64 bits; positions of x's leading sizes."""
+    n = inv_freq.numel()
+    angle = (positions.double()[..., None] * inv_freq.double())[..., None, :] * (-1 if back else 1)
+    x = x.double()
+    a, b = (x[..., 0:2 * n:2], x[..., 1:2 * n:2]) if interleaved else (x[..., :n], x[..., n:2 * n])
+    c, s = torch.cos(angle), torch.sin(angle)
+    pair = ((a * c - b * s) * factor, (b * c + a * s) * factor)
+    mag = (a.abs() + b.abs()) * abs(factor)
+    put = (lambda p, q: torch.stack((p, q), -1).flatten(-2)) if interleaved else (lambda p, q: torch.cat((p, q), -1))
+    rest = x[..., 2 * n:]
+    return torch.cat((put(*pair), rest), -1), torch.cat((put(mag, mag), torch.zeros_like(rest)), -1)
+
+
+def near(got, want, mag):
+    dt = got.dtype
+    bound = torch.finfo(dt).eps / 2 * (want.abs() + LOST[dt] * mag) + LOST[dt] * mag
+    bad = (got.double() - want).abs() > bound
+    assert got.shape == want.shape and not bool(bad.any()), f"{int(bad.sum())} of {bad.numel()} off, by up to {float(((got.double() - want).abs() / mag.clamp_min(1e-30)).max()):.3g} of the magnitudes"
+
+
+def frequencies(n, base=1e4, dtype=torch.float64):
+    return (base ** (-torch.arange(n, dtype=torch.float64) / max(n, 1))).to(dtype).cuda()
+
+
+# lead, query heads, key heads, dim, turned, interleaved, type, first position, factor
+CASES = [((1, 1), 12, 2, 128, 128, False, BF, 0, 1.0), ((1,), 1, 1, 2, 2, True, BF, 5, 1.0), ((2, 37), 28, 4, 128, 128, False, BF, 0, 1.0), ((3, 701), 7, 1, 96, 48, True, F32, 10 ** 6, 1.0),
+         ((5,), 3, 2, 10, 6, False, F32, 3, 1.0), ((130,), 16, 16, 64, 64, True, BF, 1 << 20, 1.2), ((33,), 2, 1, 256, 64, False, BF, 7, 0.5), ((9,), 5, 5, 512, 512, False, F32, 9, 1.0),
+         ((9,), 5, 1, 512, 510, True, BF, 9, 1.0), ((2, 3, 5), 4, 2, 80, 32, False, BF, 1 << 24, 1.0), ((4100,), 32, 8, 128, 128, True, BF, 100, 1.0), ((2100,), 32, 32, 64, 32, False, F32, 0, 1.1),
+         ((3, 1031), 40, 1, 112, 96, False, BF, 0, 1.0)]
+
+
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_against_64_bits(case):
+    from metis_hip import rotary
+    lead, hq, hk, dim, part, inter, dt, first, factor = CASES[case]
+    g = torch.Generator().manual_seed(case)
+    q, k, gq, gk = (torch.randn(*lead, h, dim, generator=g).to(dt).cuda() for h in (hq, hk, hq, hk))
+    q, k = q.requires_grad_(), k.requires_grad_()
+    positions = (first + torch.randint(0, 4000, lead, generator=g)).cuda()
+    inv = frequencies(part // 2)
+    yq, yk = rotary(q, k, positions, inv, interleaved=inter, factor=factor)
+    grads = torch.autograd.grad((yq, yk), (q, k), (gq, gk))
+    with torch.no_grad():
+        for got, x, back in ((yq, q, False), (yk, k, False), (grads[0], gq, True), (grads[1], gk, True)):
+            assert got.dtype == dt and got.is_contiguous()
+            near(got, *turned(x, positions, inv, inter, factor, back))
+        # not recorded: the same bits
+        assert all(torch.equal(a, b) for a, b in zip(rotary(q, k, positions, inv, interleaved=inter, factor=factor), (yq, yk)))
+
+
+def test_parts_of_a_products_rows_and_broadcast_positions():
+    """Strides of tokens and heads, rows that are no multiple of 16 bytes, transposed and expanded heads, positions of one sequence for all: the bits of dense operands."""
+    from metis_hip import ops, rotary
+    g = torch.Generator().manual_seed(3)
+    inv = frequencies(32)
+    for width, first in ((12 * 64, 0), (12 * 64 + 3, 0), (12 * 64 + 8, 8), (12 * 64 + 8, 5)):
+        rows = torch.randn(2, 19, width, generator=g).to(BF).cuda()[..., first:first + 768]
+        q, k = rows[..., :512].unflatten(-1, (8, 64)), rows[..., 512:].unflatten(-1, (4, 64))
+        for positions in (torch.arange(19).cuda(), torch.arange(19).cuda()[None], torch.arange(38).reshape(2, 19).cuda()):
+            same = positions.expand(2, 19) if positions.numel() == 19 else positions
+            want = ops.rotary(q.contiguous(), k.contiguous(), same.contiguous(), inv)
+            assert all(torch.equal(a, b) for a, b in zip(rotary(q, k, positions, inv), want))
+            lead = [t.detach().requires_grad_() for t in (q, k)]
+            assert all(torch.equal(a, b) for a, b in zip(rotary(*lead, positions, inv), want))
+    # [batch, heads, tokens, dim] turned round, one key head for many, every second head
+    a = torch.randn(2, 6, 19, 64, generator=g).to(BF).cuda()
+    one = torch.randn(2, 19, 1, 64, generator=g).to(BF).cuda().expand(2, 19, 5, 64)
+    positions = torch.arange(19).cuda()
+    for q, k in ((a.transpose(1, 2), one), (a.transpose(1, 2)[:, :, ::2], one[:, :, :1]), (a.transpose(1, 2)[:, ::2], one[:, ::2])):
+        at = positions[:q.shape[1]]
+        assert all(torch.equal(x, y) for x, y in zip(rotary(q, k, at, inv), rotary(q.contiguous(), k.contiguous(), at, inv)))
+    # dimensions that are not dense
+    wide = torch.randn(7, 3, 128, generator=g).to(BF).cuda()[..., ::2]
+    at = torch.arange(7).cuda()
+    assert all(torch.equal(x, y) for x, y in zip(rotary(wide, wide, at, inv), rotary(wide.contiguous(), wide.contiguous(), at, inv)))
+
+
+def test_gradients_of_broadcast_heads():
+    """A key head expanded over five: its gradient is the sum of theirs."""
+    from metis_hip import rotary
+    g = torch.Generator().manual_seed(4)
+    q, k = torch.randn(11, 5, 64, generator=g).cuda().requires_grad_(), torch.randn(11, 1, 64, generator=g).cuda().requires_grad_()
+    at, inv = torch.arange(11).cuda(), frequencies(32)
+    gq, gk = torch.randn(11, 5, 64, generator=g).cuda(), torch.randn(11, 5, 64, generator=g).cuda()
+    got = torch.autograd.grad(rotary(q, k.expand(11, 5, 64), at, inv), (q, k), (gq, gk))
+    with torch.no_grad():
+        want, mag = turned(gk, at, inv, False, 1.0, True)
+        near(got[0], *turned(gq, at, inv, False, 1.0, True))
+        assert bool(((got[1].double() - want.sum(1, keepdim=True)).abs() <= 2.0 ** -18 * mag.sum(1, keepdim=True)).all())
+
+
+def test_one_result_used():
+    from metis_hip import rotary
+    g = torch.Generator().manual_seed(5)
+    q, k, w = (torch.randn(9, h, 64, generator=g).to(BF).cuda().requires_grad_() for h in (4, 2, 4))
+    at, inv = torch.arange(9).cuda(), frequencies(16)
+    both = torch.autograd.grad(rotary(q, k, at, inv), (q, k), (w.detach(), k.detach()))
+    (alone,) = torch.autograd.grad(rotary(q, k, at, inv)[0], q, w.detach())
+    assert torch.equal(alone, both[0])
+    (alone,) = torch.autograd.grad(rotary(q, k.detach(), at, inv)[0], q, w.detach())
+    assert torch.equal(alone, both[0])
+    (alone,) = torch.autograd.grad(rotary(q.detach(), k, at, inv)[1], k, k.detach())
+    assert torch.equal(alone, both[1])
+
+
+def test_gradients_against_differences():
+    """The derivative along a direction, by central differences in binary32: the operator is linear in its operands, so what they are off by is rounding alone, 2^-18 of
+    the magnitudes over the step."""
+    from metis_hip import rotary
+    g = torch.Generator().manual_seed(6)
+    q, k, dq, dk, gq, gk = (torch.randn(13, h, 40, generator=g).cuda() for h in (3, 2, 3, 2, 3, 2))
+    at, inv = (1000 * torch.arange(13)).cuda(), frequencies(20)
+    q, k = q.requires_grad_(), k.requires_grad_()
+    grads = torch.autograd.grad(rotary(q, k, at, inv, interleaved=True, factor=1.5), (q, k), (gq, gk))
+    with torch.no_grad():
+        along = sum(float((a.double() * b.double()).sum()) for a, b in zip(grads, (dq, dk)))
+        ends = []
+        for h in (0.5, -0.5):
+            out = rotary(q + h * dq, k + h * dk, at, inv, interleaved=True, factor=1.5)
+            ends.append(sum((a.double() * b.double()).sum() for a, b in zip(out, (gq, gk))))
+        mag = sum(float((a.abs() * (b.abs() + c.abs())).sum()) for a, b, c in ((gq, q, dq), (gk, k, dk)))
+        assert abs(float(ends[0] - ends[1]) - along) <= 2.0 ** -18 * 2 * 1.5 * 2 * mag
+
+
+def test_turned_back_and_lengths_kept():
+    """Turned by a position and by its negative is where it was, within twice the bound; a single column pair turned by a quarter comes out exactly there."""
+    from metis_hip import ops
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(64, 4, 128, generator=g).cuda()
+    at, inv = torch.randint(-(1 << 20), 1 << 20, (64,), generator=g).cuda(), frequencies(64)
+    y, _ = ops.rotary(x, x, at, inv)
+    z, _ = ops.rotary(y, y, -at, inv)
+    mag = x.double().abs()[..., :64] + x.double().abs()[..., 64:]
+    assert bool(((z.double() - x.double()).abs() <= 2.0 ** -17 * torch.cat((mag, mag), -1)).all())
+    back, _ = ops.rotary(y, y, at, inv, back=True)
+    assert torch.equal(back, z)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.float64])
+def test_a_models_own_frequencies(dt):
+    from metis_hip import rotary
+    g = torch.Generator().manual_seed(8)
+    q, k = torch.randn(50, 4, 128, generator=g).to(BF).cuda(), torch.randn(50, 2, 128, generator=g).to(BF).cuda()
+    inv, at = frequencies(64, 1e6, dt), (131072 + torch.arange(50)).cuda()
+    for got, x in zip(rotary(q, k, at, inv), (q, k)):
+        near(got, *turned(x, at, inv, False, 1.0))
+
+
+def test_no_tokens_and_refusals():
+    from metis_hip import rotary
+    inv, at = frequencies(32), torch.arange(5).cuda()
+    for grad in (False, True):
+        q, k = torch.zeros(0, 4, 64, device="cuda", requires_grad=grad), torch.zeros(0, 2, 64, device="cuda")
+        out = rotary(q, k, at[:0], inv)
+        assert out[0].shape == q.shape and out[1].shape == k.shape
+    q, k = torch.zeros(5, 4, 64, device="cuda", dtype=BF), torch.zeros(5, 2, 64, device="cuda", dtype=BF)
+    for args in ((q, k.float(), at, inv), (q.half(), k.half(), at, inv), (q, k[:4], at, inv), (q, k, at[:4], inv), (q, k, at.int(), inv), (q, k, at, inv.half()), (q, k, at, inv[:, None]),
+                 (q, k, at, torch.cat((inv, inv))), (q, k, at, inv[:0]), (q, k, at, torch.stack((inv, inv), 1)[:, 0]), (q[..., :63], k[..., :63], at, inv[:31]), (q[0], k[0], at, inv),
+                 (q, k[..., :32], at, inv), (q, k, at, inv.cpu()), (q, k, at.cpu(), inv), (q[:, :0], k, at, inv)):
+        for leaf in (args[0], args[0].detach().clone().requires_grad_()):
+            with pytest.raises(ValueError):
+                rotary(leaf, *args[1:])
+    with pytest.raises(ValueError, match="inv_freq"):
+        rotary(q, k, at, inv.clone().requires_grad_())
+
+
+def test_not_a_number_stays_in_its_pair():
+    from metis_hip import rotary
+    q = torch.ones(3, 2, 64, device="cuda", dtype=BF)
+    q[1, 0, 3] = float("nan")
+    y, _ = rotary(q, q, torch.arange(3).cuda(), frequencies(16))
+    bad = torch.zeros_like(y, dtype=torch.bool)
+    bad[1, 0, 3] = bad[1, 0, 19] = True
+    assert torch.equal(y.isnan(), bad)
+
+
+def test_streams_graphs_traces_and_second_derivatives():
+    """Another stream's bits; replays of a captured forward and backward on changed values; a recorded trace; what is refused."""
+    import torch.autograd.forward_ad as fwd
+    from metis_hip import rotary
+    g = torch.Generator().manual_seed(9)
+    inv = frequencies(64)
+
+    def values():
+        return [torch.randn(2, 65, h, 128, generator=g).to(BF).cuda() for h in (6, 2, 6, 2)] + [torch.randint(0, 5000, (2, 65), generator=g).cuda()]
+
+    def step(q, k, gq, gk, at):
+        y = rotary(q, k, at, inv)
+        return [*(t.detach() for t in y), *torch.autograd.grad(y, (q, k), (gq, gk))]
+
+    def eager(q, k, *more):
+        return step(q.detach().clone().requires_grad_(), k.detach().clone().requires_grad_(), *more)
+
+    held = values()
+    want = eager(*held)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        got = eager(*held)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    held[0].requires_grad_(), held[1].requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*held)
+    for _ in range(3):
+        with torch.no_grad():
+            for a, b in zip(held, values()):
+                a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager(*held)))
+    q, k, gq, gk, at = values()
+    traced = torch.jit.trace(lambda q, k, at: rotary(q, k, at, inv), (q.clone().requires_grad_(), k, at), check_trace=False)
+    q, k, gq, gk, at = values()
+    q.requires_grad_()
+    results = []
+    for run in (traced, lambda q, k, at: rotary(q, k, at, inv)):
+        y = run(q, k, at)
+        results.append([y[0].detach(), y[1].detach(), *torch.autograd.grad(y[0], q, gq)])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    first, = torch.autograd.grad(rotary(q, k, at, inv)[0].float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        first.float().sum().backward()
+    with fwd.dual_level(), pytest.raises(NotImplementedError, match="jvp"):
+        rotary(fwd.make_dual(q, torch.ones_like(q)), k, at, inv)
+
+
+def test_beyond_32_bits_of_elements():
+    """2^32 elements and more of queries, the same rows again and again."""
+    from metis_hip import ops
+    rows, times = 4096, 260
+    g = torch.Generator(device="cuda").manual_seed(10)
+    q = torch.randn(rows, 32, 128, generator=g, device="cuda").to(BF)
+    at, inv = torch.arange(rows, device="cuda"), frequencies(64)
+    want, _ = ops.rotary(q, q[:, :1], at, inv)
+    many = q.repeat(times, 1, 1)
+    assert many.numel() > 1 << 32
+    got, _ = ops.rotary(many.view(times, rows, 32, 128), many.view(times, rows, 32, 128)[:, :, :1], at, inv)
+    assert all(torch.equal(got[i], want) for i in range(times))
+    del many, got
+    torch.cuda.empty_cache()

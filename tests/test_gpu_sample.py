@@ -1,0 +1,245 @@
+"""sample_tokens on the device against its definition in 64 bits: equal tokens.
+
+A token may differ from the definition's only where the random number's goal, or a threshold, lies within the weights' error of a border: weights and sums are accurate to
+2^-40 or better, so over the thousands of rows here with some 10^5 borders each that is not to be expected.  Log-probabilities are rounded to binary32 once: half a
+step, and 2^-40 of the magnitudes."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def definition(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(tokens, log-probabilities) in 64 bits; the settings numbers or vectors."""
+    rows, V = logits.shape
+    def column(s):
+        return torch.as_tensor(s, dtype=torch.float64, device=logits.device).expand(rows)[:, None]
+    temperature, top_k, top_p, min_p = map(column, (temperature, top_k, top_p, min_p))
+    x = logits.double()
+    ranked, order = torch.sort(x, dim=1, descending=True, stable=True)
+    w = torch.where(ranked == ranked[:, :1], 1.0, torch.exp((ranked - ranked[:, :1]) / temperature))
+    rank = torch.arange(V, device=logits.device)
+    keep = (rank < top_k) | (top_k == 0)
+    upto = torch.cumsum(torch.where(keep, w, 0.0), 1)
+    before = torch.nn.functional.pad(upto[:, :-1], (1, 0))
+    keep &= (before < top_p * upto[:, -1:]) | (top_p >= 1.0)
+    keep &= w >= min_p
+    upto = torch.cumsum(torch.zeros_like(x).scatter_(1, order, torch.where(keep, w, 0.0)), 1)
+    tokens = torch.searchsorted(upto, uniforms.double()[:, None] * upto[:, -1:], right=True)
+    place = (order == tokens).double().argmax(1, keepdim=True)
+    logp = torch.log(w.gather(1, place)) - torch.log(w.sum(1, keepdim=True))
+    empty = ranked[:, 0] == -torch.inf                                 # (binary32's lowest number is -inf in bf16)
+    return torch.where(empty, -1, tokens[:, 0]), torch.where(empty, torch.nan, logp[:, 0])
+
+
+def check(logits, uniforms, **settings):
+    from metis_hip import sample_tokens
+    tokens, logp = sample_tokens(logits, uniforms, **settings)
+    rows, V = uniforms.numel(), logits.shape[-1]
+    assert tokens.shape == logp.shape == uniforms.shape and tokens.dtype == torch.int64 and logp.dtype == F32
+    want, want_logp = definition(logits.reshape(rows, V), uniforms.reshape(rows), **{k: s.reshape(rows) if isinstance(s, torch.Tensor) else s for k, s in settings.items()})
+    off = tokens.reshape(rows) != want
+    assert not bool(off.any()), (settings, tokens.reshape(rows)[off][:5], want[off][:5], uniforms.reshape(rows)[off][:5])
+    bound = 2.0 ** -24 * want_logp.abs() + 2.0 ** -38 * (want_logp.abs() + 1 + math.log(V))
+    assert bool((((logp.reshape(rows).double() - want_logp).abs() <= bound) | (want_logp.isnan() & logp.reshape(rows).isnan())).all())
+    return tokens, logp
+
+
+def rows_of(seed, rows, V, dtype, spread=2.0, peaks=6):
+    g = torch.Generator().manual_seed(seed)
+    x = spread * torch.randn(rows, V, generator=g)
+    if peaks:
+        x.scatter_add_(1, torch.randint(V, (rows, peaks), generator=g), 8 * torch.rand(rows, peaks, generator=g))
+    return x.to(dtype).cuda(), torch.rand(rows, generator=g).cuda()
+
+
+SETTINGS = [dict(), dict(temperature=0.6), dict(top_k=1), dict(top_k=50), dict(top_p=0.9), dict(min_p=0.05), dict(temperature=1.7, top_k=300, top_p=0.8, min_p=0.001), dict(top_p=1e-9),
+            dict(top_p=0.999999), dict(top_k=7, top_p=0.5), dict(min_p=1.0), dict(temperature=1e-3), dict(temperature=50.0, top_p=0.7), dict(top_k=10 ** 9, top_p=2.0)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,V", [(40, 1), (40, 2), (40, 7), (200, 64), (60, 1000), (33, 4096), (20, 32003), (9, 131072)])
+def test_against_the_definition(rows, V, dtype):
+    logits, u = rows_of(rows + V, rows, V, dtype)
+    for settings in SETTINGS:
+        check(logits, u, **settings)
+
+
+def test_the_whole_range_of_the_random_number():
+    """One row's distribution under 4097 numbers from 0 to the largest below 1."""
+    u = torch.arange(4097, dtype=torch.float32) / 4097
+    u[-1] = 1 - 2.0 ** -24
+    for dtype, V in ((BF, 501), (F32, 501), (F32, 20001)):
+        logits, _ = rows_of(V, 1, V, dtype)
+        for settings in (dict(), dict(top_k=20), dict(top_p=0.9), dict(min_p=0.1)):
+            tokens, _ = check(logits.expand(4097, V), u.cuda(), **settings)
+            assert bool((tokens[1:] >= tokens[:-1]).all())
+
+
+def test_equal_logits():
+    """Ties go to the lower index, however many there are: rows of one value, of two, of a few, with more of them than are sorted at once."""
+    for V in (3, 100, 2048, 2049, 5000, 70001):
+        g = torch.Generator().manual_seed(V)
+        u = torch.rand(16, generator=g).cuda()
+        for values in ((0.0,), (1.5, -0.25), (0.0, -0.0), (3.0, 2.9, 2.8, -1.0)):
+            logits = torch.tensor(values)[torch.randint(len(values), (16, V), generator=g)].cuda()
+            for settings in (dict(), dict(top_k=max(1, V // 3)), dict(top_p=0.37), dict(top_k=max(1, V // 2), top_p=0.61), dict(top_k=2), dict(min_p=0.9)):
+                check(logits, u, **settings)
+                check(logits.to(BF), u, **settings)
+
+
+@pytest.mark.parametrize("scale", [1e-6, 1e-3, 0.02, 1e4, 1e30])
+def test_flat_and_steep_rows(scale):
+    """Logits that all lie in one bin (an untrained head's), and such that all but one have no weight left."""
+    for V in (300, 40000):
+        g = torch.Generator().manual_seed(V)
+        logits, u = (scale * torch.randn(8, V, generator=g)).cuda(), torch.rand(8, generator=g).cuda()
+        for settings in (dict(), dict(top_k=V // 5), dict(top_p=0.83), dict(top_k=V // 2, top_p=0.5), dict(top_k=2500, top_p=0.9), dict(min_p=0.3)):
+            check(logits, u, **settings)
+            check(logits.to(BF), u, **settings)
+
+
+def test_masked_and_infinite_logits():
+    from metis_hip import sample_tokens
+    inf = float("inf")
+    logits, u = rows_of(5, 12, 3001, F32)
+    masked = logits.clone()
+    masked[:, 100:] = -inf
+    masked[1], masked[1, 2999] = -inf, -5.0
+    masked[2, :99] = torch.finfo(F32).min
+    masked[3] = torch.finfo(F32).min
+    for settings in (dict(), dict(top_k=50), dict(top_k=2000), dict(top_p=0.9), dict(min_p=0.01), dict(top_k=500, top_p=0.99)):
+        tokens, _ = check(masked, u, **settings)
+        assert int(tokens[1]) == 2999 and bool((tokens[[0, *range(4, 12)]] < 100).all())
+        check(masked.to(BF), u, **settings)
+    some = logits.clone()
+    some[:, ::1000] = inf                                              # all the weight, evenly
+    tokens, logp = sample_tokens(some, u)
+    assert torch.equal(tokens, 1000 * (u * 4).long()) and bool((logp + math.log(4)).abs().max() < 2.0 ** -20)
+    tokens, _ = sample_tokens(some, u, top_k=2, top_p=0.9)
+    assert torch.equal(tokens, 1000 * (u * 2).long())
+    none = logits.clone()
+    none[0], none[3, 7], none[5] = -inf, float("nan"), float("nan")
+    want = sample_tokens(logits, u, top_p=0.9)
+    got = sample_tokens(none, u, top_p=0.9)
+    bad = torch.zeros(12, dtype=torch.bool, device="cuda")
+    bad[[0, 3, 5]] = True
+    assert bool((got[0][bad] == -1).all()) and bool(got[1][bad].isnan().all())
+    assert torch.equal(got[0][~bad], want[0][~bad]) and torch.equal(got[1][~bad], want[1][~bad])
+
+
+def test_settings_for_each_row():
+    """Tensors of any number type in any of the settings, numbers beside them; rows with settings or numbers out of range say so and leave the others alone."""
+    from metis_hip import sample_tokens
+    g = torch.Generator().manual_seed(6)
+    logits, u = rows_of(6, 32, 5003, BF)
+    t, k, p, m = (0.5 + torch.rand(32, generator=g)).cuda(), torch.randint(0, 60, (32,), generator=g).cuda(), (0.3 + 0.7 * torch.rand(32, generator=g).double()).cuda(), (0.1 * torch.rand(32, generator=g)).cuda()
+    check(logits, u, temperature=t, top_k=k, top_p=p, min_p=m)
+    check(logits, u, temperature=t)
+    check(logits, u, top_k=k.int(), top_p=0.9)
+    check(logits, u, top_p=p, min_p=0.01, temperature=0.8)
+    whole = sample_tokens(logits, u, temperature=0.5, top_k=40, top_p=0.9, min_p=0.01)
+    full = torch.full((32,), 0.5, device="cuda")
+    assert all(torch.equal(a, b) for a, b in zip(whole, sample_tokens(logits, u, temperature=full, top_k=40, top_p=0.9, min_p=0.01)))
+    nan, inf = float("nan"), float("inf")
+    for name, bads in (("temperature", (0.0, -1.0, nan, inf)), ("top_k", (-1.0, nan)), ("top_p", (0.0, -0.5, nan)), ("min_p", (-0.1, 1.5, nan))):
+        good = {"temperature": 0.5, "top_k": 40.0, "top_p": 0.9, "min_p": 0.01}
+        column = torch.full((32,), good[name], dtype=torch.float64, device="cuda")
+        column[:len(bads)] = torch.tensor(bads, dtype=torch.float64)
+        tokens, logp = sample_tokens(logits, u, **{**good, name: column, "top_k": column if name == "top_k" else 40})
+        assert bool((tokens[:len(bads)] == -1).all()) and bool(logp[:len(bads)].isnan().all())
+        assert torch.equal(tokens[len(bads):], whole[0][len(bads):]) and torch.equal(logp[len(bads):], whole[1][len(bads):])
+    odd = u.clone()
+    odd[:4] = torch.tensor([1.0, -1e-9, nan, inf])
+    tokens, logp = sample_tokens(logits, odd)
+    assert bool((tokens[:4] == -1).all()) and bool(logp[:4].isnan().all()) and torch.equal(tokens[4:], sample_tokens(logits, u)[0][4:])
+
+
+def test_shapes_strides_and_alignment():
+    from metis_hip import sample_tokens
+    g = torch.Generator().manual_seed(7)
+    for dtype in (BF, F32):
+        wide = (3 * torch.randn(6, 1511, generator=g)).to(dtype).cuda()
+        u = torch.rand(6, generator=g).cuda()
+        for first in (0, 1, 3, 4, 8):
+            part = wide[:, first:first + 1499]
+            tokens, logp = check(part, u, top_p=0.95)
+            dense = sample_tokens(part.contiguous(), u, top_p=0.95)
+            assert torch.equal(tokens, dense[0]) and torch.equal(logp, dense[1])
+        check(wide[::2], u[::2].contiguous(), top_k=30)
+        check(wide.t().contiguous().t(), u, top_k=30)
+        check(wide.view(2, 3, 1511), u.view(2, 3), top_p=0.9)
+        check(wide.view(2, 3, 1511), u.view(2, 3), top_p=0.9, temperature=(0.5 + u).view(2, 3))
+        check(wide[:1].expand(6, 1511), u)
+        one = sample_tokens(wide[0], u[0])
+        assert one[0].shape == () and int(one[0]) == int(sample_tokens(wide[:1], u[:1])[0])
+    empty = sample_tokens(torch.zeros(0, 50, device="cuda"), torch.zeros(0, device="cuda"))
+    assert empty[0].shape == (0,) and empty[0].dtype == torch.int64 and empty[1].shape == (0,)
+
+
+def test_equal_calls_streams_and_graphs():
+    """The same inputs give the same bits, on any stream and in replays on changed logits, numbers and settings."""
+    from metis_hip import sample_tokens
+    logits, u = rows_of(8, 50, 30011, BF)
+    t = (0.5 + torch.rand(50, generator=torch.Generator().manual_seed(8))).cuda()
+    want = sample_tokens(logits, u, temperature=t, top_k=900, top_p=0.97)
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got.append(sample_tokens(logits, u, temperature=t, top_k=900, top_p=0.97))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for run in got for a, b in zip(run, want))
+    held = logits.clone(), u.clone(), t.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = sample_tokens(held[0], held[1], temperature=held[2], top_k=900, top_p=0.97)
+    for k in range(3):
+        new = rows_of(20 + k, 50, 30011, BF)
+        held[0].copy_(new[0]), held[1].copy_(new[1]), held[2].add_(0.1)
+        graph.replay()
+        eager = sample_tokens(held[0], held[1], temperature=held[2], top_k=900, top_p=0.97)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+def test_the_largest_vocabulary():
+    logits, u = rows_of(9, 3, 1 << 22, F32)
+    for settings in (dict(), dict(top_k=100000, top_p=0.9), dict(top_p=0.5), dict(min_p=0.01)):
+        check(logits, u, **settings)
+    flat = torch.zeros(2, 1 << 22, device="cuda")
+    check(flat, u[:2], top_p=0.6)
+
+
+def test_beyond_32_bits_of_elements():
+    from metis_hip import sample_tokens
+    rows = 33000
+    logits, _ = rows_of(10, 64, 131072, BF)
+    many = logits.repeat(rows // 64 + 1, 1)
+    u = torch.rand(many.shape[0], generator=torch.Generator().manual_seed(10)).cuda()
+    assert many.numel() > 1 << 32
+    u[-64:] = u[:64]
+    tokens, logp = sample_tokens(many, u, top_p=0.9)
+    assert torch.equal(tokens[-64:], tokens[:64]) and torch.equal(logp[-64:], logp[:64])
+    check(logits, u[:64].contiguous(), top_p=0.9)
+    del many
+    torch.cuda.empty_cache()
+
+
+def test_refusals():
+    from metis_hip import MetisHipError, sample_tokens
+    logits, u = rows_of(11, 4, 100, F32)
+    for args, more in (((logits.half(), u), {}), ((logits, u.double()), {}), ((logits, u[:3]), {}), ((logits[:, :0], u), {}), ((logits, u), dict(temperature=0.0)), ((logits, u), dict(temperature=-1.0)),
+                       ((logits, u), dict(temperature=float("nan"))), ((logits, u), dict(top_k=-1)), ((logits, u), dict(top_p=0.0)), ((logits, u), dict(top_p=float("nan"))),
+                       ((logits, u), dict(min_p=1.1)), ((logits, u), dict(min_p=-0.1)), ((logits, u), dict(temperature=u[:3])), ((logits, u), dict(top_p=u.cpu())), ((logits, u.cpu()), {}),
+                       ((logits.requires_grad_(), u), {})):
+        with pytest.raises(ValueError):
+            sample_tokens(*args, **more)
+        logits = logits.detach()
+    with pytest.raises(MetisHipError, match="no CPU path"):
+        sample_tokens(logits.cpu(), u.cpu())
+    with torch.no_grad():
+        sample_tokens(logits.requires_grad_(), u)
