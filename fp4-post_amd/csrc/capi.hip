@@ -718,10 +718,12 @@ int metis_cache_copy_pages(void* keys, void* values, int64_t layers, int64_t pag
     return copy_pages(keys, values, layers, pages, page_bytes, sources, destinations, count, (hipStream_t)stream);
 }
 
+size_t metis_sample_tokens_workspace_bytes(int64_t rows, int64_t vocab) { return sample_tokens_workspace_bytes(rows, vocab); }
+
 int metis_sample_tokens(const void* logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const float* uniforms, const double* parameters, const double* row_parameters,
-                        int64_t* tokens, float* logprobs, void* stream)
+                        int64_t* tokens, float* logprobs, void* workspace, size_t workspace_bytes, void* stream)
 {
-    return sample_tokens(logits, ld, dtype, rows, vocab, uniforms, parameters, row_parameters, tokens, logprobs, (hipStream_t)stream);
+    return sample_tokens(logits, ld, dtype, rows, vocab, uniforms, parameters, row_parameters, tokens, logprobs, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

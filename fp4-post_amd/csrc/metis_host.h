@@ -145,8 +145,9 @@ int paged_attention(const void* q, int64_t q_seq, int64_t q_head, int64_t seqs, 
                     float value_scale, void* out, void* workspace, size_t workspace_bytes, hipStream_t st);
 int copy_pages(void* keys, void* values, int64_t layers, int64_t pages, int64_t page_bytes, const int64_t* from, const int64_t* to, int64_t count, hipStream_t st);
 // a token of each row's distribution by a given random number; sample.hip
+size_t sample_tokens_workspace_bytes(int64_t rows, int64_t vocab);
 int sample_tokens(const void* logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const float* uniforms, const double* parameters, const double* row_parameters,
-                  int64_t* tokens, float* logprobs, hipStream_t st);
+                  int64_t* tokens, float* logprobs, void* workspace, size_t workspace_bytes, hipStream_t st);
 int gemm_nvfp4(const void* a_codes, const void* a_scales, const float* a_unit, const void* b_codes, const void* b_scales,
                const float* b_unit, int64_t M, int64_t N, int64_t K, const void* t, const void* u, int64_t r,
                const void* bias, void* out, int out_dtype, hipStream_t st, void* workspace = nullptr,

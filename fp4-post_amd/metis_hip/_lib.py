@@ -142,7 +142,8 @@ SIGNATURES = {
     "metis_paged_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
     "metis_paged_attention": (_i32, [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _f32, _f32, _f32, _vp, _vp, _sz, _vp]),
     "metis_cache_copy_pages": (_i32, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
-    "metis_sample_tokens": (_i32, [_vp, _i64, _i32, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "metis_sample_tokens_workspace_bytes": (_sz, [_i64, _i64]),
+    "metis_sample_tokens": (_i32, [_vp, _i64, _i32, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 
 _lib = None

@@ -1731,6 +1731,11 @@ def copy_pages(keys: torch.Tensor, values: torch.Tensor, sources, destinations) 
 
 
 @functools.lru_cache(maxsize=4096)
+def _sample_bytes(rows: int, V: int, device_index: int) -> int:
+    return int(load().metis_sample_tokens_workspace_bytes(rows, V))         # depends on the device's CU count only
+
+
+@functools.lru_cache(maxsize=4096)
 def _sample_parameters(*settings: float) -> ctypes.Array:
     return (ctypes.c_double * 4)(*settings)
 
@@ -1746,12 +1751,12 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
         raise ValueError(f"sample_tokens: uniforms are float32 {tuple(lead)}, not {uniforms.dtype} {tuple(uniforms.shape)}")
     settings = (temperature, top_k, top_p, min_p)
     each = any(isinstance(s, torch.Tensor) for s in settings)
-    for name, s, ok in zip(("temperature", "top_k", "top_p", "min_p"), settings, (lambda s: 0.0 < s < float("inf"), lambda s: s >= 0, lambda s: s > 0.0, lambda s: 0.0 <= s <= 1.0)):
+    for name, s, ok in zip(("temperature", "top_k", "top_p", "min_p"), settings, (lambda s: 0.0 < s <= 2.0 ** 64, lambda s: s >= 0, lambda s: s > 0.0, lambda s: 0.0 <= s <= 1.0)):
         if isinstance(s, torch.Tensor):
             if s.shape != lead or s.device != logits.device or s.is_complex():
                 raise ValueError(f"sample_tokens: {name} is a number, or a tensor {tuple(lead)} on the logits' device, not {tuple(s.shape)} on {s.device}")
         elif not ok(s):
-            raise ValueError(f"sample_tokens: temperature is positive, top_k at least 0 (all), top_p positive, min_p from 0 to 1: not {name} = {s}")
+            raise ValueError(f"sample_tokens: temperature is positive (up to 2^64), top_k at least 0 (all), top_p positive, min_p from 0 to 1: not {name} = {s}")
     rows = uniforms.numel()
     if rows == 0:
         return torch.empty(lead, dtype=torch.int64, device=logits.device), torch.empty(lead, dtype=torch.float32, device=logits.device)
@@ -1764,11 +1769,12 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
                                    for s in settings], -1).contiguous(), None
     else:
         own, common = None, _sample_parameters(*map(float, settings))
-    new = _lib.call("metis_sample_tokens", logits.get_device(), ((I64, *lead), (F32, *lead)),
-                    (x, x.stride(0) if rows > 1 else V, dt, rows, V, uniforms.contiguous(), common and ctypes.addressof(common), own, "0", "1", _stream()))
+    need = _sample_bytes(rows, V, logits.get_device())
+    new = _lib.call("metis_sample_tokens", logits.get_device(), ((I64, *lead), (F32, *lead), (U8, need)),
+                    (x, x.stride(0) if rows > 1 else V, dt, rows, V, uniforms.contiguous(), common and ctypes.addressof(common), own, "0", "1", "2", need, _stream()))
     if new.__class__ is int:
         check(new, "metis_sample_tokens", logits.shape)
-    return new
+    return new[:2]
 
 
 @functools.lru_cache(maxsize=16)

@@ -1097,17 +1097,21 @@ int metis_cache_copy_pages(void *keys, void *values, int64_t layers, int64_t pag
  *   K3  those of K2 with w >= min_p
  *   token = the lowest index i in K3 with sum_{j <= i, j in K3} w_j > u sum(K3),
  *   logprob = log w_token - log sum_i w_i, over all tokens: its log-probability under softmax(x / temperature)
- * Weights and sums in 64 bits; the same inputs give the same token always.
+ * Weights and sums in 64 bits (with top_k the sum in logprob, of all tokens, in binary32: within 2^-18 of the value in 64
+ * bits); the same inputs give the same results always.
  *   logits      bf16 or float [rows, vocab], row stride ld; vocab up to 2^22.  -inf: never drawn
  *   uniforms    float [rows] in [0, 1)
- *   parameters  HOST double[4]: temperature > 0, top_k >= 0, top_p > 0, min_p in [0, 1]; or row_parameters, device
+ *   parameters  HOST double[4]: 0 < temperature <= 2^64, top_k >= 0, top_p > 0, min_p in [0, 1]; or row_parameters, device
  *               double [rows, 4], which is then used in its place
+ *   workspace   metis_sample_tokens_workspace_bytes(rows, vocab) bytes (0: none), no initialisation needed
  *   A row without a finite or infinite largest logit (all -inf, or a NaN), or with parameters or a number outside their
  *   ranges, has token -1 and logprob NaN.
  */
+size_t metis_sample_tokens_workspace_bytes(int64_t rows, int64_t vocab);
 int metis_sample_tokens(const void *logits, int64_t ld, int dtype, int64_t rows, int64_t vocab,
                         const float *uniforms, const double *parameters,
-                        const double *row_parameters, int64_t *tokens, float *logprobs, void *stream);
+                        const double *row_parameters, int64_t *tokens, float *logprobs,
+                        void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

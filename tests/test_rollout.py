@@ -90,9 +90,9 @@ def test_copies_refuse_before_a_launch():
 def test_sampling_refuses_before_a_launch():
     L = _lib.load()
 
-    def call(parameters=(1.0, 0.0, 1.0, 0.0), logits=4096, ld=100, dtype=1, rows=4, vocab=100, uniforms=4096, each=None, tokens=4096, logprobs=4096):
+    def call(parameters=(1.0, 0.0, 1.0, 0.0), logits=4096, ld=100, dtype=1, rows=4, vocab=100, uniforms=4096, each=None, tokens=4096, logprobs=4096, workspace=4096, size=1 << 24):
         p = None if parameters is None else ctypes.cast((ctypes.c_double * 4)(*parameters), ctypes.c_void_p)
-        return L.metis_sample_tokens(logits, ld, dtype, rows, vocab, uniforms, p, each, tokens, logprobs, None)
+        return L.metis_sample_tokens(logits, ld, dtype, rows, vocab, uniforms, p, each, tokens, logprobs, workspace, size, None)
 
     nan = float("nan")
     for more in (dict(logits=None), dict(logits=4098), dict(ld=99), dict(ld=-1), dict(dtype=2), dict(rows=-1), dict(rows=1 << 32), dict(vocab=0), dict(vocab=(1 << 22) + 1, ld=1 << 23), dict(uniforms=None),
