@@ -22,9 +22,9 @@ struct AttendArgs {
     const void *q, *keys, *values;
     const int *tables, *lengths;
     void* out;
-    float* partial;                                                // [pair, tile, split][16 heads][dim + 2]: sums, then maximum and sum of the weights
+    float *sums, *stats;                                           // of splits: [seq, head, split][dim], and [seq, head, split][2]: maximum and sum of the weights
     int64_t q_seq, q_head, table_stride;
-    int q_heads, kv_heads, group, pages, page_shift, width, splits, chunk, tiles;
+    int q_heads, kv_heads, group, pages, page_shift, width, splits, chunk, tiles, pairs;
     float scale, value_scale;                                      // scale: of the scores, with log2 e
 };
 
@@ -44,8 +44,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(const AttendArgs
     constexpr int D = 32 * DT, S = TOK / 32, T = TOK / 16, NV = D / 16;
     constexpr bool WIDE = F8 && TOK == 64;                         // sixteen neighbouring tokens to a lane, one 16-byte load of values for both steps; else eight a step
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    const int split = blockIdx.x % a.splits;
-    int rest = blockIdx.x / a.splits;
+    // the splits of all sequences one after the other: neighbouring workgroups, which lie on different XCDs, have the same split of other sequences and heads, so that a
+    // ragged batch's late splits, which only the long sequences have, do not leave XCDs without work
+    const int split = blockIdx.x / a.pairs;
+    int rest = blockIdx.x - split * a.pairs;
     const int tile = rest % a.tiles;
     rest /= a.tiles;
     const int kv = rest % a.kv_heads, seq = rest / a.kv_heads;
@@ -76,39 +78,63 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(const AttendArgs
     const char* values = static_cast<const char*>(a.values) + kv * head_bytes;
     const int mask = (1 << a.page_shift) - 1;
 
+    // The pages of a block are asked for a block ahead (the first one's before anything is known of the length): KP of a lane's keys, VL of its values.  A run of eight
+    // tokens (WIDE: sixteen) lies in one page.
+    constexpr int KP = WIDE ? 1 : S, VL = WIDE ? 1 : S, VW = F8 && !WIDE ? 2 : 4;              // VL: loads of a dimension too, and their words
+    const int r = n >> 2, last = a.width - 1;
+    int kpage[KP], vpage[VL];
+    const auto ask = [&](int t0) {
+#pragma unroll
+        for (int s = 0; s < KP; ++s) kpage[s] = table[max(min((t0 + (WIDE ? 16 * r : 32 * s + 8 * r)) >> a.page_shift, last), 0)];
+#pragma unroll
+        for (int s = 0; s < VL; ++s) vpage[s] = table[max(min((t0 + (WIDE ? 16 * g : 32 * s + 8 * g)) >> a.page_shift, last), 0)];
+    };
+    if (last >= 0) ask(begin + wave * TOK);
+
     for (int t0 = begin + wave * TOK; t0 < end; t0 += kWaves * TOK) {
-        uint32_t bad = 0;                                          // bit t: the page of this lane's key of tile t is none
-        uint4 kx[T][F8 ? DT / 2 : DT];
+        uint32_t bad = 0;                                          // bit s: the page of this lane's s-th run of keys is none
+        size_t kat[KP], vat[VL];
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-            const int r = n >> 2, j = n & 3;
-            const int tok = t0 + (WIDE ? 16 * r + 4 * t + j : 32 * (t >> 1) + 8 * r + 4 * (t & 1) + j);
-            int page = tok < end ? table[tok >> a.page_shift] : 0;
-            if ((uint32_t)page >= (uint32_t)a.pages) { page = 0; bad |= 1u << t; }
-            const char* row = keys + (size_t)page * page_bytes + (size_t)(tok & mask) * (D * unit);
-#pragma unroll
-            for (int c = 0; c < (F8 ? DT / 2 : DT); ++c) kx[t][c] = *reinterpret_cast<const uint4*>(row + 64 * c + 16 * g);
+        for (int s = 0; s < KP; ++s) {
+            const int tok = t0 + (WIDE ? 16 * r : 32 * s + 8 * r);
+            const bool none = (uint32_t)kpage[s] >= (uint32_t)a.pages;
+            if (none && tok < end) bad |= 1u << s;
+            kat[s] = (size_t)(none || tok >= end ? 0 : kpage[s]) * page_bytes + (size_t)(tok & mask) * (D * unit);
         }
-        constexpr int VL = WIDE ? 1 : S, VW = F8 && !WIDE ? 2 : 4; // loads of a dimension, and their words
-        uint32_t vx[NV][VL][VW];
 #pragma unroll
         for (int s = 0; s < VL; ++s) {
             const int tok = t0 + (WIDE ? 16 * g : 32 * s + 8 * g);
-            int page = tok < end ? table[tok >> a.page_shift] : 0;
-            if ((uint32_t)page >= (uint32_t)a.pages) page = 0;
-            const char* col = values + (size_t)page * page_bytes + (size_t)(tok & mask) * unit;
+            vat[s] = (size_t)((uint32_t)vpage[s] >= (uint32_t)a.pages || tok >= end ? 0 : vpage[s]) * page_bytes + (size_t)(tok & mask) * unit;
+        }
+        uint4 kx[T][F8 ? DT / 2 : DT];
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const char* at = col + (((size_t)(16 * i + n) << a.page_shift) * unit);
-                if constexpr (VW == 4) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(at);
-                    vx[i][s][0] = w.x; vx[i][s][1] = w.y; vx[i][s][2] = w.z; vx[i][s][3] = w.w;
-                } else {
-                    const uint2 w = *reinterpret_cast<const uint2*>(at);
-                    vx[i][s][0] = w.x; vx[i][s][1] = w.y;
+        for (int t = 0; t < T; ++t) {
+            // the token of row n of score tile t: number n & 3 of four
+            const char* row = keys + kat[WIDE ? 0 : t >> 1] + (size_t)((WIDE ? 4 * t : 4 * (t & 1)) + (n & 3)) * (D * unit);
+#pragma unroll
+            for (int c = 0; c < (F8 ? DT / 2 : DT); ++c) kx[t][c] = *reinterpret_cast<const uint4*>(row + 64 * c + 16 * g);
+        }
+        uint32_t vx[NV][VL][VW];
+        constexpr bool LATE = DT == 8 && !F8;                      // (keys and values at once do not fit the registers)
+        const auto load_values = [&] {
+#pragma unroll
+            for (int s = 0; s < VL; ++s) {
+                const char* col = values + vat[s];
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const char* at = col + (((size_t)(16 * i + n) << a.page_shift) * unit);
+                    if constexpr (VW == 4) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(at);
+                        vx[i][s][0] = w.x; vx[i][s][1] = w.y; vx[i][s][2] = w.z; vx[i][s][3] = w.w;
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2*>(at);
+                        vx[i][s][0] = w.x; vx[i][s][1] = w.y;
+                    }
                 }
             }
-        }
+        };
+        if constexpr (!LATE) load_values();
+        ask(t0 + kWaves * TOK);
 
         float p[TOK / 4];                                          // scores, then weights, of the lane's tokens in their order
 #pragma unroll
@@ -124,6 +150,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(const AttendArgs
 #pragma unroll
             for (int j = 0; j < 4; ++j) p[4 * t + j] = acc[j] * a.scale;
         }
+        if constexpr (LATE) {
+            __builtin_amdgcn_sched_barrier(0);
+            load_values();
+        }
         // tokens behind the end have no weight; a token whose page is none makes the result NaN
         const bool tail = t0 + TOK > end;
         if (tail || __any(bad != 0)) {
@@ -133,7 +163,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(const AttendArgs
                 for (int j = 0; j < 4; ++j) {
                     const int tok = t0 + (WIDE ? 16 * g + 4 * t + j : 32 * (t >> 1) + 8 * g + 4 * (t & 1) + j);
                     const int from = 4 * g + j;                    // the lane that loaded this row's key
-                    const bool none = (__shfl((int)bad, from, 64) >> t) & 1;
+                    const bool none = (__shfl((int)bad, from, 64) >> (WIDE ? 0 : t >> 1)) & 1;
                     if (tok >= end) p[4 * t + j] = -INFINITY;
                     else if (none) p[4 * t + j] = __builtin_nanf("");
                 }
@@ -224,52 +254,65 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(const AttendArgs
             const float v = lie ? __builtin_nanf("") : length == 0 ? 0.0f : num / den * a.value_scale;
             static_cast<uint16_t*>(a.out)[((size_t)seq * a.q_heads + kv * a.group + tile * kHeadTile + head) * D + d] = (uint16_t)bf16_bits(v);
         } else {
-            float* to = a.partial + (((size_t)seq * a.q_heads + kv * a.group + tile * kHeadTile + head) * a.splits + split) * (D + 2);
-            to[d] = num;
+            const size_t row = ((size_t)seq * a.q_heads + kv * a.group + tile * kHeadTile + head) * a.splits + split;
+            a.sums[row * D + d] = num;
             if (d == 0) {
-                to[D] = top;
-                to[D + 1] = den;
+                a.stats[2 * row] = top;
+                a.stats[2 * row + 1] = den;
             }
         }
     }
 }
 
-// The splits' sums of one head together.
+// The splits' sums of one head together: a lane has four dimensions of every G-th split.  Bound by the way to memory and back, twice: the maxima, then the sums, eight splits
+// of a lane on their way at once.
+constexpr int kJoinThreads = 512;
 template <int DT>
-__global__ __launch_bounds__(256) void attend_join_kernel(const AttendArgs a)
+__global__ __launch_bounds__(kJoinThreads) void attend_join_kernel(const AttendArgs a)
 {
-    constexpr int D = 32 * DT, G = 256 / D > 0 ? 256 / D : 1;      // splits at a time
-    const int row = blockIdx.x, seq = row / a.q_heads;
+    constexpr int D = 32 * DT, LANES = D / 4, G = kJoinThreads / LANES;
+    const int row = blockIdx.x, seq = row / a.q_heads, tid = threadIdx.x;
     const int capacity = a.width << a.page_shift, said = a.lengths[seq], length = said < 0 ? 0 : said > capacity ? capacity : said;
     const int splits = max(1, (length + a.chunk - 1) / a.chunk);
-    const float* from = a.partial + (size_t)row * a.splits * (D + 2);
+    const float2* stats = reinterpret_cast<const float2*>(a.stats) + (size_t)row * a.splits;
+    const float4* sums = reinterpret_cast<const float4*>(a.sums) + (size_t)row * a.splits * LANES;
+    __shared__ float tops[kJoinThreads / 64], dens[G];
+    __shared__ float4 nums[G][LANES];
     float top = -INFINITY;
-    for (int s = threadIdx.x & 63; s < splits; s += 64) top = fmaxf(top, from[(size_t)s * (D + 2) + D]);
+    for (int s = tid; s < splits; s += kJoinThreads) top = fmaxf(top, stats[s].x);
     top = wave_max(top);
+    if ((tid & 63) == 0) tops[tid >> 6] = top;
+    __syncthreads();
+    top = tops[0];
+#pragma unroll
+    for (int i = 1; i < kJoinThreads / 64; ++i) top = fmaxf(top, tops[i]);
     const float base = top == -INFINITY ? 0.0f : top;
-    const int d = threadIdx.x % D, k = threadIdx.x / D;
-    float num = 0.0f, den = 0.0f;
-    if (k < G)
-        for (int s = k; s < splits; s += G) {
-            const float* part = from + (size_t)s * (D + 2);
-            const float f = __builtin_amdgcn_exp2f(part[D] - base);
-            num = fmaf(part[d], f, num);
-            den = fmaf(part[D + 1], f, den);
-        }
-    __shared__ float nums[G][D], dens[G];
+    const int lane = tid % LANES, k = tid / LANES;
+    float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float den = 0.0f;
     if (k < G) {
-        nums[k][d] = num;
-        if (d == 0) dens[k] = den;
+#pragma unroll 8
+        for (int s = k; s < splits; s += G) {
+            const float2 st = stats[s];
+            const float4 v = sums[(size_t)s * LANES + lane];
+            const float f = __builtin_amdgcn_exp2f(st.x - base);
+            num.x = fmaf(v.x, f, num.x); num.y = fmaf(v.y, f, num.y); num.z = fmaf(v.z, f, num.z); num.w = fmaf(v.w, f, num.w);
+            den = fmaf(st.y, f, den);
+        }
+        nums[k][lane] = num;
+        if (lane == 0) dens[k] = den;
     }
     __syncthreads();
-    if (k != 0) return;
-#pragma unroll
-    for (int i = 1; i < G; ++i) {
-        num += nums[i][d];
+    if (tid >= LANES) return;
+    const int parts = min(G, splits);
+    for (int i = 1; i < parts; ++i) {
+        const float4 v = nums[i][lane];
+        num.x += v.x; num.y += v.y; num.z += v.z; num.w += v.w;
         den += dens[i];
     }
-    const float v = said != length ? __builtin_nanf("") : length == 0 ? 0.0f : num / den * a.value_scale;
-    static_cast<uint16_t*>(a.out)[(size_t)row * D + d] = (uint16_t)bf16_bits(v);
+    const float f = said != length ? __builtin_nanf("") : length == 0 ? 0.0f : a.value_scale / den;
+    uint2* out = reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (size_t)row * D) + lane;
+    *out = length == 0 && said == length ? make_uint2(0u, 0u) : make_uint2(rb_pair(num.x * f, num.y * f), rb_pair(num.z * f, num.w * f));
 }
 
 // Tokens of a split.  One sequence of few tokens is left whole (no second launch); else as many splits as give every compute unit two workgroups, of 256 tokens at least
@@ -301,7 +344,7 @@ int paged_attention(const void* q, int64_t q_seq, int64_t q_head, int64_t seqs, 
         return METIS_E_ARG;
     if (dim <= 0 || dim > 256 || dim % (f8 ? 64 : 32) || page < 16 || page > 4096 || (page & (page - 1))) return METIS_E_ARG;
     if (seqs == 0) return METIS_OK;
-    if (!out || (uintptr_t)out % 2 || !lengths || (uintptr_t)lengths % 4 || (width > 0 && (!tables || (uintptr_t)tables % 4)) || !q || (uintptr_t)q % 16 || q_seq % 8 || q_head % 8)
+    if (!out || (uintptr_t)out % 8 || !lengths || (uintptr_t)lengths % 4 || (width > 0 && (!tables || (uintptr_t)tables % 4)) || !q || (uintptr_t)q % 16 || q_seq % 8 || q_head % 8)
         return METIS_E_ARG;
     if (pages > 0 ? (!keys || !values || ((uintptr_t)keys | (uintptr_t)values) % 16) : width > 0) return METIS_E_ARG;
     if (width > INT32_MAX / page || seqs > ((int64_t)1 << 46) / q_heads / dim) return METIS_E_ARG;
@@ -310,12 +353,13 @@ int paged_attention(const void* q, int64_t q_seq, int64_t q_head, int64_t seqs, 
     if (pairs > INT32_MAX / splits || seqs * q_heads > INT32_MAX) return METIS_E_TOO_LARGE;
     if (splits > 1 && (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < (size_t)seqs * (size_t)q_heads * (size_t)splits * (size_t)(dim + 2) * 4)) return METIS_E_WORKSPACE;
     AttendArgs a = {};
-    a.q = q; a.keys = keys; a.values = values; a.tables = tables; a.lengths = lengths; a.out = out; a.partial = static_cast<float*>(workspace);
+    a.q = q; a.keys = keys; a.values = values; a.tables = tables; a.lengths = lengths; a.out = out; a.sums = static_cast<float*>(workspace);
     a.q_seq = q_seq; a.q_head = q_head; a.table_stride = table_stride;
     a.q_heads = (int)q_heads; a.kv_heads = (int)kv_heads; a.group = (int)(q_heads / kv_heads); a.pages = (int)pages; a.page_shift = __builtin_ctzll((unsigned long long)page);
-    a.width = (int)width; a.splits = (int)splits; a.chunk = (int)chunk; a.tiles = (int)tiles;
+    a.width = (int)width; a.splits = (int)splits; a.chunk = (int)chunk; a.tiles = (int)tiles; a.pairs = (int)pairs;
     a.scale = (float)((double)scale * (double)key_scale * 1.4426950408889634);
     a.value_scale = value_scale;
+    if (splits > 1) a.stats = a.sums + (size_t)seqs * (size_t)q_heads * (size_t)splits * (size_t)dim;
     const dim3 grid((unsigned)(pairs * splits)), block(64 * kWaves), rows((unsigned)(seqs * q_heads));
 #define METIS_ATT(DT, F, TOK) hipLaunchKernelGGL((attend_kernel<DT, F, TOK>), grid, block, 0, st, a)
     if (f8) {
@@ -340,7 +384,7 @@ int paged_attention(const void* q, int64_t q_seq, int64_t q_head, int64_t seqs, 
 #undef METIS_ATT
     if (splits > 1) {
         switch (dim / 32) {
-#define METIS_JOIN(DT) case DT: hipLaunchKernelGGL((attend_join_kernel<DT>), rows, dim3(256), 0, st, a); break
+#define METIS_JOIN(DT) case DT: hipLaunchKernelGGL((attend_join_kernel<DT>), rows, dim3(kJoinThreads), 0, st, a); break
             METIS_JOIN(1); METIS_JOIN(2); METIS_JOIN(3); METIS_JOIN(4); METIS_JOIN(5); METIS_JOIN(6); METIS_JOIN(7); METIS_JOIN(8);
 #undef METIS_JOIN
         }

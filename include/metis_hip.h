@@ -1067,7 +1067,7 @@ int metis_rotary_append(const void *q, int64_t q_token, int64_t q_head, int64_t 
  *            of 0 gives 0; one that is negative or larger than the table's pages, or a page that the cache does not
  *            have, makes the sequence's results NaN
  *   page     a power of two from 16 to 4096; dim a multiple of 32 up to 256 (e4m3: of 64); kv_heads divides q_heads
- *   out      dense [seqs, q_heads, dim]
+ *   out      dense [seqs, q_heads, dim], 8-byte aligned
  *   workspace metis_paged_attention_workspace_bytes(.., width * page) bytes, no initialisation needed
  */
 size_t metis_paged_attention_workspace_bytes(int64_t seqs, int64_t q_heads, int64_t kv_heads,
