@@ -78,64 +78,75 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(const AttendArgs
     const char* values = static_cast<const char*>(a.values) + kv * head_bytes;
     const int mask = (1 << a.page_shift) - 1;
 
-    // The pages of a block are asked for a block ahead (the first one's before anything is known of the length): KP of a lane's keys, VL of its values.  A run of eight
-    // tokens (WIDE: sixteen) lies in one page.
-    constexpr int KP = WIDE ? 1 : S, VL = WIDE ? 1 : S, VW = F8 && !WIDE ? 2 : 4;              // VL: loads of a dimension too, and their words
+    // Three things are on their way at a time: a block's values while its scores are formed, the next block's keys from then on, and the pages of the one after that (PIPE; where
+    // keys and values do not fit the registers side by side, the values come after the scores).  The first block's pages are asked for before anything is known of the
+    // length.  A run of eight tokens (WIDE: sixteen) lies in one page: KP runs of a lane's keys, VL of its values (loads of a dimension too, of VW words).
+    constexpr int KP = WIDE ? 1 : S, VL = WIDE ? 1 : S, VW = F8 && !WIDE ? 2 : 4, KC = F8 ? DT / 2 : DT, STEP = kWaves * TOK;
+    constexpr bool PIPE = F8 || DT < 7;
     const int r = n >> 2, last = a.width - 1;
     int kpage[KP], vpage[VL];
-    const auto ask = [&](int t0) {
+    const auto page_of = [&](int tok) { return table[max(min(tok >> a.page_shift, last), 0)]; };
+    const auto ask_keys = [&](int t0) {
 #pragma unroll
-        for (int s = 0; s < KP; ++s) kpage[s] = table[max(min((t0 + (WIDE ? 16 * r : 32 * s + 8 * r)) >> a.page_shift, last), 0)];
-#pragma unroll
-        for (int s = 0; s < VL; ++s) vpage[s] = table[max(min((t0 + (WIDE ? 16 * g : 32 * s + 8 * g)) >> a.page_shift, last), 0)];
+        for (int s = 0; s < KP; ++s) kpage[s] = page_of(t0 + (WIDE ? 16 * r : 32 * s + 8 * r));
     };
-    if (last >= 0) ask(begin + wave * TOK);
-
-    for (int t0 = begin + wave * TOK; t0 < end; t0 += kWaves * TOK) {
-        uint32_t bad = 0;                                          // bit s: the page of this lane's s-th run of keys is none
-        size_t kat[KP], vat[VL];
+    const auto ask_values = [&](int t0) {
+#pragma unroll
+        for (int s = 0; s < VL; ++s) vpage[s] = page_of(t0 + (WIDE ? 16 * g : 32 * s + 8 * g));
+    };
+    uint4 kx[T][KC];
+    uint32_t vx[NV][VL][VW], bad = 0;                              // bit s of bad: the page of this lane's s-th run of keys is none
+    const auto load_keys = [&](int t0) {
+        const char* run[KP];
+        bad = 0;
 #pragma unroll
         for (int s = 0; s < KP; ++s) {
             const int tok = t0 + (WIDE ? 16 * r : 32 * s + 8 * r);
             const bool none = (uint32_t)kpage[s] >= (uint32_t)a.pages;
             if (none && tok < end) bad |= 1u << s;
-            kat[s] = (size_t)(none || tok >= end ? 0 : kpage[s]) * page_bytes + (size_t)(tok & mask) * (D * unit);
+            run[s] = keys + (size_t)(none || tok >= end ? 0 : kpage[s]) * page_bytes + (size_t)((tok & mask) + (n & 3)) * (D * unit) + 16 * g;
         }
+#pragma unroll
+        for (int t = 0; t < T; ++t)                                // (the token of row n of score tile t: number n & 3 of four)
+#pragma unroll
+            for (int c = 0; c < KC; ++c) kx[t][c] = *reinterpret_cast<const uint4*>(run[WIDE ? 0 : t >> 1] + (WIDE ? 4 * t : 4 * (t & 1)) * (int)(D * unit) + 64 * c);
+    };
+    const auto load_values = [&](int t0) {
 #pragma unroll
         for (int s = 0; s < VL; ++s) {
             const int tok = t0 + (WIDE ? 16 * g : 32 * s + 8 * g);
-            vat[s] = (size_t)((uint32_t)vpage[s] >= (uint32_t)a.pages || tok >= end ? 0 : vpage[s]) * page_bytes + (size_t)(tok & mask) * unit;
-        }
-        uint4 kx[T][F8 ? DT / 2 : DT];
+            const char* col = values + (size_t)((uint32_t)vpage[s] >= (uint32_t)a.pages || tok >= end ? 0 : vpage[s]) * page_bytes + (size_t)(tok & mask) * unit + (((size_t)n << a.page_shift) * unit);
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-            // the token of row n of score tile t: number n & 3 of four
-            const char* row = keys + kat[WIDE ? 0 : t >> 1] + (size_t)((WIDE ? 4 * t : 4 * (t & 1)) + (n & 3)) * (D * unit);
-#pragma unroll
-            for (int c = 0; c < (F8 ? DT / 2 : DT); ++c) kx[t][c] = *reinterpret_cast<const uint4*>(row + 64 * c + 16 * g);
-        }
-        uint32_t vx[NV][VL][VW];
-        constexpr bool LATE = DT == 8 && !F8;                      // (keys and values at once do not fit the registers)
-        const auto load_values = [&] {
-#pragma unroll
-            for (int s = 0; s < VL; ++s) {
-                const char* col = values + vat[s];
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const char* at = col + (((size_t)(16 * i + n) << a.page_shift) * unit);
-                    if constexpr (VW == 4) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(at);
-                        vx[i][s][0] = w.x; vx[i][s][1] = w.y; vx[i][s][2] = w.z; vx[i][s][3] = w.w;
-                    } else {
-                        const uint2 w = *reinterpret_cast<const uint2*>(at);
-                        vx[i][s][0] = w.x; vx[i][s][1] = w.y;
-                    }
+            for (int i = 0; i < NV; ++i) {
+                const char* at = col + (((size_t)(16 * i) << a.page_shift) * unit);
+                if constexpr (VW == 4) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(at);
+                    vx[i][s][0] = w.x; vx[i][s][1] = w.y; vx[i][s][2] = w.z; vx[i][s][3] = w.w;
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2*>(at);
+                    vx[i][s][0] = w.x; vx[i][s][1] = w.y;
                 }
             }
-        };
-        if constexpr (!LATE) load_values();
-        ask(t0 + kWaves * TOK);
-
+        }
+    };
+    int t0 = begin + wave * TOK;
+    if (last >= 0) {
+        ask_keys(t0);
+        ask_values(t0);
+    }
+    if (PIPE && t0 < end) {
+        load_keys(t0);
+        ask_keys(t0 + STEP);
+    }
+    for (; t0 < end; t0 += STEP) {
+        if constexpr (PIPE) {
+            load_values(t0);
+            ask_values(t0 + STEP);
+            __builtin_amdgcn_sched_barrier(0);
+        } else {
+            load_keys(t0);
+            ask_keys(t0 + STEP);
+        }
         float p[TOK / 4];                                          // scores, then weights, of the lane's tokens in their order
 #pragma unroll
         for (int t = 0; t < T; ++t) {
@@ -150,36 +161,42 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(const AttendArgs
 #pragma unroll
             for (int j = 0; j < 4; ++j) p[4 * t + j] = acc[j] * a.scale;
         }
-        if constexpr (LATE) {
-            __builtin_amdgcn_sched_barrier(0);
-            load_values();
-        }
-        // tokens behind the end have no weight; a token whose page is none makes the result NaN
-        const bool tail = t0 + TOK > end;
-        if (tail || __any(bad != 0)) {
+        if (__any(bad != 0)) {                                     // a token whose page is none makes the result NaN
+            const uint32_t mine = (uint32_t)__shfl((int)bad, 4 * g, 64);          // (a lane whose keys' rows are this lane's scores)
 #pragma unroll
-            for (int t = 0; t < T; ++t) {
+            for (int t = 0; t < T; ++t)
+                if (mine >> (WIDE ? 0 : t >> 1) & 1) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int tok = t0 + (WIDE ? 16 * g + 4 * t + j : 32 * (t >> 1) + 8 * g + 4 * (t & 1) + j);
-                    const int from = 4 * g + j;                    // the lane that loaded this row's key
-                    const bool none = (__shfl((int)bad, from, 64) >> (WIDE ? 0 : t >> 1)) & 1;
-                    if (tok >= end) p[4 * t + j] = -INFINITY;
-                    else if (none) p[4 * t + j] = __builtin_nanf("");
+                    for (int j = 0; j < 4; ++j) p[4 * t + j] = __builtin_nanf("");
                 }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (PIPE) {
+            if (t0 + STEP < end) {
+                load_keys(t0 + STEP);
+                ask_keys(t0 + 2 * STEP);
             }
-            if (tail) {                                            // (what lies behind the end may be anything: 0 times it has to be 0)
+        } else {
+            load_values(t0);
+            ask_values(t0 + STEP);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (t0 + TOK > end) {                                      // tokens behind the end have no weight, and what lies there may be anything: 0 times it has to be 0
 #pragma unroll
-                for (int s = 0; s < VL; ++s) {
-                    const int left = end - (t0 + (WIDE ? 16 * g : 32 * s + 8 * g));        // tokens of this load that count
-                    constexpr int PER = F8 ? 4 : 2;                                        // of a word
+            for (int t = 0; t < T; ++t)
 #pragma unroll
-                    for (int w = 0; w < VW; ++w) {
-                        const int k = min(max(left - PER * w, 0), PER);
-                        const uint32_t keep = k == PER ? ~0u : (1u << (32 / PER * k)) - 1u;
+                for (int j = 0; j < 4; ++j)
+                    if (t0 + (WIDE ? 16 * g + 4 * t + j : 32 * (t >> 1) + 8 * g + 4 * (t & 1) + j) >= end) p[4 * t + j] = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < NV; ++i) vx[i][s][w] &= keep;
-                    }
+            for (int s = 0; s < VL; ++s) {
+                const int left = end - (t0 + (WIDE ? 16 * g : 32 * s + 8 * g));            // tokens of this load that count
+                constexpr int PER = F8 ? 4 : 2;                                            // of a word
+#pragma unroll
+                for (int w = 0; w < VW; ++w) {
+                    const int k = min(max(left - PER * w, 0), PER);
+                    const uint32_t keep = k == PER ? ~0u : (1u << (32 / PER * k)) - 1u;
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) vx[i][s][w] &= keep;
                 }
             }
         }
@@ -315,14 +332,14 @@ __global__ __launch_bounds__(kJoinThreads) void attend_join_kernel(const AttendA
     *out = length == 0 && said == length ? make_uint2(0u, 0u) : make_uint2(rb_pair(num.x * f, num.y * f), rb_pair(num.z * f, num.w * f));
 }
 
-// Tokens of a split.  One sequence of few tokens is left whole (no second launch); else as many splits as give every compute unit two workgroups, of 256 tokens at least
-// (one block for each wave), so that long sequences of a ragged batch have many workgroups and short ones few.
+// Tokens of a split.  Where the pairs of sequence and head fill the device, sequences of up to 4096 tokens are left whole (the joining launch costs 5 to 9 us: 64 sequences of
+// 4096 tokens, 4 heads of the cache, 94 us whole, 102 in halves), longer ones are cut so that a ragged batch's long ones do not end alone; else there are as many splits
+// as give every compute unit a workgroup, of 256 tokens at least (a block for each wave).  512 tokens are never cut: two blocks a wave take less than the joining launch.
 static int64_t split_tokens(int64_t pairs, int64_t capacity)
 {
-    const int64_t block = 64 * kWaves, want = 2 * (int64_t)device_cus();
-    int64_t splits = (want + pairs - 1) / pairs;
+    const int64_t block = 64 * kWaves, most = 4096, splits = (device_cus() + pairs - 1) / pairs;
     int64_t chunk = (capacity + splits - 1) / splits;
-    if (chunk > 1024) chunk = 1024;                                // a ragged batch: at most 1024 tokens of one sequence in a workgroup
+    if (chunk > most) chunk = most;
     chunk = (chunk + block - 1) / block * block;
     return capacity <= 2 * block ? 2 * block : chunk;
 }
@@ -347,7 +364,7 @@ int paged_attention(const void* q, int64_t q_seq, int64_t q_head, int64_t seqs, 
     if (!out || (uintptr_t)out % 8 || !lengths || (uintptr_t)lengths % 4 || (width > 0 && (!tables || (uintptr_t)tables % 4)) || !q || (uintptr_t)q % 16 || q_seq % 8 || q_head % 8)
         return METIS_E_ARG;
     if (pages > 0 ? (!keys || !values || ((uintptr_t)keys | (uintptr_t)values) % 16) : width > 0) return METIS_E_ARG;
-    if (width > INT32_MAX / page || seqs > ((int64_t)1 << 46) / q_heads / dim) return METIS_E_ARG;
+    if (width > (INT32_MAX - 65536) / page || seqs > ((int64_t)1 << 46) / q_heads / dim) return METIS_E_ARG;
     const int64_t capacity = width * page, tiles = (q_heads / kv_heads + kHeadTile - 1) / kHeadTile, pairs = seqs * kv_heads * tiles;
     const int64_t chunk = split_tokens(pairs, capacity > 0 ? capacity : 1), splits = capacity > 0 ? (capacity + chunk - 1) / chunk : 1;
     if (pairs > INT32_MAX / splits || seqs * q_heads > INT32_MAX) return METIS_E_TOO_LARGE;

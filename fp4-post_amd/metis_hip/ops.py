@@ -1689,8 +1689,8 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, t
     if seqs == 0:
         return torch.empty_like(q, memory_format=torch.contiguous_format)
     width = tables.shape[1]
-    if width > 0 and pages == 0 or width * page >= 1 << 31:
-        raise ValueError(f"paged_attention: tables of a cache with pages, of less than 2^31 tokens a sequence, not {tuple(tables.shape)} of pages of {page}")
+    if width > 0 and pages == 0 or width * page > (1 << 31) - (1 << 17):
+        raise ValueError(f"paged_attention: tables of a cache with pages, of up to 2^31 - 2^17 tokens a sequence, not {tuple(tables.shape)} of pages of {page}")
     if width > 1 and tables.stride(1) != 1:
         tables = tables.contiguous()
     if q.stride(2) != 1 or (heads > 1 and q.stride(1) % 8) or (seqs > 1 and q.stride(0) % 8) or q.data_ptr() % 16:
