@@ -302,6 +302,14 @@ PyMethodDef methods[] = {{"call", reinterpret_cast<PyCFunction>(reinterpret_cast
                           "recorded_swiglu(gate, up): swiglu of checked arguments as a node of autograd"},
                          {"recorded_rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&metis_recorded_rotary)), METH_FASTCALL,
                           "recorded_rotary(q, k, positions, inv_freq, interleaved, factor): rotary of checked arguments as a node of autograd"},
+                         {"rotary_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&metis_host_rotary_append)), METH_FASTCALL,
+                          "rotary_append(q, k, v, positions, inv_freq, slots, keys, values, interleaved, factor, key_scale, value_scale): the turned q, or None where it takes more than the entry point"},
+                         {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&metis_host_paged_attention)), METH_FASTCALL,
+                          "paged_attention(q, keys, values, tables, lengths, scale, key_scale, value_scale): its result, or None likewise"},
+                         {"copy_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&metis_host_copy_pages)), METH_FASTCALL,
+                          "copy_pages(keys, values, sources, destinations): True, or None likewise"},
+                         {"sample_tokens", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&metis_host_sample_tokens)), METH_FASTCALL,
+                          "sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p): tokens and log-probabilities, or None likewise"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_metis_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1647,6 +1647,7 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     for name, t in (("positions", positions), ("slots", slots)):
         if t.shape != (tokens,) or t.dtype != torch.int64:
             raise ValueError(f"rotary_append: {name} are int64 [{tokens}], not {t.dtype} {tuple(t.shape)}")
+    factor, key_scale, value_scale = float(factor), float(key_scale), float(value_scale)
     _check_scales("rotary_append", key_scale, value_scale)
     if tokens == 0:
         return torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -1682,7 +1683,7 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, t
         raise ValueError(f"paged_attention: pages of a power of two from 16 to 4096 tokens, not {page}")
     if tables.dim() != 2 or tables.shape[0] != seqs or tables.dtype != torch.int32 or lengths.shape != (seqs,) or lengths.dtype != torch.int32:
         raise ValueError(f"paged_attention: tables int32 [{seqs}, pages] and lengths int32 [{seqs}], not {tables.dtype} {tuple(tables.shape)} and {lengths.dtype} {tuple(lengths.shape)}")
-    scale = dim ** -0.5 if scale is None else float(scale)
+    scale, key_scale, value_scale = dim ** -0.5 if scale is None else float(scale), float(key_scale), float(value_scale)
     if not abs(scale) < float("inf"):
         raise ValueError(f"paged_attention: a finite scale, not {scale}")
     _check_scales("paged_attention", key_scale, value_scale)

@@ -12,7 +12,7 @@ from dataclasses import dataclass
 import torch
 from torch import nn
 
-from . import ops
+from . import _lib, ops
 from .bitlinear import _transformed
 
 
@@ -47,9 +47,15 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
                written and makes the token's query NaN; no two tokens may have one place
     keys       [pages, kv_heads, page, dim], values [pages, kv_heads, dim, page] of one layer, bf16 or float8_e4m3fn: there the numbers are value / scale,
                rounded to nearest, 448 for everything beyond it"""
-    _no_gradients("rotary_append", q, k, v)
-    args = q, k, v, positions, inv_freq, slots, keys, values, bool(interleaved), float(factor), float(key_scale), float(value_scale)
-    return _Recorded.apply(ops.rotary_append, *args) if _transformed() else ops.rotary_append(*args)
+    args = q, k, v, positions, inv_freq, slots, keys, values, bool(interleaved), factor, key_scale, value_scale
+    if _transformed():
+        _no_gradients("rotary_append", q, k, v)
+        return _Recorded.apply(ops.rotary_append, *args)
+    out = _lib.host().rotary_append(*args)
+    if out is None:                                                # (refused, or copied first)
+        _no_gradients("rotary_append", q, k, v)
+        out = ops.rotary_append(*args)
+    return out
 
 
 def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, *, scale: float | None = None,
@@ -60,15 +66,22 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, t
     keys, values   as in rotary_append, turned keys; dim a multiple of 32 up to 256 (float8_e4m3fn: of 64), pages of a power of two from 16 to 4096 tokens
     tables   int32 [seqs, n]: the pages of each sequence in order; lengths int32 [seqs]: its tokens.  What stands in a table behind them, or in a page, counts
              for nothing.  A length of 0 gives 0; a negative one, one that the table has no pages for, and a page that the cache does not have give NaN"""
-    _no_gradients("paged_attention", q, keys, values)
-    args = q, keys, values, tables, lengths, scale, float(key_scale), float(value_scale)
-    return _Recorded.apply(ops.paged_attention, *args) if _transformed() else ops.paged_attention(*args)
+    args = q, keys, values, tables, lengths, scale, key_scale, value_scale
+    if _transformed():
+        _no_gradients("paged_attention", q, keys, values)
+        return _Recorded.apply(ops.paged_attention, *args)
+    out = _lib.host().paged_attention(*args)
+    if out is None:
+        _no_gradients("paged_attention", q, keys, values)
+        out = ops.paged_attention(*args)
+    return out
 
 
 def copy_pages(keys: torch.Tensor, values: torch.Tensor, sources: Sequence[int], destinations: Sequence[int]) -> None:
     """Copies whole pages, sources[i] to destinations[i], in all layers of a cache: keys [layers, pages, kv_heads, page, dim], values [layers, pages, kv_heads, dim,
     page].  The numbers are the host's.  No page may be written twice, or written and read."""
-    ops.copy_pages(keys, values, sources, destinations)
+    if _lib.host().copy_pages(keys, values, sources, destinations) is None:
+        ops.copy_pages(keys, values, sources, destinations)
 
 
 def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: float | torch.Tensor = 1.0, top_k: int | torch.Tensor = 0,
@@ -83,9 +96,15 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: 
 
     The log-probability is that under softmax(logits / temperature), before anything is left out: what token_logprobs gives for it, and a GRPO step takes its
     ratios to.  A row of nothing but -inf, one with a NaN, or one whose settings or number are out of range has token -1 and NaN."""
-    _no_gradients("sample_tokens", logits)
     args = logits, uniforms, temperature, top_k, top_p, min_p
-    return _Recorded.apply(ops.sample_tokens, *args) if _transformed() else ops.sample_tokens(*args)
+    if _transformed():
+        _no_gradients("sample_tokens", logits)
+        return _Recorded.apply(ops.sample_tokens, *args)
+    out = _lib.host().sample_tokens(*args)
+    if out is None:
+        _no_gradients("sample_tokens", logits)
+        out = ops.sample_tokens(*args)
+    return out
 
 
 @dataclass
