@@ -411,7 +411,7 @@ int paged_attention(const void* q, int64_t q_seq, int64_t q_head, int64_t seqs, 
 
 // ---------------------------------------------------------------------------------------------- copies of pages
 // The pairs travel with the launch: nothing has to be brought to the device first.
-constexpr int kCopyPairs = 240;
+constexpr int kCopyPairs = 448;                                    // (a launch's arguments hold 4 KB)
 struct CopyArgs {
     char *keys, *values;
     uint64_t page_bytes, layer_bytes;
@@ -433,11 +433,14 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(const CopyArgs a)
     char* to = base + (size_t)a.to[pair] * a.page_bytes;
     const uint64_t at = (uint64_t)piece * kCopyPiece + threadIdx.x * 16;
     if ((uint64_t)(piece + 1) * kCopyPiece <= a.page_bytes) {
-        uint4 w[kCopyPiece / 4096];
-#pragma unroll
-        for (int i = 0; i < kCopyPiece / 4096; ++i) w[i] = *reinterpret_cast<const uint4*>(from + at + 4096 * i);
-#pragma unroll
-        for (int i = 0; i < kCopyPiece / 4096; ++i) *reinterpret_cast<uint4*>(to + at + 4096 * i) = w[i];
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        const u32x4* src = reinterpret_cast<const u32x4*>(from + at);
+        u32x4* dst = reinterpret_cast<u32x4*>(to + at);
+        const u32x4 w0 = src[0], w1 = src[256], w2 = src[512], w3 = src[768];
+        dst[0] = w0;
+        dst[256] = w1;
+        dst[512] = w2;
+        dst[768] = w3;
     } else {
         for (int i = 0; i < kCopyPiece / 4096; ++i)
             if (at + 4096 * i < a.page_bytes) *reinterpret_cast<uint4*>(to + at + 4096 * i) = *reinterpret_cast<const uint4*>(from + at + 4096 * i);
