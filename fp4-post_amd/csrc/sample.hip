@@ -2,14 +2,15 @@
 //   w_i = exp((x_i - max x) / T);  the tokens in order of falling logits, of equal ones the lower index first;
 //   K1 the first k of them, K2 those of K1 with less than p sum(K1) of weight before them, K3 those of K2 with w >= min_p;
 //   the lowest index i of K3 with  sum_{j <= i, j in K3} w_j > u sum(K3),   log p_i = log w_i - log sum_i w_i  (of all tokens, not of K3 alone)
-// The vocabulary is not sorted.  A token's depth is the binary logarithm of 1 / w, its bin the depth in 1/64.  One pass adds up all weights and takes out the tokens of the
-// bins down to one that the thresholds lie above of as a rule:
-//   k  at least k tokens lie in the bins down to the one that holds the k-th largest of 4096 maxima over disjoint shares of the row;
-//   p  some 3000 tokens lie down to the 2130th largest of them, and some 16000 down to the 4013th (where the first are not enough); and with W0 the weights of those maxima (less than all weights), tokens deeper than
-//      log2(2 V / ((1 - p) W0)) have together less than half of what K2 leaves out.
+// The vocabulary is not sorted.  A token's depth is the binary logarithm of 1 / w, its bin the depth in 1/64.  A first pass finds the row's maximum (with p, also a sum of all
+// weights that is good to a few digits) and 4096 maxima over disjoint shares of the row, a second one adds up all weights and takes out the tokens that a threshold lies
+// among as a rule:
+//   k  those in the bins down to the one that holds the k-th largest of the maxima: at least k;
+//   p  those in a window of bins around the one in which the weights reach p of their sum, by a guess: where M of S shares have a maximum in the bins down to one, about
+//      V (1 - (1 - M / S)^(S / V)) tokens lie there (to some 3 percent where that are 16000); those above the window are kept, and added up by stretches of 512 indices at once.
 // They are sorted where they are few; else they are counted (k) and their weights added up (p) by bins, in whole numbers, so that the order of the additions does not
-// count, and the tokens of the bin that holds a threshold are sorted.  What is kept is added up by stretches of 512 indices for the draw, in whole numbers again.  Where
-// the thresholds lie deeper (large k, flat rows), further passes over the row do the same with all tokens, and narrow a bin of too many by digits of its logits and indices.
+// count, and the tokens of the bin that holds a threshold are sorted.  What is kept of them is added to the stretches' sums for the draw, in whole numbers again.  Where
+// the thresholds lie elsewhere (large k, flat rows), further passes over the row do the same with all tokens, and narrow a bin of too many by digits of its logits and indices.
 // Weights are accurate to 2^-44 and sums are held in 64 bits: with some 10^5 tokens next to each other in the running sum, what binary32 is off would take another
 // token now and then.  Each pass is a chain of some twenty 64-bit operations for each token, and what it must not do is go through LDS for each (one LDS
 // operation of a compute unit's sixteen waves costs as much as sixteen of these on its four SIMDs): there are no tables, sums over lanes go by DPP.
@@ -24,9 +25,11 @@ namespace metis {
 constexpr int kSampleThreads = 1024;                               // of the workgroup that has a row to itself
 constexpr int kPartThreads = 256;                                  // of one that has a part of a row
 constexpr int kBins = 4096;                                        // 64 octaves; the last one holds everything below them
-constexpr int kTaken = 24576, kPartTaken = 8192;                   // tokens that are taken out of a row, and of a part of one
+constexpr int kTaken = 16384, kPartTaken = 8192;                   // tokens that are taken out of a row, and of a part of one
 constexpr int kList = 1024;                                        // tokens that can be sorted
-constexpr int kShares = 4096, kSharesDown = 2130, kSharesFar = 4013;   // maxima of a row, and how many of them lie in the bins that p takes tokens out of, first and then
+constexpr int kShares = 4096;                                      // maxima of a row
+constexpr int kSharesOfK = 3900;                                   // the largest k that tokens are taken out for: some 12500
+constexpr double kLowTemperatures = 0x1p100;                       // 1 / T from which depths do not fit binary32
 constexpr double kUnit = 0x1p41;                                   // a weight of its bin's octave, as a whole number
 constexpr double kKeptUnit = 0x1p50;                               // a kept weight of a stretch
 
@@ -38,11 +41,12 @@ struct SampleArgs {
     double temperature, top_k, top_p, min_p;
     int64_t* tokens;
     float* logprobs;
-    // of rows in parts: [rows][kShares] maxima, [rows][parts] sums of weights, [rows][kBins] sums of stretches, [rows][kTaken] indices and their numbers
-    float* tops;
-    double* sums;
+    // of rows in parts: [rows][kShares] maxima, [rows][kBins] sums of stretches, [rows][kTaken] indices and their numbers
+    float *tops, *guesses, *rests;                                 // (and [rows][parts][2] largest logits and guessed sums, [rows][kShares] what they hold besides the maxima)
+    double* sums;                                                  // [rows][parts][2]: of all weights, of those above the window
     double* stretches;
     uint32_t *taken, *filled;
+    int* limits;                                                   // [rows][2]
     int rows, vocab, parts;
 };
 
@@ -105,7 +109,7 @@ template <int THREADS, class V> __device__ __forceinline__ V scan(V v, V* waves,
 template <bool F32> struct LogitRow {
     const char* base;
     int vocab, shift, pieces;
-    __device__ LogitRow(const void* p, int vocab_) : base(static_cast<const char*>(p)), vocab(vocab_)
+    __device__ __forceinline__ LogitRow(const void* p, int vocab_) : base(static_cast<const char*>(p)), vocab(vocab_)
     {
         shift = (int)(reinterpret_cast<uintptr_t>(p) % (F32 ? 32 : 16)) / (F32 ? 4 : 2);
         pieces = (vocab + shift + 7) / 8;
@@ -172,13 +176,15 @@ template <bool F32> struct LogitRow {
 struct Weigher {
     double top, rate;                                              // the row's maximum; log2(e) / T
     float least, top32, rate32, cut;                               // what lies 2000 octaves deep or more has no weight: logits below `least` are that
+    double far;                                                    // 2000 octaves
     bool single;
-    __device__ Weigher(float top_, double rate_) : top((double)top_), rate(rate_), cut(top_)
+    __device__ __forceinline__ Weigher(float top_, double rate_) : top((double)top_), rate(rate_), cut(top_)
     {
         const double deep = top - 2000.0 / rate_;
         single = !(top_ < INFINITY) || !(deep > -3.4e38) || !((float)deep < top_);
         if (single) { top = 0.0; rate = 1.0; }
         least = single ? -2000.0f : (float)deep;
+        far = 2000.0 / rate;
         top32 = (float)top;
         rate32 = (float)rate;
     }
@@ -202,31 +208,37 @@ struct Weigher {
         return {fma(d, rate, -(double)octave), bin, octave};
     }
     __device__ __forceinline__ static int octave_of(int bin) { return (bin + 32) >> 6; }
-    // p r + c; HOT: for all tokens (as the compiler writes it, it first copies c to where the sum goes; the constants of those for a few stay out of the registers)
-    template <bool HOT> __device__ __forceinline__ static double step(double p, double r, double c)
-    {
-        if constexpr (!HOT) return fma(p, r, c);
-        double v;
-        asm("v_fma_f64 %0, %1, %2, %3" : "=v"(v) : "v"(p), "v"(r), "v"(c));
-        return v;
-    }
     // 2^-r: a polynomial through 2^-r at nine Chebyshev points of |r| <= 0.508, and 1 at 0; within 2^-44.4
-    template <bool HOT = false> __device__ __forceinline__ static double part(double r)
+    static constexpr double C[9] = {-0.6931471805599453, 0.24022650695799835, -0.05550410866475214, 0.00961812916457961, -0.0013333558182304001, 0.0001540345096151519, -1.52526837656183e-05,
+                                    1.3256508477029382e-06, -1.020392955712988e-07};
+    __device__ __forceinline__ static double part(double r)
     {
-        double p = step<HOT>(-1.020392955712988e-07, r, 1.3256508477029382e-06);
-        p = step<HOT>(p, r, -1.52526837656183e-05);
-        p = step<HOT>(p, r, 0.0001540345096151519);
-        p = step<HOT>(p, r, -0.0013333558182304001);
-        p = step<HOT>(p, r, 0.00961812916457961);
-        p = step<HOT>(p, r, -0.05550410866475214);
-        p = step<HOT>(p, r, 0.24022650695799835);
-        p = step<HOT>(p, r, -0.6931471805599453);
+        double p = C[8];
+#pragma unroll
+        for (int i = 7; i >= 0; --i) p = fma(p, r, C[i]);
         return fma(p, r, 1.0);
     }
-    template <bool HOT = false> __device__ __forceinline__ double weight(float x) const
+    // two of them for the passes over all tokens, side by side, as they are to be issued: the compiler copies each constant to where the sum goes
+    __device__ __forceinline__ static void parts(double r, double q, double& a, double& b)
+    {
+        asm("v_fma_f64 %0, %4, %2, %5\n\tv_fma_f64 %1, %4, %3, %5\n\tv_fma_f64 %0, %0, %2, %6\n\tv_fma_f64 %1, %1, %3, %6\n\tv_fma_f64 %0, %0, %2, %7\n\tv_fma_f64 %1, %1, %3, %7\n\t"
+            "v_fma_f64 %0, %0, %2, %8\n\tv_fma_f64 %1, %1, %3, %8\n\tv_fma_f64 %0, %0, %2, %9\n\tv_fma_f64 %1, %1, %3, %9\n\tv_fma_f64 %0, %0, %2, %10\n\tv_fma_f64 %1, %1, %3, %10\n\t"
+            "v_fma_f64 %0, %0, %2, %11\n\tv_fma_f64 %1, %1, %3, %11\n\tv_fma_f64 %0, %0, %2, %12\n\tv_fma_f64 %1, %1, %3, %12\n\tv_fma_f64 %0, %0, %2, 1.0\n\tv_fma_f64 %1, %1, %3, 1.0"
+            : "=&v"(a), "=&v"(b)
+            : "v"(r), "v"(q), "v"(C[8]), "v"(C[7]), "v"(C[6]), "v"(C[5]), "v"(C[4]), "v"(C[3]), "v"(C[2]), "v"(C[1]), "v"(C[0]));
+    }
+    __device__ __forceinline__ double weight(float x) const
     {
         const Depth d = depth(x);
-        return ldexp(part<HOT>(d.r), -d.octave);
+        return ldexp(part(d.r), -d.octave);
+    }
+    // the same for two tokens of a pass over all: 0 from 2000 octaves on, as above; the octave to the nearest, read off a sum again
+    __device__ __forceinline__ void weights(float x, float y, double& a, double& b) const
+    {
+        const double d = fmin(top - (double)x, far), e = fmin(top - (double)y, far), o = fma(d, -rate, 0x1.8p52), p = fma(e, -rate, 0x1.8p52);
+        parts(fma(d, rate, o - 0x1.8p52), fma(e, rate, p - 0x1.8p52), a, b);
+        a = ldexp(a, (int)__double_as_longlong(o));
+        b = ldexp(b, (int)__double_as_longlong(p));
     }
     // a weight as a whole number of its bin's units (read off the bits of a sum with 2^52), and the unit
     __device__ __forceinline__ static uint64_t units(double part, Depth d)
@@ -255,7 +267,7 @@ __device__ __forceinline__ uint64_t place(float x, int i) { return (uint64_t)fal
 struct RowSettings {
     double temperature, top_k, top_p, min_p, u;
     bool by_k, by_p;
-    __device__ RowSettings(const SampleArgs& a, int r)
+    __device__ __forceinline__ RowSettings(const SampleArgs& a, int r)
     {
         const double* own = a.row_parameters ? a.row_parameters + 4 * (size_t)r : nullptr;
         temperature = own ? own[0] : a.temperature;
@@ -266,11 +278,11 @@ struct RowSettings {
         by_k = top_k >= 1.0 && top_k < (double)a.vocab;
         by_p = top_p < 1.0;
     }
-    __device__ bool fit() const
+    __device__ __forceinline__ bool fit() const
     {
         return temperature > 0.0 && temperature <= 0x1p64 && u >= 0.0 && u < 1.0 && top_k >= 0.0 && top_p > 0.0 && min_p >= 0.0 && min_p <= 1.0;
     }
-    __device__ double rate() const { return 1.4426950408889634 / temperature; }
+    __device__ __forceinline__ double rate() const { return 1.4426950408889634 / temperature; }
 };
 
 // What a workgroup holds of a row or of a part of one.
@@ -287,6 +299,7 @@ template <int THREADS, int TAKEN> struct SampleShared {
 };
 using PartShared = SampleShared<kPartThreads, kPartTaken>;
 struct RowShared : SampleShared<kSampleThreads, kTaken> {
+    double above[kBins];                                           // sums of the stretches: of the tokens above the window
     uint32_t count[kBins];
     uint64_t list[kList];
     uint64_t digit_weight[256];
@@ -308,10 +321,14 @@ template <int THREADS> __device__ __forceinline__ float largest(float top, float
     return __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(wave_max(top))));
 }
 // The largest logits of this thread's pieces (first, first + step, ..), dealt to `slots` shares (a power of two up to SLOTS; -inf: of an empty one); NaN where one is.
-template <bool F32, int SLOTS> __device__ __forceinline__ void own_largest(const LogitRow<F32>& row, int first, int end, int step, int slots, float (&top)[SLOTS])
+// guess: with rate > 0 the sum of their weights as seen from the largest of them, `most_of_all`, in binary32.
+template <bool F32, int SLOTS>
+__device__ __forceinline__ void own_largest(const LogitRow<F32>& row, int first, int end, int step, int slots, float rate, float (&top)[SLOTS], float& most_of_all, float& guess)
 {
     bool nan = false;
     int turn = 0;
+    guess = 0.0f;
+    most_of_all = -INFINITY;
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k) top[k] = -INFINITY;
     row.each(first, end, step, [&](const float* x, int) {
@@ -324,62 +341,142 @@ template <bool F32, int SLOTS> __device__ __forceinline__ void own_largest(const
 #pragma unroll
         for (int k = 0; k < SLOTS; ++k) top[k] = k == (turn & (slots - 1)) ? fmaxf(top[k], most) : top[k];
         ++turn;
+        if (rate > 0.0f) {
+            const float now = fmaxf(most_of_all, most), from = now == -INFINITY ? 0.0f : now;
+            guess *= __builtin_amdgcn_exp2f((most_of_all - from) * rate);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) guess += __builtin_amdgcn_exp2f((x[j] - from) * rate);
+            most_of_all = now;
+        }
     });
     if (nan) top[0] = __builtin_nanf("");
 }
+// the rate that weights are guessed with: 0 where nobody asks
+__device__ __forceinline__ float guess_rate(const RowSettings& set) { return set.by_p && !set.by_k ? (float)set.rate() : 0.0f; }
+// One logit with as much weight as all that a thread guessed but its shares' maxima: where two of the row's largest lie in the same share, the other one.
+template <int SLOTS> __device__ __forceinline__ float rest_of(const float (&top)[SLOTS], float most, float guess, float rate)
+{
+#pragma unroll
+    for (int k = 0; k < SLOTS; ++k) guess -= top[k] > -INFINITY ? __builtin_amdgcn_exp2f((top[k] - most) * rate) : 0.0f;
+    return guess > 0.0f ? most + __log2f(guess) / rate : -INFINITY;
+}
+// the row's sum of weights from what was guessed for some of it, as seen from the row's maximum
+template <int THREADS> __device__ __forceinline__ float guessed_sum(float most, float guess, float top, float rate, float* waves)
+{
+    float all;
+    scan<THREADS>(guess > 0.0f ? guess * __builtin_amdgcn_exp2f((most - top) * rate) : 0.0f, waves, all);
+    return all;
+}
 
-// Bins down to which at least so many of the shares' maxima lie (the last one where there is none).  s.weight is used.
-template <int THREADS, class S>
-__device__ __forceinline__ void bins_of_shares(S& s, const Weigher& w, const float (&mine)[kShares / THREADS], uint32_t need, uint32_t need_far, int& bin, int& far)
-{
-    const int tid = threadIdx.x;
-    constexpr int per = kBins / THREADS;
-    uint32_t* const count = reinterpret_cast<uint32_t*>(s.weight);
-    for (int b = tid; b < kBins / 2; b += THREADS) s.weight[b] = 0;
-    if (tid < 2) s.found_bins[tid] = kBins - 1;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kShares / THREADS; ++j) atomicAdd(&count[min(w.depth(w.settled(mine[j])).bin, kBins - 1)], 1u);
-    __syncthreads();
-    uint32_t c[per], n = 0, all;
-#pragma unroll
-    for (int j = 0; j < per; ++j) {
-        c[j] = count[per * tid + j];
-        n += c[j];
-    }
-    uint32_t upto = scan<THREADS>(n, s.waves_n, all) - n;
-#pragma unroll
-    for (int j = 0; j < per; ++j) {
-        if (upto < need && upto + c[j] >= need) s.found_bins[0] = per * tid + j;
-        if (upto < need_far && upto + c[j] >= need_far) s.found_bins[1] = per * tid + j;
-        upto += c[j];
-    }
-    __syncthreads();
-    bin = s.found_bins[0];
-    far = s.found_bins[1];
-}
-// The deepest bin that p's threshold can lie in.
-template <int THREADS, class S> __device__ __forceinline__ int deepest_p(S& s, const RowSettings& set, const Weigher& w, const float (&mine)[kShares / THREADS], int vocab)
-{
-    double known = 0.0, all;
-#pragma unroll
-    for (int j = 0; j < kShares / THREADS; ++j) known += w.weight(w.settled(mine[j]));
-    scan<THREADS>(known, s.waves_d, all);
-    // (W0's tokens are in the row, each once, so W >= W0; two more bins make good what W0 and the bins are rounded by)
-    const double bins = (log2(2.0 * (double)vocab) - log2((1.0 - set.top_p) * all)) * 64.0 + 2.0;
-    return bins < (double)(kBins - 1) ? max((int)bins, 0) : kBins - 1;
-}
-// The bins down to which tokens are taken out, first and then (-1: none are: no thresholds, or so large a k that another pass is needed anyhow), and the deepest one that counts.
+// The bins whose tokens are taken out, `first` (0: nothing lies above them) to `last` (-1: none are: no thresholds, or so large a k or so flat a row that further passes are
+// needed anyhow).
 struct Limits {
-    int first = -1, far = -1, deepest = kBins - 1;
-    template <int THREADS, class S> __device__ __forceinline__ void find(S& s, const RowSettings& set, const Weigher& w, const float (&mine)[kShares / THREADS], int vocab)
+    int first = 0, last = -1;
+    // rest: what the guess says besides the maxima (rest_of).  s.weight and s.taken are used
+    template <int THREADS, int RESTS, class S>
+    __device__ __forceinline__ void find(S& s, const RowSettings& set, const Weigher& w, const float (&mine)[kShares / THREADS], const float (&rest)[RESTS], float guess, int vocab, int pieces)
     {
-        if (set.by_k ? set.top_k > (double)kSharesFar : !set.by_p) return;
-        bins_of_shares<THREADS>(s, w, mine, set.by_k ? (uint32_t)set.top_k : (uint32_t)kSharesDown, (uint32_t)kSharesFar, first, far);
-        if (set.by_k) return;
-        deepest = deepest_p<THREADS>(s, set, w, mine, vocab);
-        first = min(first, deepest);
-        far = min(far, deepest);
+        if (set.by_k ? set.top_k > (double)kSharesOfK : !set.by_p) return;
+        const int tid = threadIdx.x;
+        constexpr int per = kBins / THREADS;
+        uint32_t* const count = reinterpret_cast<uint32_t*>(s.weight);
+        unsigned long long* const weight = reinterpret_cast<unsigned long long*>(s.taken);               // of the maxima, in units of 2^-40
+        static_assert(sizeof s.taken >= kBins * 8, "");
+        for (int b = tid; b < kBins / 2; b += THREADS) s.weight[b] = 0;
+        for (int b = tid; b < kBins; b += THREADS) weight[b] = 0;
+        if (tid < 2) s.found_bins[tid] = tid ? INT32_MAX : kBins - 1;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kShares / THREADS; ++j) {
+            const auto d = w.depth(w.settled(mine[j]));
+            atomicAdd(&count[min(d.bin, kBins - 1)], 1u);
+            if (!set.by_k) atomicAdd(&weight[min(d.bin, kBins - 1)], (unsigned long long)(__builtin_amdgcn_exp2f(-(float)((double)d.octave + d.r)) * 0x1p40f));
+        }
+        if (!set.by_k) {
+#pragma unroll
+            for (int j = 0; j < RESTS; ++j) {                      // (what many small ones add up to is less)
+                const auto d = w.depth(fminf(w.settled(rest[j]), w.top32));
+                const float v = __builtin_amdgcn_exp2f(-(float)((double)d.octave + d.r));
+                if (v > 0.002f * guess) atomicAdd(&weight[min(d.bin, kBins - 1)], (unsigned long long)(v * 0x1p40f));
+            }
+        }
+        __syncthreads();
+        uint32_t c[per], n = 0, all;
+#pragma unroll
+        for (int j = 0; j < per; ++j) {
+            c[j] = count[per * tid + j];
+            n += c[j];
+        }
+        const uint32_t before = scan<THREADS>(n, s.waves_n, all) - n;
+        uint32_t m = before;
+        if (set.by_k) {
+            const uint32_t need = (uint32_t)set.top_k;
+#pragma unroll
+            for (int j = 0; j < per; ++j) {
+                if (m < need && m + c[j] >= need) s.found_bins[0] = per * tid + j;
+                m += c[j];
+            }
+            __syncthreads();
+            last = s.found_bins[0];
+            return;
+        }
+        // the weights of the maxima, and of the others that are guessed to lie in the same bins
+        const float shares = (float)min(pieces, kShares), most = shares * 0.995f;
+        const auto tokens = [&](uint32_t m) __attribute__((always_inline)) { return (float)vocab * (1.0f - __builtin_amdgcn_exp2f(__log2f(1.0f - fminf((float)m, most) / shares) * (shares / (float)vocab))); };
+        if (!(guess < INFINITY)) guess = 1.0f;                     // (rows of infinities)
+        const float plain = 0.002f * guess;                        // a hidden token of more weight is known from `rest`
+        float known[per], hidden[per], square[per], sum = 0.0f, sum_hidden = 0.0f, sum_square = 0.0f, told = tokens(before), whole;
+#pragma unroll
+        for (int j = 0; j < per; ++j) {
+            m += c[j];
+            const float now = c[j] ? tokens(m) : told;
+            known[j] = (float)weight[per * tid + j] * 0x1p-40f;
+            const float each = __builtin_amdgcn_exp2f((float)(per * tid + j) * (-1.0f / 64.0f));
+            hidden[j] = each > plain ? 0.0f : fmaxf(now - told - (float)c[j], 0.0f) * each;
+            square[j] = hidden[j] * each;
+            sum += known[j] + hidden[j];
+            sum_hidden += hidden[j];
+            sum_square += square[j];
+            told = now;
+        }
+        float* const waves = reinterpret_cast<float*>(s.waves_n);
+        float front = scan<THREADS>(sum, waves, whole) - sum, front_hidden = scan<THREADS>(sum_hidden, waves, whole) - sum_hidden;
+        float front_square = scan<THREADS>(sum_square, waves, whole) - sum_square;
+        // The window: where the guess is that far from p of the sum that it may be off by that.  (Of n hidden tokens the deviation is sqrt(n) where they are few, 2.1 sqrt(n) where
+        // 6000 of 131072 lie down to there, 2.9 sqrt(n) where 12000 do.)
+        const float goal = (float)set.top_p * guess;
+        const auto error = [&]() __attribute__((always_inline)) { return 0.001f * guess + 0.02f * front_hidden + 6.0f * __builtin_amdgcn_sqrtf(fmaxf(front_square, 0.0f)); };
+        m = before;
+        float off = error();
+        bool upper = tid > 0 && front + off >= goal, lower = tid > 0 && front - off >= goal;             // (a bin has passed the goal)
+#pragma unroll
+        for (int j = 0; j < per; ++j) {
+            m += c[j];
+            front += known[j] + hidden[j];
+            front_hidden += hidden[j];
+            front_square += square[j];
+            off = error();
+            if (!upper && front + off >= goal) { atomicMin(&s.found_bins[0], per * tid + j); upper = true; }
+            if (!lower && front - off >= goal && (float)m <= most) { atomicMin(&s.found_bins[1], per * tid + j); lower = true; }
+        }
+        __syncthreads();
+        first = s.found_bins[0];
+        last = s.found_bins[1];
+        // what a short list holds is taken out from the top on
+        if (last < kBins && last / per == tid) {
+            m = before;
+            for (int j = 0; j <= last % per; ++j) m += c[j];
+            s.found_i = (int)tokens(m);
+        }
+        __syncthreads();
+        if (last >= kBins) {                                       // (a guess that ends before it gets there)
+            last = vocab <= kTaken ? kBins - 1 : -1;
+            first = first == kBins - 1 ? 0 : first;
+        } else if (s.found_i < kList / 2) {
+            first = 0;
+        }
+        // (all tokens above the window are kept: none is less than min_p)
+        if (set.min_p > 0.0) first = min(first, max((int)(fmin(-log2(set.min_p), 64.0) * 64.0) - 2, 0));
     }
 };
 
@@ -399,61 +496,72 @@ template <class W, class F> __device__ __forceinline__ void each_of_eight(const 
     }
 }
 
-// Takes the indices of the tokens down to bin `limit` (and of some of the next one: those that are not below a bound in binary32; never of -inf) out of pieces first,
-// first + step, .., multiples of 64 lanes (s.filled counts them, also those that s.taken has no room for); returns the thread's sum of all weights (SUM).  With k that sum is
-// for the log-probability alone, and formed in binary32 by eights (a weight is off by 2^-19 at a depth of 40 octaves, 2^-22 where it counts).
-template <bool F32, bool SUM, int TAKEN, class S>
-__device__ __forceinline__ double take_down(S& s, const RowSettings& set, const LogitRow<F32>& row, const Weigher& w, int limit, int first, int end, int step)
+// Takes the indices of the tokens of the window's bins (and of some of the next ones: those that are not beyond its bounds in binary32; never of -inf) out of pieces first,
+// first + step, .., multiples of 64 lanes (s.filled counts them, also those that s.taken has no room for); returns the thread's sum of all weights, and in `upper` that of the
+// tokens above the window, which go into stretches[] as well (by stretches).  With k the sum is for the log-probability alone, and formed in binary32 by eights (a weight is off
+// by 2^-19 at a depth of 40 octaves, 2^-22 where it counts).
+struct Window {
+    float lowest, highest;
+    __device__ __forceinline__ Window(const Limits& limits, const Weigher& w)
+    {
+        lowest = limits.last < 0 ? INFINITY : fmaxf(w.lowest(limits.last), -3.4028234e38f);
+        highest = w.highest(limits.first);
+    }
+};
+template <bool F32, int TAKEN, class S>
+__device__ __forceinline__ double take_down(S& s, const RowSettings& set, const LogitRow<F32>& row, const Weigher& w, const Limits& limits, int first, int end, int step, double* stretches,
+                                            double& upper)
 {
     double sum = 0.0;
-    const float lowest = limit < 0 ? INFINITY : fmaxf(w.lowest(limit), -3.4028234e38f);
-    const auto take = [&](const float* x, float most, int i) {
-        if (!__any(most >= lowest)) return;
-        uint32_t n = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) n += x[j] >= lowest ? 1u : 0u;
+    upper = 0.0;
+    const Window window(limits, w);
+    const auto take = [&](const float* x, uint32_t n, int i) __attribute__((always_inline)) {
+        if (!__any(n > 0)) return;
         const uint32_t upto = wave_scan(n);
         uint32_t at = 0;
         if ((threadIdx.x & 63) == 63) at = atomicAdd(&s.filled, upto);
         at = lane_value(at, 63) + upto - n;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (x[j] >= lowest) {
+            if (x[j] >= window.lowest && x[j] <= window.highest) {
                 if (at < (uint32_t)TAKEN) s.taken[at] = (uint32_t)(i + j);
                 ++at;
             }
     };
-    if constexpr (!SUM) {
+    if (set.by_k && w.rate < kLowTemperatures) {
         row.each(first, end, step, [&](float* x, int p) {
             w.settle(x);
-            float most = x[0];
-#pragma unroll
-            for (int j = 1; j < 8; ++j) most = fmaxf(most, x[j]);
-            take(x, most, row.index(p));
-        });
-    } else if (set.by_k) {
-        row.each(first, end, step, [&](float* x, int p) {
-            w.settle(x);
-            float eight = 0.0f, most = -INFINITY;
+            float eight = 0.0f;
+            uint32_t n = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 eight += __builtin_amdgcn_exp2f((x[j] - w.top32) * w.rate32);
-                most = fmaxf(most, x[j]);
+                n += x[j] >= window.lowest ? 1u : 0u;
             }
             sum += (double)eight;
-            take(x, most, row.index(p));
+            take(x, n, row.index(p));
         });
     } else {
         row.each(first, end, step, [&](float* x, int p) {
             w.settle(x);
-            float most = -INFINITY;
+            uint32_t n = 0;
+            double over = 0.0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                sum += w.template weight<true>(x[j]);
-                most = fmaxf(most, x[j]);
-                if (j % 2) __builtin_amdgcn_sched_barrier(0);      // (two tokens' chains side by side are enough, and eight want more registers than there are)
+            for (int j = 0; j < 8; j += 2) {
+                double v[2];
+                w.weights(x[j], x[j + 1], v[0], v[1]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    sum += v[e];
+                    over = fma(v[e], __longlong_as_double((long long)((uint64_t)(x[j + e] > window.highest ? 0x3ff00000u : 0u) << 32)), over);
+                    n += x[j + e] >= window.lowest && x[j + e] <= window.highest ? 1u : 0u;
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            take(x, most, row.index(p));
+            upper += over;
+            if (__any(over > 0.0)) over = wave_scan(over);
+            if ((threadIdx.x & 63) == 63 && p / 64 < kBins) stretches[p / 64] = over;
+            take(x, n, row.index(p));
         });
     }
     return sum;
@@ -469,15 +577,17 @@ template <bool F32> __device__ __forceinline__ void fill_bins(RowShared& s, cons
     row.each(tid, row.pieces, kSampleThreads, [&](float* x, int) {
         w.settle(x);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const auto d = w.depth(x[j]);
-            const int b = min(d.bin, kBins - 1);
-            if (set.by_p) {
-                const uint64_t units = w.units(w.template part<true>(d.r), d);
-                if (b <= limit) atomicAdd((unsigned long long*)&s.weight[b], (unsigned long long)units);
+        for (int j = 0; j < 8; j += 2) {
+            const Weigher::Depth d[2] = {w.depth(x[j]), w.depth(x[j + 1])};
+            double v[2];
+            if (set.by_p) w.parts(d[0].r, d[1].r, v[0], v[1]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int b = min(d[e].bin, kBins - 1);
+                if (set.by_p && b <= limit) atomicAdd((unsigned long long*)&s.weight[b], (unsigned long long)w.units(v[e], d[e]));
+                if (set.by_k) atomicAdd(&s.count[b], 1u);
             }
-            if (set.by_k) atomicAdd(&s.count[b], 1u);
-            if (j % 2) __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0);                     // (two tokens' chains side by side are enough, and eight want more registers than there are)
         }
     });
     __syncthreads();
@@ -737,7 +847,7 @@ struct Kept {
     float floor, edge;                                             // nothing below `floor` is kept (a wide bound); the threshold's logit
     int edge_index;                                                // and index
     bool whole;                                                    // all tokens are kept
-    __device__ Kept(uint64_t threshold_, const RowSettings& set, const Weigher& w) : threshold(threshold_), min_p(set.min_p)
+    __device__ __forceinline__ Kept(uint64_t threshold_, const RowSettings& set, const Weigher& w) : threshold(threshold_), min_p(set.min_p)
     {
         edge = threshold == ~0ull ? -INFINITY : risen((uint32_t)(threshold >> 24));
         edge_index = threshold == ~0ull ? INT32_MAX : (int)(threshold & 0xffffffu);
@@ -752,15 +862,31 @@ struct Kept {
         const double v = w.weight(x);
         return v >= min_p ? v : 0.0;
     }
-    // of eight neighbours, i the index of the first
-    __device__ __forceinline__ double eight(const Weigher& w, const float* x, int i) const
+    // of eight neighbours, i the index of the first; PASS: in a pass over the row
+    template <bool PASS> __device__ __forceinline__ double eight(const Weigher& w, const float* x, int i) const
     {
         double sum = 0.0;
         if (whole) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                sum += w.template weight<true>(x[j]);
-                if (j % 2) __builtin_amdgcn_sched_barrier(0);
+            for (int j = 0; j < 8; j += 2) {
+                double v[2];
+                w.weights(x[j], x[j + 1], v[0], v[1]);
+                sum += v[0] + v[1];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            return sum;
+        }
+        float most = x[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) most = fmaxf(most, x[j]);
+        if (PASS && __popcll(__ballot(most >= floor)) > 16) {                        // (many: all weights, side by side, are sooner there)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                double v[2];
+                w.weights(x[j], x[j + 1], v[0], v[1]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) sum += may(x[j + e], i + j + e) && v[e] >= min_p ? v[e] : 0.0;
+                __builtin_amdgcn_sched_barrier(0);
             }
             return sum;
         }
@@ -770,19 +896,22 @@ struct Kept {
     }
 };
 
-// K1's and K2's threshold from the sorted list of n tokens, K1's among them.
-__device__ __forceinline__ uint64_t threshold_of_list(RowShared& s, const RowSettings& set, const Weigher& w, uint32_t n)
+// K1's and K2's threshold from the sorted list of the window's n tokens, K1's among them; without k, `total` is the sum of all weights and `upper` of those above the window, and
+// the answer false where K2 ends elsewhere.
+__device__ __forceinline__ bool threshold_of_list(RowShared& s, const RowSettings& set, const Weigher& w, uint32_t n, double total, double upper, uint64_t& threshold)
 {
     const int tid = thread_anew();
-    const uint32_t limit = min((uint32_t)set.top_k, n);
+    const uint32_t limit = set.by_k ? min((uint32_t)set.top_k, n) : n;
     double all;
     const double v = tid < (int)limit ? w.weight(risen((uint32_t)(s.list[tid] >> 24))) : 0.0;
-    const double before = scan<kSampleThreads>(v, s.waves_d, all) - v, goal = set.by_p ? set.top_p * all : INFINITY;
+    const double before = upper + (scan<kSampleThreads>(v, s.waves_d, all) - v), goal = set.by_p ? set.top_p * (set.by_k ? all : total) : INFINITY;
+    if (!set.by_k && (upper >= goal || upper + all < goal)) return false;
     if (tid == 0) s.found_i = 0;
     __syncthreads();
     if (tid < (int)limit && before < goal) atomicMax(&s.found_i, tid);
     __syncthreads();
-    return s.list[s.found_i];
+    threshold = s.list[s.found_i];
+    return true;
 }
 
 // The token from the row's stretches of 512: `chosen` is the one that the goal falls into, `front` the weight in front of it (-1: a rounding put the goal behind every
@@ -799,7 +928,7 @@ __device__ __forceinline__ void draw_from_stretch(const SampleArgs& a, int r, co
     row.load(p).expand(x);                                         // (pieces behind the row: -inf)
     w.settle(x);
     const int i = row.index(p);
-    const double mine = kept.eight(w, x, i), incl = wave_scan(mine);
+    const double mine = kept.eight<false>(w, x, i), incl = wave_scan(mine);
     double at = front + (incl - mine);
     int found = -1, behind = -1;
 #pragma unroll 1
@@ -826,79 +955,76 @@ __device__ __forceinline__ void draw_from_stretch(const SampleArgs& a, int r, co
     }
 }
 
-// Thresholds and the draw.  total: the sum of all weights (< 0: it is what is kept); limits.first: the bin down to which s.filled tokens were taken out.  ready: there are no thresholds, and the sums of the stretches are in s.weight.
+// Thresholds and the draw.  total: the sum of all weights (< 0: it is what is kept); limits: the bins of which s.filled tokens were taken out, `upper` the weights above them.
+// ready: there are no thresholds, and the sums of the stretches are in s.weight.
 template <bool F32>
-__device__ __forceinline__ void finish_row(RowShared& s, const SampleArgs& a, int r, const RowSettings& set, const LogitRow<F32>& row, const Weigher& w, double total, const Limits& limits,
-                                           bool ready)
+__device__ __forceinline__ void finish_row(RowShared& s, const SampleArgs& a, int r, const RowSettings& set, const LogitRow<F32>& row, const Weigher& w, double total, double upper,
+                                           const Limits& limits, bool ready)
 {
     const int tid = threadIdx.x;
     constexpr int per = kBins / kSampleThreads;
-    int limit = limits.first;
-    uint32_t filled = s.filled;
+    const uint32_t filled = s.filled;
     uint64_t threshold = ~0ull;
     double kept_sum = total;                                       // sum(K1)
     int last = kBins;                                              // the bin that K1 ends in
-    // what was taken out is all that may be kept, but for p with a threshold further down
     const int stretches = (row.pieces + 63) / 64;
-    bool taken = limit >= 0 && stretches <= kBins && filled <= (uint32_t)kTaken;
-    if (taken && set.by_k && filled <= (uint32_t)kList) {
+    bool taken = limits.last >= 0 && stretches <= kBins && filled <= (uint32_t)kTaken, found_in_list = false;
+    if (taken && filled <= (uint32_t)kList) {
         const uint32_t n = take_again(s, row, w, filled, -1);
         sort_list(s, list_size(n));
-        threshold = threshold_of_list(s, set, w, n);
-    } else {
-        bool refill = (set.by_k || set.by_p) && !taken;
-        if (taken) fill_bins_again(s, row, w, filled, limit);
-        bool far = false;                                          // the second, larger number of tokens was taken out
+        taken = found_in_list = threshold_of_list(s, set, w, n, total, upper, threshold);
+    }
+    if (!found_in_list && (set.by_k || set.by_p)) {
+        // the deepest bin that p's threshold can lie in: V tokens further down have less than half of what K2 leaves out
+        const auto pass = [&]() __attribute__((always_inline)) {
+            const double bins = (log2(2.0 * (double)a.vocab) - log2((1.0 - set.top_p) * total)) * 64.0 + 2.0;
+            taken = false;
+            fill_bins<F32>(s, set, row, w, set.by_k || !(bins < (double)(kBins - 1)) ? kBins - 1 : max((int)bins, 0));
+        };
+        if (taken) fill_bins_again(s, row, w, filled, limits.last);
+        else pass();
 #pragma unroll 1
         for (int stage = 0; stage < 2; ++stage) {                  // top_k, then top_p
             if (!(stage ? set.by_p : set.by_k)) continue;
             // the bin: k by the bins' counts, p by their weights
             const double goal = stage ? set.top_p * kept_sum : (double)(uint32_t)set.top_k;
-            const auto held = [&](int b) { return stage ? (double)s.weight[b] * w.unit(b) : (double)s.count[b]; };
-            double sum, above;
+            const auto held = [&](int b) __attribute__((always_inline)) { return stage ? (double)s.weight[b] * w.unit(b) : (double)s.count[b]; };
+            int b;
+            uint32_t n;
+            double in_front;
+#pragma unroll 1
             for (;;) {
-                sum = 0.0;
+                double sum = 0.0, all;
 #pragma unroll
                 for (int j = 0; j < per; ++j) sum += held(per * tid + j);
                 if (tid == 0) s.found_i = -1;
-                double all;
-                above = scan<kSampleThreads>(sum, s.waves_d, all) - sum;
-                if (!refill && !(taken && all < goal)) break;
-                if (taken && !far && !set.by_k && limits.far > limit) {                  // further down
-                    far = true;
-                    limit = limits.far;
-                    if (tid == 0) s.filled = 0;
-                    __syncthreads();
-                    take_down<F32, false, kTaken>(s, set, row, w, limit, tid, (row.pieces + 63) / 64 * 64, kSampleThreads);
-                    __syncthreads();
-                    filled = s.filled;
-                    if (filled <= (uint32_t)kTaken) {
-                        fill_bins_again(s, row, w, filled, limit);
-                        continue;
-                    }
+                const double over = taken && !set.by_k ? upper : 0.0;                    // (nothing lies above what k takes out)
+                double front = over + (scan<kSampleThreads>(sum, s.waves_d, all) - sum);
+                if (taken && (over + all < goal || (over > 0.0 && over >= goal))) {      // the window missed it
+                    pass();
+                    continue;
                 }
-                taken = refill = false;                            // by another pass
-                fill_bins<F32>(s, set, row, w, limits.deepest);
-            }
-            double front = above;
 #pragma unroll
-            for (int j = 0; j < per; ++j) {
-                const int b = per * tid + j;
-                const double here = held(b), up = stage && b == last ? kept_sum : front + here;
-                // (one bin at most: the sums rise)
-                if (here > 0.0 && b <= last && front < goal && up >= goal) {
-                    s.found_i = b;
-                    s.found_d[0] = front;
+                for (int j = 0; j < per; ++j) {
+                    const int at = per * tid + j;
+                    const double here = held(at), up = stage && at == last ? kept_sum : front + here;
+                    // (one bin at most: the sums rise)
+                    if (here > 0.0 && at <= last && front < goal && up >= goal) {
+                        s.found_i = at;
+                        s.found_d[0] = front;
+                    }
+                    front += here;
                 }
-                front += here;
+                __syncthreads();
+                b = s.found_i;
+                in_front = s.found_d[0];
+                __syncthreads();
+                n = b < 0 ? 0 : taken ? take_again(s, row, w, filled, b) : take_out<F32>(s, row, w, b, 0, 0);
+                if (!taken || (b >= 0 && n <= (uint32_t)kList)) break;
+                pass();
             }
-            __syncthreads();
-            const int b = s.found_i;
-            const double in_front = s.found_d[0];
-            __syncthreads();
             if (b < 0) continue;
             const Wanted want = {stage == 1, stage ? 0 : (uint32_t)goal - (uint32_t)in_front, stage ? (goal - in_front) / w.unit(b) : 0.0};
-            uint32_t n = taken ? take_again(s, row, w, filled, b) : take_out<F32>(s, row, w, b, 0, 0);
             Narrowed at;
             if (n > (uint32_t)kList) {
                 at = narrow<F32>(s, row, w, b, n, want);
@@ -949,7 +1075,7 @@ __device__ __forceinline__ void finish_row(RowShared& s, const SampleArgs& a, in
                 __syncthreads();
                 row.each(first * 64 + tid, (first + here) * 64, kSampleThreads, [&](float* x, int p) {
                     w.settle(x);
-                    const double sum = wave_scan(kept.eight(w, x, row.index(p)));
+                    const double sum = wave_scan(kept.template eight<true>(w, x, row.index(p)));
                     if ((tid & 63) == 63) stretch[p / 64 - first] = sum;
                 });
                 __syncthreads();
@@ -957,17 +1083,27 @@ __device__ __forceinline__ void finish_row(RowShared& s, const SampleArgs& a, in
             double v[per], sum = 0.0, all;
 #pragma unroll
             for (int j = 0; j < per; ++j) {
-                v[j] = per * tid + j >= here ? 0.0 : taken ? (double)s.weight[per * tid + j] * (1.0 / kKeptUnit) : stretch[per * tid + j];
+                v[j] = per * tid + j >= here ? 0.0 : taken ? (double)s.weight[per * tid + j] * (1.0 / kKeptUnit) + (set.by_k ? 0.0 : s.above[per * tid + j]) : stretch[per * tid + j];
                 sum += v[j];
             }
             const double incl = scan<kSampleThreads>(sum, s.waves_d, all);
             if (round == 1) {
                 double at = done + (incl - sum);
+                int hit = -1, live = -1;
 #pragma unroll
                 for (int j = 0; j < per; ++j) {
-                    if (v[j] > 0.0 && at + v[j] > goal) atomicMin(&s.found_i, first + per * tid + j);
-                    if (v[j] > 0.0) atomicMax((int*)&s.filled, first + per * tid + j);
                     at += v[j];
+                    if (v[j] > 0.0) {
+                        if (hit < 0 && at > goal) hit = first + per * tid + j;
+                        live = first + per * tid + j;
+                    }
+                }
+                const uint64_t hits = __ballot(hit >= 0), lives = __ballot(live >= 0);
+                hit = lane_value(hit, hits ? __ffsll((unsigned long long)hits) - 1 : 0);
+                live = lane_value(live, lives ? 63 - __clzll((unsigned long long)lives) : 0);
+                if ((thread_anew() & 63) == 0) {
+                    if (hits) atomicMin(&s.found_i, hit);
+                    if (lives) atomicMax((int*)&s.filled, live);
                 }
                 __syncthreads();
                 const int f = s.found_i - first;
@@ -1001,57 +1137,74 @@ template <bool F32>
 __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs a)
 {
     __shared__ RowShared s;
-    const int tid = threadIdx.x, r = blockIdx.x;
+    const int r = blockIdx.x;
     const RowSettings set(a, r);
     const LogitRow<F32> row(static_cast<const char*>(a.logits) + (size_t)r * a.ld * (F32 ? 4 : 2), a.vocab);
     constexpr int SLOTS = kShares / kSampleThreads;
-    float mine[SLOTS];
-    own_largest<F32, SLOTS>(row, tid, row.pieces, kSampleThreads, SLOTS, mine);
+    float mine[SLOTS], most, guess;
+    own_largest<F32, SLOTS>(row, threadIdx.x, row.pieces, kSampleThreads, SLOTS, guess_rate(set), mine, most, guess);
     float top = mine[0];                                           // (a NaN is there)
 #pragma unroll
     for (int k = 1; k < SLOTS; ++k) top = top != top ? top : fmaxf(top, mine[k]);
     top = largest<kSampleThreads>(top, s.tops);
     if (!(top > -INFINITY) || !set.fit()) {                        // nothing to draw from, or no way to
-        if (tid == 0) {
+        if (thread_anew() == 0) {
             a.tokens[r] = -1;
             a.logprobs[r] = __builtin_nanf("");
         }
         return;
     }
     const Weigher w(top, set.rate());
+    const float rest[1] = {guess_rate(set) > 0.0f ? rest_of(mine, most, guess, guess_rate(set)) : -INFINITY};
+    if (guess_rate(set) > 0.0f) guess = guessed_sum<kSampleThreads>(most, guess, top, guess_rate(set), reinterpret_cast<float*>(s.waves_n));
     Limits limits;
-    limits.find<kSampleThreads>(s, set, w, mine, a.vocab);
-    if (tid == 0) s.filled = 0;
+    limits.find<kSampleThreads>(s, set, w, mine, rest, guess, a.vocab, row.pieces);
+    if (thread_anew() == 0) s.filled = 0;
     __syncthreads();
-    double total = -1.0;
-    if (set.by_k || set.by_p || set.min_p > 0.0)
-        scan<kSampleThreads>(take_down<F32, true, kTaken>(s, set, row, w, limits.first, tid, (row.pieces + 63) / 64 * 64, kSampleThreads), s.waves_d, total);
-    finish_row<F32>(s, a, r, set, row, w, total, limits, false);
+    double total = -1.0, upper = 0.0;
+    if (set.by_k || set.by_p || set.min_p > 0.0) {
+        double some;
+        const double own = take_down<F32, kTaken>(s, set, row, w, limits, thread_anew(), (row.pieces + 63) / 64 * 64, kSampleThreads, s.above, some);
+        scan<kSampleThreads>(own, s.waves_d, total);
+        scan<kSampleThreads>(some, s.waves_d, upper);
+    }
+    finish_row<F32>(s, a, r, set, row, w, total, upper, limits, false);
 }
 
 // whether a row's stretches of 512 tokens fit in place of its bins
 __device__ __forceinline__ bool stretches_fit(int pieces) { return (pieces + 63) / 64 <= kBins; }
 
-// Rows in parts, three launches.  1: the maxima of the row's shares; the stretches' sums and the number of tokens taken out cleared.
+// Rows in parts, three launches.  1: the maxima of the row's shares, and the guess of the weights' sum; the number of tokens taken out cleared.
 template <bool F32>
 __global__ __launch_bounds__(kPartThreads) void sample_tops_kernel(const SampleArgs a)
 {
+    __shared__ float waves[kPartThreads / 64];
     const int r = blockIdx.x / a.parts, part = blockIdx.x - r * a.parts, tid = threadIdx.x;
+    const RowSettings set(a, r);
     const LogitRow<F32> row(static_cast<const char*>(a.logits) + (size_t)r * a.ld * (F32 ? 4 : 2), a.vocab);
     const int at = part * kPartThreads + tid, all = a.parts * kPartThreads;
     // (a thread's pieces are dealt to several shares, or several threads have one)
     constexpr int SLOTS = kShares / kSampleThreads;
     const int slots = max(kShares / all, 1), per = max(all / kShares, 1);
-    float top[SLOTS];
-    own_largest<F32, SLOTS>(row, at, row.pieces, all, slots, top);
-    for (int o = 1; o < per; o <<= 1) {                            // (one slot then)
-        const float other = __shfl_xor(top[0], o, 64);
-        top[0] = top[0] != top[0] || other != other ? __builtin_nanf("") : fmaxf(top[0], other);
+    const float rate = guess_rate(set);
+    float top[SLOTS], most, guess;
+    own_largest<F32, SLOTS>(row, at, row.pieces, all, slots, rate, top, most, guess);
+    if (rate > 0.0f) {
+        const float highest = largest<kPartThreads>(most, waves);
+        __syncthreads();
+        const float sum = guessed_sum<kPartThreads>(most, guess, highest, rate, waves);
+        if (tid < 2) a.guesses[2 * ((size_t)r * a.parts + part) + tid] = tid ? sum : highest;
     }
+    for (int o = 1; o < per; o <<= 1) {                            // (one slot then)
+        const float other = __shfl_xor(top[0], o, 64), other_most = __shfl_xor(most, o, 64), other_guess = __shfl_xor(guess, o, 64), both = fmaxf(most, other_most);
+        top[0] = top[0] != top[0] || other != other ? __builtin_nanf("") : fmaxf(top[0], other);
+        guess = (guess > 0.0f ? guess * __builtin_amdgcn_exp2f((most - both) * rate) : 0.0f) + (other_guess > 0.0f ? other_guess * __builtin_amdgcn_exp2f((other_most - both) * rate) : 0.0f);
+        most = both;
+    }
+    if (rate > 0.0f && at % per == 0) a.rests[(size_t)r * kShares + at / per] = rest_of(top, most, guess, rate);
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k)
         if (k < slots && at % per == 0) a.tops[(size_t)r * kShares + k * all + at / per] = top[k];
-    for (int b = at; b < kBins; b += all) a.stretches[(size_t)r * kBins + b] = 0.0;
     if (at == 0) a.filled[r] = 0;
 }
 
@@ -1080,31 +1233,47 @@ __global__ __launch_bounds__(kPartThreads) void sample_bins_kernel(const SampleA
     const float top = row_top<kPartThreads>(a, r, mine, s.tops);
     if (!(top > -INFINITY) || !set.fit()) return;
     const Weigher w(top, set.rate());
+    float guess = 0.0f, rest[kShares / kPartThreads];
+#pragma unroll
+    for (int j = 0; j < kShares / kPartThreads; ++j) rest[j] = guess_rate(set) > 0.0f && j < a.parts ? a.rests[(size_t)r * kShares + j * kPartThreads + tid] : -INFINITY;
+    if (guess_rate(set) > 0.0f) {
+        const float* const told = a.guesses + 2 * (size_t)r * a.parts;
+        guess = guessed_sum<kPartThreads>(tid < a.parts ? told[2 * tid] : -INFINITY, tid < a.parts ? told[2 * tid + 1] : 0.0f, top, guess_rate(set), reinterpret_cast<float*>(s.waves_n));
+    }
     Limits limits;
-    limits.find<kPartThreads>(s, set, w, mine, a.vocab);
-    const int limit = limits.first;
+    limits.find<kPartThreads>(s, set, w, mine, rest, guess, a.vocab, row.pieces);
+    if (part == 0 && tid == 0) {
+        a.limits[2 * (size_t)r] = limits.first;
+        a.limits[2 * (size_t)r + 1] = limits.last;
+    }
     if (tid == 0) s.filled = 0;
     __syncthreads();
-    double sum = 0.0;
+    double sum = 0.0, some = 0.0;
     if (set.by_k || set.by_p || !stretches_fit(row.pieces)) {
-        sum = take_down<F32, true, kPartTaken>(s, set, row, w, limit, part * kPartThreads + tid, (row.pieces + 63) / 64 * 64, a.parts * kPartThreads);
+        sum = take_down<F32, kPartTaken>(s, set, row, w, limits, part * kPartThreads + tid, (row.pieces + 63) / 64 * 64, a.parts * kPartThreads, a.stretches + (size_t)r * kBins, some);
     } else {
         // no thresholds: the stretches' sums, in place of the bins
         const Kept kept(~0ull, set, w);
         row.each(part * kPartThreads + tid, (row.pieces + 63) / 64 * 64, a.parts * kPartThreads, [&](float* x, int p) {
             w.settle(x);
-            const double some = wave_scan(kept.eight(w, x, row.index(p)));
+            const double some = wave_scan(kept.template eight<true>(w, x, row.index(p)));
             if ((tid & 63) == 63) a.stretches[(size_t)r * kBins + p / 64] = some;
             if (!kept.whole) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) sum += w.template weight<true>(x[j]);
+                for (int j = 0; j < 8; j += 2) {
+                    double v[2];
+                    w.weights(x[j], x[j + 1], v[0], v[1]);
+                    sum += v[0] + v[1];
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         });
     }
-    double all;
+    double all, upper;
     scan<kPartThreads>(sum, s.waves_d, all);
-    if (tid == 0) a.sums[(size_t)r * a.parts + part] = all;
-    if (limit < 0) return;
+    scan<kPartThreads>(some, s.waves_d, upper);
+    if (tid < 2) a.sums[2 * ((size_t)r * a.parts + part) + tid] = tid ? upper : all;
+    if (limits.last < 0) return;
     // (more than there is room for, here or there: the number says so)
     const uint32_t n = s.filled;
     if (tid == 0) s.found_i = (int)atomicAdd(&a.filled[r], n > (uint32_t)kPartTaken ? (uint32_t)kTaken + 1 : n);
@@ -1133,15 +1302,18 @@ __global__ __launch_bounds__(kSampleThreads) void sample_finish_kernel(const Sam
     const Weigher w(top, set.rate());
     const bool ready = !set.by_k && !set.by_p && stretches_fit(row.pieces);
     const uint32_t filled = a.filled[r];
-    Limits limits;
-    limits.find<kSampleThreads>(s, set, w, mine, a.vocab);         // (as the launch before found them)
+    Limits limits;                                                 // (those that the launch before took: sums in another order might give others)
+    limits.first = a.limits[2 * (size_t)r];
+    limits.last = a.limits[2 * (size_t)r + 1];
     if (tid == 0) s.filled = filled;
-    if (ready)
-        for (int b = tid; b < kBins; b += kSampleThreads) s.weight[b] = __double_as_longlong(a.stretches[(size_t)r * kBins + b]);
+    const int stretches = min((row.pieces + 63) / 64, kBins);
+    for (int b = tid; b < stretches; b += kSampleThreads) (ready ? reinterpret_cast<double*>(s.weight) : s.above)[b] = a.stretches[(size_t)r * kBins + b];
     for (uint32_t i = tid; i < filled && i < (uint32_t)kTaken; i += kSampleThreads) s.taken[i] = a.taken[(size_t)r * kTaken + i];
-    double total;
-    scan<kSampleThreads>(tid < a.parts ? a.sums[(size_t)r * a.parts + tid] : 0.0, s.waves_d, total);
-    finish_row<F32>(s, a, r, set, row, w, ready && !(set.min_p > 0.0) ? -1.0 : total, limits, ready);
+    const double* const sums = a.sums + 2 * (size_t)r * a.parts;
+    double total, upper;
+    scan<kSampleThreads>(tid < a.parts ? sums[2 * tid] : 0.0, s.waves_d, total);
+    scan<kSampleThreads>(tid < a.parts ? sums[2 * tid + 1] : 0.0, s.waves_d, upper);
+    finish_row<F32>(s, a, r, set, row, w, ready && !(set.min_p > 0.0) ? -1.0 : total, upper, limits, ready);
 }
 
 // Workgroups that share a row, or 0 for one workgroup and one launch: rows that fill a quarter of the device or more, and vocabularies of a few pieces a thread.
@@ -1154,16 +1326,19 @@ static int row_parts(int64_t rows, int64_t vocab)
 }
 
 struct SampleSpace {
-    size_t tops, sums, stretches, taken, filled, bytes;
+    size_t tops, guesses, rests, sums, stretches, taken, filled, limits, bytes;
     SampleSpace(int64_t rows, int parts)
     {
         const size_t n = (size_t)rows;
         stretches = 0;
-        taken = n * kBins * 8;
-        sums = taken + n * kTaken * 4;
-        tops = sums + n * (size_t)parts * 8;
-        filled = tops + n * kShares * 4;
-        bytes = filled + n * 4;
+        sums = n * kBins * 8;
+        taken = sums + n * (size_t)parts * 16;
+        tops = taken + n * kTaken * 4;
+        guesses = tops + n * kShares * 4;
+        rests = guesses + n * (size_t)parts * 8;
+        filled = rests + n * kShares * 4;
+        limits = filled + n * 4;
+        bytes = limits + n * 8;
     }
 };
 size_t sample_tokens_workspace_bytes(int64_t rows, int64_t vocab)
@@ -1196,10 +1371,13 @@ int sample_tokens(const void* logits, int64_t ld, int dtype, int64_t rows, int64
         if (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < space.bytes) return METIS_E_WORKSPACE;
         char* base = static_cast<char*>(workspace);
         a.tops = reinterpret_cast<float*>(base + space.tops);
+        a.guesses = reinterpret_cast<float*>(base + space.guesses);
+        a.rests = reinterpret_cast<float*>(base + space.rests);
         a.sums = reinterpret_cast<double*>(base + space.sums);
         a.stretches = reinterpret_cast<double*>(base + space.stretches);
         a.taken = reinterpret_cast<uint32_t*>(base + space.taken);
         a.filled = reinterpret_cast<uint32_t*>(base + space.filled);
+        a.limits = reinterpret_cast<int*>(base + space.limits);
     }
     const dim3 grid((unsigned)rows), parts((unsigned)(rows * (a.parts ? a.parts : 1)));
 #define METIS_SAMPLE(F)                                                                                                             \
