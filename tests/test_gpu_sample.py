@@ -245,3 +245,53 @@ def test_refusals():
         sample_tokens(logits.cpu(), u.cpu())
     with torch.no_grad():
         sample_tokens(logits.requires_grad_(), u)
+
+
+@pytest.mark.parametrize("rows", [5, 70])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_thresholds_at_any_depth(rows, dtype):
+    """From a token to most of the vocabulary kept, rows in parts and rows alone: thresholds among a few tokens, some thousands, and where nothing was taken out for them."""
+    for spread, peaks in ((0.5, 0), (2.2, 40), (2.2, 3), (4.0, 0)):
+        logits, u = rows_of(rows + peaks, rows, 131072, dtype, spread, peaks)
+        for settings in [dict(top_p=p) for p in (0.3, 0.9, 0.95, 0.99, 0.9999)] + [dict(top_k=k) for k in (1024, 1025, 2900, 3900, 3901, 50000)] + \
+                        [dict(top_k=3000, top_p=0.97), dict(top_k=20000, top_p=0.6), dict(top_p=0.95, min_p=0.01), dict(top_p=0.97, min_p=1e-5), dict(min_p=1e-6), dict(top_p=0.95, temperature=2.0)]:
+            check(logits, u, **settings)
+
+
+@pytest.mark.parametrize("rows", [3, 70])
+def test_rows_with_an_order(rows):
+    """Vocabularies in order: rising, falling, in steps, the largest logits side by side or at even distances, all of them at one end."""
+    g = torch.Generator().manual_seed(rows)
+    u = torch.rand(rows, generator=g).cuda()
+    for V in (2000, 50021):
+        base = torch.sort(2.0 * torch.randn(rows, V, generator=g), 1)[0]
+        beside, apart, end = (2.0 * torch.randn(rows, V, generator=g) for _ in range(3))
+        for at in (0, 1, V // 2, V // 2 + 1, V // 2 + 2, V - 2, V - 1):
+            beside[:, at] += 12
+        apart[:, ::V // 30] += 9
+        end[:, -300:] += 7
+        for x in (base, base.flip(1), (4 * base).round() / 4, beside, apart, end):
+            for settings in (dict(), dict(top_p=0.5), dict(top_p=0.95), dict(top_p=0.999), dict(top_k=40), dict(top_k=1500), dict(top_k=600, top_p=0.9), dict(top_p=0.9, min_p=0.02)):
+                check(x.cuda(), u, **settings)
+                check(x.to(BF).cuda(), u, **settings)
+
+
+def test_a_row_alone_and_among_others():
+    """Rows that several workgroups share draw what the same rows draw that have one each."""
+    from metis_hip import sample_tokens
+    logits, u = rows_of(9, 80, 40009, BF, 2.2, 30)
+    for settings in (dict(), dict(top_k=50), dict(top_p=0.95), dict(top_k=4000, top_p=0.9), dict(temperature=0.7, min_p=0.01)):
+        tokens, logp = sample_tokens(logits, u, **settings)
+        for r in range(0, 80, 9):
+            token, lp = sample_tokens(logits[r:r + 1], u[r:r + 1], **settings)
+            assert int(token) == int(tokens[r]) and abs(float(lp) - float(logp[r])) <= 2.0 ** -22 * (1 + abs(float(lp))) + (2.0 ** -17 if settings.get("top_k") else 0)
+
+
+def test_smallest_and_largest_temperatures():
+    g = torch.Generator().manual_seed(11)
+    u = torch.rand(20, generator=g).cuda()
+    for V in (50, 20000):
+        x = torch.randn(20, V, generator=g)
+        for scale, t in ((1e-35, 1e-35), (1e-30, 3e-31), (1e15, 1e15), (1.0, 2.0 ** 64), (1.0, 1e-300), (3e38, 1e-3)):
+            for settings in (dict(), dict(top_k=10), dict(top_k=3000), dict(top_p=0.9), dict(top_k=30, top_p=0.8, min_p=0.05)):
+                check((scale * x.clamp(-1, 1)).cuda(), u, temperature=t, **settings)
