@@ -2,7 +2,9 @@
 //   (y1, y2) = f (x1 cos a - x2 sin a, x2 cos a + x1 sin a),   a = position * inv_freq[i]
 // for the pairs (i, i + R/2) or (2i, 2i + 1) of a head's first R columns; the columns behind them are copied.  The gradient is the same turn by -a.
 // Bound by memory.  The angle is formed in 64 bits and reduced to a part of a turn in [-1/2, 1/2] before it is rounded to binary32 (a position of 2^20 times a frequency
-// near one has 20 bits before the point, so binary32 would leave 4 behind it); its sine and cosine serve all heads of a token that a lane goes through.
+// near one has 20 bits before the point, so binary32 would leave 4 behind it); its sine and cosine serve all heads of a token that a lane goes through.  8192 tokens of 28 + 4
+// heads of 128 bf16 numbers (134 MB) in 27 us, 65536 in 181 (5.9 TB/s, a large copy 4.9 to 6.9); a token of 12 + 2 heads into a cache in 2.6, 4099 of
+// 28 + 4 heads (76 MB) in 15.
 #include "chunk8.h"
 #include "metis_host.h"
 
@@ -224,10 +226,12 @@ int rotary(const void* q, int64_t q_token, int64_t q_head, int64_t q_heads, cons
     a.q_heads = (int)q_heads; a.k_heads = (int)k_heads; a.dim = (int)dim; a.half = (int)(turned / 2); a.freq64 = freq_dtype == METIS_DTYPE_F64; a.interleaved = interleaved;
     a.units = (int)(dim / (2 * N)); a.turned_units = (int)(turned / (2 * N));
     a.factor = factor; a.sign = back ? -1.0f : 1.0f; a.key_scale = key_scale; a.value_scale = value_scale; a.page = (int)page;
-    // Where the device does not hold all heads' pieces at once, a lane goes through four heads with one set of sines; else every head has lanes of its own.
+    // A lane goes through two heads with one set of sines from two waves' pieces for each of the device's SIMDs on, else every head has lanes of its own (two heads / one / four of
+    // each token, 28 + 4 of 128 numbers: 64 tokens 3.9 / 3.5 / 4.7 us, 512 4.3 / 4.5 / 5.2, 4096 12.4 / 14.6 / 11.9, 8192 26.9 / 28.1 / 28.3, 65536 181 / 194 / 195;
+    // 12 + 2 heads: 512 tokens 4.0 / 3.6 / 4.8, 1024 4.3 / 4.4 / 5.1, 16384 24.4 / 27.2 / 25.9).
     const int heads = a.q_heads + a.k_heads;
-    const bool many = (double)tokens * heads * a.units > (double)device_cus() * 2048;
-    a.head_lanes = many ? (heads + 3) / 4 : heads;
+    const bool two = (double)tokens * heads * a.units > (double)device_cus() * 512;
+    a.head_lanes = two ? (heads + 1) / 2 : heads;
     if (a.head_lanes > 256 / a.units) a.head_lanes = 256 / a.units;
     a.tok_lanes = 256 / (a.units * a.head_lanes);
     const int64_t blocks = (tokens + a.tok_lanes - 1) / a.tok_lanes, v_items = cached ? tokens * k_heads * (dim / (N == 8 ? 8 : 1)) : 0;

@@ -1316,13 +1316,17 @@ __global__ __launch_bounds__(kSampleThreads) void sample_finish_kernel(const Sam
     finish_row<F32>(s, a, r, set, row, w, ready && !(set.min_p > 0.0) ? -1.0 : total, upper, limits, ready);
 }
 
-// Workgroups that share a row, or 0 for one workgroup and one launch: rows that fill a quarter of the device or more, and vocabularies of a few pieces a thread.
+// Workgroups that share a row, or 0 for one workgroup and one launch.  Three launches and the row's sums on their way through memory cost 10 us or so, and a workgroup alone
+// needs 25 us (top_k) to 70 (top_p) for 131072 tokens: rows are shared out from 65536 tokens on, as long as they fill an eighth of the device or less (from 131072: a quarter).
+// In parts and alone, no thresholds / top_k = 50 / top_p = 0.95: a row of 131072 19 / 26 / 33 and 39 / 34 / 80 us, of 65536 19 / 26 / 33 and 25 / 26 / 52, of 50000 20 / 27 / 33 and
+// 21 / 24 / 43, of 32003 21 / 28 / 36 and 18 / 23 / 34; 64 rows of 131072 35 / 38 / 70 and 39 / 34 / 85, of 65536 27 / 33 / 52 and 25 / 26 / 52.
 static int row_parts(int64_t rows, int64_t vocab)
 {
     const int64_t room = (int64_t)device_cus() / rows;
+    if (vocab < 65536 || room < 4 || rows * 131072 > (int64_t)device_cus() / 4 * vocab) return 0;
     int parts = 4;                                                 // (as many threads as a row has alone, or more)
     while (parts < 32 && parts * 2 <= room && vocab >= (int64_t)parts * 2 * kPartThreads * 16) parts *= 2;
-    return room >= 4 && vocab >= 4 * kPartThreads * 16 ? parts : 0;
+    return parts;
 }
 
 struct SampleSpace {

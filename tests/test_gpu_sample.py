@@ -295,3 +295,12 @@ def test_smallest_and_largest_temperatures():
         for scale, t in ((1e-35, 1e-35), (1e-30, 3e-31), (1e15, 1e15), (1.0, 2.0 ** 64), (1.0, 1e-300), (3e38, 1e-3)):
             for settings in (dict(), dict(top_k=10), dict(top_k=3000), dict(top_p=0.9), dict(top_k=30, top_p=0.8, min_p=0.05)):
                 check((scale * x.clamp(-1, 1)).cuda(), u, temperature=t, **settings)
+
+
+@pytest.mark.parametrize("rows,V", [(1, 65535), (1, 65536), (31, 70003), (64, 140001), (65, 140001), (2, 1 << 20)])
+def test_rows_in_parts(rows, V):
+    """Sizes on both sides of those from which several workgroups share a row."""
+    for dtype in (BF, F32):
+        logits, u = rows_of(V + rows, rows, V, dtype, 2.2, 20)
+        for settings in (dict(), dict(top_k=50), dict(top_k=2000, top_p=0.9), dict(top_p=0.95), dict(top_p=0.5, min_p=0.001), dict(top_k=V // 2), dict(temperature=3.0, top_p=0.8)):
+            check(logits, u, **settings)
