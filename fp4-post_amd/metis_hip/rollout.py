@@ -152,6 +152,8 @@ class PagedCache:
 
     def new(self, count: int = 1) -> list[int]:
         """So many empty sequences."""
+        if count < 0:
+            raise ValueError(f"PagedCache: a number of sequences, not {count}")
         ids = list(range(self._next, self._next + count))
         self._next += count
         for i in ids:

@@ -290,3 +290,19 @@ def test_the_attention_modules_parameters_and_frequencies():
     step = cache.extend(cache.new(2), [1, 2])
     with pytest.raises(ValueError, match="one new token"):
         module(torch.zeros(2, 64, dtype=BF), cache, 0, step)
+
+
+def test_numbers_of_sequences():
+    """Fewer than none are refused, and the books are as they were; none are none."""
+    cache = PagedCache(1, 4, 1, 64, device="cpu")
+    (s,) = cache.new()
+    cache.extend([s], [20])
+    for call in (lambda: cache.new(-1), lambda: cache.fork(s, -1), lambda: cache.fork(s, -2)):
+        with pytest.raises(ValueError, match="number of sequences"):
+            call()
+    assert cache.new(0) == cache.fork(s, 0) == []
+    (t,) = cache.fork(s)
+    cache.free([s])
+    assert cache.free_pages == 2 and cache.pages(t) == (0, 1)
+    cache.free([t])
+    assert cache.free_pages == 4 and cache.new() == [2]
