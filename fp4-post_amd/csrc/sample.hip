@@ -15,6 +15,9 @@
 // token now and then.  Each pass is a chain of some twenty 64-bit operations for each token, and what it must not do is go through LDS for each (one LDS
 // operation of a compute unit's sixteen waves costs as much as sixteen of these on its four SIMDs): there are no tables, sums over lanes go by DPP.
 // Rows that do not fill the device are shared out to several workgroups for the passes over all tokens, in launches of their own.
+// 256 rows of 131072 bf16 logits (67 MB, 14 us at a large copy's rate): no thresholds 43 us, top_k = 50 37, top_p = 0.95 87 to 105 (the row that keeps most, 12000 to 14000 tokens,
+// sets the time; most rows take 58 to 70: 10 for the first pass, 5 for the guess of the sum, 5 for the window, 35 for the weights in 64 bits, 13 for the list, the stretches and
+// the draw).  A row whose nucleus lies beyond 20000 tokens takes 170.  One row of 131072 binary32 logits with all settings 26 us: 3.4 + 9.0 + 13.7 in three launches.
 #include <type_traits>
 
 #include "metis_device.h"
