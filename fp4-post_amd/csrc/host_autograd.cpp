@@ -1,5 +1,6 @@
 // residual_norm, swiglu and rotary as nodes of torch's autograd, in compiled code.  Host code only: the arithmetic is libmetis_hip.so's, the checks of arguments are
-// made by the Python functions that call these (metis_hip/block.py, metis_hip/ops.py).
+// made by the Python functions that call these (metis_hip/block.py, metis_hip/ops.py); rotary's are made here first, and what does not pass them is Python's (host time of a rotation and
+// its gradient 44 to 75 us on different hosts before, 39 now).
 //
 // All are kernels of some tens of microseconds in a training step, and a node written in Python costs more than that: recorded, run backward in the
 // engine's own thread (which has to get the interpreter first) and allocated for.  One token x 1536, forward and all gradients: 101 us through
@@ -177,10 +178,14 @@ struct HeadRows {
         if (!given.defined()) return;
         heads = given.size(-2);
         const int64_t dim = given.size(-1);
+        token = heads * dim;
+        head = dim;
+        t = given;
+        if (t.is_contiguous()) return;
         t = given.reshape({tokens, heads, dim});
         if (t.stride(2) != 1) t = t.contiguous();
-        token = tokens > 1 ? t.stride(0) : heads * dim;
-        head = heads > 1 ? t.stride(1) : dim;
+        if (tokens > 1) token = t.stride(0);
+        if (heads > 1) head = t.stride(1);
     }
 };
 
@@ -223,6 +228,28 @@ struct Rotary : torch::autograd::Function<Rotary> {
         return once(std::move(given));
     }
 };
+
+// Whether rotary takes the arguments as they are, positions dense (what is wrong with others the Python functions say).
+bool plain_rotary(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq)
+{
+    const int64_t lead = q.dim() - 2;
+    const auto type = q.scalar_type(), freq = inv_freq.scalar_type();
+    if (!q.is_cuda() || !k.is_cuda() || !positions.is_cuda() || !inv_freq.is_cuda() || lead < 1 || k.dim() != lead + 2 || k.scalar_type() != type ||
+        (type != at::kBFloat16 && type != at::kFloat) || (freq != at::kDouble && freq != at::kFloat) || positions.scalar_type() != at::kLong || inv_freq.requires_grad())
+        return false;
+    const auto device = q.get_device();
+    const int64_t dim = q.size(lead + 1), n = inv_freq.numel();
+    if (k.get_device() != device || positions.get_device() != device || inv_freq.get_device() != device || k.size(lead + 1) != dim || dim % 2 || dim <= 0 || dim > 512 || q.size(lead) <= 0 ||
+        q.size(lead) > 65536 || k.size(lead) <= 0 || k.size(lead) > 65536 || inv_freq.dim() != 1 || n <= 0 || 2 * n > dim || !inv_freq.is_contiguous() || !positions.is_contiguous())
+        return false;
+    int64_t ones = 0;
+    while (ones < positions.dim() && positions.size(ones) == 1) ++ones;
+    const int64_t own = positions.dim() - ones;
+    if (own > lead) return false;
+    for (int64_t i = 0; i < lead; ++i)
+        if (k.size(i) != q.size(i) || (i >= lead - own && positions.size(i - (lead - own) + ones) != q.size(i))) return false;
+    return true;
+}
 
 // The interpreter's lock given up: an allocation may wait for the device.
 struct Unlocked {
@@ -302,8 +329,8 @@ PyObject* metis_recorded_rotary(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
     Tensor t[4];
-    if (n != 6) {
-        PyErr_SetString(PyExc_TypeError, "recorded_rotary(q, k, positions, inv_freq, interleaved, factor)");
+    if (n != 7) {
+        PyErr_SetString(PyExc_TypeError, "recorded_rotary(q, k, positions, inv_freq, interleaved, factor, checked)");
         return nullptr;
     }
     for (int i = 0; i < 4; ++i) {
@@ -316,10 +343,16 @@ PyObject* metis_recorded_rotary(PyObject*, PyObject* const* a, Py_ssize_t n)
     const int interleaved = PyObject_IsTrue(a[4]);
     const double factor = PyFloat_AsDouble(a[5]);
     if (PyErr_Occurred()) return nullptr;
+    if (a[6] != Py_True) {
+        for (int i = 0; i < 4; ++i)
+            if (!THPVariable_CheckExact(a[i])) Py_RETURN_NONE;
+        if (!plain_rotary(t[0], t[1], t[2], t[3])) Py_RETURN_NONE;
+    }
     variable_list r;
     {
         Unlocked unlocked;
-        r = Rotary::apply(t[0], t[1], t[2], t[3], interleaved != 0, factor);
+        if (at::GradMode::is_enabled() && (t[0].requires_grad() || t[1].requires_grad())) r = Rotary::apply(t[0], t[1], t[2], t[3], interleaved != 0, factor);
+        else r = Rotary::turn(t[0], t[1], t[2], t[3], interleaved != 0, factor, false);
     }
     PyObject* q = THPVariable_Wrap(std::move(r[0]));
     PyObject* k = q ? THPVariable_Wrap(std::move(r[1])) : nullptr;

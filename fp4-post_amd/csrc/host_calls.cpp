@@ -301,7 +301,7 @@ PyMethodDef methods[] = {{"call", reinterpret_cast<PyCFunction>(reinterpret_cast
                          {"recorded_swiglu", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&metis_recorded_swiglu)), METH_FASTCALL,
                           "recorded_swiglu(gate, up): swiglu of checked arguments as a node of autograd"},
                          {"recorded_rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&metis_recorded_rotary)), METH_FASTCALL,
-                          "recorded_rotary(q, k, positions, inv_freq, interleaved, factor): rotary of checked arguments as a node of autograd"},
+                          "recorded_rotary(q, k, positions, inv_freq, interleaved, factor, checked): rotary as a node of autograd, or without one where nothing asks for it; None for arguments that are neither checked nor plain"},
                          {"rotary_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&metis_host_rotary_append)), METH_FASTCALL,
                           "rotary_append(q, k, v, positions, inv_freq, slots, keys, values, interleaved, factor, key_scale, value_scale): the turned q, or None where it takes more than the entry point"},
                          {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&metis_host_paged_attention)), METH_FASTCALL,

@@ -168,13 +168,18 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: 
 
     The angles are formed in 64 bits.  The results are dense.  Differentiable (once, in reverse) in q and k."""
     factor = float(factor)
-    if inv_freq.requires_grad:
-        raise ValueError("rotary: no gradient of inv_freq")
     if _transformed():
+        if inv_freq.requires_grad:
+            raise ValueError("rotary: no gradient of inv_freq")
         return _Rotary.apply(q, k, positions, inv_freq, bool(interleaved), factor)
+    out = _lib.host().recorded_rotary(q, k, positions, inv_freq, interleaved, factor, False)
+    if out is not None:
+        return out
+    if inv_freq.requires_grad:                                     # (refused, or positions made dense first)
+        raise ValueError("rotary: no gradient of inv_freq")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
         ops._check_rotary("rotary", q, k, positions, inv_freq)
-        return _lib.host().recorded_rotary(q, k, ops._flat_positions("rotary", positions, q.shape[:-2]), inv_freq, interleaved, factor)
+        return _lib.host().recorded_rotary(q, k, ops._flat_positions("rotary", positions, q.shape[:-2]), inv_freq, interleaved, factor, True)
     return ops.rotary(q, k, positions, inv_freq, interleaved, factor)
 
 
