@@ -252,3 +252,110 @@ def test_traced_calls_and_tangents():
                      lambda: sample_tokens(fwd.make_dual(torch.zeros(2, 5).cuda(), torch.ones(2, 5).cuda()), u)):
             with pytest.raises(NotImplementedError, match="jvp"):
                 call()
+
+
+def test_calls_of_several_threads():
+    """Four threads, each on a stream of its own, make the calls of a step at once (the interpreter is given up inside them): the results of one after the other."""
+    import threading
+    from metis_hip import paged_attention, rotary, rotary_append, rotary_frequencies, sample_tokens
+    inv = rotary_frequencies(64)[0].cuda()
+
+    def step(seed, rounds):
+        g = torch.Generator().manual_seed(seed)
+        q, k, v = (torch.randn(9, h, 64, generator=g).to(BF).cuda() for h in (6, 2, 2))
+        keys, values = torch.zeros(20, 2, 16, 64, dtype=BF, device="cuda"), torch.zeros(20, 2, 64, 16, dtype=BF, device="cuda")
+        positions, slots = torch.arange(9).cuda(), torch.randperm(160, generator=g)[:9].cuda()
+        tables, lengths = torch.arange(20, dtype=torch.int32).reshape(2, 10).cuda(), torch.tensor([160, 33], dtype=torch.int32).cuda()
+        logits, u = 3 * torch.randn(70, 5003, generator=g).to(BF).cuda(), torch.rand(70, generator=g).cuda()
+        for _ in range(rounds):
+            leaf = q.clone().requires_grad_()
+            turned, _ = rotary(leaf, k, positions, inv)
+            (grad,) = torch.autograd.grad(turned, leaf, q)
+            new = rotary_append(q, k, v, positions, inv, slots, keys, values)
+            o = paged_attention(new[:2], keys, values, tables, lengths)
+            out = [turned.detach(), grad, new, o, *sample_tokens(logits, u, top_p=0.9), *sample_tokens(logits[:2], u[:2], top_k=30)]
+        return out
+
+    want = [step(seed, 1) for seed in range(4)]
+    torch.cuda.synchronize()
+    got, failed = [None] * 4, []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got[i] = step(i, 20)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                                         # (shown by the test's own thread)
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for mine, exact in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(mine, exact))
+
+
+def test_arguments_of_other_kinds():
+    """What the compiled calls leave to Python gives the same: parameters, numbers of other types, tuples of pages, strided and misaligned tensors, positions of a batch."""
+    from metis_hip import copy_pages, paged_attention, rotary, rotary_append, rotary_frequencies, sample_tokens
+    g = torch.Generator().manual_seed(3)
+    inv = rotary_frequencies(64)[0].cuda()
+    q, k, v = (torch.randn(4, 5, h, 64, generator=g).to(BF).cuda() for h in (6, 2, 2))
+    positions = torch.randint(900, (4, 5), generator=g).cuda()
+    want = rotary(q, k, positions, inv)
+    with torch.no_grad():
+        for args in ((nn.Parameter(q), k, positions, inv), (q, k, positions.t().contiguous().t(), inv), (q.transpose(0, 1).contiguous().transpose(0, 1), k, positions, inv),
+                     (torch.cat((q, k), 2)[:, :, :6], torch.cat((q, k), 2)[:, :, 6:], positions, inv), (torch.stack((q, q), -1)[..., 0], k, positions, inv)):
+            assert all(torch.equal(a, b) for a, b in zip(rotary(*args), want))
+    flat, slots = [t.flatten(0, 1) for t in (q, k, v)], torch.randperm(48, generator=g)[:20].cuda()
+    def fresh():
+        return torch.zeros(3, 2, 16, 64, dtype=BF, device="cuda"), torch.zeros(3, 2, 64, 16, dtype=BF, device="cuda")
+    keys, values = fresh()
+    new = rotary_append(*flat, positions.flatten(), inv, slots, keys, values)
+    wide = torch.zeros(20, 10, 65, dtype=BF, device="cuda")
+    wide[:, :6, 1:], wide[:, 6:8, 1:], wide[:, 8:, 1:] = flat
+    for args in ((wide[:, :6, 1:], wide[:, 6:8, 1:], wide[:, 8:, 1:], positions.flatten(), inv, slots), (*flat, positions.flatten(), inv, torch.stack((slots, slots), 1)[:, 0])):
+        other = fresh()
+        assert torch.equal(rotary_append(*args, *other), new) and torch.equal(other[0], keys) and torch.equal(other[1], values)
+    tables, lengths = torch.tensor([[0, 1, 2], [2, 0, 0]], dtype=torch.int32).cuda(), torch.tensor([48, 9], dtype=torch.int32).cuda()
+    o = paged_attention(new[:2], keys, values, tables, lengths)
+    for args in ((wide[:2, :6, 1:].copy_(new[:2]), keys, values, tables, lengths), (new[:2], keys, values, torch.stack((tables, tables), -1)[..., 0], torch.stack((lengths, lengths), 1)[:, 0])):
+        assert torch.equal(paged_attention(*args), o)
+    assert torch.equal(paged_attention(new[:2], keys, values, tables, lengths, scale=torch.tensor(0.125)), o)
+    pool = [torch.stack((t, t + 1)) for t in (keys, values)]
+    moved = [t.clone() for t in pool]
+    copy_pages(*moved, [0], [2])
+    for sources, destinations in (((0,), (2,)), (torch.tensor([0]), torch.tensor([2]))):
+        other = [t.clone() for t in pool]
+        copy_pages(*other, sources, destinations)
+        assert all(torch.equal(a, b) for a, b in zip(other, moved))
+    logits, u = torch.randn(6, 700, generator=g).cuda(), torch.rand(6, generator=g).cuda()
+    want = sample_tokens(logits, u, temperature=0.5, top_k=20)
+    for settings in (dict(temperature=torch.full((6,), 0.5, device="cuda"), top_k=20), dict(temperature=0.5, top_k=torch.full((6,), 20, device="cuda"))):
+        assert all(torch.equal(a, b) for a, b in zip(sample_tokens(logits, u, **settings), want))
+    for other in (logits.t().contiguous().t(), torch.cat((logits, logits), 1)[:, :700], torch.cat((logits[:, :1], logits), 1)[:, 1:]):
+        assert all(torch.equal(a, b) for a, b in zip(sample_tokens(other, torch.stack((u, u), 1)[:, 0], temperature=0.5, top_k=20), want))
+
+
+def test_a_captured_draw_from_a_nucleus():
+    """Rows in parts and rows alone, captured and replayed on other logits, with eager calls of the same sizes between the replays."""
+    from metis_hip import sample_tokens
+    g = torch.Generator().manual_seed(4)
+    logits = [3 * torch.randn(r, v, generator=g).cuda() for r, v in ((2, 70001), (80, 20011))]
+    u = [torch.rand(r, generator=g).cuda() for r in (2, 80)]
+    held = [t.clone() for t in logits]
+    draws = [sample_tokens(x, n, top_p=0.9) for x, n in zip(held, u)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        draws = [sample_tokens(x, n, top_p=0.9) for x, n in zip(held, u)]
+    for turn in range(4):
+        for h, x in zip(held, logits):
+            h.copy_(x.roll(turn * 7, 1) * (1 + turn / 2))
+        graph.replay()
+        eager = [sample_tokens(h, n, top_p=0.9) for h, n in zip(held, u)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for got, want in zip(draws, eager) for a, b in zip(got, want))
