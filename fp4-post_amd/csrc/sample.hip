@@ -3,11 +3,11 @@
 //   K1 the first k of them, K2 those of K1 with less than p sum(K1) of weight before them, K3 those of K2 with w >= min_p;
 //   the lowest index i of K3 with  sum_{j <= i, j in K3} w_j > u sum(K3),   log p_i = log w_i - log sum_i w_i  (of all tokens, not of K3 alone)
 // The vocabulary is not sorted.  A token's depth is the binary logarithm of 1 / w, its bin the depth in 1/64.  A first pass finds the row's maximum (with p, also a sum of all
-// weights that is good to a few digits) and 4096 maxima over disjoint shares of the row, a second one adds up all weights and takes out the tokens that a threshold lies
+// weights that is good to a few digits) and 8192 maxima over disjoint shares of the row, a second one adds up all weights and takes out the tokens that a threshold lies
 // among as a rule:
 //   k  those in the bins down to the one that holds the k-th largest of the maxima: at least k;
 //   p  those in a window of bins around the one in which the weights reach p of their sum, by a guess: where M of S shares have a maximum in the bins down to one, about
-//      V (1 - (1 - M / S)^(S / V)) tokens lie there (to some 3 percent where that are 16000); those above the window are kept, and added up by stretches of 512 indices at once.
+//      V (1 - (1 - M / S)^(S / V)) tokens lie there (to 1.3 percent where that are 12000 of 131072); those above the window are kept, and added up by stretches of 512 indices at once.
 // They are sorted where they are few; else they are counted (k) and their weights added up (p) by bins, in whole numbers, so that the order of the additions does not
 // count, and the tokens of the bin that holds a threshold are sorted.  What is kept of them is added to the stretches' sums for the draw, in whole numbers again.  Where
 // the thresholds lie elsewhere (large k, flat rows), further passes over the row do the same with all tokens, and narrow a bin of too many by digits of its logits and indices.
@@ -15,9 +15,9 @@
 // token now and then.  Each pass is a chain of some twenty 64-bit operations for each token, and what it must not do is go through LDS for each (one LDS
 // operation of a compute unit's sixteen waves costs as much as sixteen of these on its four SIMDs): there are no tables, sums over lanes go by DPP.
 // Rows that do not fill the device are shared out to several workgroups for the passes over all tokens, in launches of their own.
-// 256 rows of 131072 bf16 logits (67 MB, 14 us at a large copy's rate): no thresholds 43 us, top_k = 50 37, top_p = 0.95 87 to 105 (the row that keeps most, 12000 to 14000 tokens,
-// sets the time; most rows take 58 to 70: 10 for the first pass, 5 for the guess of the sum, 5 for the window, 35 for the weights in 64 bits, 13 for the list, the stretches and
-// the draw).  A row whose nucleus lies beyond 20000 tokens takes 170.  One row of 131072 binary32 logits with all settings 26 us: 3.4 + 9.0 + 13.7 in three launches.
+// 256 rows of 131072 bf16 logits (67 MB, 14 us at a large copy's rate): no thresholds 43 us, top_k = 50 38, top_p = 0.95 88 to 106 (the row that keeps most, 12000 to 14000 tokens,
+// sets the time; most rows take 62 to 72: 12 for the first pass, 5 for the guess of the sum, 7 for the window, 35 for the weights in 64 bits, 4 to 14 for the list, 6 for the
+// stretches and the draw).  A row whose nucleus lies beyond 30000 of them takes 168.  One row of 131072 binary32 logits with all settings 26 us: 3.3 + 11 + 12.5 in three launches.
 #include <type_traits>
 
 #include "metis_device.h"
@@ -30,8 +30,7 @@ constexpr int kPartThreads = 256;                                  // of one tha
 constexpr int kBins = 4096;                                        // 64 octaves; the last one holds everything below them
 constexpr int kTaken = 16384, kPartTaken = 8192;                   // tokens that are taken out of a row, and of a part of one
 constexpr int kList = 1024;                                        // tokens that can be sorted
-constexpr int kShares = 4096;                                      // maxima of a row
-constexpr int kSharesOfK = 3900;                                   // the largest k that tokens are taken out for: some 12500
+constexpr int kShares = 8192;                                      // maxima of a row
 constexpr double kLowTemperatures = 0x1p100;                       // 1 / T from which depths do not fit binary32
 constexpr double kUnit = 0x1p41;                                   // a weight of its bin's octave, as a whole number
 constexpr double kKeptUnit = 0x1p50;                               // a kept weight of a stretch
@@ -49,7 +48,7 @@ struct SampleArgs {
     double* sums;                                                  // [rows][parts][2]: of all weights, of those above the window
     double* stretches;
     uint32_t *taken, *filled;
-    int* limits;                                                   // [rows][2]
+    int* limits;                                                   // [rows][3]: the window's bins, the largest logit
     int rows, vocab, parts;
 };
 
@@ -106,6 +105,28 @@ template <int THREADS, class V> __device__ __forceinline__ V scan(V v, V* waves,
     const V sums = wave_scan(lane < THREADS / 64 ? waves[lane] : (V)0);
     all = lane_value(sums, THREADS / 64 - 1);
     return wave > 0 ? v + lane_value(sums, wave - 1) : v;
+}
+
+// N of them at once: exclusive
+template <int THREADS, int N> __device__ __forceinline__ void scan_several(float (&v)[N], float* waves)
+{
+    const int tid = thread_anew(), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    float own[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        own[i] = v[i];
+        v[i] = wave_scan(v[i]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (lane == 63) waves[i * (THREADS / 64) + wave] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float sums = wave_scan(lane < THREADS / 64 ? waves[i * (THREADS / 64) + lane] : 0.0f);
+        v[i] = (wave > 0 ? v[i] + lane_value(sums, wave - 1) : v[i]) - own[i];
+    }
 }
 
 // a row's logits in pieces of eight whose addresses are multiples of 16 bytes: the first and the last may reach beyond the row (those are -inf, with indices >= vocab)
@@ -296,6 +317,7 @@ template <int THREADS, int TAKEN> struct SampleShared {
     double waves_d[WAVES];
     uint64_t waves_u[WAVES];
     uint32_t waves_n[WAVES];
+    float waves_f[3 * WAVES];
     float tops[WAVES];
     int found_i, found_bins[2];
     uint32_t filled;
@@ -375,15 +397,18 @@ template <int THREADS> __device__ __forceinline__ float guessed_sum(float most, 
 // needed anyhow).
 struct Limits {
     int first = 0, last = -1;
+    __device__ __forceinline__ static float bin_weight(int b) { return __builtin_amdgcn_exp2f((float)b * (-1.0f / 64.0f)); }
     // rest: what the guess says besides the maxima (rest_of).  s.weight and s.taken are used
     template <int THREADS, int RESTS, class S>
     __device__ __forceinline__ void find(S& s, const RowSettings& set, const Weigher& w, const float (&mine)[kShares / THREADS], const float (&rest)[RESTS], float guess, int vocab, int pieces)
     {
-        if (set.by_k ? set.top_k > (double)kSharesOfK : !set.by_p) return;
+        const int filled_shares = min(pieces, kShares);
+        // (k up to 5/6 of the shares: some 14000 of 131072 tokens)
+        if (set.by_k ? vocab > kTaken && set.top_k > (double)(filled_shares / 6 * 5) : !set.by_p) return;
         const int tid = threadIdx.x;
         constexpr int per = kBins / THREADS;
         uint32_t* const count = reinterpret_cast<uint32_t*>(s.weight);
-        unsigned long long* const weight = reinterpret_cast<unsigned long long*>(s.taken);               // of the maxima, in units of 2^-40
+        unsigned long long* const weight = reinterpret_cast<unsigned long long*>(s.taken);               // beside what the counts say, in units of 2^-40 (signed)
         static_assert(sizeof s.taken >= kBins * 8, "");
         for (int b = tid; b < kBins / 2; b += THREADS) s.weight[b] = 0;
         for (int b = tid; b < kBins; b += THREADS) weight[b] = 0;
@@ -391,9 +416,18 @@ struct Limits {
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < kShares / THREADS; ++j) {
-            const auto d = w.depth(w.settled(mine[j]));
-            atomicAdd(&count[min(d.bin, kBins - 1)], 1u);
-            if (!set.by_k) atomicAdd(&weight[min(d.bin, kBins - 1)], (unsigned long long)(__builtin_amdgcn_exp2f(-(float)((double)d.octave + d.r)) * 0x1p40f));
+            // (empty shares: what many lanes add to one place goes there one by one)
+            if (pieces >= kShares || mine[j] > -INFINITY) atomicAdd(&count[min(w.depth(w.settled(mine[j])).bin, kBins - 1)], 1u);
+        }
+        if (!set.by_k) {                                           // of the heavy ones the weight itself, where the bin's is off by up to half a percent
+            const float heavy = w.settled(w.top32) - 9.0f / w.rate32;              // (2^-9 < 0.002; the sum is at least 1)
+#pragma unroll
+            for (int j = 0; j < kShares / THREADS; ++j) {
+                if (!(w.settled(mine[j]) > heavy)) continue;
+                const auto d = w.depth(w.settled(mine[j]));
+                const float v = __builtin_amdgcn_exp2f(-(float)((double)d.octave + d.r));
+                atomicAdd(&weight[min(d.bin, kBins - 1)], (unsigned long long)(long long)((v - bin_weight(d.bin)) * 0x1p40f));
+            }
         }
         if (!set.by_k) {
 #pragma unroll
@@ -424,17 +458,17 @@ struct Limits {
             return;
         }
         // the weights of the maxima, and of the others that are guessed to lie in the same bins
-        const float shares = (float)min(pieces, kShares), most = shares * 0.995f;
+        const float shares = (float)filled_shares, most = shares * 0.995f;
         const auto tokens = [&](uint32_t m) __attribute__((always_inline)) { return (float)vocab * (1.0f - __builtin_amdgcn_exp2f(__log2f(1.0f - fminf((float)m, most) / shares) * (shares / (float)vocab))); };
         if (!(guess < INFINITY)) guess = 1.0f;                     // (rows of infinities)
         const float plain = 0.002f * guess;                        // a hidden token of more weight is known from `rest`
-        float known[per], hidden[per], square[per], sum = 0.0f, sum_hidden = 0.0f, sum_square = 0.0f, told = tokens(before), whole;
+        float known[per], hidden[per], square[per], sum = 0.0f, sum_hidden = 0.0f, sum_square = 0.0f, told = tokens(before);
 #pragma unroll
         for (int j = 0; j < per; ++j) {
             m += c[j];
             const float now = c[j] ? tokens(m) : told;
-            known[j] = (float)weight[per * tid + j] * 0x1p-40f;
-            const float each = __builtin_amdgcn_exp2f((float)(per * tid + j) * (-1.0f / 64.0f));
+            const float each = bin_weight(per * tid + j);
+            known[j] = fmaf((float)c[j], each, (float)(long long)weight[per * tid + j] * 0x1p-40f);
             hidden[j] = each > plain ? 0.0f : fmaxf(now - told - (float)c[j], 0.0f) * each;
             square[j] = hidden[j] * each;
             sum += known[j] + hidden[j];
@@ -442,11 +476,11 @@ struct Limits {
             sum_square += square[j];
             told = now;
         }
-        float* const waves = reinterpret_cast<float*>(s.waves_n);
-        float front = scan<THREADS>(sum, waves, whole) - sum, front_hidden = scan<THREADS>(sum_hidden, waves, whole) - sum_hidden;
-        float front_square = scan<THREADS>(sum_square, waves, whole) - sum_square;
+        float fronts[3] = {sum, sum_hidden, sum_square};
+        scan_several<THREADS>(fronts, s.waves_f);
+        float front = fronts[0], front_hidden = fronts[1], front_square = fronts[2];
         // The window: where the guess is that far from p of the sum that it may be off by that.  (Of n hidden tokens the deviation is sqrt(n) where they are few, 2.1 sqrt(n) where
-        // 6000 of 131072 lie down to there, 2.9 sqrt(n) where 12000 do.)
+        // 12000 of 131072 lie down to there.)
         const float goal = (float)set.top_p * guess;
         const auto error = [&]() __attribute__((always_inline)) { return 0.001f * guess + 0.02f * front_hidden + 6.0f * __builtin_amdgcn_sqrtf(fmaxf(front_square, 0.0f)); };
         m = before;
@@ -1186,9 +1220,8 @@ __global__ __launch_bounds__(kPartThreads) void sample_tops_kernel(const SampleA
     const RowSettings set(a, r);
     const LogitRow<F32> row(static_cast<const char*>(a.logits) + (size_t)r * a.ld * (F32 ? 4 : 2), a.vocab);
     const int at = part * kPartThreads + tid, all = a.parts * kPartThreads;
-    // (a thread's pieces are dealt to several shares, or several threads have one)
-    constexpr int SLOTS = kShares / kSampleThreads;
-    const int slots = max(kShares / all, 1), per = max(all / kShares, 1);
+    constexpr int SLOTS = kShares / (4 * kPartThreads);            // (a thread's pieces are dealt to several shares)
+    const int slots = kShares / all;
     const float rate = guess_rate(set);
     float top[SLOTS], most, guess;
     own_largest<F32, SLOTS>(row, at, row.pieces, all, slots, rate, top, most, guess);
@@ -1198,30 +1231,24 @@ __global__ __launch_bounds__(kPartThreads) void sample_tops_kernel(const SampleA
         const float sum = guessed_sum<kPartThreads>(most, guess, highest, rate, waves);
         if (tid < 2) a.guesses[2 * ((size_t)r * a.parts + part) + tid] = tid ? sum : highest;
     }
-    for (int o = 1; o < per; o <<= 1) {                            // (one slot then)
-        const float other = __shfl_xor(top[0], o, 64), other_most = __shfl_xor(most, o, 64), other_guess = __shfl_xor(guess, o, 64), both = fmaxf(most, other_most);
-        top[0] = top[0] != top[0] || other != other ? __builtin_nanf("") : fmaxf(top[0], other);
-        guess = (guess > 0.0f ? guess * __builtin_amdgcn_exp2f((most - both) * rate) : 0.0f) + (other_guess > 0.0f ? other_guess * __builtin_amdgcn_exp2f((other_most - both) * rate) : 0.0f);
-        most = both;
-    }
-    if (rate > 0.0f && at % per == 0) a.rests[(size_t)r * kShares + at / per] = rest_of(top, most, guess, rate);
+    if (rate > 0.0f) a.rests[(size_t)r * kShares + at] = rest_of(top, most, guess, rate);
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k)
-        if (k < slots && at % per == 0) a.tops[(size_t)r * kShares + k * all + at / per] = top[k];
+        if (k < slots) a.tops[(size_t)r * kShares + k * all + at] = top[k];
     if (at == 0) a.filled[r] = 0;
 }
 
-template <int THREADS> __device__ __forceinline__ float row_top(const SampleArgs& a, int r, float (&mine)[kShares / THREADS], float* waves)
+__device__ __forceinline__ float row_top(const SampleArgs& a, int r, float (&mine)[kShares / kPartThreads], float* waves)
 {
     float top = -INFINITY;
     bool nan = false;
 #pragma unroll
-    for (int j = 0; j < kShares / THREADS; ++j) {
-        mine[j] = a.tops[(size_t)r * kShares + threadIdx.x + j * THREADS];
+    for (int j = 0; j < kShares / kPartThreads; ++j) {
+        mine[j] = a.tops[(size_t)r * kShares + threadIdx.x + j * kPartThreads];
         nan |= mine[j] != mine[j];
         top = fmaxf(top, mine[j]);
     }
-    return largest<THREADS>(nan ? __builtin_nanf("") : top, waves);
+    return largest<kPartThreads>(nan ? __builtin_nanf("") : top, waves);
 }
 
 // 2: the sum of all weights, and the tokens that are taken out or the stretches' sums
@@ -1233,7 +1260,8 @@ __global__ __launch_bounds__(kPartThreads) void sample_bins_kernel(const SampleA
     const RowSettings set(a, r);
     const LogitRow<F32> row(static_cast<const char*>(a.logits) + (size_t)r * a.ld * (F32 ? 4 : 2), a.vocab);
     float mine[kShares / kPartThreads];
-    const float top = row_top<kPartThreads>(a, r, mine, s.tops);
+    const float top = row_top(a, r, mine, s.tops);
+    if (part == 0 && tid == 0) a.limits[3 * (size_t)r + 2] = __float_as_int(top);
     if (!(top > -INFINITY) || !set.fit()) return;
     const Weigher w(top, set.rate());
     float guess = 0.0f, rest[kShares / kPartThreads];
@@ -1246,8 +1274,8 @@ __global__ __launch_bounds__(kPartThreads) void sample_bins_kernel(const SampleA
     Limits limits;
     limits.find<kPartThreads>(s, set, w, mine, rest, guess, a.vocab, row.pieces);
     if (part == 0 && tid == 0) {
-        a.limits[2 * (size_t)r] = limits.first;
-        a.limits[2 * (size_t)r + 1] = limits.last;
+        a.limits[3 * (size_t)r] = limits.first;
+        a.limits[3 * (size_t)r + 1] = limits.last;
     }
     if (tid == 0) s.filled = 0;
     __syncthreads();
@@ -1293,8 +1321,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_finish_kernel(const Sam
     const int tid = threadIdx.x, r = blockIdx.x;
     const RowSettings set(a, r);
     const LogitRow<F32> row(static_cast<const char*>(a.logits) + (size_t)r * a.ld * (F32 ? 4 : 2), a.vocab);
-    float mine[kShares / kSampleThreads];
-    const float top = row_top<kSampleThreads>(a, r, mine, s.tops);
+    const float top = __int_as_float(a.limits[3 * (size_t)r + 2]);
     if (!(top > -INFINITY) || !set.fit()) {
         if (tid == 0) {
             a.tokens[r] = -1;
@@ -1306,8 +1333,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_finish_kernel(const Sam
     const bool ready = !set.by_k && !set.by_p && stretches_fit(row.pieces);
     const uint32_t filled = a.filled[r];
     Limits limits;                                                 // (those that the launch before took: sums in another order might give others)
-    limits.first = a.limits[2 * (size_t)r];
-    limits.last = a.limits[2 * (size_t)r + 1];
+    limits.first = a.limits[3 * (size_t)r];
+    limits.last = a.limits[3 * (size_t)r + 1];
     if (tid == 0) s.filled = filled;
     const int stretches = min((row.pieces + 63) / 64, kBins);
     for (int b = tid; b < stretches; b += kSampleThreads) (ready ? reinterpret_cast<double*>(s.weight) : s.above)[b] = a.stretches[(size_t)r * kBins + b];
@@ -1320,9 +1347,9 @@ __global__ __launch_bounds__(kSampleThreads) void sample_finish_kernel(const Sam
 }
 
 // Workgroups that share a row, or 0 for one workgroup and one launch.  Three launches and the row's sums on their way through memory cost 10 us or so, and a workgroup alone
-// needs 25 us (top_k) to 70 (top_p) for 131072 tokens: rows are shared out from 65536 tokens on, as long as they fill an eighth of the device or less (from 131072: a quarter).
-// In parts and alone, no thresholds / top_k = 50 / top_p = 0.95: a row of 131072 19 / 26 / 33 and 39 / 34 / 80 us, of 65536 19 / 26 / 33 and 25 / 26 / 52, of 50000 20 / 27 / 33 and
-// 21 / 24 / 43, of 32003 21 / 28 / 36 and 18 / 23 / 34; 64 rows of 131072 35 / 38 / 70 and 39 / 34 / 85, of 65536 27 / 33 / 52 and 25 / 26 / 52.
+// needs 35 us (top_k) to 65 and more (top_p) for 131072 tokens: rows are shared out from 65536 tokens on, as long as they fill an eighth of the device or less (from 131072: a
+// quarter).  In parts and alone, no thresholds / top_k = 50 / top_p = 0.95: a row of 131072 18 / 27 / 40 and 41 / 37 / 70, of 65536 19 / 27 / 36 and 25 / 28 / 45, of 50000 20 / 27 / 33
+// and 21 / 24 / 35, of 32003 21 / 28 / 36 and 18 / 22 / 30; 64 rows of 131072 35 / 40 / 78 and 41 / 37 / 85, of 65536 27 / 33 / 52 and 26 / 28 / 54.
 static int row_parts(int64_t rows, int64_t vocab)
 {
     const int64_t room = (int64_t)device_cus() / rows;
@@ -1345,7 +1372,7 @@ struct SampleSpace {
         rests = guesses + n * (size_t)parts * 8;
         filled = rests + n * kShares * 4;
         limits = filled + n * 4;
-        bytes = limits + n * 8;
+        bytes = limits + n * 12;
     }
 };
 size_t sample_tokens_workspace_bytes(int64_t rows, int64_t vocab)
