@@ -3,7 +3,7 @@
 //   K1 the first k of them, K2 those of K1 with less than p sum(K1) of weight before them, K3 those of K2 with w >= min_p;
 //   the lowest index i of K3 with  sum_{j <= i, j in K3} w_j > u sum(K3),   log p_i = log w_i - log sum_i w_i  (of all tokens, not of K3 alone)
 // The vocabulary is not sorted.  A token's depth is the binary logarithm of 1 / w, its bin the depth in 1/64.  A first pass finds the row's maximum (with p, also a sum of all
-// weights that is good to a few digits) and 8192 maxima over disjoint shares of the row, a second one adds up all weights and takes out the tokens that a threshold lies
+// weights that is good to a few digits) and 8192 maxima over disjoint shares of the row (up to 8192 tokens: each one of them), a second one adds up all weights and takes out the tokens that a threshold lies
 // among as a rule:
 //   k  those in the bins down to the one that holds the k-th largest of the maxima: at least k;
 //   p  those in a window of bins around the one in which the weights reach p of their sum, by a guess: where M of S shares have a maximum in the bins down to one, about
@@ -346,7 +346,7 @@ template <int THREADS> __device__ __forceinline__ float largest(float top, float
     return __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(wave_max(top))));
 }
 // The largest logits of this thread's pieces (first, first + step, ..), dealt to `slots` shares (a power of two up to SLOTS; -inf: of an empty one); NaN where one is.
-// guess: with rate > 0 the sum of their weights as seen from the largest of them, `most_of_all`, in binary32.
+// Where a thread has one piece at most, its eight logits are the shares.  guess: with rate > 0 the sum of their weights as seen from the largest of them, `most_of_all`, in binary32.
 template <bool F32, int SLOTS>
 __device__ __forceinline__ void own_largest(const LogitRow<F32>& row, int first, int end, int step, int slots, float rate, float (&top)[SLOTS], float& most_of_all, float& guess)
 {
@@ -363,8 +363,13 @@ __device__ __forceinline__ void own_largest(const LogitRow<F32>& row, int first,
             nan |= x[j] != x[j];
             most = fmaxf(most, x[j]);
         }
+        if (SLOTS == 8 && slots == 8 && end <= step) {
 #pragma unroll
-        for (int k = 0; k < SLOTS; ++k) top[k] = k == (turn & (slots - 1)) ? fmaxf(top[k], most) : top[k];
+            for (int k = 0; k < SLOTS; ++k) top[k] = x[k % 8];
+        } else {
+#pragma unroll
+            for (int k = 0; k < SLOTS; ++k) top[k] = k == (turn & (slots - 1)) ? fmaxf(top[k], most) : top[k];
+        }
         ++turn;
         if (rate > 0.0f) {
             const float now = fmaxf(most_of_all, most), from = now == -INFINITY ? 0.0f : now;
@@ -402,7 +407,8 @@ struct Limits {
     template <int THREADS, int RESTS, class S>
     __device__ __forceinline__ void find(S& s, const RowSettings& set, const Weigher& w, const float (&mine)[kShares / THREADS], const float (&rest)[RESTS], float guess, int vocab, int pieces)
     {
-        const int filled_shares = min(pieces, kShares);
+        const bool exact = pieces <= THREADS && kShares == 8 * THREADS;        // every token is a share
+        const int filled_shares = exact ? vocab : min(pieces, kShares);
         // (k up to 5/6 of the shares: some 14000 of 131072 tokens)
         if (set.by_k ? vocab > kTaken && set.top_k > (double)(filled_shares / 6 * 5) : !set.by_p) return;
         const int tid = threadIdx.x;
@@ -458,8 +464,8 @@ struct Limits {
             return;
         }
         // the weights of the maxima, and of the others that are guessed to lie in the same bins
-        const float shares = (float)filled_shares, most = shares * 0.995f;
-        const auto tokens = [&](uint32_t m) __attribute__((always_inline)) { return (float)vocab * (1.0f - __builtin_amdgcn_exp2f(__log2f(1.0f - fminf((float)m, most) / shares) * (shares / (float)vocab))); };
+        const float shares = (float)filled_shares, most = exact ? shares : shares * 0.995f;
+        const auto tokens = [&](uint32_t m) __attribute__((always_inline)) { return exact ? (float)m : (float)vocab * (1.0f - __builtin_amdgcn_exp2f(__log2f(1.0f - fminf((float)m, most) / shares) * (shares / (float)vocab))); };
         if (!(guess < INFINITY)) guess = 1.0f;                     // (rows of infinities)
         const float plain = 0.002f * guess;                        // a hidden token of more weight is known from `rest`
         float known[per], hidden[per], square[per], sum = 0.0f, sum_hidden = 0.0f, sum_square = 0.0f, told = tokens(before);

@@ -304,3 +304,14 @@ def test_rows_in_parts(rows, V):
         logits, u = rows_of(V + rows, rows, V, dtype, 2.2, 20)
         for settings in (dict(), dict(top_k=50), dict(top_k=2000, top_p=0.9), dict(top_p=0.95), dict(top_p=0.5, min_p=0.001), dict(top_k=V // 2), dict(temperature=3.0, top_p=0.8)):
             check(logits, u, **settings)
+
+
+@pytest.mark.parametrize("V", [1023, 1025, 4001, 8177, 8184, 8185, 8192, 8193, 8200])
+def test_sizes_around_the_lists(V):
+    """Vocabularies on both sides of what is sorted at once and of where every token is a share, at every alignment; thresholds far down, and beyond 64 octaves."""
+    for dtype in (BF, F32):
+        wide, u = rows_of(V, 20, V + 8, dtype, 2.2, 20)
+        for first in (0, 1, 5, 8):
+            logits = wide[:, first:first + V]
+            for settings in (dict(top_k=20), dict(top_k=V - 1), dict(top_k=V // 2, top_p=0.9), dict(top_p=0.95), dict(top_p=0.9999), dict(temperature=0.05, top_k=V // 2), dict(temperature=0.03, top_p=0.999)):
+                check(logits, u, **settings)
