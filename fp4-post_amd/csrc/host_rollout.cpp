@@ -5,6 +5,7 @@
 // 16 -> 7.1.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <cmath>
 #include <limits>
 #include <vector>
 #include <ATen/core/grad_mode.h>

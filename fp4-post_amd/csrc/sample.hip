@@ -426,7 +426,7 @@ struct Limits {
             if (pieces >= kShares || mine[j] > -INFINITY) atomicAdd(&count[min(w.depth(w.settled(mine[j])).bin, kBins - 1)], 1u);
         }
         if (!set.by_k) {                                           // of the heavy ones the weight itself, where the bin's is off by up to half a percent
-            const float heavy = w.settled(w.top32) - 9.0f / w.rate32;              // (2^-9 < 0.002; the sum is at least 1)
+            const float heavy = w.top32 - 9.0f / w.rate32;         // (2^-9 < 0.002; the sum is at least 1)
 #pragma unroll
             for (int j = 0; j < kShares / THREADS; ++j) {
                 if (!(w.settled(mine[j]) > heavy)) continue;
