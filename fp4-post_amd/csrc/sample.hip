@@ -17,7 +17,7 @@
 // Rows that do not fill the device are shared out to several workgroups for the passes over all tokens, in launches of their own.
 // 256 rows of 131072 bf16 logits (67 MB, 14 us at a large copy's rate): no thresholds 43 us, top_k = 50 38, top_p = 0.95 88 to 106 (the row that keeps most, 12000 to 14000 tokens,
 // sets the time; most rows take 62 to 72: 12 for the first pass, 5 for the guess of the sum, 7 for the window, 35 for the weights in 64 bits, 4 to 14 for the list, 6 for the
-// stretches and the draw).  A row whose nucleus lies beyond 30000 of them takes 168.  One row of 131072 binary32 logits with all settings 26 us: 3.3 + 11 + 12.5 in three launches.
+// stretches and the draw).  Rows that keep more than 27000 of them take 150 to 168.  One row of 131072 binary32 logits with all settings 26 us: 3.3 + 11 + 12.5 in three launches.
 #include <type_traits>
 
 #include "metis_device.h"
@@ -493,7 +493,7 @@ struct Limits {
         scan_several<THREADS>(fronts, s.waves_f);
         float front = fronts[0], front_hidden = fronts[1], front_square = fronts[2];
         // The window: where the guess is that far from p of the sum that it may be off by that.  (Of n hidden tokens the deviation is sqrt(n) where they are few, 2.1 sqrt(n) where
-        // 12000 of 131072 lie down to there.  Of 1200 rows of 131072 with 1 to 30000 tokens kept the window missed none.)
+        // 12000 of 131072 lie down to there.  Of 1200 rows of 131072 the window missed none that keeps up to 27000 tokens.)
         const float goal = (float)set.top_p * guess;
         const auto error = [&]() __attribute__((always_inline)) { return 0.001f * guess + 0.02f * front_hidden + 6.0f * __builtin_amdgcn_sqrtf(fmaxf(front_square, 0.0f)); };
         m = before;
