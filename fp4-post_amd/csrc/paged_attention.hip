@@ -9,6 +9,8 @@
 // which costs nothing: the matrix cores are idle most of the time.  28 query and 4 cache heads of 128 numbers, keys and values from memory: 64 ragged sequences of up to 4096
 // tokens in pages of 64 (277 MB) 65 us, one of 131072 (268 MB) 54 with the joining launch's 5 (5.0 TB/s), 48 ragged ones of up to 16384 tokens of 8 e4m3 heads (811 MB) 155
 // (5.2 TB/s); a large copy moves 4.9.  One sequence of 411 tokens 8: lengths, table, a block's keys and values one after the other.
+#include <cmath>
+
 #include "metis_device.h"
 #include "metis_host.h"
 
@@ -334,16 +336,30 @@ __global__ __launch_bounds__(kJoinThreads) void attend_join_kernel(const AttendA
     *out = length == 0 && said == length ? make_uint2(0u, 0u) : make_uint2(rb_pair(num.x * f, num.y * f), rb_pair(num.z * f, num.w * f));
 }
 
-// Tokens of a split.  Where the pairs of sequence and head fill the device, sequences of up to 4096 tokens are left whole (the joining launch costs 5 to 9 us: 64 sequences of
-// 4096 tokens, 4 heads of the cache, 94 us whole, 102 in halves), longer ones are cut so that a ragged batch's long ones do not end alone; else there are as many splits
-// as give every compute unit a workgroup, of 256 tokens at least (a block for each wave).  512 tokens are never cut: two blocks a wave take less than the joining launch.
+// Tokens of a split: up to 4096, and so many splits that the workgroups fill the rounds that the device's compute units take them in.  A round that is not full costs as
+// much as one that is, a split the joining launch (5 to 9 us) and its way through memory (64 sequences of 4096 tokens, 4 heads of the cache: 92 us whole, 102 in halves); so the
+// fewest splits that fill 0.85 of the rounds are taken (0.8 where the sequences are cut in any case), or of six more the best.  Uniform and ragged sequences of up to 4096
+// tokens, this and in the fewest splits that reach every compute unit: 48 of them 79 and 84, 54 and 61 us; 65 of them 111 and 133, 62 and 102; 80 of them 128 and 139, 96 and 109;
+// 160 of them 246 and 236, 170 and 207; 130 of them 211 and 222, 131 and 123.  512 tokens are never cut: two blocks a wave take less than the joining launch.
 static int64_t split_tokens(int64_t pairs, int64_t capacity)
 {
-    const int64_t block = 64 * kWaves, most = 4096, splits = (device_cus() + pairs - 1) / pairs;
-    int64_t chunk = (capacity + splits - 1) / splits;
-    if (chunk > most) chunk = most;
-    chunk = (chunk + block - 1) / block * block;
-    return capacity <= 2 * block ? 2 * block : chunk;
+    const int64_t block = 64 * kWaves, most = 4096, cus = device_cus();
+    if (capacity <= 2 * block) return 2 * block;
+    const int64_t fewest = (capacity + most - 1) / most;
+    const int64_t splits = cus / pairs > fewest ? cus / pairs : fewest;
+    int64_t chosen = 0;
+    const double enough = fewest > 1 ? 0.8 : 0.85;
+    double best = 0.0;
+    for (int64_t k = splits; k < splits + 6; ++k) {
+        const int64_t chunk = ((capacity + k - 1) / k + block - 1) / block * block;
+        if (chosen && (chunk < 3 * block || best >= enough)) break;
+        const double rounds = (double)pairs * (double)((capacity + chunk - 1) / chunk) / (double)cus, fill = rounds / ceil(rounds);
+        if (!chosen || fill > best) {
+            chosen = chunk;
+            best = fill;
+        }
+    }
+    return chosen;
 }
 
 size_t paged_attention_workspace_bytes(int64_t seqs, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t capacity)

@@ -404,3 +404,20 @@ def test_copies_beyond_32_bits_of_bytes():
         assert torch.equal(t[:, 0], t[:, -1]) and torch.equal(t[:, -5], t[:, -2]) and not bool(t[:, 1].any()) and bool(t[:, -1].any())
     del keys, values, t
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("seqs,longest", [(2, 1300), (33, 2600), (65, 1700), (100, 900)])
+def test_splits_of_batches_that_do_not_fill_the_rounds(seqs, longest):
+    """Batches whose sequences and heads are a little more, or a little less, than the device has compute units: cut in two to six, lengths on both sides of the cuts."""
+    g = torch.Generator().manual_seed(seqs)
+    lengths = [longest] + torch.randint(1, longest + 1, (seqs - 1,), generator=g).tolist()
+    for n in (256, 512, 513, 768, 769, 1024):
+        if n <= longest:
+            lengths[1 + (n // 256) % (seqs - 1)] = n
+    pages = sum(-(-n // 64) for n in lengths)
+    keys, values = cache(g, pages, 4, 64, 64)
+    tables = tables_of(g, lengths, 64, pages)
+    q = torch.randn(seqs, 8, 64, generator=g).to(BF).cuda()
+    from metis_hip import paged_attention
+    got = paged_attention(q, keys, values, tables, torch.tensor(lengths, dtype=torch.int32).cuda())
+    check(got, q, keys, values, tables, lengths)
