@@ -1,6 +1,6 @@
 // residual_norm, swiglu and rotary as nodes of torch's autograd, in compiled code.  Host code only: the arithmetic is libmetis_hip.so's, the checks of arguments are
 // made by the Python functions that call these (metis_hip/block.py, metis_hip/ops.py); rotary's are made here first, and what does not pass them is Python's (host time of a rotation and
-// its gradient 44 to 75 us on different hosts before, 39 now).
+// its gradient 44 to 75 us on different hosts before, 39 to 62 now, of which the engine's way to its thread and back is 28).
 //
 // All are kernels of some tens of microseconds in a training step, and a node written in Python costs more than that: recorded, run backward in the
 // engine's own thread (which has to get the interpreter first) and allocated for.  One token x 1536, forward and all gradients: 101 us through
