@@ -1104,7 +1104,7 @@ __device__ __forceinline__ void finish_row(RowShared& s, const SampleArgs& a, in
     double* const stretch = reinterpret_cast<double*>(s.weight);
     __syncthreads();
     if (taken) {
-        for (int k = tid; k < kBins; k += kSampleThreads) s.weight[k] = 0;
+        for (int k = tid; k < stretches; k += kSampleThreads) s.weight[k] = 0;
         __syncthreads();
         each_taken(s, row, w, filled, [&](float x, int index) {
             const double v = kept.one(w, x, index);
@@ -1113,7 +1113,7 @@ __device__ __forceinline__ void finish_row(RowShared& s, const SampleArgs& a, in
         });
         __syncthreads();
     }
-    double done = 0.0, goal = 0.0, chosen_front = 0.0;
+    double done = 0.0, goal = 0.0, chosen_front = 0.0, v[per], sum = 0.0, incl = 0.0, all = 0.0;
     int chosen = -1;
 #pragma unroll 1
     for (int round = 0; round < 2; ++round) {                      // the sum first, then the place (one pass where the stretches fit)
@@ -1130,13 +1130,17 @@ __device__ __forceinline__ void finish_row(RowShared& s, const SampleArgs& a, in
                 });
                 __syncthreads();
             }
-            double v[per], sum = 0.0, all;
+            if (round == 0 || stretches > kBins) {
+                sum = 0.0;
 #pragma unroll
-            for (int j = 0; j < per; ++j) {
-                v[j] = per * tid + j >= here ? 0.0 : taken ? (double)s.weight[per * tid + j] * (1.0 / kKeptUnit) + (set.by_k ? 0.0 : s.above[per * tid + j]) : stretch[per * tid + j];
-                sum += v[j];
+                for (int j = 0; j < per; ++j) {
+                    v[j] = per * tid + j >= here ? 0.0
+                           : taken               ? (double)s.weight[per * tid + j] * (1.0 / kKeptUnit) + (set.by_k ? 0.0 : s.above[per * tid + j])
+                                                 : stretch[per * tid + j];
+                    sum += v[j];
+                }
+                incl = scan<kSampleThreads>(sum, s.waves_d, all);
             }
-            const double incl = scan<kSampleThreads>(sum, s.waves_d, all);
             if (round == 1) {
                 double at = done + (incl - sum);
                 int hit = -1, live = -1;
