@@ -114,6 +114,7 @@ class CacheStep:
     slots: torch.Tensor         # int64 [tokens]
     tables: torch.Tensor        # int32 [seqs, pages of the longest]
     lengths: torch.Tensor       # int32 [seqs], the new tokens among them
+    counts: tuple[int, ...] | None = None  # new tokens of each sequence; None (of a step made by hand): not told
 
 
 class PagedCache:
@@ -220,7 +221,7 @@ class PagedCache:
         width = max((len(t) for t in tables), default=0)
         filled = [t + [0] * (width - len(t)) for t in tables]
         return CacheStep(self._there(positions, torch.int64), self._there(slots, torch.int64), self._there(filled, torch.int32).reshape(len(filled), width),
-                         self._there(lengths, torch.int32))
+                         self._there(lengths, torch.int32), tuple(counts))
 
     def compact(self) -> int:
         """Moves pages so that those in use are the first ones; returns how many were moved."""
@@ -261,10 +262,11 @@ class CachedAttention(nn.Module):
 
     @torch.no_grad()
     def forward(self, x: torch.Tensor, cache: PagedCache, layer: int, step: CacheStep) -> torch.Tensor:
-        """x [seqs, hidden], the newest token of each of the step's sequences."""
-        if x.dim() != 2 or x.shape[0] != step.lengths.shape[0] or step.slots.shape != step.lengths.shape:
-            raise ValueError(f"CachedAttention: one new token of each sequence, [{step.lengths.shape[0]}, hidden] for a step of as many tokens, not {tuple(x.shape)} and "
-                             f"{step.slots.shape[0]}")
+        """x [seqs, hidden], the newest token of each of the step's sequences (a step without counts is taken to be of one token each)."""
+        seqs = step.lengths.shape[0]
+        if x.dim() != 2 or x.shape[0] != seqs or step.slots.shape != step.lengths.shape or (step.counts is not None and step.counts != (1,) * seqs):
+            raise ValueError(f"CachedAttention: one new token of each sequence, [{seqs}, hidden] for a step of as many tokens, not {tuple(x.shape)} and "
+                             f"{step.slots.shape[0] if step.counts is None else list(step.counts)}")
         q, k, v = (proj(x).to(torch.bfloat16).unflatten(-1, (-1, self.head_dim)) for proj in (self.q_proj, self.k_proj, self.v_proj))
         keys, values = cache.keys[layer], cache.values[layer]
         q = rotary_append(q, k, v, step.positions, self.inv_freq, step.slots, keys, values, interleaved=self.interleaved, factor=self.factor, key_scale=cache.key_scale,

@@ -306,3 +306,24 @@ def test_numbers_of_sequences():
     assert cache.free_pages == 2 and cache.pages(t) == (0, 1)
     cache.free([t])
     assert cache.free_pages == 4 and cache.new() == [2]
+
+
+def test_the_attention_module_wants_one_token_of_each_sequence():
+    """As many new tokens as sequences are not enough: two of one and none of the other would attend over the other's tokens.  A step made by hand need not say its counts."""
+    from dataclasses import replace
+    linear = lambda n, m: torch.nn.Linear(n, m, bias=False, dtype=BF)
+    module = CachedAttention(linear(64, 128), linear(64, 64), linear(64, 64), linear(128, 64), 32, rotary_frequencies(32, 1e6)[0])
+    cache = PagedCache(1, 8, 2, 32, device="cpu")
+    a, b, c = cache.new(3)
+    x = torch.zeros(2, 64, dtype=BF)
+    step = cache.extend([a, b], [2, 0])
+    assert step.counts == (2, 0) and step.slots.shape == step.lengths.shape
+    with pytest.raises(ValueError, match="one new token"):
+        module(x, cache, 0, step)
+    with pytest.raises(ValueError, match="one new token"):
+        module(torch.zeros(3, 64, dtype=BF), cache, 0, cache.extend([a, b, c], [0, 3, 0]))
+    step = cache.extend([a, b])
+    assert step.counts == (1, 1)
+    for good in (step, replace(step, counts=None), replace(step, tables=torch.nn.functional.pad(step.tables, (0, 3)))):
+        with pytest.raises(MetisHipError, match="no CPU path"):      # (it gets as far as the device's calls)
+            module(x, cache, 0, good)
