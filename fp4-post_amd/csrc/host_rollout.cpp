@@ -66,7 +66,9 @@ int cache_type(const Tensor& keys, const Tensor& values)
         return -1;
     return keys.scalar_type() == at::kBFloat16 ? METIS_DTYPE_BF16 : keys.scalar_type() == at::kFloat8_e4m3fn ? METIS_DTYPE_E4M3 : -1;
 }
-template <class T> T* data(const Tensor& t) { return static_cast<T*>(const_cast<void*>(t.const_data_ptr())); }
+template <class T> const T* data(const Tensor& t) { return static_cast<const T*>(t.const_data_ptr()); }
+// of a tensor that the call writes: one that shares its numbers until it is written (a lazy clone) gets its own
+template <class T> T* written(const Tensor& t) { return static_cast<T*>(t.mutable_data_ptr()); }
 
 }  // namespace
 
@@ -97,7 +99,7 @@ PyObject* metis_host_rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n)
         out = at::empty({tokens, q.size(1), dim}, q.options().memory_format(at::MemoryFormat::Contiguous));
         rc = metis_rotary_append(data<void>(q), qt, qh, q.size(1), data<void>(k), kt, kh, k.size(1), data<void>(v), vt, vh, data<int64_t>(positions), data<void>(inv_freq),
                                  wide ? METIS_DTYPE_F64 : METIS_DTYPE_F32, data<int64_t>(slots), tokens, dim, 2 * half, interleaved, static_cast<float>(factor), keys.size(0), keys.size(2), type,
-                                 static_cast<float>(key_scale), static_cast<float>(value_scale), data<void>(keys), data<void>(values), data<void>(out), stream_of(q));
+                                 static_cast<float>(key_scale), static_cast<float>(value_scale), written<void>(keys), written<void>(values), written<void>(out), stream_of(q));
     }
     return rc == METIS_OK ? THPVariable_Wrap(std::move(out)) : not_here();
     END_HANDLE_TH_ERRORS
@@ -130,8 +132,8 @@ PyObject* metis_host_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n
         Tensor workspace;
         if (need > 16) workspace = at::empty({static_cast<int64_t>(need)}, options.dtype(at::kByte));
         rc = metis_paged_attention(data<void>(q), qs, qh, seqs, heads, keys.size(1), dim, data<void>(keys), data<void>(values), keys.size(0), page, type, data<int32_t>(tables), tables.stride(0),
-                                   width, data<int32_t>(lengths), static_cast<float>(scale), static_cast<float>(key_scale), static_cast<float>(value_scale), data<void>(out),
-                                   need > 16 ? data<void>(workspace) : nullptr, need, stream_of(q));
+                                   width, data<int32_t>(lengths), static_cast<float>(scale), static_cast<float>(key_scale), static_cast<float>(value_scale), written<void>(out),
+                                   need > 16 ? written<void>(workspace) : nullptr, need, stream_of(q));
     }
     return rc == METIS_OK ? THPVariable_Wrap(std::move(out)) : not_here();
     END_HANDLE_TH_ERRORS
@@ -158,7 +160,7 @@ PyObject* metis_host_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n)
             pages[static_cast<size_t>(which * count + i)] = p;
         }
     const int64_t size = keys.size(2) * keys.size(3) * keys.size(4) * static_cast<int64_t>(keys.element_size());
-    const int rc = metis_cache_copy_pages(data<void>(keys), data<void>(values), keys.size(0), keys.size(1), size, pages.data(), pages.data() + count, count, stream_of(keys));
+    const int rc = metis_cache_copy_pages(written<void>(keys), written<void>(values), keys.size(0), keys.size(1), size, pages.data(), pages.data() + count, count, stream_of(keys));
     if (rc != METIS_OK) return not_here();
     Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS
@@ -190,7 +192,7 @@ PyObject* metis_host_sample_tokens(PyObject*, PyObject* const* a, Py_ssize_t n)
         Tensor workspace;
         if (need) workspace = at::empty({static_cast<int64_t>(need)}, options.dtype(at::kByte));
         rc = metis_sample_tokens(data<void>(logits), count > 1 ? logits.stride(0) : vocab, f32 ? METIS_DTYPE_F32 : METIS_DTYPE_BF16, count, vocab, data<float>(uniforms), settings, nullptr,
-                                 data<int64_t>(tokens), data<float>(logprobs), need ? data<void>(workspace) : nullptr, need, stream_of(logits));
+                                 written<int64_t>(tokens), written<float>(logprobs), need ? written<void>(workspace) : nullptr, need, stream_of(logits));
     }
     if (rc != METIS_OK) return not_here();
     PyObject* first = THPVariable_Wrap(std::move(tokens));

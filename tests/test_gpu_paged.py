@@ -421,3 +421,29 @@ def test_splits_of_batches_that_do_not_fill_the_rounds(seqs, longest):
     from metis_hip import paged_attention
     got = paged_attention(q, keys, values, tables, torch.tensor(lengths, dtype=torch.int32).cuda())
     check(got, q, keys, values, tables, lengths)
+
+
+@pytest.mark.parametrize("other_path", [False, True])
+def test_lazy_clones_of_a_cache_keep_their_numbers(other_path):
+    """A cache that shares its storage with a lazy clone until one of them is written: an append and a copy of pages write to the one that was named, on the compiled
+    path and on Python's (a tuple of pages, slots that have to be made dense)."""
+    from metis_hip import copy_pages, rotary_append
+    g = torch.Generator().manual_seed(15)
+    keys, values = cache(g, 4, 2, 16, 64)
+    q, k, v = (torch.randn(5, h, 64, generator=g).to(BF).cuda() for h in (4, 2, 2))
+    at, slots = torch.arange(5).cuda(), torch.arange(10, 20, 2).cuda()
+    if other_path:
+        slots = torch.stack((slots, slots), 1)[:, 0]
+    want = keys.clone(), values.clone()
+    before = want[0].clone(), want[1].clone()
+    rotary_append(q, k, v, at, frequencies(32), slots, *want)
+    shared = torch._lazy_clone(keys), torch._lazy_clone(values)
+    rotary_append(q, k, v, at, frequencies(32), slots, *shared)
+    assert torch.equal(shared[0], want[0]) and torch.equal(shared[1], want[1]) and not torch.equal(want[0], before[0])
+    assert torch.equal(keys, before[0]) and torch.equal(values, before[1])
+    pool = keys[None], values[None]
+    shared = torch._lazy_clone(pool[0]), torch._lazy_clone(pool[1])
+    copy_pages(*shared, (0,) if other_path else [0], (3,) if other_path else [3])
+    for t, old in zip(shared, before):
+        assert torch.equal(t[0, 3], old[0]) and torch.equal(t[0, :3], old[:3])
+    assert torch.equal(keys, before[0]) and torch.equal(values, before[1])
