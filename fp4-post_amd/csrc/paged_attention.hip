@@ -5,9 +5,9 @@
 //   scores^T [tokens, heads] = K q^T        K is the first operand as it lies in its page (a row is a token)
 //   o^T [dim, heads] = V^T p^T              V is kept transposed in its page (a row is a dimension, its tokens side by side)
 // and the tokens are dealt to the rows of the first product in an order that leaves a lane with exactly the eight (two times eight) neighbouring tokens of one head
-// that the second product wants from it: no value crosses lanes but the maximum.  The probabilities enter the second product as two bf16 terms (2^-16 of them is lost),
-// which costs nothing: the matrix cores are idle most of the time.  28 query and 4 cache heads of 128 numbers, keys and values from memory: 64 ragged sequences of up to 4096
-// tokens in pages of 64 (277 MB) 65 us, one of 131072 (268 MB) 54 with the joining launch's 5 (5.0 TB/s), 48 ragged ones of up to 16384 tokens of 8 e4m3 heads (811 MB) 155
+// that the second product wants from it: no value crosses lanes but the maximum.  The probabilities enter the second product as two bf16 terms, which
+// costs nothing, as the matrix cores are idle most of the time: each is good to 2^-16 of itself and to 2^-126 of the sequence's largest.
+// 28 query and 4 cache heads of 128 numbers, keys and values from memory: 64 ragged sequences of up to 4096 tokens in pages of 64 (277 MB) 65 us, one of 131072 (268 MB) 54 with the joining launch's 5 (5.0 TB/s), 48 ragged ones of up to 16384 tokens of 8 e4m3 heads (811 MB) 155
 // (5.2 TB/s); a large copy moves 4.9.  One sequence of 411 tokens 8: lengths, table, a block's keys and values one after the other.
 #include <cmath>
 
@@ -227,8 +227,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(const AttendArgs
             for (int w = 0; w < 4; ++w) {
                 const float x = p[8 * s + 2 * w], y = p[8 * s + 2 * w + 1];
                 hi[w] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);      // both cut off
-                // what is left of them is positive: an infinite value keeps its sign in both products (2^-100 is lost in any weight that counts)
-                lo[w] = rb_pair(fmaxf(x - bf16_lo(hi[w]), 0x1p-100f), fmaxf(y - bf16_hi(hi[w]), 0x1p-100f));
+                // What is left of a weight stays positive, so that an infinite value keeps its sign in both products: 2^-126 at least, binary32's smallest step, and nothing
+                // where the weight is nothing.
+                lo[w] = rb_pair(fmaxf(x - bf16_lo(hi[w]), fminf(x, 0x1p-126f)), fmaxf(y - bf16_hi(hi[w]), fminf(y, 0x1p-126f)));
             }
             const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, make_uint4(hi[0], hi[1], hi[2], hi[3])), pl = __builtin_bit_cast(bf16x8_t, make_uint4(lo[0], lo[1], lo[2], lo[3]));
 #pragma unroll

@@ -1060,7 +1060,8 @@ int metis_rotary_append(const void *q, int64_t q_token, int64_t q_head, int64_t 
 
 /*
  * softmax(scale q K^T) V of one new token of each sequence over the cached tokens of the sequence (its own among them):
- * scores and sums in binary32, the result rounded once to bf16.  Query head h reads head h / (q_heads / kv_heads) of the cache.
+ * scores and sums in binary32, each weight in the sum of values within 2^-16 of itself and 2^-126 of the largest (one that is
+ * nothing in binary32 is nothing), the result rounded once to bf16.  Query head h reads head h / (q_heads / kv_heads) of the cache.
  *   q        bf16 [seqs, q_heads, dim], strides of sequences and heads in elements, multiples of 8; 16-byte aligned
  *   tables   int32 [seqs, width], row stride table_stride: the pages of each sequence in order; lengths int32 [seqs]: its
  *            tokens.  What lies behind a length, in the table or in the last page, is not read into any result.  A length

@@ -447,3 +447,26 @@ def test_lazy_clones_of_a_cache_keep_their_numbers(other_path):
     for t, old in zip(shared, before):
         assert torch.equal(t[0, 3], old[0]) and torch.equal(t[0, :3], old[:3])
     assert torch.equal(keys, before[0]) and torch.equal(values, before[1])
+
+
+@pytest.mark.parametrize("lengths", [[40, 700], [3000, 90]])
+def test_weights_of_nothing_carry_nothing(lengths):
+    """Tokens of which nothing is left beside the likeliest (a weight of 2^-490, 2^-104) with values that would show if they had a little more: the formula's result.  Scores
+    that are all -inf have no weights: NaN, whatever the values."""
+    from metis_hip import paged_attention
+    g = torch.Generator().manual_seed(16)
+    pages = sum(-(-n // 16) for n in lengths)
+    keys, values = cache(g, pages, 1, 16, 128)
+    tables, n = tables_of(g, lengths, 16, pages), torch.tensor(lengths, dtype=torch.int32).cuda()
+    q = torch.ones(2, 4, 128, dtype=BF, device="cuda")
+    for one, much in ((30.0, 2.0 ** 100), (6.375, 2.0 ** 104)):
+        k, v = torch.zeros_like(keys), values * much
+        for i in range(2):
+            k[tables[i, 1].long(), :, 5] = one                          # token 21 has all the weight
+            v[tables[i, 1].long(), :, :, 5] = values[tables[i, 1].long(), :, :, 5]
+        check(paged_attention(q, k, v, tables, n), q, k, v, tables, lengths)
+    k = keys.clone()
+    k[tables[0, :-(-lengths[0] // 16)].long()] = -float("inf")
+    got = paged_attention(q, k, values, tables, n)
+    assert bool(got[0].isnan().all())
+    check(got[1:], q[1:], k, values, tables[1:], lengths[1:])
