@@ -39,6 +39,8 @@ inline int carve_workspace(void* p, size_t bytes, int64_t rows, int64_t cols, Wo
 
 // compute units of the current device (cached per device ordinal)
 int device_cus();
+// whether one launch takes so many workgroups: it has fewer than 2^32 work-items
+static inline bool launch_takes(int64_t workgroups, int threads) { return workgroups <= (int64_t)UINT32_MAX / threads; }
 
 // Measurement switches (kernel variants and shape overrides read from the environment) exist only in a
 // -DMETIS_MEASURE build of the library; the shipped library reads no environment variables.

@@ -386,7 +386,7 @@ int paged_attention(const void* q, int64_t q_seq, int64_t q_head, int64_t seqs, 
     if (width > (INT32_MAX - 65536) / page || seqs > ((int64_t)1 << 46) / q_heads / dim) return METIS_E_ARG;
     const int64_t capacity = width * page, tiles = (q_heads / kv_heads + kHeadTile - 1) / kHeadTile, pairs = seqs * kv_heads * tiles;
     const int64_t chunk = split_tokens(pairs, capacity > 0 ? capacity : 1), splits = capacity > 0 ? (capacity + chunk - 1) / chunk : 1;
-    if (pairs > INT32_MAX / splits || seqs * q_heads > INT32_MAX) return METIS_E_TOO_LARGE;
+    if (pairs > INT32_MAX / splits || !launch_takes(pairs * splits, 64 * kWaves) || (splits > 1 && !launch_takes(seqs * q_heads, kJoinThreads))) return METIS_E_TOO_LARGE;
     if (splits > 1 && (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < (size_t)seqs * (size_t)q_heads * (size_t)splits * (size_t)(dim + 2) * 4)) return METIS_E_WORKSPACE;
     AttendArgs a = {};
     a.q = q; a.keys = keys; a.values = values; a.tables = tables; a.lengths = lengths; a.out = out; a.sums = static_cast<float*>(workspace);
@@ -489,11 +489,13 @@ int copy_pages(void* keys, void* values, int64_t layers, int64_t pages, int64_t 
     a.keys = static_cast<char*>(keys); a.values = static_cast<char*>(values);
     a.page_bytes = (uint64_t)page_bytes; a.layer_bytes = (uint64_t)page_bytes * (uint64_t)pages;
     a.pieces = (int)((page_bytes + kCopyPiece - 1) / kCopyPiece);
+    if (layers > INT32_MAX / 2 / a.pieces || !launch_takes(2 * layers * a.pieces, 256)) return METIS_E_TOO_LARGE;
     const int64_t one = 2 * layers * a.pieces;
-    if (layers > INT32_MAX / 2 / a.pieces || one > INT32_MAX / kCopyPairs) return METIS_E_TOO_LARGE;
     a.layers = (int)layers;
-    for (int64_t done = 0; done < count; done += kCopyPairs) {
-        a.count = (int)(count - done < kCopyPairs ? count - done : kCopyPairs);
+    int64_t most = kCopyPairs;                                     // pairs of a launch
+    while (!launch_takes(one * most, 256)) most /= 2;
+    for (int64_t done = 0; done < count; done += most) {
+        a.count = (int)(count - done < most ? count - done : most);
         for (int i = 0; i < a.count; ++i) {
             a.from[i] = (int)from[done + i];
             a.to[i] = (int)to[done + i];

@@ -235,7 +235,7 @@ int rotary(const void* q, int64_t q_token, int64_t q_head, int64_t q_heads, cons
     if (a.head_lanes > 256 / a.units) a.head_lanes = 256 / a.units;
     a.tok_lanes = 256 / (a.units * a.head_lanes);
     const int64_t blocks = (tokens + a.tok_lanes - 1) / a.tok_lanes, v_items = cached ? tokens * k_heads * (dim / (N == 8 ? 8 : 1)) : 0;
-    if (blocks + (v_items + 255) / 256 > INT32_MAX) return METIS_E_TOO_LARGE;
+    if (!launch_takes(blocks + (v_items + 255) / 256, 256)) return METIS_E_TOO_LARGE;
     a.rotate_blocks = (int)blocks;
     const dim3 grid((unsigned)(blocks + (v_items + 255) / 256)), block(256);
 #define METIS_ROT(F, C) do { if (whole) hipLaunchKernelGGL((rotary_kernel<F, 8, C>), grid, block, 0, st, a); else hipLaunchKernelGGL((rotary_kernel<F, 1, C>), grid, block, 0, st, a); } while (0)

@@ -1430,21 +1430,34 @@ int sample_tokens(const void* logits, int64_t ld, int dtype, int64_t rows, int64
         a.filled = reinterpret_cast<uint32_t*>(base + space.filled);
         a.limits = reinterpret_cast<int*>(base + space.limits);
     }
-    const dim3 grid((unsigned)rows), parts((unsigned)(rows * (a.parts ? a.parts : 1)));
-#define METIS_SAMPLE(F)                                                                                                             \
-    do {                                                                                                                            \
-        if (!a.parts) {                                                                                                             \
-            hipLaunchKernelGGL(sample_kernel<F>, grid, dim3(kSampleThreads), 0, st, a);                                             \
-        } else {                                                                                                                    \
-            hipLaunchKernelGGL(sample_tops_kernel<F>, parts, dim3(kPartThreads), 0, st, a);                                         \
-            hipLaunchKernelGGL(sample_bins_kernel<F>, parts, dim3(kPartThreads), 0, st, a);                                         \
-            hipLaunchKernelGGL(sample_finish_kernel<F>, grid, dim3(kSampleThreads), 0, st, a);                                      \
-        }                                                                                                                           \
+    const bool f32 = dtype == METIS_DTYPE_F32;
+    if (a.parts) {                                                 // (rows that a small part of the device's compute units takes)
+        const dim3 grid((unsigned)rows), parts((unsigned)(rows * a.parts));
+#define METIS_SAMPLE_PARTS(F)                                                                   \
+    do {                                                                                        \
+        hipLaunchKernelGGL(sample_tops_kernel<F>, parts, dim3(kPartThreads), 0, st, a);         \
+        hipLaunchKernelGGL(sample_bins_kernel<F>, parts, dim3(kPartThreads), 0, st, a);         \
+        hipLaunchKernelGGL(sample_finish_kernel<F>, grid, dim3(kSampleThreads), 0, st, a);      \
     } while (0)
-    if (dtype == METIS_DTYPE_F32) METIS_SAMPLE(true);
-    else METIS_SAMPLE(false);
-#undef METIS_SAMPLE
-    return hipGetLastError() == hipSuccess ? METIS_OK : METIS_E_LAUNCH;
+        if (f32) METIS_SAMPLE_PARTS(true);
+        else METIS_SAMPLE_PARTS(false);
+#undef METIS_SAMPLE_PARTS
+        return hipGetLastError() == hipSuccess ? METIS_OK : METIS_E_LAUNCH;
+    }
+    constexpr int64_t most = (int64_t)UINT32_MAX / kSampleThreads;                    // rows of a launch
+    for (int64_t first = 0; first < rows; first += most) {
+        SampleArgs some = a;
+        some.logits = static_cast<const char*>(logits) + (size_t)first * (size_t)ld * (f32 ? 4 : 2);
+        some.uniforms += first;
+        if (some.row_parameters) some.row_parameters += 4 * first;
+        some.tokens += first;
+        some.logprobs += first;
+        some.rows = (int)(rows - first < most ? rows - first : most);
+        if (f32) hipLaunchKernelGGL(sample_kernel<true>, dim3((unsigned)some.rows), dim3(kSampleThreads), 0, st, some);
+        else hipLaunchKernelGGL(sample_kernel<false>, dim3((unsigned)some.rows), dim3(kSampleThreads), 0, st, some);
+        if (hipGetLastError() != hipSuccess) return METIS_E_LAUNCH;
+    }
+    return METIS_OK;
 }
 
 }  // namespace metis

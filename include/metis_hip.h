@@ -1032,6 +1032,8 @@ int metis_head_logprobs_backward(const void *hidden, int64_t ld_hidden, const vo
  *   inv_freq   [turned / 2], float or double (freq_dtype METIS_DTYPE_F32 / _F64)
  *   dim        even, up to 512; turned even, 0 to dim.  16-byte aligned pointers and strides with turned and dim - turned
  *              multiples of 16 are read in whole pieces
+ * One launch: METIS_E_TOO_LARGE where it would have 2^32 work-items or more (with elements read one by one, 2^24 tokens of one
+ * head of 512 do).  So for metis_rotary_append.
  */
 int metis_rotary(const void *q, int64_t q_token, int64_t q_head, int64_t q_heads, const void *k,
                  int64_t k_token, int64_t k_head, int64_t k_heads, const int64_t *positions,
@@ -1070,6 +1072,8 @@ int metis_rotary_append(const void *q, int64_t q_token, int64_t q_head, int64_t 
  *   page     a power of two from 16 to 4096; dim a multiple of 32 up to 256 (e4m3: of 64); kv_heads divides q_heads
  *   out      dense [seqs, q_heads, dim], 8-byte aligned
  *   workspace metis_paged_attention_workspace_bytes(.., width * page) bytes, no initialisation needed
+ * METIS_E_TOO_LARGE where a launch would have 2^32 work-items or more: 2^24 workgroups (a sequence's share of up to 4096 tokens
+ * for 16 query heads of one head of the cache is one), or, of sequences in shares, 2^23 rows of a sequence and query head.
  */
 size_t metis_paged_attention_workspace_bytes(int64_t seqs, int64_t q_heads, int64_t kv_heads,
                                              int64_t dim, int64_t capacity);

@@ -315,3 +315,12 @@ def test_sizes_around_the_lists(V):
             logits = wide[:, first:first + V]
             for settings in (dict(top_k=20), dict(top_k=V - 1), dict(top_k=V // 2, top_p=0.9), dict(top_p=0.95), dict(top_p=0.9999), dict(temperature=0.05, top_k=V // 2), dict(temperature=0.03, top_p=0.999)):
                 check(logits, u, **settings)
+
+
+def test_more_rows_than_a_launch_takes():
+    """A row is a workgroup, and a launch has fewer than 2^32 work-items: 2^22 + 5 rows, with numbers of their own and settings of their own."""
+    rows = (1 << 22) + 5
+    g = torch.Generator(device="cuda").manual_seed(12)
+    logits, u = (2 * torch.randn(rows, 8, generator=g, device="cuda")).to(BF), torch.rand(rows, generator=g, device="cuda")
+    check(logits, u, top_p=0.8)
+    check(logits, u, temperature=0.5 + torch.rand(rows, generator=g, device="cuda"), top_k=5)

@@ -327,3 +327,17 @@ def test_the_attention_module_wants_one_token_of_each_sequence():
     for good in (step, replace(step, counts=None), replace(step, tables=torch.nn.functional.pad(step.tables, (0, 3)))):
         with pytest.raises(MetisHipError, match="no CPU path"):      # (it gets as far as the device's calls)
             module(x, cache, 0, good)
+
+
+def test_calls_of_more_than_a_launch_takes():
+    """A launch has fewer than 2^32 work-items.  Rotations, appends and attention beyond it say that they are too large, and nothing is launched."""
+    L = _lib.load()
+    wide = dict(dim=512, turned=512, q_token=511, q_heads=1, k_heads=1, k_token=511, q_head=512, k_head=512)
+    assert L.metis_rotary(*{**ROTARY, **wide, "tokens": 1 << 24, "npos": 1}.values()) == _lib.E_TOO_LARGE
+    assert L.metis_rotary(*{**ROTARY, "tokens": 1 << 31, "npos": 1, "q_token": 64, "k_token": 64}.values()) == _lib.E_TOO_LARGE
+    assert L.metis_rotary_append(*{**APPEND, "v_token": 127, "tokens": 1 << 25}.values()) == _lib.E_TOO_LARGE
+    big = 1 << 60
+    assert L.metis_paged_attention(*{**ATTEND, "seqs": 1 << 23}.values()) == _lib.E_TOO_LARGE
+    assert L.metis_paged_attention(*{**ATTEND, "seqs": 1 << 18, "heads": 32, "kv": 1, "width": 1024, "bytes": big}.values()) == _lib.E_TOO_LARGE
+    a = (ctypes.c_int64 * 1)(0)
+    assert L.metis_cache_copy_pages(4096, 4096, 1 << 20, 8, 1 << 20, ctypes.cast(a, ctypes.c_void_p), ctypes.cast((ctypes.c_int64 * 1)(1), ctypes.c_void_p), 1, None) == _lib.E_TOO_LARGE
