@@ -253,10 +253,11 @@ struct Weigher {
     }
     __device__ __forceinline__ double weight(float x) const
     {
-        const Depth d = depth(x);
-        return ldexp(part(d.r), -d.octave);
+        const double d = fmin(top - (double)x, far), o = fma(d, -rate, 0x1.8p52);
+        return ldexp(part(fma(d, rate, o - 0x1.8p52)), (int)__double_as_longlong(o));
     }
-    // the same for two tokens of a pass over all: 0 from 2000 octaves on, as above; the octave to the nearest, read off a sum again
+    // The same bits for two tokens of a pass over all (a token next to min_p is one of the kept in the sums and in the draw, or in neither): 0 from 2000 octaves on; the octave to
+    // the nearest, read off a sum again.
     __device__ __forceinline__ void weights(float x, float y, double& a, double& b) const
     {
         const double d = fmin(top - (double)x, far), e = fmin(top - (double)y, far), o = fma(d, -rate, 0x1.8p52), p = fma(e, -rate, 0x1.8p52);
@@ -994,14 +995,16 @@ __device__ __forceinline__ void draw_from_stretch(const SampleArgs& a, int r, co
         }
     }
     const uint64_t hits = __ballot(found >= 0), live = __ballot(behind >= 0);
-    const int who = hits ? __ffsll((unsigned long long)hits) - 1 : 63 - __clzll((unsigned long long)live);
-    if (lane == who) {
+    const int who = hits ? __ffsll((unsigned long long)hits) - 1 : live ? 63 - __clzll((unsigned long long)live) : 0;
+    if (lane != who) return;
+    if (!hits && !live) {                                          // (a stretch is chosen for a weight that the draw sees too)
+        answer(a, r, -1, __builtin_nan(""));
+    } else {
         const int j = hits ? found : behind;
         float xt = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) xt = e == j ? x[e] : xt;
-        a.tokens[r] = i + j;
-        a.logprobs[r] = (float)(w.log_weight(xt) - log(total));
+        answer(a, r, i + j, w.log_weight(xt) - log(total));
     }
 }
 
@@ -1202,10 +1205,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
     for (int k = 1; k < SLOTS; ++k) top = top != top ? top : fmaxf(top, mine[k]);
     top = largest<kSampleThreads>(top, s.tops);
     if (!(top > -INFINITY) || !set.fit()) {                        // nothing to draw from, or no way to
-        if (thread_anew() == 0) {
-            a.tokens[r] = -1;
-            a.logprobs[r] = __builtin_nanf("");
-        }
+        if (thread_anew() == 0) answer(a, r, -1, __builtin_nan(""));
         return;
     }
     const Weigher w(top, set.rate());
@@ -1340,10 +1340,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_finish_kernel(const Sam
     const LogitRow<F32> row(static_cast<const char*>(a.logits) + (size_t)r * a.ld * (F32 ? 4 : 2), a.vocab);
     const float top = __int_as_float(a.limits[3 * (size_t)r + 2]);
     if (!(top > -INFINITY) || !set.fit()) {
-        if (tid == 0) {
-            a.tokens[r] = -1;
-            a.logprobs[r] = __builtin_nanf("");
-        }
+        if (tid == 0) answer(a, r, -1, __builtin_nan(""));
         return;
     }
     const Weigher w(top, set.rate());

@@ -324,3 +324,25 @@ def test_more_rows_than_a_launch_takes():
     logits, u = (2 * torch.randn(rows, 8, generator=g, device="cuda")).to(BF), torch.rand(rows, generator=g, device="cuda")
     check(logits, u, top_p=0.8)
     check(logits, u, temperature=0.5 + torch.rand(rows, generator=g, device="cuda"), top_k=5)
+
+
+def test_a_token_next_to_min_p():
+    """One other token beside a row's largest, 4096 settings of min_p within 2^-41 of its weight and 511 tokens just below them around it: it is kept, or it is not, in
+    the sums and in the draw alike, so every row has one of the two.  Depths within 1/64 of half an octave, where an octave is rounded one way or the other."""
+    from metis_hip import sample_tokens
+    rows = 4096
+    for depth in (0.4925, 0.495, 0.4975, 0.4999, 0.5001, 1.496, 3.4993):
+        x = torch.tensor(-depth * math.log(2)).item()
+        logits = torch.full((rows, 1024), -50.0)
+        logits[:, 0], logits[:, 512:], logits[:, 600] = 0.0, x - math.log(2) / 128, x
+        weight = math.exp(float(logits[0, 600]))
+        min_p = (weight * (1 + torch.arange(-rows // 2, rows // 2, dtype=torch.float64) * 2.0 ** -52)).cuda()
+        u = torch.full((rows,), 0.999, device="cuda")
+        del_me = [torch.full((rows,), -7, dtype=d, device="cuda") for d in (torch.int64, F32, torch.int64, F32)]
+        del del_me                                                      # (what is not written shows)
+        tokens, logp = sample_tokens(logits.cuda(), u, min_p=min_p)
+        assert bool(((tokens == 0) | (tokens == 600)).all()), tokens[(tokens != 0) & (tokens != 600)][:5]
+        assert int(tokens[0]) == 600 and int(tokens[-1]) == 0 and bool((tokens[1:] <= tokens[:-1]).all())
+        total = torch.logsumexp(logits[0].double(), 0)
+        want = torch.where(tokens == 600, logits[0, 600].double().cuda(), 0.0) - total.cuda()
+        assert bool(((logp.double() - want).abs() <= 2.0 ** -22).all())
