@@ -11,8 +11,9 @@
 // They are sorted where they are few; else they are counted (k) and their weights added up (p) by bins, in whole numbers, so that the order of the additions does not
 // count, and the tokens of the bin that holds a threshold are sorted.  What is kept of them is added to the stretches' sums for the draw, in whole numbers again.  Where
 // the thresholds lie elsewhere (large k, flat rows), further passes over the row do the same with all tokens, and narrow a bin of too many by digits of its logits and indices.
-// Weights are accurate to 2^-44 and sums are held in 64 bits: with some 10^5 tokens next to each other in the running sum, what binary32 is off would take another
-// token now and then.  Each pass is a chain of some twenty 64-bit operations for each token, and what it must not do is go through LDS for each (one LDS
+// A weight is accurate to 2^-44 of itself and sums are held in 64 bits: with some 10^5 tokens next to each other in the running sum, what binary32 is off would take another
+// token now and then.  Whole numbers round once more: of the taken tokens each kept weight to 2^-54 of the largest (one below 2^-53 is 2^-53), in the bins, where they only say
+// where a threshold lies, to 2^-41.5 of itself (beyond 64 octaves to 2^-105 of the largest).  Each pass is a chain of some twenty 64-bit operations for each token, and what it must not do is go through LDS for each (one LDS
 // operation of a compute unit's sixteen waves costs as much as sixteen of these on its four SIMDs): there are no tables, sums over lanes go by DPP.
 // Rows that do not fill the device are shared out to several workgroups for the passes over all tokens, in launches of their own.
 // 256 rows of 131072 bf16 logits (67 MB, 14 us at a large copy's rate): no thresholds 43 us, top_k = 50 38, top_p = 0.95 88 to 106 (the row that keeps most, 12000 to 14000 tokens,
@@ -33,7 +34,7 @@ constexpr int kList = 1024;                                        // tokens tha
 constexpr int kShares = 8192;                                      // maxima of a row
 constexpr double kLowTemperatures = 0x1p100;                       // 1 / T from which depths do not fit binary32
 constexpr double kUnit = 0x1p41;                                   // a weight of its bin's octave, as a whole number
-constexpr double kKeptUnit = 0x1p50;                               // a kept weight of a stretch
+constexpr double kKeptUnit = 0x1p53;                               // a kept weight of a stretch (512 of them have room in 64 bits)
 
 struct SampleArgs {
     const void* logits;
@@ -1112,7 +1113,7 @@ __device__ __forceinline__ void finish_row(RowShared& s, const SampleArgs& a, in
         each_taken(s, row, w, filled, [&](float x, int index) {
             const double v = kept.one(w, x, index);
             // (no less than one unit: the number 0 falls into the first kept token, however little it weighs)
-            if (v > 0.0) atomicAdd((unsigned long long*)&s.weight[(index + row.shift) / 512], (unsigned long long)fmax(v * kKeptUnit, 1.0));
+            if (v > 0.0) atomicAdd((unsigned long long*)&s.weight[(index + row.shift) / 512], (unsigned long long)(fmax(v * kKeptUnit, 1.0) + 0.5));
         });
         __syncthreads();
     }

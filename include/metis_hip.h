@@ -1102,8 +1102,9 @@ int metis_cache_copy_pages(void *keys, void *values, int64_t layers, int64_t pag
  *   K3  those of K2 with w >= min_p
  *   token = the lowest index i in K3 with sum_{j <= i, j in K3} w_j > u sum(K3),
  *   logprob = log w_token - log sum_i w_i, over all tokens: its log-probability under softmax(x / temperature)
- * Weights and sums in 64 bits (with top_k the sum in logprob, of all tokens, in binary32: within 2^-18 of the value in 64
- * bits); the same inputs give the same results always.
+ * Weights good to 2^-44 of themselves, sums in 64 bits or in whole numbers of 2^-53 of the largest weight (in the search for a
+ * threshold 2^-41.5 of each weight); with top_k the sum in logprob, of all tokens, in binary32: within 2^-18 of the value in 64
+ * bits.  The same inputs give the same results always.
  *   logits      bf16 or float [rows, vocab], row stride ld; vocab up to 2^22.  -inf: never drawn
  *   uniforms    float [rows] in [0, 1)
  *   parameters  HOST double[4]: 0 < temperature <= 2^64, top_k >= 0, top_p > 0, min_p in [0, 1]; or row_parameters, device

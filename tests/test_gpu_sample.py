@@ -346,3 +346,20 @@ def test_a_token_next_to_min_p():
         total = torch.logsumexp(logits[0].double(), 0)
         want = torch.where(tokens == 600, logits[0, 600].double().cuda(), 0.0) - total.cuda()
         assert bool(((logp.double() - want).abs() <= 2.0 ** -22).all())
+
+
+def test_numbers_next_to_the_borders_of_many_tokens():
+    """12000 kept tokens behind a heavy one, together as heavy as it, numbers whose goal lies 2^-42 to 2^-39.5 beside a border: the definition's token.  The weights are good to
+    2^-44 and the whole numbers of the sums to 2^-54 apiece, in either direction; 12000 of them cut off would move the borders by 2^-38."""
+    rows, V, k = 300, 14000, 12000
+    g = torch.Generator().manual_seed(13)
+    logits = torch.sort(-8.9 - 0.7 * torch.rand(rows, V, generator=g), 1, descending=True)[0]
+    logits[:, 0] = 0.0
+    upto = torch.cumsum(torch.exp(logits[:, :k].double()), 1)
+    borders, whole = upto[:, 1:3000], upto[:, -1:]
+    u = (borders / whole).float()
+    off = (u.double() * whole - borders).abs()
+    row, at = torch.nonzero((off > 2.0 ** -42) & (off < 2.0 ** -39.5), as_tuple=True)
+    assert row.numel() >= 10
+    check(logits[row].cuda(), u[row, at].cuda(), top_k=k)
+    check(logits[row].cuda(), u[row, at].cuda(), top_k=k, top_p=1 - 1e-12)
