@@ -1051,26 +1051,33 @@ __device__ __forceinline__ void finish_row(RowShared& s, const SampleArgs& a, in
                 double sum = 0.0, all;
 #pragma unroll
                 for (int j = 0; j < per; ++j) sum += held(per * tid + j);
-                if (tid == 0) s.found_i = -1;
+                if (tid == 0) s.found_i = INT32_MAX;
                 const double over = taken && !set.by_k ? upper : 0.0;                    // (nothing lies above what k takes out)
                 double front = over + (scan<kSampleThreads>(sum, s.waves_d, all) - sum);
                 if (taken && (over + all < goal || (over > 0.0 && over >= goal))) {      // the window missed it
                     pass();
                     continue;
                 }
+                // The first bin that reaches the goal.  (Where a thread's sums begin and where the one before it ended, two roundings of one sum, a goal may lie between them: then
+                // it is the latter's bin, or the former's first.)
+                int mine = INT32_MAX;
+                double mine_front = 0.0;
 #pragma unroll
                 for (int j = 0; j < per; ++j) {
                     const int at = per * tid + j;
                     const double here = held(at), up = stage && at == last ? kept_sum : front + here;
-                    // (one bin at most: the sums rise)
-                    if (here > 0.0 && at <= last && front < goal && up >= goal) {
-                        s.found_i = at;
-                        s.found_d[0] = front;
+                    if (mine == INT32_MAX && here > 0.0 && at <= last && up >= goal) {
+                        mine = at;
+                        mine_front = front;
                     }
                     front += here;
                 }
+                const uint64_t reach = __ballot(mine != INT32_MAX);
+                if (reach && (tid & 63) == __ffsll((unsigned long long)reach) - 1) atomicMin(&s.found_i, mine);
                 __syncthreads();
-                b = s.found_i;
+                b = s.found_i == INT32_MAX ? -1 : s.found_i;
+                if (mine == b) s.found_d[0] = mine_front;
+                __syncthreads();
                 in_front = s.found_d[0];
                 __syncthreads();
                 n = b < 0 ? 0 : taken ? take_again(s, row, w, filled, b) : take_out<F32>(s, row, w, b, 0, 0);

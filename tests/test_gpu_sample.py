@@ -363,3 +363,21 @@ def test_numbers_next_to_the_borders_of_many_tokens():
     assert row.numel() >= 10
     check(logits[row].cuda(), u[row, at].cuda(), top_k=k)
     check(logits[row].cuda(), u[row, at].cuda(), top_k=k, top_p=1 - 1e-12)
+
+
+def test_nuclei_that_end_between_two_threads_bins():
+    """A row of 2^19 tokens in order, whose nucleus is set to every number within 64 steps of the weight down to a border of bins that neighbouring threads add up: two
+    roundings of one sum, 2^-45 apart.  The largest number draws the nucleus's last token or the one before it; without a threshold it would draw one of the row's last.
+    (The weights in the bins are good to 2^-41.5 each, so the border lies within 64 steps of where it is in 64 bits.)"""
+    from metis_hip import sample_tokens
+    V, rows = 1 << 19, 128
+    x = torch.sort(torch.randn(V, generator=torch.Generator().manual_seed(1)), descending=True)[0].cuda()
+    upto = torch.cumsum(torch.exp(x.double() - x[0].double()), 0)
+    bins = torch.round((x[0].double() - x.double()) / math.log(2) * 64)
+    logits, u = x.expand(rows, V).contiguous(), torch.full((rows,), 1 - 2.0 ** -24, device="cuda")
+    for last in (235, 271, 275, 283, 295, 299, 363, 399, 427, 439):
+        n = int((bins <= last).sum())
+        p = float(upto[n - 1] / upto[-1])
+        top_p = (p + torch.arange(-rows // 2, rows // 2, dtype=torch.float64) * math.ulp(p)).cuda()
+        tokens, _ = sample_tokens(logits, u, top_p=top_p)
+        assert bool(((tokens - n).abs() <= 2).all()), (last, n, tokens[(tokens - n).abs() > 2])
