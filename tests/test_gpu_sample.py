@@ -381,3 +381,60 @@ def test_nuclei_that_end_between_two_threads_bins():
         top_p = (p + torch.arange(-rows // 2, rows // 2, dtype=torch.float64) * math.ulp(p)).cuda()
         tokens, _ = sample_tokens(logits, u, top_p=top_p)
         assert bool(((tokens - n).abs() <= 2).all()), (last, n, tokens[(tokens - n).abs() > 2])
+
+
+def test_the_same_rows_in_parts_and_alone():
+    """80 rows of 131072 tokens have a workgroup each, one of them alone is shared by several: equal tokens, and log-probabilities within the orders of their sums."""
+    from metis_hip import _lib, sample_tokens
+    V = 131072
+    assert _lib.load().metis_sample_tokens_workspace_bytes(80, V) == 0 and _lib.load().metis_sample_tokens_workspace_bytes(1, V) > 0
+    for dtype in (BF, F32):
+        logits, u = rows_of(21, 80, V, dtype, 2.2, 30)
+        for settings in (dict(), dict(top_k=50), dict(top_p=0.95), dict(top_k=4000, top_p=0.9), dict(top_k=60000), dict(top_p=0.999), dict(temperature=0.7, min_p=0.01)):
+            tokens, logp = sample_tokens(logits, u, **settings)
+            for r in range(0, 80, 9):
+                token, lp = sample_tokens(logits[r:r + 1], u[r:r + 1], **settings)
+                off = 2.0 ** -23 * (1 + abs(float(lp))) + (2.0 ** -17 if settings.get("top_k") else 0)        # (a rounding each, and with top_k two binary32 sums within 2^-18)
+                assert int(token) == int(tokens[r]) and abs(float(lp) - float(logp[r])) <= off
+
+
+def test_rows_in_parts_side_by_side():
+    """Rows that several workgroups share, called again and again on streams and from threads at once, each with a workspace of its own: the same bits, whatever the order in
+    which the workgroups take tokens out."""
+    import threading
+    from metis_hip import _lib, sample_tokens
+    calls = []
+    for rows, V, settings in ((2, 70001, dict(top_p=0.95)), (2, 70001, dict(top_k=3000, top_p=0.9)), (5, 131072, dict(top_p=0.99)), (1, 262144, dict(top_k=50)), (3, 131072, dict())):
+        assert _lib.load().metis_sample_tokens_workspace_bytes(rows, V) > 0
+        for dtype in (BF, F32):
+            calls.append((*rows_of(V + rows, rows, V, dtype, 2.2, 20), settings))
+    want = [sample_tokens(x, u, **settings) for x, u, settings in calls]
+    for x, u, settings in calls:
+        check(x, u, **settings)
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(6):
+        for x, u, settings in calls:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got.append(sample_tokens(x, u, **settings))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i, run in enumerate(got) for a, b in zip(run, want[i % len(calls)]))
+    told, failed = [None] * 4, []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                told[i] = [[sample_tokens(x, u, **settings) for x, u, settings in calls] for _ in range(5)]
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                                         # (shown by the test's own thread)
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for mine in told:
+        for round_ in mine:
+            assert all(torch.equal(a, b) for one, exact in zip(round_, want) for a, b in zip(one, exact))
