@@ -6,7 +6,6 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <cmath>
-#include <limits>
 #include <vector>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
@@ -48,7 +47,9 @@ bool number(PyObject* o, double* v)
     if (*v == -1.0 && PyErr_Occurred()) { PyErr_Clear(); return false; }
     return true;
 }
-bool positive(double v) { return v > 0.0 && v < std::numeric_limits<double>::infinity(); }
+// (in binary32, as the entry points take them)
+bool finite32(double v) { return std::isfinite(static_cast<float>(v)); }
+bool positive(double v) { return static_cast<float>(v) > 0.0f && finite32(v); }
 uintptr_t address(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()); }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 // [.., heads, dim] with dense dimensions; the strides of its rows and heads (of a single one: none that counts)
@@ -116,7 +117,7 @@ PyObject* metis_host_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n
     const int type = cache_type(keys, values);
     if (type < 0 || q.dim() != 3 || q.scalar_type() != at::kBFloat16 || q.size(0) == 0 || q.size(2) != keys.size(3) || tables.dim() != 2 || tables.size(0) != q.size(0) ||
         tables.scalar_type() != at::kInt || (tables.size(1) > 1 && tables.stride(1) != 1) || lengths.dim() != 1 || lengths.size(0) != q.size(0) || lengths.scalar_type() != at::kInt ||
-        !lengths.is_contiguous() || !positive(key_scale) || !positive(value_scale) || !(std::abs(scale) < std::numeric_limits<double>::infinity()))
+        !lengths.is_contiguous() || !positive(key_scale) || !positive(value_scale) || !finite32(scale))
         return not_here();
     const int64_t seqs = q.size(0), heads = q.size(1), dim = q.size(2), width = tables.size(1), page = keys.size(2);
     int64_t qs, qh;

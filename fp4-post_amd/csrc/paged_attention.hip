@@ -378,6 +378,7 @@ int paged_attention(const void* q, int64_t q_seq, int64_t q_head, int64_t seqs, 
     if (seqs < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads > 65536 || q_heads % kv_heads || pages < 0 || pages > INT32_MAX || width < 0 || q_seq < 0 || q_head < 0 || table_stride < 0 ||
         (cache_dtype != METIS_DTYPE_BF16 && !f8))
         return METIS_E_ARG;
+    if (!(fabsf(scale) < INFINITY) || !(key_scale > 0.0f && key_scale < INFINITY) || !(value_scale > 0.0f && value_scale < INFINITY)) return METIS_E_ARG;
     if (dim <= 0 || dim > 256 || dim % (f8 ? 64 : 32) || page < 16 || page > 4096 || (page & (page - 1))) return METIS_E_ARG;
     if (seqs == 0) return METIS_OK;
     if (!out || (uintptr_t)out % 8 || !lengths || (uintptr_t)lengths % 4 || (width > 0 && (!tables || (uintptr_t)tables % 4)) || !q || (uintptr_t)q % 16 || q_seq % 8 || q_head % 8)

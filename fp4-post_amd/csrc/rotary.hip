@@ -202,7 +202,7 @@ int rotary(const void* q, int64_t q_token, int64_t q_head, int64_t q_heads, cons
         turned > dim || turned % 2 || (dtype != METIS_DTYPE_BF16 && dtype != METIS_DTYPE_F32) || (freq_dtype != METIS_DTYPE_F32 && freq_dtype != METIS_DTYPE_F64))
         return METIS_E_ARG;
     if (cached && (dtype != METIS_DTYPE_BF16 || k_heads == 0 || pages <= 0 || page <= 0 || page > 4096 || (cache_dtype != METIS_DTYPE_BF16 && cache_dtype != METIS_DTYPE_E4M3) ||
-                   !(key_scale > 0.0f) || !(value_scale > 0.0f)))
+                   !(key_scale > 0.0f && key_scale < INFINITY) || !(value_scale > 0.0f && value_scale < INFINITY)))
         return METIS_E_ARG;
     if (tokens == 0 || q_heads + k_heads == 0) return METIS_OK;
     if (tokens > (int64_t)1 << 31 || npos <= 0 || tokens % npos || !positions || (turned && !inv_freq)) return METIS_E_ARG;

@@ -1626,9 +1626,13 @@ def _check_cache(what: str, keys: torch.Tensor, values: torch.Tensor, layers: bo
         raise ValueError(f"{what}: values have their dimensions in front of their tokens, [.., dim, page] beside keys of [.., page, dim]: {tuple(keys.shape)}, {tuple(values.shape)}")
 
 
-def _check_scales(what: str, key_scale: float, value_scale: float) -> None:
-    if not 0.0 < key_scale < float("inf") or not 0.0 < value_scale < float("inf"):
-        raise ValueError(f"{what}: positive scales of keys and values, not {key_scale} and {value_scale}")
+def _check_scales(what: str, key_scale: float, value_scale: float, scale: float = 1.0) -> None:
+    """Scales as the kernels hold them, in binary32."""
+    key, value, scores = (ctypes.c_float(s).value for s in (key_scale, value_scale, scale))
+    if not 0.0 < key < float("inf") or not 0.0 < value < float("inf"):
+        raise ValueError(f"{what}: positive scales of keys and values (in binary32), not {key_scale} and {value_scale}")
+    if not abs(scores) < float("inf"):
+        raise ValueError(f"{what}: a finite scale (in binary32), not {scale}")
 
 
 @_on_own_device
@@ -1684,9 +1688,7 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, t
     if tables.dim() != 2 or tables.shape[0] != seqs or tables.dtype != torch.int32 or lengths.shape != (seqs,) or lengths.dtype != torch.int32:
         raise ValueError(f"paged_attention: tables int32 [{seqs}, pages] and lengths int32 [{seqs}], not {tables.dtype} {tuple(tables.shape)} and {lengths.dtype} {tuple(lengths.shape)}")
     scale, key_scale, value_scale = dim ** -0.5 if scale is None else float(scale), float(key_scale), float(value_scale)
-    if not abs(scale) < float("inf"):
-        raise ValueError(f"paged_attention: a finite scale, not {scale}")
-    _check_scales("paged_attention", key_scale, value_scale)
+    _check_scales("paged_attention", key_scale, value_scale, scale)
     if seqs == 0:
         return torch.empty_like(q, memory_format=torch.contiguous_format)
     width = tables.shape[1]

@@ -1044,7 +1044,7 @@ int metis_rotary(const void *q, int64_t q_token, int64_t q_head, int64_t q_heads
 /*
  * A paged cache of one layer: keys [pages, heads, page, dim] and values [pages, heads, dim, page] (a value's dimensions lie
  * `page` elements apart, its neighbours in time side by side), bf16 or e4m3 with one scale for all keys and one for all
- * values (a cached number times the scale is the value).  A place is page number * page + offset.
+ * values, positive and finite (a cached number times the scale is the value).  A place is page number * page + offset.
  *
  * metis_rotary_append: metis_rotary of new tokens' q and k (bf16), the turned keys and the values written to the cache at
  * each token's place, e4m3 rounded to nearest with 448 for everything beyond it.

@@ -470,3 +470,21 @@ def test_weights_of_nothing_carry_nothing(lengths):
     got = paged_attention(q, k, values, tables, n)
     assert bool(got[0].isnan().all())
     check(got[1:], q[1:], k, values, tables[1:], lengths[1:])
+
+
+def test_scales_that_binary32_does_not_have_are_refused():
+    from metis_hip import paged_attention, rotary_append
+    g = torch.Generator().manual_seed(17)
+    keys, values = cache(g, 4, 2, 16, 64)
+    q, k, v = (torch.zeros(5, h, 64, dtype=BF, device="cuda") for h in (4, 2, 2))
+    at, inv, tables = torch.arange(5).cuda(), frequencies(32), torch.zeros(5, 1, dtype=torch.int32, device="cuda")
+    for bad in (1e-50, 1e300):
+        for more in (dict(key_scale=bad), dict(value_scale=bad)):
+            with pytest.raises(ValueError, match="scales"):
+                rotary_append(q, k, v, at, inv, at, keys, values, **more)
+            with pytest.raises(ValueError, match="scales"):
+                paged_attention(q, keys, values, tables, at.int(), **more)
+    for bad in (1e300, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="finite scale"):
+            paged_attention(q, keys, values, tables, at.int(), scale=bad)
+    assert bool(paged_attention(q, keys, values, tables, at.int(), scale=0.0).isfinite().all())

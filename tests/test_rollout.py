@@ -341,3 +341,18 @@ def test_calls_of_more_than_a_launch_takes():
     assert L.metis_paged_attention(*{**ATTEND, "seqs": 1 << 18, "heads": 32, "kv": 1, "width": 1024, "bytes": big}.values()) == _lib.E_TOO_LARGE
     a = (ctypes.c_int64 * 1)(0)
     assert L.metis_cache_copy_pages(4096, 4096, 1 << 20, 8, 1 << 20, ctypes.cast(a, ctypes.c_void_p), ctypes.cast((ctypes.c_int64 * 1)(1), ctypes.c_void_p), 1, None) == _lib.E_TOO_LARGE
+
+
+def test_scales_that_binary32_does_not_have():
+    """Scales of the cache are positive and finite, and so held in binary32: one that is nothing there would make all scores alike."""
+    L = _lib.load()
+    inf, nan = float("inf"), float("nan")
+    for bad in (inf, 0.0, -1.0, nan, 1e-50):
+        assert L.metis_rotary_append(*{**APPEND, "key_scale": bad}.values()) == L.metis_rotary_append(*{**APPEND, "value_scale": bad}.values()) == _lib.E_ARG
+        assert L.metis_paged_attention(*{**ATTEND, "key_scale": bad}.values()) == L.metis_paged_attention(*{**ATTEND, "value_scale": bad}.values()) == _lib.E_ARG
+    for bad in (inf, -inf, nan):
+        assert L.metis_paged_attention(*{**ATTEND, "scale": bad}.values()) == _lib.E_ARG
+    for bad in (1e-50, 1e300, nan):
+        for more in (dict(key_scale=bad), dict(value_scale=bad)):
+            with pytest.raises(ValueError, match="scales"):
+                PagedCache(1, 4, 1, 64, device="cpu", **more)
