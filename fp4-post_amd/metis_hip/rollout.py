@@ -30,10 +30,10 @@ class _Recorded(torch.autograd.Function):
         raise RuntimeError("metis_hip: a call without gradients")
 
 
-def _no_gradients(what: str, *tensors: torch.Tensor) -> None:
+def _no_gradients(what: str, *args) -> None:
     if torch.is_grad_enabled():
-        for t in tensors:
-            if t.requires_grad:
+        for t in args:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
                 raise ValueError(f"{what}: no gradients; call it under torch.no_grad()")
 
 
@@ -49,11 +49,11 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
                rounded to nearest, 448 for everything beyond it"""
     args = q, k, v, positions, inv_freq, slots, keys, values, bool(interleaved), factor, key_scale, value_scale
     if _transformed():
-        _no_gradients("rotary_append", q, k, v)
+        _no_gradients("rotary_append", *args)
         return _Recorded.apply(ops.rotary_append, *args)
     out = _lib.host().rotary_append(*args)
     if out is None:                                                # (refused, or copied first)
-        _no_gradients("rotary_append", q, k, v)
+        _no_gradients("rotary_append", *args)
         out = ops.rotary_append(*args)
     return out
 
@@ -68,11 +68,11 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, t
              for nothing.  A length of 0 gives 0; a negative one, one that the table has no pages for, and a page that the cache does not have give NaN"""
     args = q, keys, values, tables, lengths, scale, key_scale, value_scale
     if _transformed():
-        _no_gradients("paged_attention", q, keys, values)
+        _no_gradients("paged_attention", *args)
         return _Recorded.apply(ops.paged_attention, *args)
     out = _lib.host().paged_attention(*args)
     if out is None:
-        _no_gradients("paged_attention", q, keys, values)
+        _no_gradients("paged_attention", *args)
         out = ops.paged_attention(*args)
     return out
 
@@ -81,6 +81,7 @@ def copy_pages(keys: torch.Tensor, values: torch.Tensor, sources: Sequence[int],
     """Copies whole pages, sources[i] to destinations[i], in all layers of a cache: keys [layers, pages, kv_heads, page, dim], values [layers, pages, kv_heads, dim,
     page].  The numbers are the host's.  No page may be written twice, or written and read."""
     if _lib.host().copy_pages(keys, values, sources, destinations) is None:
+        _no_gradients("copy_pages", keys, values)
         ops.copy_pages(keys, values, sources, destinations)
 
 
@@ -98,11 +99,11 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: 
     ratios to.  A row of nothing but -inf, one with a NaN, or one whose settings or number are out of range has token -1 and NaN."""
     args = logits, uniforms, temperature, top_k, top_p, min_p
     if _transformed():
-        _no_gradients("sample_tokens", logits)
+        _no_gradients("sample_tokens", *args)
         return _Recorded.apply(ops.sample_tokens, *args)
     out = _lib.host().sample_tokens(*args)
     if out is None:
-        _no_gradients("sample_tokens", logits)
+        _no_gradients("sample_tokens", *args)
         out = ops.sample_tokens(*args)
     return out
 

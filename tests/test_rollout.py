@@ -356,3 +356,18 @@ def test_scales_that_binary32_does_not_have():
         for more in (dict(key_scale=bad), dict(value_scale=bad)):
             with pytest.raises(ValueError, match="scales"):
                 PagedCache(1, 4, 1, 64, device="cpu", **more)
+
+
+def test_gradients_of_any_argument_are_refused():
+    """Frequencies, settings and caches too: whoever asks for their gradients would get none."""
+    q, at, inv, u = torch.zeros(2, 4, 64, dtype=BF), torch.arange(2), torch.ones(32), torch.zeros(2)
+    keys, values, logits = torch.zeros(3, 4, 16, 64, dtype=BF), torch.zeros(3, 4, 64, 16, dtype=BF), torch.zeros(2, 5)
+    ask = lambda t: t.clone().requires_grad_()
+    for call in (lambda: rotary_append(q, q, q, at, ask(inv), at, keys, values), lambda: rotary_append(q, q, q, at, inv, at, ask(keys), values),
+                 lambda: rotary_append(q, q, q, at, inv, at, keys, ask(values)), lambda: copy_pages(ask(keys[None]), values[None], [0], [1]),
+                 lambda: paged_attention(q, keys, ask(values), at.int()[:, None], at.int()), lambda: sample_tokens(logits, ask(u)), lambda: sample_tokens(logits, u, temperature=ask(u)),
+                 lambda: sample_tokens(logits, u, top_p=ask(u)), lambda: sample_tokens(ask(logits), u)):
+        with pytest.raises(ValueError, match="no gradients"):
+            call()
+        with torch.no_grad(), pytest.raises(MetisHipError, match="no CPU path"):
+            call()
