@@ -1,7 +1,7 @@
 // Queries and keys turned by the angles of their positions, and the same for new tokens with their keys and values written into the pages of a cache:
 //   (y1, y2) = f (x1 cos a - x2 sin a, x2 cos a + x1 sin a),   a = position * inv_freq[i]
 // for the pairs (i, i + R/2) or (2i, 2i + 1) of a head's first R columns; the columns behind them are copied.  The gradient is the same turn by -a.
-// Bound by memory.  The angle is formed in 64 bits and reduced to a part of a turn in [-1/2, 1/2] before it is rounded to binary32 (a position of 2^20 times a frequency
+// Bound by memory.  The angle is formed in 64 bits and reduced to a part of a turn in [-1/2, 1/2] before anything is rounded to binary32 (a position of 2^20 times a frequency
 // near one has 20 bits before the point, so binary32 would leave 4 behind it); its sine and cosine serve all heads of a token that a lane goes through.  8192 tokens of 28 + 4
 // heads of 128 bf16 numbers (134 MB) in 27 us, 65536 in 181 (5.9 TB/s, a large copy 4.9 to 6.9); a token of 12 + 2 heads into a cache in 2.6, 4099 of
 // 28 + 4 heads (76 MB) in 15.
@@ -70,6 +70,27 @@ template <int N> __device__ __forceinline__ void put_e4m3(uint8_t* p, const floa
     }
 }
 
+// Sine and cosine of a part of a turn for binary32, rounded once: the nearest quarter turn is taken off in 64 bits, and the series of sin(2 pi t) and cos(2 pi t) for what is left,
+// |t| <= 1/8, are added up in 64 bits as well (a 64-bit product takes as long as one in binary32 that is not packed); what is cut off of them is under 2^-33.
+__device__ __forceinline__ void sine_cosine(double turns, float& si, float& co)
+{
+    constexpr double S[6] = {6.283185307179586, -41.34170224039976, 81.60524927607506, -76.70585975306139, 42.058693944897655, -15.09464257682299};
+    constexpr double C[6] = {1.0, -19.739208802178716, 64.9393940226683, -85.45681720669373, 60.24464137187666, -26.4262567833744};
+    const double magic = fma(turns, 4.0, 0x1.8p52), t = fma(magic - 0x1.8p52, -0.25, turns), t2 = t * t;
+    const int quarter = (int)__double_as_longlong(magic);
+    double s = S[5], c = C[5];
+#pragma unroll
+    for (int i = 4; i >= 0; --i) {
+        s = fma(s, t2, S[i]);
+        c = fma(c, t2, C[i]);
+    }
+    const float a = (float)(s * t), b = (float)c;
+    si = quarter & 1 ? b : a;
+    co = quarter & 1 ? a : b;
+    si = quarter & 2 ? -si : si;
+    co = (quarter + 1) & 2 ? -co : co;
+}
+
 // CACHE 0: none; 1: bf16; 2: e4m3.  A workgroup takes tok_lanes tokens, head_lanes of their heads at a time.
 template <bool F32, int N, int CACHE>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a)
@@ -111,7 +132,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a)
             turns -= rint(turns);
             float si, co;
             if constexpr (F32) {
-                sincospif(2.0f * (float)turns, &si, &co);
+                sine_cosine(turns, si, co);
             } else {                                               // (the hardware's sine of a part of a turn is off by less than 2^-20; bf16 has 2^-9)
                 si = __builtin_amdgcn_sinf((float)turns);
                 co = __builtin_amdgcn_cosf((float)turns);

@@ -5,6 +5,8 @@ sine, the cosine and two products lose, all relative to |x1| + |x2|.  For binary
 part's own rounding to binary32 moves the angle by 2 pi 2^-26, the products and the sum by 2^-23: under 2^-19.  For bf16 the hardware's sine and cosine
 are taken, which are off by at most 2^-18 (over all multiples of 2^-24 of a turn 2^-20.5 was seen): under 2^-16.  The angles are formed in 64 bits here and there:
 positions up to 2^24 times frequencies up to one leave 2^-29 of an angle."""
+import math
+
 import pytest
 import torch
 
@@ -256,3 +258,31 @@ def test_beyond_32_bits_of_elements():
     assert all(torch.equal(got[i], want) for i in range(times))
     del many, got
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_binary32_is_as_good_as_a_64_bit_sine_rounded_once(interleaved):
+    """The error's norm beside that of the formula in binary32 with 64-bit sines and cosines rounded once: the same but for the order of roundings, which moves the norm
+    of some 10^6 of them by 10^-3; a part of a turn rounded to binary32 first would add a quarter.  Quarter turns are exact."""
+    from metis_hip import rotary
+    g = torch.Generator().manual_seed(18)
+    inv = frequencies(48, 1e6)
+    q, k = (torch.randn(1500, h, 96, generator=g).cuda() for h in (9, 2))
+    at = torch.randint(-(1 << 20), 1 << 20, (1500,), generator=g).cuda()
+    got, _ = rotary(q, k, at, inv, interleaved=interleaved)
+    want, _ = turned(q, at, inv, interleaved, 1.0)
+    angle = (at.double()[:, None] * inv)[:, None, :]
+    c, s = torch.cos(angle).float(), torch.sin(angle).float()
+    a, b = (q[..., 0::2], q[..., 1::2]) if interleaved else (q[..., :48], q[..., 48:])
+    pair = a * c - b * s, b * c + a * s
+    plain = torch.stack(pair, -1).flatten(-2) if interleaved else torch.cat(pair, -1)
+    off, plain_off = ((x.double() - want).norm() for x in (got, plain))
+    assert float(off) <= 1.01 * float(plain_off), (float(off / want.norm()), float(plain_off / want.norm()))
+    turns = torch.full((1,), 2 * math.pi / 4, dtype=torch.float64, device="cuda")
+    x = torch.randn(8, 1, 2, generator=g).cuda()
+    y, _ = rotary(x, x, torch.arange(-4, 4).cuda(), turns)
+    # (the 64-bit quarter of a turn is off by 2^-53 of it)
+    for i, n in enumerate(range(-4, 4)):
+        re, im = x[i, 0].tolist()
+        exact = [(re, im), (-im, re), (-re, -im), (im, -re)][n % 4]
+        assert all(abs(u - v) <= 2.0 ** -50 * (abs(re) + abs(im)) for u, v in zip(y[i, 0].tolist(), exact))
