@@ -7,7 +7,7 @@
 // and the tokens are dealt to the rows of the first product in an order that leaves a lane with exactly the eight (two times eight) neighbouring tokens of one head
 // that the second product wants from it: no value crosses lanes but the maximum.  The probabilities enter the second product as two bf16 terms, which
 // costs nothing, as the matrix cores are idle most of the time: each is good to 2^-16 of itself and to 2^-126 of the sequence's largest.
-// 28 query and 4 cache heads of 128 numbers, keys and values from memory: 64 ragged sequences of up to 4096 tokens in pages of 64 (277 MB) 65 us, one of 131072 (268 MB) 54 with the joining launch's 5 (5.0 TB/s), 48 ragged ones of up to 16384 tokens of 8 e4m3 heads (811 MB) 155
+// 28 query and 4 cache heads of 128 numbers, keys and values from memory: 64 ragged sequences of up to 4096 tokens in pages of 16 (276 MB) 65 us (in pages of 64 79), one of 131072 (268 MB) 54 with the joining launch's 5 (5.0 TB/s), 48 ragged ones of up to 16384 tokens of 8 e4m3 heads (811 MB) 155
 // (5.2 TB/s); a large copy moves 4.9.  One sequence of 411 tokens 8: lengths, table, a block's keys and values one after the other.
 #include <cmath>
 
@@ -338,10 +338,11 @@ __global__ __launch_bounds__(kJoinThreads) void attend_join_kernel(const AttendA
 }
 
 // Tokens of a split: up to 4096, and so many splits that the workgroups fill the rounds that the device's compute units take them in.  A round that is not full costs as
-// much as one that is, a split the joining launch (5 to 9 us) and its way through memory (64 sequences of 4096 tokens, 4 heads of the cache: 92 us whole, 102 in halves); so the
+// much as one that is, a split the joining launch (5 to 9 us) and its way through memory (64 sequences of 4096 tokens, 4 heads of the cache: 93 us whole, 102 in halves); so the
 // fewest splits that fill 0.85 of the rounds are taken (0.8 where the sequences are cut in any case), or of six more the best.  Uniform and ragged sequences of up to 4096
-// tokens, this and in the fewest splits that reach every compute unit: 48 of them 79 and 84, 54 and 61 us; 65 of them 111 and 133, 62 and 102; 80 of them 128 and 139, 96 and 109;
-// 160 of them 246 and 236, 170 and 207; 130 of them 211 and 222, 131 and 123.  512 tokens are never cut: two blocks a wave take less than the joining launch.
+// tokens, this and in the fewest splits that reach every compute unit, from memory (a GB and more of caches in turn, pages of 64): 48 of them 80 and 79, 68 and 75 us; 65 of them
+// 115 and 150, 74 and 111; 80 of them 133 and 154, 97 and 111; 160 of them 246 and 250, 171 and 208; 130 of them 213 and 240, 132 and 124, the one that loses.  512 tokens are never
+// cut: two blocks a wave take less than the joining launch.
 static int64_t split_tokens(int64_t pairs, int64_t capacity)
 {
     const int64_t block = 64 * kWaves, most = 4096, cus = device_cus();

@@ -3,8 +3,9 @@
 // for the pairs (i, i + R/2) or (2i, 2i + 1) of a head's first R columns; the columns behind them are copied.  The gradient is the same turn by -a.
 // Bound by memory.  The angle is formed in 64 bits and reduced to a part of a turn in [-1/2, 1/2] before anything is rounded to binary32 (a position of 2^20 times a frequency
 // near one has 20 bits before the point, so binary32 would leave 4 behind it); its sine and cosine serve all heads of a token that a lane goes through.  8192 tokens of 28 + 4
-// heads of 128 bf16 numbers (134 MB) in 27 us, 65536 in 181 (5.9 TB/s, a large copy 4.9 to 6.9); a token of 12 + 2 heads into a cache in 2.6, 4099 of
-// 28 + 4 heads (76 MB) in 15.
+// heads of 128 bf16 numbers (134 MB) in 27 us, 65536 in 181 (5.9 TB/s, a large copy 4.9 to 6.9); binary32 (268 MB) 48 us by halves, 64 in neighbouring pairs, where a lane has 64
+// bytes side by side and each of its four loads takes 16 of every 64 bytes.  A token of 12 + 2 heads into a cache in 2.6, 4099 of 28 + 4 heads (76 MB) in 15 (from memory 19), into an
+// e4m3 one 19 (71 MB), 32768 tokens 115 and 112.
 #include "chunk8.h"
 #include "metis_host.h"
 

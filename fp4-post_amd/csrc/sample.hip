@@ -13,12 +13,13 @@
 // the thresholds lie elsewhere (large k, flat rows), further passes over the row do the same with all tokens, and narrow a bin of too many by digits of its logits and indices.
 // A weight is accurate to 2^-44 of itself and sums are held in 64 bits: with some 10^5 tokens next to each other in the running sum, what binary32 is off would take another
 // token now and then.  Whole numbers round once more: of the taken tokens each kept weight to 2^-54 of the largest (one below 2^-53 is 2^-53), in the bins, where they only say
-// where a threshold lies, to 2^-41.5 of itself (beyond 64 octaves to 2^-105 of the largest).  Each pass is a chain of some twenty 64-bit operations for each token, and what it must not do is go through LDS for each (one LDS
-// operation of a compute unit's sixteen waves costs as much as sixteen of these on its four SIMDs): there are no tables, sums over lanes go by DPP.
+// where a threshold lies, to 2^-41.5 of itself (beyond 64 octaves to 2^-105 of the largest).  Each pass is a chain of 25 instructions for each token, 17 of them 64-bit, and an LDS operation beside it
+// would cost as much as sixteen of these (a compute unit's sixteen waves share one LDS and have four SIMDs): there are no tables, sums over lanes go by DPP.  An LDS operation in
+// place of the chain, a count of a bf16 row's logits by their bits, has not been tried.
 // Rows that do not fill the device are shared out to several workgroups for the passes over all tokens, in launches of their own.
-// 256 rows of 131072 bf16 logits (67 MB, 14 us at a large copy's rate): no thresholds 43 us, top_k = 50 38, top_p = 0.95 88 to 106 (the row that keeps most, 12000 to 14000 tokens,
+// 256 rows of 131072 bf16 logits (67 MB, 14 us at a large copy's rate): no thresholds 43 us, top_k = 50 38, top_p = 0.95 83 to 106 (the row that keeps most, 12000 to 14000 tokens,
 // sets the time; most rows take 62 to 72: 12 for the first pass, 5 for the guess of the sum, 7 for the window, 35 for the weights in 64 bits, 4 to 14 for the list, 6 for the
-// stretches and the draw).  Rows that keep more than 27000 of them take 150 to 168.  One row of 131072 binary32 logits with all settings 26 us: 3.3 + 11 + 12.5 in three launches.
+// stretches and the draw).  Rows that keep more than 27000 of them take 150 to 168.  One row of 131072 binary32 logits with all settings 25 us: 3.4 + 11.4 + 11.2 in three launches.
 #include <type_traits>
 
 #include "metis_device.h"
