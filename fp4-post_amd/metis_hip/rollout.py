@@ -8,6 +8,7 @@ from __future__ import annotations
 
 from collections.abc import Sequence
 from dataclasses import dataclass
+from operator import index
 
 import torch
 from torch import nn
@@ -185,7 +186,7 @@ class PagedCache:
     def extend(self, seqs: Sequence[int], counts: Sequence[int] | int = 1) -> CacheStep:
         """Room for new tokens of these sequences, so many of each, and where they go.  Raises MemoryError, and changes nothing, where the pages do not suffice.  Host work
         for every page of the sequences: 0.5 ms for 64 of 4096 tokens in pages of 16, once a step."""
-        counts = [counts] * len(seqs) if isinstance(counts, int) else list(counts)
+        counts = [counts] * len(seqs) if isinstance(counts, int) else [index(n) for n in counts]        # (whole numbers, before the books change)
         if len(counts) != len(seqs) or len(set(seqs)) != len(seqs) or any(s not in self._pages for s in seqs) or any(n < 0 for n in counts):
             raise ValueError(f"PagedCache: sequences of this cache, each once, and a number of new tokens for each: {list(seqs)}, {counts}")
         page, need, writers = self.page, 0, {}

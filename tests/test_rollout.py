@@ -371,3 +371,18 @@ def test_gradients_of_any_argument_are_refused():
             call()
         with torch.no_grad(), pytest.raises(MetisHipError, match="no CPU path"):
             call()
+
+
+def test_counts_that_are_no_whole_numbers():
+    """Refused before a page is taken; whole numbers of other types are taken as such."""
+    import numpy as np
+    cache = PagedCache(1, 8, 1, 64, device="cpu")
+    a, b = cache.new(2)
+    cache.extend([a], [20])
+    for counts in ([1.5, 1], [1, 40.5], [1, None], ["1", 1]):
+        before = cache.free_pages, [(cache.pages(s), cache.length(s)) for s in (a, b)], list(cache._users)
+        with pytest.raises(TypeError):
+            cache.extend([a, b], counts)
+        assert before == (cache.free_pages, [(cache.pages(s), cache.length(s)) for s in (a, b)], list(cache._users))
+    step = cache.extend([a, b], np.array([1, 17]))
+    assert step.counts == (1, 17) and step.lengths.tolist() == [21, 17] and all(type(n) is int for n in step.counts) and type(cache.length(a)) is int
